@@ -18,7 +18,7 @@ HPRMS_OK = 0
 HPRMS_E_INVALID = -22
 HPRMS_E_LAUNCH = -5
 HPRMS_E_RANGE = -34
-DTYPE_BF16, DTYPE_FP16 = 0, 1
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2  # FP32: gradients only
 STREAM_COPY, STREAM_RELU = 0, 1
 MAX_PARTS = 8
 # the `mode` numbering of hprms_select_config / hprms_kernel_configs
@@ -37,6 +37,15 @@ SYMBOLS = (
     "hprms_fused_add_rmsnorm_mx",
     "hprms_streamer",
     "hprms_rmsnorm",
+    "hprms_rmsnorm_backward_workspace",
+    "hprms_rmsnorm_backward",
+    "hprms_linear_cross_entropy_workspace",
+    "hprms_linear_cross_entropy",
+    "hprms_linear_cross_entropy_backward_workspace",
+    "hprms_linear_cross_entropy_backward",
+    "hprms_grad_norm_workspace",
+    "hprms_grad_norm",
+    "hprms_clip_grad_norm",
     "hprms_fused_add_rmsnorm_config",
     "hprms_select_config",
     "hprms_select_config_cu",
@@ -80,6 +89,19 @@ def _bind(L, bench):
     L.hprms_reduce_add_rmsnorm.argtypes = [vp, ctypes.POINTER(vp), ci, vp, vp, i64, i64, i64, i64, i64, ci,
                                            cd, vp]
     L.hprms_fused_add_rmsnorm_mx.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, ci, ci, cd, vp]
+    pvp, pi64, pci = ctypes.POINTER(vp), ctypes.POINTER(i64), ctypes.POINTER(ci)
+    L.hprms_rmsnorm_backward_workspace.argtypes = [i64, i64]
+    L.hprms_rmsnorm_backward.argtypes = [vp] * 7 + [i64] * 7 + [ci, ci, cd, vp]
+    L.hprms_linear_cross_entropy_workspace.argtypes = [i64, i64, i64]
+    L.hprms_linear_cross_entropy.argtypes = [vp] * 6 + [i64] * 7 + [ci, vp]
+    L.hprms_linear_cross_entropy_backward_workspace.argtypes = [i64, i64, i64]
+    L.hprms_linear_cross_entropy_backward.argtypes = [vp] * 8 + [i64] * 9 + [ci, vp]
+    L.hprms_grad_norm_workspace.argtypes = [pi64, ci]
+    L.hprms_grad_norm.argtypes = [vp, pvp, pci, pi64, ci, vp, i64, vp]
+    L.hprms_clip_grad_norm.argtypes = [vp, pvp, pci, pvp, pci, pi64, ci, cd, vp, i64, vp]
+    for name in ("hprms_rmsnorm_backward_workspace", "hprms_linear_cross_entropy_workspace",
+                 "hprms_linear_cross_entropy_backward_workspace", "hprms_grad_norm_workspace"):
+        getattr(L, name).restype = i64
     L.hprms_streamer.argtypes = [vp, vp, i64, i64, i64, i64, ci, ci, vp]
     L.hprms_select_config.argtypes = [i64, i64, ci, ci, ctypes.POINTER(Config)]
     L.hprms_select_config_cu.argtypes = [i64, i64, ci, ci, ci, ctypes.POINTER(Config)]
@@ -95,7 +117,9 @@ def _bind(L, bench):
              "hprms_fused_add_rmsnorm_fp8_ub",
              "hprms_fused_add_rmsnorm_out",
              "hprms_reduce_add_rmsnorm",
-             "hprms_fused_add_rmsnorm_mx", "hprms_streamer", "hprms_select_config", "hprms_select_config_cu",
+             "hprms_fused_add_rmsnorm_mx", "hprms_rmsnorm_backward", "hprms_linear_cross_entropy",
+             "hprms_linear_cross_entropy_backward", "hprms_grad_norm", "hprms_clip_grad_norm",
+             "hprms_streamer", "hprms_select_config", "hprms_select_config_cu",
              "hprms_device_cu_count", "hprms_kernel_configs", "hprms_set_batch_invariant", "hprms_batch_invariant"]
     if bench:
         L.hprms_bench_fused_timeline.argtypes = [vp, vp, vp, i64, i64, ci, cd, ctypes.POINTER(Config), vp, vp]
@@ -210,6 +234,65 @@ class Library:
         return self._check(self.lib().hprms_rmsnorm(out_ptr, in_ptr, weight_ptr, rows, hidden, out_stride,
                                                     in_stride, dtype, eps, stream))
 
+    def _bytes(self, n):
+        if n < 0:
+            raise HprmsError(n, self.last_error())
+        return n
+
+    def rmsnorm_backward_workspace(self, rows, hidden):
+        return self._bytes(self.lib().hprms_rmsnorm_backward_workspace(rows, hidden))
+
+    def rmsnorm_backward(self, dinput_ptr, dweight_ptr, dout_ptr, input_ptr, weight_ptr, dresidual_ptr, workspace_ptr,
+                         workspace_size, rows, hidden, dinput_stride, dout_stride, input_stride, dresidual_stride,
+                         dtype, dweight_dtype, eps, stream=0):
+        return self._check(self.lib().hprms_rmsnorm_backward(
+            dinput_ptr, dweight_ptr, dout_ptr, input_ptr, weight_ptr, dresidual_ptr, workspace_ptr, workspace_size,
+            rows, hidden, dinput_stride, dout_stride, input_stride, dresidual_stride, dtype, dweight_dtype, eps,
+            stream))
+
+    def linear_cross_entropy_workspace(self, rows, hidden, vocab):
+        return self._bytes(self.lib().hprms_linear_cross_entropy_workspace(rows, hidden, vocab))
+
+    def linear_cross_entropy(self, loss_ptr, lse_ptr, hidden_ptr, weight_ptr, target_ptr, workspace_ptr,
+                             workspace_size, rows, hidden, vocab, hidden_stride, weight_stride, ignore_index, dtype,
+                             stream=0):
+        return self._check(self.lib().hprms_linear_cross_entropy(
+            loss_ptr, lse_ptr, hidden_ptr, weight_ptr, target_ptr, workspace_ptr, workspace_size, rows, hidden, vocab,
+            hidden_stride, weight_stride, ignore_index, dtype, stream))
+
+    def linear_cross_entropy_backward_workspace(self, rows, hidden, vocab):
+        return self._bytes(self.lib().hprms_linear_cross_entropy_backward_workspace(rows, hidden, vocab))
+
+    def linear_cross_entropy_backward(self, dhidden_ptr, dweight_ptr, dloss_ptr, hidden_ptr, weight_ptr, target_ptr,
+                                      lse_ptr, workspace_ptr, workspace_size, rows, hidden, vocab, dhidden_stride,
+                                      dweight_stride, hidden_stride, weight_stride, ignore_index, dtype, stream=0):
+        return self._check(self.lib().hprms_linear_cross_entropy_backward(
+            dhidden_ptr, dweight_ptr, dloss_ptr, hidden_ptr, weight_ptr, target_ptr, lse_ptr, workspace_ptr,
+            workspace_size, rows, hidden, vocab, dhidden_stride, dweight_stride, hidden_stride, weight_stride,
+            ignore_index, dtype, stream))
+
+    @staticmethod
+    def _arrays(ptrs, dtypes, counts):
+        n = len(counts)
+        return ((ctypes.c_void_p * max(1, n))(*ptrs), (ctypes.c_int * max(1, n))(*dtypes),
+                (ctypes.c_int64 * max(1, n))(*counts), n)
+
+    def grad_norm_workspace(self, counts):
+        arr = (ctypes.c_int64 * max(1, len(counts)))(*counts)
+        return self._bytes(self.lib().hprms_grad_norm_workspace(arr, len(counts)))
+
+    def grad_norm(self, norm_ptr, grad_ptrs, dtypes, counts, workspace_ptr, workspace_size, stream=0):
+        """``grad_ptrs``, ``dtypes`` and ``counts``: sequences of one length."""
+        g, d, c, n = self._arrays(grad_ptrs, dtypes, counts)
+        return self._check(self.lib().hprms_grad_norm(norm_ptr, g, d, c, n, workspace_ptr, workspace_size, stream))
+
+    def clip_grad_norm(self, norm_ptr, out_ptrs, out_dtypes, grad_ptrs, dtypes, counts, max_norm, workspace_ptr,
+                       workspace_size, stream=0):
+        g, d, c, n = self._arrays(grad_ptrs, dtypes, counts)
+        o, od, _, _ = self._arrays(out_ptrs, out_dtypes, counts)
+        return self._check(self.lib().hprms_clip_grad_norm(norm_ptr, o, od, g, d, c, n, max_norm, workspace_ptr,
+                                                           workspace_size, stream))
+
     def streamer(self, out_ptr, in_ptr, rows, hidden, out_stride, in_stride, dtype, op, stream=0):
         return self._check(self.lib().hprms_streamer(out_ptr, in_ptr, rows, hidden, out_stride, in_stride, dtype,
                                                      op, stream))
@@ -292,6 +375,15 @@ fused_add_rmsnorm_out = PRODUCT.fused_add_rmsnorm_out
 reduce_add_rmsnorm = PRODUCT.reduce_add_rmsnorm
 fused_add_rmsnorm_mx = PRODUCT.fused_add_rmsnorm_mx
 rmsnorm = PRODUCT.rmsnorm
+rmsnorm_backward_workspace = PRODUCT.rmsnorm_backward_workspace
+rmsnorm_backward = PRODUCT.rmsnorm_backward
+linear_cross_entropy_workspace = PRODUCT.linear_cross_entropy_workspace
+linear_cross_entropy = PRODUCT.linear_cross_entropy
+linear_cross_entropy_backward_workspace = PRODUCT.linear_cross_entropy_backward_workspace
+linear_cross_entropy_backward = PRODUCT.linear_cross_entropy_backward
+grad_norm_workspace = PRODUCT.grad_norm_workspace
+grad_norm = PRODUCT.grad_norm
+clip_grad_norm = PRODUCT.clip_grad_norm
 streamer = PRODUCT.streamer
 select_config = PRODUCT.select_config
 device_cu_count = PRODUCT.device_cu_count

@@ -77,18 +77,21 @@ def _atomic(dst, build_fn):
 def build_kernels(bench=True):
     """Compiles every translation unit of csrc/ at once into a scratch
     directory, then links libhprms.so and (with `bench`) libhprms_bench.so.
-    The two share the variant and general-tier objects; hprms.hip is compiled
+    The two share the variant, general-tier and training objects; hprms.hip is compiled
     once per library (HPRMS_BENCH_BUILD adds the bench-only shapes and entry
     point)."""
     hipcc = shutil.which("hipcc") or os.path.join(ROCM, "bin", "hipcc")
-    units = [("hprms.hip", []), ("hprms_unaligned.hip", []), ("hprms_tail.hip", []), ("hprms_general.hip", [])]
+    shared_units = ["hprms_unaligned.hip", "hprms_tail.hip", "hprms_general.hip", "hprms_norm_grad.hip",
+                    "hprms_grad_norm.hip", "hprms_loss.hip"]
+    units = [("hprms.hip", [])] + [(name, []) for name in shared_units]
     if bench:
         units += [("hprms.hip", ["-DHPRMS_BENCH_BUILD"]), ("hprms_ceiling.hip", [])]
     with tempfile.TemporaryDirectory(prefix="hprms_build_") as tmp:
         objs = [os.path.join(tmp, f"{i}_{name}.o") for i, (name, _) in enumerate(units)]
         _run_parallel([[hipcc, *HIP_FLAGS, *defs, "-c", f"-I{INCLUDE}", f"-I{CSRC}", os.path.join(CSRC, name),
                         "-o", obj] for (name, defs), obj in zip(units, objs)])
-        product, shared, bench_objs = objs[0], objs[1:4], objs[4:]
+        n = 1 + len(shared_units)
+        product, shared, bench_objs = objs[0], objs[1:n], objs[n:]
         _atomic(KERNEL_LIB, lambda out: _run([hipcc, *HIP_FLAGS, "-shared", product, *shared, "-o", out]))
         if bench:
             _atomic(BENCH_LIB, lambda out: _run([hipcc, *HIP_FLAGS, "-shared", *bench_objs, *shared, "-o", out]))

@@ -18,6 +18,7 @@
 #include <string.h>
 
 #include "hp_rms_norm_amd.h"
+#include "hprms_host.h"
 #include "hprms_kernels.h"
 #include "hprms_registry.h"
 
@@ -25,6 +26,8 @@ namespace hprms {
 namespace {
 
 thread_local char g_err[512] = "";
+
+}  // namespace
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -39,6 +42,8 @@ int check_launch(const char* what) {
   if (e != hipSuccess) return fail(HPRMS_E_LAUNCH, "%s: kernel launch failed: %s", what, hipGetErrorString(e));
   return HPRMS_OK;
 }
+
+namespace {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 bool aligned2(const void* p) { return ((uintptr_t)p & 1u) == 0; }
@@ -105,7 +110,6 @@ const FusedEntry* find_fused(int dtype, int mode, const hprms_config& c) {
 // CUs, rows * 256 / CUs rounded up; rounds of workgroups are counted on the
 // device's own CUs.  (The reference sizes its persistent grid from the
 // device's multiProcessorCount, hp_rms_norm/csrc/cuda/hp_rms_norm.cuh:550.)
-constexpr int kRefCUs = 256;
 constexpr int kMaxDevices = 64;
 // CUs per device ordinal, 0 until queried.  Threads that race on a first query
 // store the same value.
@@ -128,8 +132,8 @@ int device_cus(int dev) {
   return n;
 }
 
-// CUs of the current device; 256 when there is no device to ask (a launch
-// would then fail and report why)
+}  // namespace
+
 int current_cus() {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) {
@@ -139,6 +143,8 @@ int current_cus() {
   const int n = device_cus(dev);
   return n > 0 ? n : kRefCUs;
 }
+
+namespace {
 
 // ---- batch-invariant mode -----------------------------------------------------------
 // The row-count rules below pick, for one width, shapes whose lanes sum a
@@ -572,18 +578,6 @@ int64_t q_row_bytes(int mode, int64_t hidden) { return mode == 6 ? hidden / 2 : 
 
 bool has_res(int mode) { return mode != 1; }
 bool has_out(int mode) { return mode != 0; }
-
-// No buffer on any GPU spans more bytes (virtual addresses have at most 57
-// bits), and under this bound the kernels' 64-bit row offsets cannot overflow.
-constexpr int64_t kMaxExtentBytes = int64_t(1) << 56;
-
-// `rows` rows of `width` elements of `elem` bytes, `stride` elements apart,
-// span at most kMaxExtentBytes
-bool extent_ok(int64_t rows, int64_t stride, int64_t elem, int64_t width) {
-  if (rows <= 1) return true;
-  if (stride > kMaxExtentBytes / elem) return false;
-  return rows - 1 <= (kMaxExtentBytes / elem - width) / stride;
-}
 
 int check_problem(const Problem& p) {
   if (p.dtype != HPRMS_DTYPE_BF16 && p.dtype != HPRMS_DTYPE_FP16)

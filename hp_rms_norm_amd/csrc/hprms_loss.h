@@ -1,0 +1,347 @@
+// hprms_loss.h - softmax cross entropy of rows under a vocabulary projection,
+// without keeping the logits, and its gradient: device code.
+//
+// z = hidden . weight^T [rows, vocab];  lse = log(sum_v exp(z));
+// loss = lse - z[target];  p = exp(z - lse);  dz = (p - [v == target]) * dloss;
+// dhidden = dz . weight;  dweight = dz^T . hidden.
+//
+// Four matrix products on the matrix cores, each a tile loop whose epilogue
+// does the rest:
+//
+//   forward   z tiles; each leaves per row its maximum and sum of exponentials
+//             (and the target's logit); a second kernel joins the tiles.
+//   gradient  for one piece of the vocabulary at a time: the z tiles again,
+//             turned into dz, rounded to the tensors' 16-bit type and kept for
+//             this piece only; then the piece's rows of dweight and its share of
+//             dhidden, summed over the pieces in binary32.
+//
+// Rows whose target is ignore_index carry no loss: the others are listed first
+// (`index`), the products run over the listed rows alone, and an ignored row's
+// hidden values are never read.
+//
+// dz is rounded to 16 bits because the matrix cores take 16-bit operands: a
+// relative error of half a step per entry, independent between entries, as the
+// outputs' own rounding has.  Its row factor dloss is scaled by a power of two
+// that brings the largest of them to [2^14, 2^15), so that float16 holds dz
+// down to probabilities of 2^-29 (subnormal from there on); the products are
+// scaled back in binary32.
+//
+// Fragments of v_mfma_f32_16x16x32: lane l holds A[l % 16][8 (l / 16) + j] and
+// B[8 (l / 16) + j][l % 16], j = 0 ... 7, and of the product the four rows
+// 4 (l / 16) + i of column l % 16.  The operand whose index should be
+// contiguous in what the epilogue writes or reduces is A: the vocabulary for z,
+// the hidden index for both gradients.
+#pragma once
+
+#include "hprms_device.h"
+
+namespace hprms {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// 16 bytes at any 2-byte boundary
+typedef u32x4 u32x4_u __attribute__((aligned(2)));
+typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(2)));
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == HPRMS_DTYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+
+// What the row list says, written by loss_rows_kernel.
+struct LossMeta {
+  int32_t count;   // listed rows
+  float scale;     // power of two applied to dloss
+  float unscale;   // its inverse
+  int32_t pad;
+};
+
+// The arguments of every loss kernel.
+struct LossArgs {
+  const uint16_t* hidden;
+  const uint16_t* weight;
+  const int64_t* target;
+  const LossMeta* meta;
+  const int32_t* index;     // listed rows
+  int64_t hidden_stride, weight_stride;
+  int64_t ignore_index;
+  int32_t rows;             // of the call
+  int32_t width;            // elements of a hidden row
+  int32_t vocab;
+  // forward
+  float* loss;
+  float* lse;               // backward: read
+  float* target_logit;      // [rows], by list position
+  float2* partial;          // [vocabulary tiles, rows_at]: maximum and sum of exponentials
+  int32_t row_from, rows_at;  // list positions of this launch: [row_from, row_from + rows_at)
+  // backward
+  const float* dloss;
+  uint16_t* dz;             // [rows rounded up, dz_stride], by list position
+  int64_t dz_stride;
+  int32_t piece_from, piece;  // vocabulary rows of this piece
+  uint16_t* dhidden;
+  int64_t dhidden_stride;
+  uint16_t* dweight;
+  int64_t dweight_stride;
+  float* sum;               // [rows, width] shares of dhidden, by list position
+  int32_t first_piece, last_piece;
+};
+
+// ---- epilogues ------------------------------------------------------------------------
+// Each sees a wave's tile of MI x NI fragments whose first row and column are
+// m and n (this lane's: + 16 mi + 4 (lane / 16) + i and + 16 ni + lane % 16).
+
+__device__ __forceinline__ float xor16(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));
+}
+__device__ __forceinline__ float xor32(float v) { return __shfl_xor(v, 32); }
+
+// exp(x) as 2^(x log2 e); the argument is at most 0 in every use but for NaN
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+
+// Per column (list position) of the workgroup's tile: the maximum over its
+// vocabulary rows and the sum of exponentials relative to it.  A wave's 4 lanes
+// of a column join by swizzles, the WM waves stacked over the column through
+// LDS.  NaN logits leave the maximum and make the sum NaN.
+template <int MI, int NI, int WM, int WN>
+__device__ __forceinline__ void forward_epilogue(const LossArgs& a, const f32x4 (&acc)[MI][NI], int m0, int n0, int wm,
+                                                 int wn, int count, int tile, float2* lds) {
+  const int lane = threadIdx.x & 63;
+  __syncthreads();  // the tile loop's LDS reads are over
+#pragma unroll
+  for (int ni = 0; ni < NI; ++ni) {
+    const int col = wn * NI * 16 + ni * 16 + (lane & 15);
+    const int n = n0 + col;
+    const bool live = n < count;
+    const int64_t t = live ? a.target[a.index[n]] : -1;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int v = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4 + i;
+        if (v < a.vocab) top = fmaxf(top, acc[mi][ni][i]);
+        if (live && v == t && v < a.vocab) a.target_logit[n] = acc[mi][ni][i];
+      }
+    top = fmaxf(top, xor16(top));
+    top = fmaxf(top, xor32(top));
+    const float at = top == -__builtin_inff() ? 0.0f : top;  // nothing but -inf here: every exponential is 0
+    float sum = 0.0f;
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int v = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4 + i;
+        if (v < a.vocab) sum += exp_neg(acc[mi][ni][i] - at);
+      }
+    sum += xor16(sum);
+    sum += xor32(sum);
+    if ((lane >> 4) == 0) lds[wm * (WN * NI * 16) + col] = float2{top, sum};
+  }
+  __syncthreads();
+  for (int col = threadIdx.x; col < WN * NI * 16; col += WM * WN * 64) {
+    if (n0 + col >= count) continue;
+    float2 s = lds[col];
+#pragma unroll
+    for (int w = 1; w < WM; ++w) {
+      const float2 o = lds[w * (WN * NI * 16) + col];
+      const float top = fmaxf(s.x, o.x);
+      const float at = top == -__builtin_inff() ? 0.0f : top;
+      s = float2{top, s.y * exp_neg(s.x - at) + o.y * exp_neg(o.x - at)};
+    }
+    a.partial[(int64_t)tile * a.rows_at + (n0 + col - a.row_from)] = s;
+  }
+}
+
+// The piece's dz of the tile, 0 where there is no row or no vocabulary entry.
+// A target outside [0, vocab) gives NaN.
+template <int DT, int MI, int NI>
+__device__ __forceinline__ void dz_epilogue(const LossArgs& a, const f32x4 (&acc)[MI][NI], int m0, int n0, int wm,
+                                            int wn, int count) {
+  using F = Fmt<DT>;
+  const int lane = threadIdx.x & 63;
+  const float scale = a.meta->scale;
+#pragma unroll
+  for (int ni = 0; ni < NI; ++ni) {
+    const int n = n0 + (wn * NI + ni) * 16 + (lane & 15);
+    const bool live = n < count;
+    float lse = 0.0f, g = 0.0f;
+    int64_t t = -1;
+    if (live) {
+      const int row = a.index[n];
+      t = a.target[row];
+      lse = a.lse[row];
+      g = a.dloss[row] * scale;
+      if (t < 0 || t >= a.vocab) g = __builtin_nanf("");
+    }
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+      const int m = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4;
+      float d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int v = a.piece_from + m + i;
+        const float p = exp_neg(acc[mi][ni][i] - lse);
+        d[i] = live && v < a.vocab ? (v == t ? p - 1.0f : p) * g : 0.0f;
+      }
+      u32x2 o = {F::pack(d[0], d[1]), F::pack(d[2], d[3])};
+      *(u32x2*)(a.dz + (int64_t)n * a.dz_stride + m) = o;
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store_four(uint16_t* p, const float* d, int n) {
+  using F = Fmt<DT>;
+  if (n >= 4) {
+    *(u32x2_u*)p = u32x2_u{F::pack(d[0], d[1]), F::pack(d[2], d[3])};
+  } else {
+    for (int i = 0; i < n; ++i) p[i] = F::pack1(d[i]);
+  }
+}
+
+// Rows of dweight: A is the hidden index, the column the vocabulary entry.
+template <int DT, int MI, int NI>
+__device__ __forceinline__ void dweight_epilogue(const LossArgs& a, const f32x4 (&acc)[MI][NI], int m0, int n0, int wm,
+                                                 int wn) {
+  const int lane = threadIdx.x & 63;
+  const float unscale = a.meta->unscale;
+#pragma unroll
+  for (int ni = 0; ni < NI; ++ni) {
+    const int64_t v = (int64_t)a.piece_from + n0 + (wn * NI + ni) * 16 + (lane & 15);
+    if (v >= a.vocab) continue;
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+      const int m = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4;
+      float d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = acc[mi][ni][i] * unscale;
+      if (m < a.width) store_four<DT>(a.dweight + v * a.dweight_stride + m, d, a.width - m);
+    }
+  }
+}
+
+// A piece's share of dhidden: A is the hidden index, the column the list position.
+template <int DT, int MI, int NI>
+__device__ __forceinline__ void dhidden_epilogue(const LossArgs& a, const f32x4 (&acc)[MI][NI], int m0, int n0, int wm,
+                                                 int wn, int count) {
+  const int lane = threadIdx.x & 63;
+  const float unscale = a.meta->unscale;
+#pragma unroll
+  for (int ni = 0; ni < NI; ++ni) {
+    const int n = n0 + (wn * NI + ni) * 16 + (lane & 15);
+    if (n >= count) continue;
+    const int64_t row = a.index[n];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+      const int m = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4;
+      const int left = a.width - m;
+      if (left <= 0) continue;
+      float* s = a.sum + (int64_t)n * a.width + m;
+      float d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        d[i] = acc[mi][ni][i];
+        if (!a.first_piece && i < left) d[i] += s[i];
+      }
+      if (a.last_piece) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] *= unscale;
+        store_four<DT>(a.dhidden + row * a.dhidden_stride + m, d, left);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < left) s[i] = d[i];
+      }
+    }
+  }
+}
+
+// ---- operands of the general tile loop ---------------------------------------------------
+// Operand rows r (in [0, rows)) over the summed index k (in [0, depth)).
+// KMAJOR false: k contiguous, element (r, k) at base + row(r) * stride + k.
+// KMAJOR true: r contiguous, element (r, k) at base + row(k) * stride + r.
+// row(i) = list ? list[i] : i.
+struct Operand {
+  const uint16_t* base;
+  int64_t stride;
+  const int32_t* list;
+  int32_t rows, depth;
+  __device__ __forceinline__ const uint16_t* at(int32_t i) const {
+    return base + (int64_t)(list ? list[i] : i) * stride;
+  }
+};
+
+constexpr int kTile = 128;      // rows and columns of a workgroup's tile
+constexpr int kDepth = 32;      // summed entries per step
+constexpr int kLdsRow = 40;     // elements between LDS rows (80 bytes: 16-byte aligned, off the bank period)
+
+// 8 elements p[0 ... 7] of which the first n exist
+__device__ __forceinline__ u32x4 load_some(const uint16_t* p, int n) {
+  if (n >= 8) return *(const u32x4_u*)p;
+  u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < n) v[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
+  return v;
+}
+
+// Rows r0 ... r0 + 127 of an operand, entries k0 ... k0 + 31, to LDS as [row][k].
+template <bool KMAJOR>
+__device__ __forceinline__ void stage(const Operand& o, int r0, int k0, uint16_t* lds) {
+#pragma unroll
+  for (int it = 0; it < 2; ++it) {
+    const int c = threadIdx.x + it * 256;
+    if constexpr (!KMAJOR) {
+      const int r = c >> 2, k = (c & 3) * 8;
+      u32x4 v = {0, 0, 0, 0};
+      if (r0 + r < o.rows && k0 + k < o.depth) v = load_some(o.at(r0 + r) + k0 + k, o.depth - k0 - k);
+      *(u32x4*)(lds + r * kLdsRow + k) = v;
+    } else {
+      const int k = c >> 4, r = (c & 15) * 8;
+      u32x4 v = {0, 0, 0, 0};
+      if (k0 + k < o.depth && r0 + r < o.rows) v = load_some(o.at(k0 + k) + r0 + r, o.rows - r0 - r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lds[(r + j) * kLdsRow + k] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+    }
+  }
+}
+
+// 128 x 128 tile by 4 waves of 64 x 64: any sizes, strides and alignment.
+template <int DT, bool AK, bool BK>
+__device__ __forceinline__ void general_tile(const Operand& oa, const Operand& ob, int m0, int n0, uint16_t* lds,
+                                             f32x4 (&acc)[4][4]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave >> 1, wn = wave & 1;
+  uint16_t* la = lds;
+  uint16_t* lb = lds + kTile * kLdsRow;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  for (int k0 = 0; k0 < oa.depth; k0 += kDepth) {
+    __syncthreads();
+    stage<AK>(oa, m0, k0, la);
+    stage<BK>(ob, n0, k0, lb);
+    __syncthreads();
+    u32x4 fa[4], fb[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      fa[i] = *(const u32x4*)(la + (wm * 64 + i * 16 + (lane & 15)) * kLdsRow + (lane >> 4) * 8);
+      fb[i] = *(const u32x4*)(lb + (wn * 64 + i * 16 + (lane & 15)) * kLdsRow + (lane >> 4) * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = mfma16<DT>(fa[i], fb[j], acc[i][j]);
+  }
+}
+
+}  // namespace hprms

@@ -17,9 +17,13 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
+
+#include <algorithm>
+#include <vector>
 
 #include "hp_rms_norm_amd.h"
 
@@ -549,6 +553,326 @@ void rms_norm_mx_meta(at::Tensor& out, at::Tensor& scales, const at::Tensor& inp
   (void)eps;
 }
 
+// ---- training: gradients, the loss, clipping ------------------------------------------
+// Workspace of a call on the current stream: from torch's allocator, which hands
+// its memory out again only behind this call's work on that stream (and, in a
+// captured graph, keeps it to the graph).
+at::Tensor workspace_of(int64_t bytes, const at::Tensor& like) {
+  TORCH_CHECK(bytes >= 0, "hp_rms_norm: ", hprms_last_error(), " (status ", bytes, ")");
+  return at::empty({bytes > 0 ? bytes : 1}, like.options().dtype(at::kByte).requires_grad(false));
+}
+
+struct BackwardShape {
+  int64_t rows, hidden, din_stride, dout_stride, in_stride, dres_stride;
+  int dtype, dweight_dtype;
+};
+
+BackwardShape check_backward(const at::Tensor& dinput, const at::Tensor& dweight, const at::Tensor& dout,
+                             const at::Tensor& input, const at::Tensor& weight,
+                             const std::optional<at::Tensor>& dresidual) {
+  TORCH_CHECK(input.dim() >= 2, "input.dim() >= 2");
+  TORCH_CHECK(weight.dim() == 1, "weight.dim() == 1");
+  BackwardShape s;
+  s.hidden = weight.size(0);
+  s.dtype = dtype_code(input);
+  TORCH_CHECK(input.size(-1) == s.hidden, "input.size(-1) == hidden_dim");
+  TORCH_CHECK(weight.stride(0) == 1 || s.hidden <= 1, "weight.stride(0) == 1");
+  TORCH_CHECK(weight.scalar_type() == input.scalar_type(), "weight.dtype() == input.dtype()");
+  TORCH_CHECK(weight.device() == input.device(), "weight must be on input's device");
+  TORCH_CHECK(dweight.dim() == 1 && dweight.size(0) == s.hidden, "dweight must be shaped like weight");
+  TORCH_CHECK(dweight.stride(0) == 1 || s.hidden <= 1, "dweight.stride(0) == 1");
+  TORCH_CHECK(dweight.scalar_type() == input.scalar_type() || dweight.scalar_type() == at::kFloat,
+              "dweight.dtype() must be weight.dtype() or float32");
+  TORCH_CHECK(dweight.device() == input.device(), "dweight must be on input's device");
+  s.dweight_dtype = dweight.scalar_type() == at::kFloat ? HPRMS_DTYPE_FP32 : s.dtype;
+  const at::Tensor* rows[4] = {&input, &dout, &dinput, dresidual ? &*dresidual : &input};
+  for (const at::Tensor* t : rows) {
+    TORCH_CHECK(t->sizes() == input.sizes(), "dinput, dout and dresidual must be shaped like input");
+    TORCH_CHECK(t->stride(-1) == 1 || s.hidden <= 1, "rows must be contiguous (stride(-1) == 1)");
+    TORCH_CHECK(t->scalar_type() == input.scalar_type(), "dinput, dout and dresidual must have input.dtype()");
+    TORCH_CHECK(t->device() == input.device(), "all tensors must be on input's device");
+  }
+  int64_t r = 0;
+  rows_of(input, s.hidden, &s.rows, &s.in_stride);
+  rows_of(dout, s.hidden, &r, &s.dout_stride);
+  rows_of(dinput, s.hidden, &r, &s.din_stride);
+  rows_of(*rows[3], s.hidden, &r, &s.dres_stride);
+  if (s.rows > 0 && s.hidden > 0) {
+    // dinput may lie on any one of the row tensors exactly: a row is read before it is written
+    for (const at::Tensor* t : rows)
+      if (t != &dinput) at::assert_no_partial_overlap(dinput, *t);
+    at::assert_no_overlap(dinput, weight);
+    for (const at::Tensor* t : rows) at::assert_no_overlap(dweight, *t);
+    at::assert_no_overlap(dweight, weight);
+  }
+  return s;
+}
+
+void rms_norm_backward_hip(at::Tensor& dinput, at::Tensor& dweight, const at::Tensor& dout, const at::Tensor& input,
+                           const at::Tensor& weight, const std::optional<at::Tensor>& dresidual, double eps) {
+  const BackwardShape s = check_backward(dinput, dweight, dout, input, weight, dresidual);
+  if (s.hidden == 0) return;
+  c10::DeviceGuard guard(input.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(input.device().index()).stream();
+  const at::Tensor ws = workspace_of(hprms_rmsnorm_backward_workspace(s.rows, s.hidden), input);
+  check_status(hprms_rmsnorm_backward(dinput.data_ptr(), dweight.data_ptr(), dout.data_ptr(), input.data_ptr(),
+                                      weight.data_ptr(), dresidual ? dresidual->data_ptr() : nullptr, ws.data_ptr(),
+                                      ws.numel(), s.rows, s.hidden, s.din_stride, s.dout_stride, s.in_stride,
+                                      s.dres_stride, s.dtype, s.dweight_dtype, eps, stream));
+}
+
+void rms_norm_backward_meta(at::Tensor& dinput, at::Tensor& dweight, const at::Tensor& dout, const at::Tensor& input,
+                            const at::Tensor& weight, const std::optional<at::Tensor>& dresidual, double eps) {
+  (void)check_backward(dinput, dweight, dout, input, weight, dresidual);
+  (void)eps;
+}
+
+struct LossShape {
+  int64_t rows, hidden, vocab, hidden_stride, weight_stride;
+  int dtype;
+};
+
+// Rows and row stride of a [vocab, hidden] matrix.
+int64_t matrix_stride(const at::Tensor& t, int64_t hidden) {
+  const int64_t stride = t.size(0) <= 1 ? hidden : t.stride(0);
+  TORCH_CHECK(stride >= hidden, "rows of the tensor overlap (row stride ", stride, " < hidden ", hidden, ")");
+  return stride;
+}
+
+LossShape check_loss(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target,
+                     std::initializer_list<const at::Tensor*> per_row) {
+  TORCH_CHECK(hidden.dim() >= 2, "hidden.dim() >= 2");
+  TORCH_CHECK(weight.dim() == 2, "weight.dim() == 2");
+  LossShape s;
+  s.vocab = weight.size(0);
+  s.hidden = weight.size(1);
+  s.dtype = dtype_code(hidden);
+  TORCH_CHECK(hidden.size(-1) == s.hidden, "hidden.size(-1) == weight.size(1)");
+  TORCH_CHECK(s.hidden >= 1 && s.vocab >= 1, "weight must hold at least one element");
+  TORCH_CHECK(hidden.stride(-1) == 1 || s.hidden == 1, "hidden.stride(-1) == 1");
+  TORCH_CHECK(weight.stride(1) == 1 || s.hidden == 1, "weight.stride(1) == 1");
+  TORCH_CHECK(weight.scalar_type() == hidden.scalar_type(), "weight.dtype() == hidden.dtype()");
+  TORCH_CHECK(weight.device() == hidden.device() && target.device() == hidden.device(),
+              "hidden, weight and target must be on the same device");
+  TORCH_CHECK(target.scalar_type() == at::kLong, "target.dtype() == int64");
+  TORCH_CHECK(target.sizes() == hidden.sizes().slice(0, hidden.dim() - 1), "target must have one element per row");
+  TORCH_CHECK(target.is_contiguous(), "target must be contiguous");
+  for (const at::Tensor* t : per_row) {
+    TORCH_CHECK(t->scalar_type() == at::kFloat, "loss, lse and dloss must be float32");
+    TORCH_CHECK(t->sizes() == target.sizes(), "loss, lse and dloss must be shaped like target");
+    TORCH_CHECK(t->is_contiguous(), "loss, lse and dloss must be contiguous");
+    TORCH_CHECK(t->device() == hidden.device(), "all tensors must be on hidden's device");
+  }
+  rows_of(hidden, s.hidden, &s.rows, &s.hidden_stride);
+  s.weight_stride = matrix_stride(weight, s.hidden);
+  return s;
+}
+
+LossShape check_loss_forward(const at::Tensor& loss, const at::Tensor& lse, const at::Tensor& hidden,
+                             const at::Tensor& weight, const at::Tensor& target) {
+  const LossShape s = check_loss(hidden, weight, target, {&loss, &lse});
+  if (s.rows > 0) {
+    at::assert_no_overlap(loss, lse);
+    for (const at::Tensor* out : {&loss, &lse})
+      for (const at::Tensor* in : {&hidden, &weight, &target}) at::assert_no_overlap(*out, *in);
+  }
+  return s;
+}
+
+void linear_cross_entropy_hip(at::Tensor& loss, at::Tensor& lse, const at::Tensor& hidden, const at::Tensor& weight,
+                              const at::Tensor& target, int64_t ignore_index) {
+  const LossShape s = check_loss_forward(loss, lse, hidden, weight, target);
+  if (s.rows == 0) return;
+  c10::DeviceGuard guard(hidden.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(hidden.device().index()).stream();
+  const at::Tensor ws = workspace_of(hprms_linear_cross_entropy_workspace(s.rows, s.hidden, s.vocab), hidden);
+  check_status(hprms_linear_cross_entropy(loss.data_ptr<float>(), lse.data_ptr<float>(), hidden.data_ptr(),
+                                          weight.data_ptr(), target.data_ptr<int64_t>(), ws.data_ptr(), ws.numel(),
+                                          s.rows, s.hidden, s.vocab, s.hidden_stride, s.weight_stride, ignore_index,
+                                          s.dtype, stream));
+}
+
+void linear_cross_entropy_meta(at::Tensor& loss, at::Tensor& lse, const at::Tensor& hidden, const at::Tensor& weight,
+                               const at::Tensor& target, int64_t ignore_index) {
+  (void)check_loss_forward(loss, lse, hidden, weight, target);
+  (void)ignore_index;
+}
+
+struct LossGradShape {
+  LossShape f;
+  int64_t dhidden_stride, dweight_stride;
+};
+
+LossGradShape check_loss_backward(const at::Tensor& dhidden, const at::Tensor& dweight, const at::Tensor& dloss,
+                                  const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target,
+                                  const at::Tensor& lse) {
+  LossGradShape s;
+  s.f = check_loss(hidden, weight, target, {&lse, &dloss});
+  TORCH_CHECK(dhidden.sizes() == hidden.sizes(), "dhidden must be shaped like hidden");
+  TORCH_CHECK(dweight.sizes() == weight.sizes(), "dweight must be shaped like weight");
+  for (const at::Tensor* t : {&dhidden, &dweight}) {
+    TORCH_CHECK(t->stride(-1) == 1 || s.f.hidden == 1, "rows must be contiguous (stride(-1) == 1)");
+    TORCH_CHECK(t->scalar_type() == hidden.scalar_type(), "dhidden and dweight must have hidden.dtype()");
+    TORCH_CHECK(t->device() == hidden.device(), "all tensors must be on hidden's device");
+  }
+  int64_t r = 0;
+  rows_of(dhidden, s.f.hidden, &r, &s.dhidden_stride);
+  s.dweight_stride = matrix_stride(dweight, s.f.hidden);
+  at::assert_no_overlap(dweight, weight);
+  if (s.f.rows > 0) {
+    at::assert_no_overlap(dhidden, dweight);
+    for (const at::Tensor* out : {&dhidden, &dweight})
+      for (const at::Tensor* in : {&hidden, &weight, &target, &lse, &dloss}) at::assert_no_overlap(*out, *in);
+  }
+  return s;
+}
+
+void linear_cross_entropy_backward_hip(at::Tensor& dhidden, at::Tensor& dweight, const at::Tensor& dloss,
+                                       const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target,
+                                       const at::Tensor& lse, int64_t ignore_index) {
+  const LossGradShape s = check_loss_backward(dhidden, dweight, dloss, hidden, weight, target, lse);
+  c10::DeviceGuard guard(hidden.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(hidden.device().index()).stream();
+  const at::Tensor ws =
+      workspace_of(hprms_linear_cross_entropy_backward_workspace(s.f.rows, s.f.hidden, s.f.vocab), hidden);
+  check_status(hprms_linear_cross_entropy_backward(
+      dhidden.data_ptr(), dweight.data_ptr(), dloss.data_ptr<float>(), hidden.data_ptr(), weight.data_ptr(),
+      target.data_ptr<int64_t>(), lse.data_ptr<float>(), ws.data_ptr(), ws.numel(), s.f.rows, s.f.hidden, s.f.vocab,
+      s.dhidden_stride, s.dweight_stride, s.f.hidden_stride, s.f.weight_stride, ignore_index, s.f.dtype, stream));
+}
+
+void linear_cross_entropy_backward_meta(at::Tensor& dhidden, at::Tensor& dweight, const at::Tensor& dloss,
+                                        const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target,
+                                        const at::Tensor& lse, int64_t ignore_index) {
+  (void)check_loss_backward(dhidden, dweight, dloss, hidden, weight, target, lse);
+  (void)ignore_index;
+}
+
+int grad_dtype_code(const at::Tensor& t) {
+  if (t.scalar_type() == at::kFloat) return HPRMS_DTYPE_FP32;
+  if (t.scalar_type() == at::kBFloat16) return HPRMS_DTYPE_BF16;
+  if (t.scalar_type() == at::kHalf) return HPRMS_DTYPE_FP16;
+  TORCH_CHECK(false, "gradients must be bfloat16, float16 or float32");
+  return -1;
+}
+
+// [first, last) bytes of a dense tensor's elements
+struct Span {
+  uintptr_t first, last;
+  size_t i;
+};
+
+Span span_of(const at::Tensor& t, size_t i) {
+  const uintptr_t p = (uintptr_t)t.data_ptr();
+  return {p, p + (uintptr_t)t.numel() * t.element_size(), i};
+}
+
+void check_grads(const at::Tensor& norm, at::TensorList grads) {
+  TORCH_CHECK(!grads.empty(), "grads must hold at least one tensor");
+  TORCH_CHECK(norm.scalar_type() == at::kFloat && norm.numel() == 1, "norm must hold one float32");
+  for (const at::Tensor& g : grads) {
+    (void)grad_dtype_code(g);
+    TORCH_CHECK(g.device() == norm.device(), "all gradients must be on one device");
+    TORCH_CHECK(g.is_non_overlapping_and_dense(), "gradients must be dense in memory");
+  }
+}
+
+void check_outs(at::TensorList outs, at::TensorList grads) {
+  TORCH_CHECK(outs.size() == grads.size(), "outs must hold one tensor per gradient");
+  for (size_t i = 0; i < outs.size(); ++i) {
+    TORCH_CHECK(outs[i].sizes() == grads[i].sizes(), "outs[i] must be shaped like grads[i]");
+    TORCH_CHECK(outs[i].is_non_overlapping_and_dense() && (outs[i].strides() == grads[i].strides() ||
+                                                           (outs[i].is_contiguous() && grads[i].is_contiguous())),
+                "outs[i] must be laid out like grads[i]");
+    TORCH_CHECK(outs[i].device() == grads[i].device(), "outs must be on the gradients' device");
+    TORCH_CHECK(outs[i].scalar_type() == grads[i].scalar_type() || outs[i].scalar_type() == at::kFloat,
+                "outs[i].dtype() must be grads[i].dtype() or float32");
+  }
+}
+
+// No output shares memory with another output, with the norm or with a
+// gradient other than its own (which it must then be, exactly).
+void check_out_spans(const at::Tensor& norm, at::TensorList outs, at::TensorList grads) {
+  std::vector<Span> spans;
+  for (size_t i = 0; i < outs.size(); ++i)
+    if (outs[i].numel() > 0) spans.push_back(span_of(outs[i], i));
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.first < b.first; });
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK(spans[i - 1].last <= spans[i].first, "two of the tensors to be written share memory");
+  auto meets = [&](const Span& s, bool own) {
+    // the first output that ends after s begins
+    auto it = std::upper_bound(spans.begin(), spans.end(), s.first,
+                               [](uintptr_t v, const Span& o) { return v < o.last; });
+    for (; it != spans.end() && it->first < s.last; ++it)
+      TORCH_CHECK(own && it->i == s.i && it->first == s.first && it->last == s.last,
+                  "a tensor to be written shares memory with another tensor");
+  };
+  for (size_t i = 0; i < grads.size(); ++i)
+    if (grads[i].numel() > 0) meets(span_of(grads[i], i), true);
+  meets(span_of(norm, 0), false);
+}
+
+struct GradArrays {
+  std::vector<void*> outs;
+  std::vector<const void*> grads;
+  std::vector<int> out_dtypes, dtypes;
+  std::vector<int64_t> counts;
+};
+
+GradArrays grad_arrays(at::TensorList outs, at::TensorList grads) {
+  GradArrays a;
+  for (const at::Tensor& t : outs) {
+    a.outs.push_back(t.data_ptr());
+    a.out_dtypes.push_back(grad_dtype_code(t));
+  }
+  for (const at::Tensor& t : grads) {
+    a.grads.push_back(t.data_ptr());
+    a.dtypes.push_back(grad_dtype_code(t));
+    a.counts.push_back(t.numel());
+  }
+  return a;
+}
+
+void grad_norm_hip(at::Tensor& norm, at::TensorList grads) {
+  check_grads(norm, grads);
+  const GradArrays a = grad_arrays({}, grads);
+  const int n = (int)grads.size();
+  c10::DeviceGuard guard(norm.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(norm.device().index()).stream();
+  const at::Tensor ws = workspace_of(hprms_grad_norm_workspace(a.counts.data(), n), norm);
+  check_status(hprms_grad_norm(norm.data_ptr<float>(), a.grads.data(), a.dtypes.data(), a.counts.data(), n,
+                               ws.data_ptr(), ws.numel(), stream));
+}
+
+void grad_norm_meta(at::Tensor& norm, at::TensorList grads) { check_grads(norm, grads); }
+
+void clip_grad_norm_out_hip(at::Tensor& norm, at::TensorList outs, at::TensorList grads, double max_norm) {
+  check_grads(norm, grads);
+  check_outs(outs, grads);
+  check_out_spans(norm, outs, grads);
+  const GradArrays a = grad_arrays(outs, grads);
+  const int n = (int)grads.size();
+  c10::DeviceGuard guard(norm.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(norm.device().index()).stream();
+  const at::Tensor ws = workspace_of(hprms_grad_norm_workspace(a.counts.data(), n), norm);
+  check_status(hprms_clip_grad_norm(norm.data_ptr<float>(), a.outs.data(), a.out_dtypes.data(), a.grads.data(),
+                                    a.dtypes.data(), a.counts.data(), n, max_norm, ws.data_ptr(), ws.numel(), stream));
+}
+
+void clip_grad_norm_out_meta(at::Tensor& norm, at::TensorList outs, at::TensorList grads, double max_norm) {
+  check_grads(norm, grads);
+  check_outs(outs, grads);
+  (void)max_norm;
+}
+
+void clip_grad_norm_hip_(at::Tensor& norm, at::TensorList grads, double max_norm) {
+  clip_grad_norm_out_hip(norm, grads, grads, max_norm);
+}
+
+void clip_grad_norm_meta_(at::Tensor& norm, at::TensorList grads, double max_norm) {
+  clip_grad_norm_out_meta(norm, grads, grads, max_norm);
+}
+
 // _C.set_batch_invariant(enable) -> previous setting; _C.batch_invariant()
 // -> current setting (hprms_set_batch_invariant / hprms_batch_invariant).
 PyObject* py_set_batch_invariant(PyObject*, PyObject* arg) {
@@ -605,6 +929,15 @@ TORCH_LIBRARY(hp_rms_norm, m) {
   m.def("reduce_add_rms_norm(Tensor(a!) out, Tensor[] parts, Tensor weight, Tensor(b!) residual, float eps) -> ()");
   m.def("rms_norm_mx_quant(Tensor(a!) out, Tensor(b!) scales, Tensor input, Tensor weight, Tensor(c!) residual, "
         "int format, float eps) -> ()");
+  m.def("rms_norm_backward(Tensor(a!) dinput, Tensor(b!) dweight, Tensor dout, Tensor input, Tensor weight, "
+        "Tensor? dresidual, float eps) -> ()");
+  m.def("linear_cross_entropy(Tensor(a!) loss, Tensor(b!) lse, Tensor hidden, Tensor weight, Tensor target, "
+        "int ignore_index) -> ()");
+  m.def("linear_cross_entropy_backward(Tensor(a!) dhidden, Tensor(b!) dweight, Tensor dloss, Tensor hidden, "
+        "Tensor weight, Tensor target, Tensor lse, int ignore_index) -> ()");
+  m.def("grad_norm(Tensor(a!) norm, Tensor[] grads) -> ()");
+  m.def("clip_grad_norm_(Tensor(a!) norm, Tensor(b!)[] grads, float max_norm) -> ()");
+  m.def("clip_grad_norm_out(Tensor(a!) norm, Tensor(b!)[] outs, Tensor[] grads, float max_norm) -> ()");
 }
 
 // ROCm builds of PyTorch expose HIP devices under the CUDA dispatch key.
@@ -620,6 +953,12 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
   m.impl("rms_norm_out", &rms_norm_out_hip);
   m.impl("reduce_add_rms_norm", &reduce_rms_norm_hip);
   m.impl("rms_norm_mx_quant", &rms_norm_mx_hip);
+  m.impl("rms_norm_backward", &rms_norm_backward_hip);
+  m.impl("linear_cross_entropy", &linear_cross_entropy_hip);
+  m.impl("linear_cross_entropy_backward", &linear_cross_entropy_backward_hip);
+  m.impl("grad_norm", &grad_norm_hip);
+  m.impl("clip_grad_norm_", &clip_grad_norm_hip_);
+  m.impl("clip_grad_norm_out", &clip_grad_norm_out_hip);
 }
 
 // Shape checks only, for fake tensors / torch.compile tracing.  Meta tensors
@@ -636,4 +975,10 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
   m.impl("rms_norm_out", &rms_norm_out_meta);
   m.impl("reduce_add_rms_norm", &reduce_rms_norm_meta);
   m.impl("rms_norm_mx_quant", &rms_norm_mx_meta);
+  m.impl("rms_norm_backward", &rms_norm_backward_meta);
+  m.impl("linear_cross_entropy", &linear_cross_entropy_meta);
+  m.impl("linear_cross_entropy_backward", &linear_cross_entropy_backward_meta);
+  m.impl("grad_norm", &grad_norm_meta);
+  m.impl("clip_grad_norm_", &clip_grad_norm_meta_);
+  m.impl("clip_grad_norm_out", &clip_grad_norm_out_meta);
 }

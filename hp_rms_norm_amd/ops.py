@@ -9,6 +9,9 @@ __all__ = ["hp_rms_norm", "relu", "relu_max0", "rms_norm", "fused_add_rms_norm",
            "hp_rms_norm_fp8_group", "fused_add_rms_norm_fp8_group",
            "reduce_add_rms_norm", "hp_rms_norm_mx",
            "fused_add_rms_norm_mxfp8", "fused_add_rms_norm_mxfp4", "MXFP8", "MXFP4",
+           "rms_norm_backward", "rms_norm_backward_out", "linear_cross_entropy", "linear_cross_entropy_out",
+           "linear_cross_entropy_backward", "linear_cross_entropy_backward_out",
+           "grad_norm", "clip_grad_norm_", "clip_grad_norm_out",
            "set_batch_invariant", "batch_invariant"]
 
 MXFP8, MXFP4 = 0, 1  # element formats of the OCP MX output
@@ -197,6 +200,108 @@ def fused_add_rms_norm_mxfp4(input, residual, weight, eps):
     q, scales = _mx_alloc(input, MXFP4)
     hp_rms_norm_mx(q, scales, input, weight, residual, eps, MXFP4)
     return q, scales
+
+
+def rms_norm_backward_out(dinput, dweight, dout, input, weight, eps, dresidual=None):
+    """Gradient of ``rms_norm`` and of ``hp_rms_norm`` / ``fused_add_rms_norm``
+    into given tensors.  ``input`` is what was normalised -- for the fused op
+    the updated residual -- and ``dout`` the gradient of the normalised output.
+    With ``r = rsqrt(mean(input^2) + eps)``: ``dinput <- r * (dout * weight) -
+    input * (r^3 * mean(dout * weight * input))``, plus ``dresidual`` (the
+    gradient that reaches the updated residual by its other uses) if given;
+    ``dweight <- sum over rows of dout * input * r``, in ``weight``'s dtype or
+    float32.  Sums are fp32, each output is rounded once.  The fused op's
+    input and residual both have the gradient ``dinput``.  ``dinput`` may be
+    ``dout``, ``dresidual`` or ``input``.  No reference counterpart."""
+    torch.ops.hp_rms_norm.rms_norm_backward.default(dinput, dweight, dout, input, weight, dresidual, eps)
+
+
+def rms_norm_backward(dout, input, weight, eps, dresidual=None):
+    """Allocating form of ``rms_norm_backward_out``: returns ``(dinput,
+    dweight)`` in the dtypes of ``input`` and ``weight``."""
+    dinput, dweight = torch.empty_like(dout), torch.empty_like(weight)
+    torch.ops.hp_rms_norm.rms_norm_backward.default(dinput, dweight, dout, input, weight, dresidual, eps)
+    return dinput, dweight
+
+
+def linear_cross_entropy_out(loss, lse, hidden, weight, target, ignore_index=-100):
+    """Softmax cross entropy of ``hidden`` rows under a vocabulary projection,
+    without keeping the logits ``z = hidden @ weight.T``: ``lse <-
+    logsumexp(z)`` and ``loss <- lse - z[target]`` per row.  ``hidden``: [..., H]
+    bf16 or fp16; ``weight``: [V, H] of the same dtype; ``target``: int64
+    [...]; ``loss`` and ``lse``: float32 like ``target``.  Products and sums
+    are fp32.  Rows whose target is ``ignore_index`` get 0 and 0 and are never
+    read (padding may hold anything); another target outside ``[0, V)`` gives
+    a NaN loss.  No reference counterpart."""
+    torch.ops.hp_rms_norm.linear_cross_entropy.default(loss, lse, hidden, weight, target, ignore_index)
+
+
+def linear_cross_entropy(hidden, weight, target, ignore_index=-100):
+    """Allocating form of ``linear_cross_entropy_out``: returns ``(loss,
+    lse)``, float32 per row; the backward call takes ``lse``."""
+    loss = torch.empty(target.shape, dtype=torch.float32, device=target.device)
+    lse = torch.empty_like(loss)
+    torch.ops.hp_rms_norm.linear_cross_entropy.default(loss, lse, hidden, weight, target, ignore_index)
+    return loss, lse
+
+
+def linear_cross_entropy_backward_out(dhidden, dweight, dloss, hidden, weight, target, lse, ignore_index=-100):
+    """Gradient of ``linear_cross_entropy`` into given tensors: with ``dz =
+    (exp(z - lse) - onehot(target)) * dloss``, ``dhidden <- dz @ weight`` and
+    ``dweight <- dz.T @ hidden``.  ``lse`` is the forward call's, ``dloss``
+    the gradient of each row's loss (float32 like ``target``; for a mean over
+    n rows, 1 / n each).  The logits are computed again, a piece of the
+    vocabulary at a time; ``dz`` is rounded to the tensors' dtype, sums are
+    fp32 and each output is rounded once.  Ignored rows get a zero
+    ``dhidden`` and no part in ``dweight``; an out-of-range target makes the
+    gradients NaN.  No reference counterpart."""
+    torch.ops.hp_rms_norm.linear_cross_entropy_backward.default(dhidden, dweight, dloss, hidden, weight, target, lse,
+                                                                ignore_index)
+
+
+def linear_cross_entropy_backward(dloss, hidden, weight, target, lse, ignore_index=-100):
+    """Allocating form of ``linear_cross_entropy_backward_out``: returns
+    ``(dhidden, dweight)``.  ``dloss`` may be any float32 tensor that expands
+    to ``target``'s shape (a scalar for a sum or mean of the losses)."""
+    dhidden, dweight = torch.empty_like(hidden), torch.empty_like(weight)
+    torch.ops.hp_rms_norm.linear_cross_entropy_backward.default(
+        dhidden, dweight, dloss.expand(target.shape).contiguous(), hidden, weight, target, lse, ignore_index)
+    return dhidden, dweight
+
+
+def grad_norm(grads):
+    """The 2-norm of all elements of ``grads`` (a sequence of bf16, fp16 or
+    fp32 tensors on one device, dense in memory in any dimension order) as a
+    float32 scalar on the device; squares are summed in fp64 in a fixed order.
+    An empty sequence raises RuntimeError: it names no device.  No reference
+    counterpart."""
+    grads = list(grads)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device if grads else None)
+    torch.ops.hp_rms_norm.grad_norm.default(norm, grads)
+    return norm
+
+
+def clip_grad_norm_(grads, max_norm):
+    """Scales ``grads`` in place by ``min(1, max_norm / (norm + 1e-6))`` with
+    ``norm = grad_norm(grads)`` (the rule of ``torch.nn.utils.
+    clip_grad_norm_``), and returns ``norm``.  Nothing waits for the device:
+    where the norm is below the limit the second pass ends at once.  No two
+    tensors may share memory.  No reference counterpart."""
+    grads = list(grads)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device if grads else None)
+    torch.ops.hp_rms_norm.clip_grad_norm_.default(norm, grads, max_norm)
+    return norm
+
+
+def clip_grad_norm_out(outs, grads, max_norm):
+    """``clip_grad_norm_`` into other tensors: ``outs[i] <- grads[i] *
+    factor``, each shaped and laid out like its gradient, of its dtype or
+    float32 (an optimizer's master gradients); ``outs[i]`` may be
+    ``grads[i]``.  Returns the norm."""
+    outs, grads = list(outs), list(grads)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device if grads else None)
+    torch.ops.hp_rms_norm.clip_grad_norm_out.default(norm, outs, grads, max_norm)
+    return norm
 
 
 def set_batch_invariant(enable):

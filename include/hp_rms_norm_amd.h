@@ -23,13 +23,14 @@
 extern "C" {
 #endif
 
-#define HPRMS_ABI_VERSION 8
+#define HPRMS_ABI_VERSION 9
 
 /* element types (the reference accepts exactly these two:
  * hp_rms_norm/csrc/cuda/hp_rms_norm.cu:29-49) */
 typedef enum {
   HPRMS_DTYPE_BF16 = 0,
-  HPRMS_DTYPE_FP16 = 1
+  HPRMS_DTYPE_FP16 = 1,
+  HPRMS_DTYPE_FP32 = 2  /* gradients only: dweight_dtype, and the dtypes of a list of gradients */
 } hprms_dtype;
 
 /* status codes */
@@ -369,6 +370,87 @@ int hprms_device_cu_count(int device);
  * configuration under it.  No counterpart in the reference. */
 int hprms_set_batch_invariant(int enable);
 int hprms_batch_invariant(void);
+
+/*
+ * Gradient of RMSNorm, plain or fused with the residual addition.  `input` is
+ * what was normalised (the fused op's updated residual), `dout` the gradient of
+ * the normalised output, `dresidual` (may be NULL) the gradient that reaches the
+ * updated residual by its other uses.  With r = 1 / sqrt(mean(input^2) + eps):
+ *   dinput[i, :] <- rne(r * (dout * weight) - input * (r^3 * mean(dout * weight * input)) + dresidual)
+ *   dweight[:]   <- sum over rows of dout * (input * r)
+ * in binary32, rounded once; dinput is the gradient of the fused op's input and
+ * of its residual alike.  `dinput` may be `dout`, `dresidual` or `input`
+ * exactly; dweight is of dweight_dtype (dtype or HPRMS_DTYPE_FP32) and is
+ * written, not added to (rows == 0 writes zeros).  The sums' order is fixed for
+ * given sizes and CU count.  `workspace`: hprms_rmsnorm_backward_workspace()
+ * bytes (a negative status for bad sizes) on the device, 16-byte aligned, free
+ * again when the call has run on `stream`; calls that may run at the same time
+ * need one each.  No counterpart in the reference, which has no gradients.
+ */
+int64_t hprms_rmsnorm_backward_workspace(int64_t rows, int64_t hidden);
+int hprms_rmsnorm_backward(void* dinput, void* dweight, const void* dout, const void* input, const void* weight,
+                           const void* dresidual, void* workspace, int64_t workspace_size, int64_t rows,
+                           int64_t hidden, int64_t dinput_row_stride, int64_t dout_row_stride,
+                           int64_t input_row_stride, int64_t dresidual_row_stride, int dtype, int dweight_dtype,
+                           double eps, hipStream_t stream);
+
+/*
+ * Softmax cross entropy of rows under a vocabulary projection, without keeping
+ * the logits z = hidden . weight^T:
+ *   lse[i] <- log(sum_v exp(z[i, v]));  loss[i] <- lse[i] - z[i, target[i]]
+ * hidden [rows, hidden_size] and weight [vocab, hidden_size] at row strides,
+ * target [rows].  Products and sums are binary32.  Rows whose target is
+ * ignore_index get loss 0 and lse 0 and are not read; any other target outside
+ * [0, vocab) gives a NaN loss.  The workspace is as for
+ * hprms_rmsnorm_backward(), 256-byte aligned, of
+ * hprms_linear_cross_entropy_workspace() bytes.  rows == 0 is a no-op.  No
+ * counterpart in the reference.
+ */
+int64_t hprms_linear_cross_entropy_workspace(int64_t rows, int64_t hidden, int64_t vocab);
+int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, const void* weight, const int64_t* target,
+                               void* workspace, int64_t workspace_size, int64_t rows, int64_t hidden_size,
+                               int64_t vocab, int64_t hidden_row_stride, int64_t weight_row_stride,
+                               int64_t ignore_index, int dtype, hipStream_t stream);
+
+/*
+ * Gradient of hprms_linear_cross_entropy(), from its lse and the gradient
+ * dloss[i] of each row's loss:
+ *   dz = (exp(z - lse) - [v == target]) * dloss;  dhidden <- dz . weight;  dweight <- dz^T . hidden
+ * The logits are computed again, a piece of the vocabulary at a time; dz is
+ * rounded to dtype (at a power-of-two scale that suits the largest dloss), the
+ * products are summed in binary32 and rounded once.  Ignored rows get a zero
+ * dhidden and no part in dweight, whatever their hidden values and dloss are; an
+ * out-of-range target gives NaN gradients.  Both outputs are written, not added
+ * to (rows == 0 zeroes dweight), and overlap none of the inputs.  Workspace:
+ * hprms_linear_cross_entropy_backward_workspace() bytes, 256-byte aligned.  No
+ * counterpart in the reference.
+ */
+int64_t hprms_linear_cross_entropy_backward_workspace(int64_t rows, int64_t hidden, int64_t vocab);
+int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const float* dloss, const void* hidden,
+                                        const void* weight, const int64_t* target, const float* lse, void* workspace,
+                                        int64_t workspace_size, int64_t rows, int64_t hidden_size, int64_t vocab,
+                                        int64_t dhidden_row_stride, int64_t dweight_row_stride,
+                                        int64_t hidden_row_stride, int64_t weight_row_stride, int64_t ignore_index,
+                                        int dtype, hipStream_t stream);
+
+/*
+ * Norm of a list of gradients: *norm <- sqrt(sum over all n tensors of g^2),
+ * with the squares summed in binary64 in a fixed order.  grads[i] holds
+ * counts[i] contiguous elements of dtypes[i] (any hprms_dtype); the arrays are
+ * host memory, read before the call returns.  Clipping also writes
+ *   outs[i] <- grads[i] * min(1, max_norm / (norm + 1e-6))
+ * with outs[i] of out_dtypes[i], the gradient's dtype or HPRMS_DTYPE_FP32;
+ * outs[i] may be grads[i], and outputs overlap nothing else.  A NaN norm gives
+ * NaN gradients.  Nothing is read back to the host.  Workspace:
+ * hprms_grad_norm_workspace() bytes, 16-byte aligned.  No counterpart in the
+ * reference.
+ */
+int64_t hprms_grad_norm_workspace(const int64_t* counts, int n);
+int hprms_grad_norm(float* norm, const void* const* grads, const int* dtypes, const int64_t* counts, int n,
+                    void* workspace, int64_t workspace_size, hipStream_t stream);
+int hprms_clip_grad_norm(float* norm, void* const* outs, const int* out_dtypes, const void* const* grads,
+                         const int* dtypes, const int64_t* counts, int n, double max_norm, void* workspace,
+                         int64_t workspace_size, hipStream_t stream);
 
 /* Lists the vector-tier configurations built into the library for (dtype,
  * mode, numbered as for hprms_select_config).  Writes up to `capacity`
