@@ -92,9 +92,9 @@ def _bind(L, bench):
     pvp, pi64, pci = ctypes.POINTER(vp), ctypes.POINTER(i64), ctypes.POINTER(ci)
     L.hprms_rmsnorm_backward_workspace.argtypes = [i64, i64]
     L.hprms_rmsnorm_backward.argtypes = [vp] * 7 + [i64] * 7 + [ci, ci, cd, vp]
-    L.hprms_linear_cross_entropy_workspace.argtypes = [i64, i64, i64]
+    L.hprms_linear_cross_entropy_workspace.argtypes = [i64, i64, i64, vp, i64]
     L.hprms_linear_cross_entropy.argtypes = [vp] * 6 + [i64] * 7 + [ci, vp]
-    L.hprms_linear_cross_entropy_backward_workspace.argtypes = [i64, i64, i64]
+    L.hprms_linear_cross_entropy_backward_workspace.argtypes = [i64, i64, i64, vp, i64]
     L.hprms_linear_cross_entropy_backward.argtypes = [vp] * 8 + [i64] * 9 + [ci, vp]
     L.hprms_grad_norm_workspace.argtypes = [pi64, ci]
     L.hprms_grad_norm.argtypes = [vp, pvp, pci, pi64, ci, vp, i64, vp]
@@ -250,8 +250,11 @@ class Library:
             rows, hidden, dinput_stride, dout_stride, input_stride, dresidual_stride, dtype, dweight_dtype, eps,
             stream))
 
-    def linear_cross_entropy_workspace(self, rows, hidden, vocab):
-        return self._bytes(self.lib().hprms_linear_cross_entropy_workspace(rows, hidden, vocab))
+    def linear_cross_entropy_workspace(self, rows, hidden, vocab, weight_ptr=0, weight_stride=None):
+        """For a weight at ``weight_ptr`` (default: any aligned address) with
+        ``weight_stride`` elements between rows (default: ``hidden``)."""
+        return self._bytes(self.lib().hprms_linear_cross_entropy_workspace(
+            rows, hidden, vocab, weight_ptr, hidden if weight_stride is None else weight_stride))
 
     def linear_cross_entropy(self, loss_ptr, lse_ptr, hidden_ptr, weight_ptr, target_ptr, workspace_ptr,
                              workspace_size, rows, hidden, vocab, hidden_stride, weight_stride, ignore_index, dtype,
@@ -260,8 +263,11 @@ class Library:
             loss_ptr, lse_ptr, hidden_ptr, weight_ptr, target_ptr, workspace_ptr, workspace_size, rows, hidden, vocab,
             hidden_stride, weight_stride, ignore_index, dtype, stream))
 
-    def linear_cross_entropy_backward_workspace(self, rows, hidden, vocab):
-        return self._bytes(self.lib().hprms_linear_cross_entropy_backward_workspace(rows, hidden, vocab))
+    def linear_cross_entropy_backward_workspace(self, rows, hidden, vocab, weight_ptr=0, weight_stride=None):
+        """For a weight at ``weight_ptr`` (default: any aligned address) with
+        ``weight_stride`` elements between rows (default: ``hidden``)."""
+        return self._bytes(self.lib().hprms_linear_cross_entropy_backward_workspace(
+            rows, hidden, vocab, weight_ptr, hidden if weight_stride is None else weight_stride))
 
     def linear_cross_entropy_backward(self, dhidden_ptr, dweight_ptr, dloss_ptr, hidden_ptr, weight_ptr, target_ptr,
                                       lse_ptr, workspace_ptr, workspace_size, rows, hidden, vocab, dhidden_stride,

@@ -30,30 +30,16 @@
 // B[8 (l / 16) + j][l % 16], j = 0 ... 7, and of the product the four rows
 // 4 (l / 16) + i of column l % 16.  The operand whose index should be
 // contiguous in what the epilogue writes or reduces is A: the vocabulary for z,
-// the hidden index for both gradients.
+// the hidden index for both gradients.  The tile loop: hprms_product.h.
 #pragma once
 
-#include "hprms_device.h"
+#include "hprms_product.h"
 
 namespace hprms {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-// 16 bytes at any 2-byte boundary
+// 8 and 16 bytes at any 2-byte boundary
 typedef u32x4 u32x4_u __attribute__((aligned(2)));
 typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(2)));
-
-template <int DT>
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-  if constexpr (DT == HPRMS_DTYPE_BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                   0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
-                                                  0);
-}
 
 // What the row list says, written by loss_rows_kernel.
 struct LossMeta {
@@ -63,35 +49,42 @@ struct LossMeta {
   int32_t pad;
 };
 
-// The arguments of every loss kernel.
+// The arguments of every loss kernel.  Listed rows are numbered by their
+// position in the list ("list position").
 struct LossArgs {
   const uint16_t* hidden;
-  const uint16_t* weight;
+  const uint16_t* weight;   // the piece's first row (the caller's, or packed)
   const int64_t* target;
   const LossMeta* meta;
-  const int32_t* index;     // listed rows
-  int64_t hidden_stride, weight_stride;
+  const int32_t* index;     // the row of each list position
+  const uint16_t* packed;   // the listed rows' hidden values, [rows, packed_width], zeros past width
+  int64_t hidden_stride;
   int64_t ignore_index;
+  int32_t weight_stride;    // elements, a multiple of 8
+  int32_t weight_width;     // readable elements of a weight row, a multiple of 8
+  int32_t packed_width;     // a multiple of 64
   int32_t rows;             // of the call
   int32_t width;            // elements of a hidden row
   int32_t vocab;
+  int32_t piece_from, piece;  // vocabulary rows of this launch
+  int32_t vocab_tiles, width_tiles;  // tiles of this launch
   // forward
   float* loss;
-  float* lse;               // backward: read
+  float* lse;               // gradient: read
   float* target_logit;      // [rows], by list position
   float2* partial;          // [vocabulary tiles, rows_at]: maximum and sum of exponentials
   int32_t row_from, rows_at;  // list positions of this launch: [row_from, row_from + rows_at)
-  // backward
+  int32_t tile_from;        // vocabulary tiles before this piece
+  // gradient
+  int32_t dz_stride;
   const float* dloss;
   uint16_t* dz;             // [rows rounded up, dz_stride], by list position
-  int64_t dz_stride;
-  int32_t piece_from, piece;  // vocabulary rows of this piece
   uint16_t* dhidden;
   int64_t dhidden_stride;
   uint16_t* dweight;
   int64_t dweight_stride;
-  float* sum;               // [rows, width] shares of dhidden, by list position
-  int32_t first_piece, last_piece;
+  float* sum;               // [splits, rows, packed_width] shares of dhidden, by list position; null: none
+  int32_t first_piece, splits;
 };
 
 // ---- epilogues ------------------------------------------------------------------------
@@ -120,15 +113,15 @@ __device__ __forceinline__ void forward_epilogue(const LossArgs& a, const f32x4 
     const int col = wn * NI * 16 + ni * 16 + (lane & 15);
     const int n = n0 + col;
     const bool live = n < count;
-    const int64_t t = live ? a.target[a.index[n]] : -1;
+    const int64_t t = live ? a.target[a.index[n]] - a.piece_from : -1;  // in the piece
     float top = -__builtin_inff();
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int v = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4 + i;
-        if (v < a.vocab) top = fmaxf(top, acc[mi][ni][i]);
-        if (live && v == t && v < a.vocab) a.target_logit[n] = acc[mi][ni][i];
+        const int v = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4 + i;  // in the piece
+        if (v < a.piece) top = fmaxf(top, acc[mi][ni][i]);
+        if (v == t && v < a.piece) a.target_logit[n] = acc[mi][ni][i];
       }
     top = fmaxf(top, xor16(top));
     top = fmaxf(top, xor32(top));
@@ -139,7 +132,7 @@ __device__ __forceinline__ void forward_epilogue(const LossArgs& a, const f32x4 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int v = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4 + i;
-        if (v < a.vocab) sum += exp_neg(acc[mi][ni][i] - at);
+        if (v < a.piece) sum += exp_neg(acc[mi][ni][i] - at);
       }
     sum += xor16(sum);
     sum += xor32(sum);
@@ -215,8 +208,9 @@ __device__ __forceinline__ void dweight_epilogue(const LossArgs& a, const f32x4 
   const float unscale = a.meta->unscale;
 #pragma unroll
   for (int ni = 0; ni < NI; ++ni) {
-    const int64_t v = (int64_t)a.piece_from + n0 + (wn * NI + ni) * 16 + (lane & 15);
-    if (v >= a.vocab) continue;
+    const int v_in = n0 + (wn * NI + ni) * 16 + (lane & 15);
+    if (v_in >= a.piece) continue;
+    const int64_t v = (int64_t)a.piece_from + v_in;
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
       const int m = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4;
@@ -228,120 +222,52 @@ __device__ __forceinline__ void dweight_epilogue(const LossArgs& a, const f32x4 
   }
 }
 
-// A piece's share of dhidden: A is the hidden index, the column the list position.
+// A piece's share of dhidden, or all of it: A is the hidden index, the column
+// the list position.  With more than one share (pieces, or splits of a piece's
+// vocabulary over workgroups) each goes to binary32 sums, which
+// loss_dhidden_kernel adds up; a share's first piece sets its sum.
 template <int DT, int MI, int NI>
 __device__ __forceinline__ void dhidden_epilogue(const LossArgs& a, const f32x4 (&acc)[MI][NI], int m0, int n0, int wm,
-                                                 int wn, int count) {
+                                                 int wn, int count, int split) {
   const int lane = threadIdx.x & 63;
   const float unscale = a.meta->unscale;
 #pragma unroll
   for (int ni = 0; ni < NI; ++ni) {
     const int n = n0 + (wn * NI + ni) * 16 + (lane & 15);
     if (n >= count) continue;
-    const int64_t row = a.index[n];
+    const int64_t row = a.sum ? 0 : a.index[n];
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
       const int m = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4;
-      const int left = a.width - m;
-      if (left <= 0) continue;
-      float* s = a.sum + (int64_t)n * a.width + m;
-      float d[4];
+      if (a.sum) {
+        if (m >= a.packed_width) continue;
+        f32x4* s = (f32x4*)(a.sum + ((int64_t)split * a.rows + n) * a.packed_width + m);
+        *s = a.first_piece ? acc[mi][ni] : acc[mi][ni] + *s;
+      } else if (m < a.width) {
+        float d[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        d[i] = acc[mi][ni][i];
-        if (!a.first_piece && i < left) d[i] += s[i];
-      }
-      if (a.last_piece) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] *= unscale;
-        store_four<DT>(a.dhidden + row * a.dhidden_stride + m, d, left);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < left) s[i] = d[i];
+        for (int i = 0; i < 4; ++i) d[i] = acc[mi][ni][i] * unscale;
+        store_four<DT>(a.dhidden + row * a.dhidden_stride + m, d, a.width - m);
       }
     }
   }
 }
 
-// ---- operands of the general tile loop ---------------------------------------------------
-// Operand rows r (in [0, rows)) over the summed index k (in [0, depth)).
-// KMAJOR false: k contiguous, element (r, k) at base + row(r) * stride + k.
-// KMAJOR true: r contiguous, element (r, k) at base + row(k) * stride + r.
-// row(i) = list ? list[i] : i.
-struct Operand {
-  const uint16_t* base;
-  int64_t stride;
-  const int32_t* list;
-  int32_t rows, depth;
-  __device__ __forceinline__ const uint16_t* at(int32_t i) const {
-    return base + (int64_t)(list ? list[i] : i) * stride;
-  }
-};
-
-constexpr int kTile = 128;      // rows and columns of a workgroup's tile
-constexpr int kDepth = 32;      // summed entries per step
-constexpr int kLdsRow = 40;     // elements between LDS rows (80 bytes: 16-byte aligned, off the bank period)
-
-// 8 elements p[0 ... 7] of which the first n exist
-__device__ __forceinline__ u32x4 load_some(const uint16_t* p, int n) {
-  if (n >= 8) return *(const u32x4_u*)p;
-  u32x4 v = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < n) v[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
-  return v;
-}
-
-// Rows r0 ... r0 + 127 of an operand, entries k0 ... k0 + 31, to LDS as [row][k].
-template <bool KMAJOR>
-__device__ __forceinline__ void stage(const Operand& o, int r0, int k0, uint16_t* lds) {
-#pragma unroll
-  for (int it = 0; it < 2; ++it) {
-    const int c = threadIdx.x + it * 256;
-    if constexpr (!KMAJOR) {
-      const int r = c >> 2, k = (c & 3) * 8;
-      u32x4 v = {0, 0, 0, 0};
-      if (r0 + r < o.rows && k0 + k < o.depth) v = load_some(o.at(r0 + r) + k0 + k, o.depth - k0 - k);
-      *(u32x4*)(lds + r * kLdsRow + k) = v;
-    } else {
-      const int k = c >> 4, r = (c & 15) * 8;
-      u32x4 v = {0, 0, 0, 0};
-      if (k0 + k < o.depth && r0 + r < o.rows) v = load_some(o.at(k0 + k) + r0 + r, o.rows - r0 - r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) lds[(r + j) * kLdsRow + k] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
-    }
-  }
-}
-
-// 128 x 128 tile by 4 waves of 64 x 64: any sizes, strides and alignment.
-template <int DT, bool AK, bool BK>
-__device__ __forceinline__ void general_tile(const Operand& oa, const Operand& ob, int m0, int n0, uint16_t* lds,
-                                             f32x4 (&acc)[4][4]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = wave >> 1, wn = wave & 1;
-  uint16_t* la = lds;
-  uint16_t* lb = lds + kTile * kLdsRow;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  for (int k0 = 0; k0 < oa.depth; k0 += kDepth) {
-    __syncthreads();
-    stage<AK>(oa, m0, k0, la);
-    stage<BK>(ob, n0, k0, lb);
-    __syncthreads();
-    u32x4 fa[4], fb[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      fa[i] = *(const u32x4*)(la + (wm * 64 + i * 16 + (lane & 15)) * kLdsRow + (lane >> 4) * 8);
-      fb[i] = *(const u32x4*)(lb + (wn * 64 + i * 16 + (lane & 15)) * kLdsRow + (lane >> 4) * 8);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mfma16<DT>(fa[i], fb[j], acc[i][j]);
-  }
+// ---- tiles of a launch ------------------------------------------------------------------
+// Tile (m, n) of workgroup b, false past the last one.  The hardware hands
+// consecutive workgroups to the 8 XCDs in turn, so XCD k takes one contiguous
+// run of tiles; in a run, `group` column tiles times some row tiles make the
+// block of tiles that an XCD's 32 CUs work on at a time, which share their
+// operands' slices in that XCD's L2.
+__device__ __forceinline__ bool tile_of(int b, int mt, int nt, int group, int* m, int* n) {
+  const int total = mt * nt, per = (total + 7) / 8;
+  const int t = (b & 7) * per + (b >> 3);
+  if ((b >> 3) >= per || t >= total) return false;
+  const int g = t / (group * mt), r = t % (group * mt);
+  const int w = nt - g * group < group ? nt - g * group : group;
+  *m = r / w;
+  *n = g * group + r % w;
+  return true;
 }
 
 }  // namespace hprms

@@ -10,10 +10,11 @@ namespace {
 
 // ---- the list of rows that carry a loss -----------------------------------------------
 // One workgroup: `index` gets the rows whose target is not ignore_index, in
-// order; with GRAD also the scale of dloss, from the largest of its finite
+// order, and `position` each row's place among them (-1: none); with GRAD also the scale of dloss, from the largest of its finite
 // magnitudes.  Without GRAD the other rows' loss and lse are set to 0.
 template <bool GRAD>
-__global__ __launch_bounds__(1024) void loss_rows_kernel(LossArgs a, LossMeta* meta, int32_t* index) {
+__global__ __launch_bounds__(1024) void loss_rows_kernel(LossArgs a, LossMeta* meta, int32_t* index,
+                                                         int32_t* position) {
   __shared__ int32_t waves[16];
   __shared__ float tops[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -31,7 +32,9 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(LossArgs a, LossMeta* m
       if (i < wave) before += waves[i];
       count += waves[i];
     }
-    if (keep) index[before + __popcll(mask & ((uint64_t(1) << lane) - 1))] = row;
+    const int32_t at = before + __popcll(mask & ((uint64_t(1) << lane) - 1));
+    if (keep) index[at] = row;
+    if (in) position[row] = keep ? at : -1;
     if constexpr (GRAD) {
       if (keep) {
         const float g = fabsf(a.dloss[row]);
@@ -60,19 +63,92 @@ __global__ __launch_bounds__(1024) void loss_rows_kernel(LossArgs a, LossMeta* m
   if (threadIdx.x == 0) *meta = LossMeta{count, scale, 1.0f / scale, 0};
 }
 
+// The listed rows' hidden values side by side, zero up to packed_width: one
+// operand layout for any width, stride and alignment, and no ignored rows in
+// the products.  With GRAD the other rows' dhidden is set to 0.
+template <bool GRAD>
+__global__ __launch_bounds__(256) void loss_pack_kernel(LossArgs a, const int32_t* position, uint16_t* packed) {
+  for (int32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int32_t at = position[row];
+    if (at < 0) {
+      if constexpr (GRAD)
+        for (int32_t i = threadIdx.x; i < a.width; i += 256) a.dhidden[(int64_t)row * a.dhidden_stride + i] = 0;
+      continue;
+    }
+    const uint16_t* from = a.hidden + (int64_t)row * a.hidden_stride;
+    uint16_t* to = packed + (int64_t)at * a.packed_width;
+    for (int32_t i = threadIdx.x * 8; i < a.packed_width; i += 256 * 8) {
+      u32x4 v = {0, 0, 0, 0};
+      if (i + 8 <= a.width) {
+        v = *(const u32x4_u*)(from + i);
+      } else {
+        for (int j = 0; j < 8; ++j)
+          if (i + j < a.width) v[j / 2] |= (uint32_t)from[i + j] << (16 * (j & 1));
+      }
+      *(u32x4*)(to + i) = v;
+    }
+  }
+}
+
+// The same for a piece of a weight whose rows the products cannot read in
+// place (an odd width, stride or alignment).
+__global__ __launch_bounds__(256) void loss_pack_weight_kernel(const uint16_t* weight, int64_t stride, int32_t rows,
+                                                               int32_t width, int32_t packed_width,
+                                                               uint16_t* packed) {
+  for (int32_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const uint16_t* from = weight + (int64_t)row * stride;
+    uint16_t* to = packed + (int64_t)row * packed_width;
+    for (int32_t i = threadIdx.x * 8; i < packed_width; i += 256 * 8) {
+      u32x4 v = {0, 0, 0, 0};
+      if (i + 8 <= width) {
+        v = *(const u32x4_u*)(from + i);
+      } else {
+        for (int j = 0; j < 8; ++j)
+          if (i + j < width) v[j / 2] |= (uint32_t)from[i + j] << (16 * (j & 1));
+      }
+      *(u32x4*)(to + i) = v;
+    }
+  }
+}
+
+// ---- operands -----------------------------------------------------------------------------
+// the piece's weight rows from row m on: k contiguous (z) ...
+__device__ __forceinline__ Operand weight_rows(const LossArgs& a, int m) {
+  return {a.weight + (int64_t)m * a.weight_stride,
+          ((int64_t)(a.piece - 1 - m) * a.weight_stride + a.weight_width) * 2, a.weight_stride};
+}
+// ... or as the summed index, from entry k on, hidden elements from m on
+__device__ __forceinline__ Operand weight_columns(const LossArgs& a, int k, int m) {
+  return {a.weight + (int64_t)k * a.weight_stride + m,
+          ((int64_t)(a.piece - 1 - k) * a.weight_stride + a.weight_width - m) * 2, a.weight_stride};
+}
+__device__ __forceinline__ Operand packed_rows(const LossArgs& a, int n, int count) {
+  return {a.packed + (int64_t)n * a.packed_width, (int64_t)(count - n) * a.packed_width * 2, a.packed_width};
+}
+__device__ __forceinline__ Operand packed_columns(const LossArgs& a, int m, int count) {
+  return {a.packed + m, ((int64_t)count * a.packed_width - m) * 2, a.packed_width};
+}
+__device__ __forceinline__ Operand dz_rows(const LossArgs& a, int n, int v, int count) {
+  return {a.dz + (int64_t)n * a.dz_stride + v, ((int64_t)(count - n) * a.dz_stride - v) * 2, a.dz_stride};
+}
+__device__ __forceinline__ Operand dz_columns(const LossArgs& a, int v, int count) {
+  return {a.dz + v, ((int64_t)count * a.dz_stride - v) * 2, a.dz_stride};
+}
+
 // ---- forward ----------------------------------------------------------------------------
-template <int DT>
-__global__ __launch_bounds__(256) void loss_forward_general_kernel(LossArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kTile * kLdsRow];
+template <class P, int DT>
+__global__ __launch_bounds__(P::NW * 64) void loss_forward_kernel(LossArgs a, int group) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[P::LDS_BYTES / 2];
   const int count = a.meta->count;
-  const int n0 = a.row_from + blockIdx.y * kTile, m0 = blockIdx.x * kTile;
-  if (n0 >= count) return;
-  f32x4 acc[4][4];
-  const Operand oa{a.weight, a.weight_stride, nullptr, a.vocab, a.width};
-  const Operand ob{a.hidden, a.hidden_stride, a.index, count, a.width};
-  general_tile<DT, false, false>(oa, ob, m0, n0, lds, acc);
+  const int here = min(count - a.row_from, a.rows_at);
+  int m, n;
+  if (here <= 0 || !tile_of(blockIdx.x, a.vocab_tiles, (here + P::NT - 1) / P::NT, group, &m, &n)) return;
+  const int m0 = m * P::MT, n0 = a.row_from + n * P::NT;
+  f32x4 acc[P::MI][P::NI];
+  P::run(weight_rows(a, m0), packed_rows(a, n0, count), a.width, lds, acc);
   const int wave = threadIdx.x >> 6;
-  forward_epilogue<4, 4, 2, 2>(a, acc, m0, n0, wave >> 1, wave & 1, count, blockIdx.x, (float2*)lds);
+  forward_epilogue<P::MI, P::NI, P::WM, P::WN>(a, acc, m0, n0, wave / P::WN, wave % P::WN,
+                                               min(count, a.row_from + a.rows_at), a.tile_from + m, (float2*)lds);
 }
 
 // Joins the tiles of RPB rows: 256 / RPB lanes per row, each over tiles in order.
@@ -109,115 +185,166 @@ __global__ __launch_bounds__(256) void loss_join_kernel(LossArgs a, int32_t tile
 }
 
 // ---- gradient ---------------------------------------------------------------------------
-template <int DT>
-__global__ __launch_bounds__(256) void loss_dz_general_kernel(LossArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kTile * kLdsRow];
+template <class P, int DT>
+__global__ __launch_bounds__(P::NW * 64) void loss_dz_kernel(LossArgs a, int group) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[P::LDS_BYTES / 2];
   const int count = a.meta->count;
-  const int n0 = blockIdx.y * kTile, m0 = blockIdx.x * kTile;
-  if (n0 >= count) return;
-  f32x4 acc[4][4];
-  const Operand oa{a.weight + (int64_t)a.piece_from * a.weight_stride, a.weight_stride, nullptr,
-                   a.vocab - a.piece_from, a.width};
-  const Operand ob{a.hidden, a.hidden_stride, a.index, count, a.width};
-  general_tile<DT, false, false>(oa, ob, m0, n0, lds, acc);
+  int m, n;
+  if (!tile_of(blockIdx.x, a.vocab_tiles, (count + P::NT - 1) / P::NT, group, &m, &n)) return;
+  const int m0 = m * P::MT, n0 = n * P::NT;
+  f32x4 acc[P::MI][P::NI];
+  P::run(weight_rows(a, m0), packed_rows(a, n0, count), a.width, lds, acc);
   const int wave = threadIdx.x >> 6;
-  dz_epilogue<DT, 4, 4>(a, acc, m0, n0, wave >> 1, wave & 1, count);
+  dz_epilogue<DT, P::MI, P::NI>(a, acc, m0, n0, wave / P::WN, wave % P::WN, count);
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void loss_dweight_general_kernel(LossArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kTile * kLdsRow];
+template <class P, int DT>
+__global__ __launch_bounds__(P::NW * 64) void loss_dweight_kernel(LossArgs a, int group) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[P::LDS_BYTES / 2];
   const int count = a.meta->count;
-  const int m0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile;
-  f32x4 acc[4][4];
-  const Operand oa{a.hidden, a.hidden_stride, a.index, a.width, count};
-  const Operand ob{a.dz, a.dz_stride, nullptr, a.piece, count};
-  general_tile<DT, true, true>(oa, ob, m0, n0, lds, acc);
+  int m, n;
+  if (!tile_of(blockIdx.x, a.width_tiles, a.vocab_tiles, group, &m, &n)) return;
+  const int m0 = m * P::MT, n0 = n * P::NT;
+  f32x4 acc[P::MI][P::NI];
+  P::run(packed_columns(a, m0, count), dz_columns(a, n0, count), count, lds, acc);
   const int wave = threadIdx.x >> 6;
-  dweight_epilogue<DT, 4, 4>(a, acc, m0, n0, wave >> 1, wave & 1);
+  dweight_epilogue<DT, P::MI, P::NI>(a, acc, m0, n0, wave / P::WN, wave % P::WN);
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void loss_dhidden_general_kernel(LossArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kTile * kLdsRow];
+// blockIdx.y: the split of the piece's vocabulary, `span` entries each
+template <class P, int DT>
+__global__ __launch_bounds__(P::NW * 64) void loss_dhidden_product_kernel(LossArgs a, int group, int span) {
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[P::LDS_BYTES / 2];
   const int count = a.meta->count;
-  const int m0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile;
-  if (n0 >= count) return;
-  f32x4 acc[4][4];
-  const Operand oa{a.weight + (int64_t)a.piece_from * a.weight_stride, a.weight_stride, nullptr, a.width, a.piece};
-  const Operand ob{a.dz, a.dz_stride, nullptr, count, a.piece};
-  general_tile<DT, true, false>(oa, ob, m0, n0, lds, acc);
+  int m, n;
+  if (!tile_of(blockIdx.x, a.width_tiles, (count + P::NT - 1) / P::NT, group, &m, &n)) return;
+  const int m0 = m * P::MT, n0 = n * P::NT;
+  const int from = blockIdx.y * span;
+  // dz holds zeros past the piece up to a tile's end, so the depth may be rounded up to whole chunks
+  const int depth = max(0, min(span, (a.piece - from + 7) & ~7));
+  f32x4 acc[P::MI][P::NI];
+  P::run(weight_columns(a, from, m0), dz_rows(a, n0, from, count), depth, lds, acc);
   const int wave = threadIdx.x >> 6;
-  dhidden_epilogue<DT, 4, 4>(a, acc, m0, n0, wave >> 1, wave & 1, count);
+  dhidden_epilogue<DT, P::MI, P::NI>(a, acc, m0, n0, wave / P::WN, wave % P::WN, count, blockIdx.y);
 }
 
-// dhidden of the rows that carry no loss
-__global__ __launch_bounds__(256) void loss_zero_rows_kernel(LossArgs a) {
-  for (int32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    if (a.target[row] != a.ignore_index) continue;
-    for (int32_t i = threadIdx.x; i < a.width; i += 256) a.dhidden[(int64_t)row * a.dhidden_stride + i] = 0;
+// dhidden from its shares
+template <int DT>
+__global__ __launch_bounds__(256) void loss_dhidden_kernel(LossArgs a) {
+  const int count = a.meta->count;
+  const float unscale = a.meta->unscale;
+  for (int32_t n = blockIdx.x; n < count; n += gridDim.x) {
+    uint16_t* to = a.dhidden + (int64_t)a.index[n] * a.dhidden_stride;
+    for (int32_t i = threadIdx.x * 4; i < a.width; i += 256 * 4) {
+      f32x4 d = {0, 0, 0, 0};
+      for (int s = 0; s < a.splits; ++s) d += *(const f32x4*)(a.sum + ((int64_t)s * a.rows + n) * a.packed_width + i);
+      const float o[4] = {d[0] * unscale, d[1] * unscale, d[2] * unscale, d[3] * unscale};
+      store_four<DT>(to + i, o, a.width - i);
+    }
   }
 }
 
 // ---- host ---------------------------------------------------------------------------------
 constexpr int64_t kMaxLossRows = int64_t(1) << 22;
-constexpr int64_t kMaxLossWidth = int64_t(1) << 24;
+constexpr int64_t kMaxLossWidth = int64_t(1) << 20;
 constexpr int64_t kMaxVocab = int64_t(1) << 28;
 constexpr int64_t kRowChunk = 16384;  // list positions per forward launch: bounds the partial sums
-constexpr int64_t kPieceElements = int64_t(1) << 27;  // of dz per piece: 256 MiB
-constexpr int64_t kMinPiece = 1024;
+constexpr int64_t kPieceElements = int64_t(1) << 27;  // of dz, and of a packed weight, per piece: 256 MiB
+constexpr int64_t kPieceUnit = 256;   // pieces are whole tiles of every kernel
+// a tile's 256 rows at this stride stay within a buffer access's 31-bit offset
+constexpr int64_t kMaxWeightStride = int64_t(1) << 21;
 
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+int64_t ceil_div(int64_t v, int64_t m) { return (v + m - 1) / m; }
 int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
+int64_t max64(int64_t a, int64_t b) { return a > b ? a : b; }
+bool aligned_to(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 int check_sizes(int64_t rows, int64_t width, int64_t vocab) {
   if (rows < 0) return fail(HPRMS_E_INVALID, "rows must be >= 0 (got %lld)", (long long)rows);
   if (width < 1) return fail(HPRMS_E_INVALID, "hidden must be >= 1 (got %lld)", (long long)width);
   if (vocab < 1) return fail(HPRMS_E_INVALID, "vocab must be >= 1 (got %lld)", (long long)vocab);
   if (rows > kMaxLossRows || width > kMaxLossWidth || vocab > kMaxVocab)
-    return fail(HPRMS_E_RANGE, "rows, hidden and vocab must be at most 2^22, 2^24 and 2^28 (got %lld, %lld, %lld)",
+    return fail(HPRMS_E_RANGE, "rows, hidden and vocab must be at most 2^22, 2^20 and 2^28 (got %lld, %lld, %lld)",
                 (long long)rows, (long long)width, (long long)vocab);
   return HPRMS_OK;
 }
 
+// The products read the weight's rows in place where 16-byte loads at 16-byte
+// boundaries cover them; otherwise a piece at a time is packed first.
+bool weight_in_place(const void* weight, int64_t stride, int64_t width) {
+  return aligned_to(weight, 16) && stride % 8 == 0 && width % 8 == 0 && stride <= kMaxWeightStride;
+}
+
+int64_t packed_width_of(int64_t width) { return round_up(width, 64); }
+
+// vocabulary rows of a packed piece
+int64_t packed_piece(int64_t width, int64_t vocab) {
+  const int64_t p = max64(kPieceElements / packed_width_of(width) / kPieceUnit * kPieceUnit, kPieceUnit);
+  return min64(p, round_up(vocab, kPieceUnit));
+}
+
+// Tiles of z by the number of rows: vocabulary rows and list positions.
+enum LogitTile { kTile16, kTile64, kTile128, kTile256 };
+LogitTile logit_tile(int64_t rows) {
+  return rows <= 16 ? kTile16 : rows <= 64 ? kTile64 : rows <= 128 ? kTile128 : kTile256;
+}
+int64_t logit_vocab_rows(LogitTile t) { return t <= kTile64 ? 128 : 256; }
+int64_t logit_rows(LogitTile t) { return t == kTile16 ? 16 : t == kTile64 ? 64 : t == kTile128 ? 128 : 256; }
+
 // Offsets of the workspace's parts, bytes.
 struct ForwardPlan {
-  int64_t index, target_logit, partial, total;
-  int64_t rows_at, tiles;
+  int64_t index, position, target_logit, packed, weight, partial, total;
+  int64_t rows_at, tiles, piece;
+  LogitTile tile;
 };
 
-ForwardPlan forward_plan(int64_t rows, int64_t vocab) {
+ForwardPlan forward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_place) {
   ForwardPlan p;
+  p.tile = logit_tile(rows);
   p.rows_at = min64(rows, kRowChunk);
-  p.tiles = (vocab + kTile - 1) / kTile;
+  p.piece = in_place ? round_up(vocab, kPieceUnit) : packed_piece(width, vocab);
+  p.tiles = ceil_div(vocab, logit_vocab_rows(p.tile));
   p.index = 256;
-  p.target_logit = p.index + round_up(rows * 4, 256);
-  p.partial = p.target_logit + round_up(rows * 4, 256);
+  p.position = p.index + round_up(rows * 4, 256);
+  p.target_logit = p.position + round_up(rows * 4, 256);
+  p.packed = p.target_logit + round_up(rows * 4, 256);
+  p.weight = p.packed + rows * packed_width_of(width) * 2;
+  p.partial = p.weight + (in_place ? 0 : p.piece * packed_width_of(width) * 2);
   p.total = p.partial + p.tiles * p.rows_at * 8;
   return p;
 }
 
 struct BackwardPlan {
-  int64_t index, dz, sum, total;
-  int64_t piece, pieces, dz_rows;
+  int64_t index, position, packed, weight, dz, sum, total;
+  int64_t piece, pieces, dz_rows, splits, span;
+  LogitTile tile;
 };
 
-BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab) {
+BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_place) {
   BackwardPlan p;
-  p.dz_rows = round_up(rows, kTile);
-  const int64_t whole = round_up(vocab, kTile);
-  p.piece = kPieceElements / (p.dz_rows > 0 ? p.dz_rows : kTile) / kTile * kTile;
-  if (p.piece < kMinPiece) p.piece = kMinPiece;
-  if (p.piece > whole) p.piece = whole;
-  p.pieces = (vocab + p.piece - 1) / p.piece;
+  p.tile = logit_tile(rows);
+  p.dz_rows = round_up(max64(rows, 1), logit_rows(p.tile));
+  p.piece = max64(kPieceElements / max64(p.dz_rows, 256) / kPieceUnit * kPieceUnit, 4 * kPieceUnit);
+  p.piece = min64(p.piece, round_up(vocab, kPieceUnit));
+  if (!in_place) p.piece = min64(p.piece, packed_piece(width, vocab));
+  p.pieces = ceil_div(vocab, p.piece);
+  // splits of a piece's vocabulary where dhidden has fewer tiles than the GPU
+  // CUs, of at least 512 entries
+  const int64_t tiles = ceil_div(width, p.tile <= kTile64 ? 128 : 256) * ceil_div(max64(rows, 1), logit_rows(p.tile));
+  const int64_t slots = (int64_t)current_cus() * (p.tile <= kTile64 ? 2 : 1);
+  p.splits = max64(1, min64(slots / tiles, p.piece / 512));
+  p.span = round_up(ceil_div(p.piece, p.splits), 64);
+  p.splits = ceil_div(p.piece, p.span);
   p.index = 256;
-  p.dz = p.index + round_up(rows * 4, 256);
+  p.position = p.index + round_up(rows * 4, 256);
+  p.packed = p.position + round_up(rows * 4, 256);
+  p.weight = p.packed + rows * packed_width_of(width) * 2;
+  p.dz = p.weight + (in_place ? 0 : p.piece * packed_width_of(width) * 2);
   p.sum = p.dz + p.dz_rows * p.piece * 2;
-  p.total = p.sum + (p.pieces > 1 ? rows * width * 4 : 0);
+  p.total = p.sum + (p.pieces * p.splits > 1 ? p.splits * rows * packed_width_of(width) * 4 : 0);
   return p;
 }
-
-bool aligned_to(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 int check_common(const void* hidden, const void* weight, const int64_t* target, int64_t rows, int64_t width,
                  int64_t vocab, int64_t hidden_stride, int64_t weight_stride, int dtype) {
@@ -242,15 +369,69 @@ int check_workspace(const void* workspace, int64_t size, int64_t need) {
   return HPRMS_OK;
 }
 
+template <int DT, bool AKO, bool BKO>
+struct Tiles {
+  typedef Product<DT, 128, 16, 4, 1, 64, 4, AKO, BKO> T16;
+  typedef Product<DT, 128, 64, 4, 1, 64, 3, AKO, BKO> T64;
+  typedef Product<DT, 256, 128, 4, 2, 32, 3, AKO, BKO> T128;
+  typedef Product<DT, 256, 256, 2, 4, 64, 2, AKO, BKO> T256;
+};
+
+// workgroups of `tiles` tiles, for tile_of
+unsigned grid_of(int64_t tiles) { return (unsigned)round_up(tiles, 8); }
+
+template <class P, int DT>
+void launch_forward(LossArgs a, int64_t here, hipStream_t stream) {
+  a.vocab_tiles = (int32_t)ceil_div(a.piece, P::MT);
+  const int64_t tiles = a.vocab_tiles * ceil_div(here, P::NT);
+  loss_forward_kernel<P, DT><<<dim3(grid_of(tiles)), dim3(P::NW * 64), 0, stream>>>(a, 4);
+}
+
+// what a call's pieces of the vocabulary share: the piece's rows, packed if need be
+struct Weight {
+  const uint16_t* base;
+  int64_t stride;
+  uint16_t* packed;  // null: in place
+};
+
+void take_piece(LossArgs& a, const Weight& w, int64_t from, int64_t piece, hipStream_t stream) {
+  a.piece_from = (int32_t)from;
+  a.piece = (int32_t)min64(piece, a.vocab - from);
+  const uint16_t* rows = w.base + from * w.stride;
+  if (!w.packed) {
+    a.weight = rows;
+    a.weight_stride = (int32_t)w.stride;
+    a.weight_width = a.width;
+    return;
+  }
+  loss_pack_weight_kernel<<<dim3((unsigned)min64(a.piece, 8192)), dim3(256), 0, stream>>>(
+      rows, w.stride, a.piece, a.width, a.packed_width, w.packed);
+  a.weight = w.packed;
+  a.weight_stride = a.packed_width;
+  a.weight_width = a.packed_width;
+}
+
 template <int DT>
-int run_forward(LossArgs a, const ForwardPlan& p, LossMeta* meta, int32_t* index, hipStream_t stream) {
-  loss_rows_kernel<false><<<dim3(1), dim3(1024), 0, stream>>>(a, meta, index);
+int run_forward(LossArgs a, const ForwardPlan& p, const Weight& w, char* ws, hipStream_t stream) {
+  typedef Tiles<DT, false, false> T;
+  loss_rows_kernel<false><<<dim3(1), dim3(1024), 0, stream>>>(a, (LossMeta*)ws, (int32_t*)(ws + p.index),
+                                                              (int32_t*)(ws + p.position));
+  loss_pack_kernel<false><<<dim3((unsigned)min64(a.rows, 8192)), dim3(256), 0, stream>>>(
+      a, (const int32_t*)(ws + p.position), (uint16_t*)(ws + p.packed));
   for (int64_t from = 0; from < a.rows; from += p.rows_at) {
     a.row_from = (int32_t)from;
-    a.rows_at = (int32_t)p.rows_at;
     const int64_t here = min64(p.rows_at, a.rows - from);
-    loss_forward_general_kernel<DT><<<dim3((unsigned)p.tiles, (unsigned)((here + kTile - 1) / kTile)), dim3(256), 0,
-                                      stream>>>(a);
+    a.tile_from = 0;
+    for (int64_t v = 0; v < a.vocab; v += p.piece) {
+      take_piece(a, w, v, p.piece, stream);
+      switch (p.tile) {
+        case kTile16: launch_forward<typename T::T16, DT>(a, here, stream); break;
+        case kTile64: launch_forward<typename T::T64, DT>(a, here, stream); break;
+        case kTile128: launch_forward<typename T::T128, DT>(a, here, stream); break;
+        case kTile256: launch_forward<typename T::T256, DT>(a, here, stream); break;
+      }
+      a.tile_from += (int32_t)ceil_div(a.piece, logit_vocab_rows(p.tile));
+    }
     if (here < 256)
       loss_join_kernel<1><<<dim3((unsigned)here), dim3(256), 0, stream>>>(a, (int32_t)p.tiles);
     else
@@ -259,23 +440,44 @@ int run_forward(LossArgs a, const ForwardPlan& p, LossMeta* meta, int32_t* index
   return check_launch("cross entropy kernel");
 }
 
-template <int DT>
-int run_backward(LossArgs a, const BackwardPlan& p, LossMeta* meta, int32_t* index, hipStream_t stream) {
-  loss_rows_kernel<true><<<dim3(1), dim3(1024), 0, stream>>>(a, meta, index);
+template <class PZ, class PW, class PH, int DT>
+void launch_piece(LossArgs a, const BackwardPlan& p, hipStream_t stream) {
+  a.vocab_tiles = (int32_t)ceil_div(a.piece, PZ::MT);
   if (a.rows > 0)
-    loss_zero_rows_kernel<<<dim3((unsigned)min64(a.rows, 4096)), dim3(256), 0, stream>>>(a);
-  const unsigned row_tiles = (unsigned)((a.rows + kTile - 1) / kTile);
-  const unsigned width_tiles = (unsigned)((a.width + kTile - 1) / kTile);
+    loss_dz_kernel<PZ, DT><<<dim3(grid_of(a.vocab_tiles * ceil_div(a.rows, PZ::NT))), dim3(PZ::NW * 64), 0, stream>>>(
+        a, 4);
+  a.vocab_tiles = (int32_t)ceil_div(a.piece, PW::NT);
+  a.width_tiles = (int32_t)ceil_div(a.width, PW::MT);
+  loss_dweight_kernel<PW, DT><<<dim3(grid_of((int64_t)a.vocab_tiles * a.width_tiles)), dim3(PW::NW * 64), 0, stream>>>(
+      a, 8);
+  a.width_tiles = (int32_t)ceil_div(a.width, PH::MT);
+  if (a.rows > 0)
+    loss_dhidden_product_kernel<PH, DT><<<dim3(grid_of(a.width_tiles * ceil_div(a.rows, PH::NT)), (unsigned)p.splits),
+                                          dim3(PH::NW * 64), 0, stream>>>(a, 4, (int)p.span);
+}
+
+template <int DT>
+int run_backward(LossArgs a, const BackwardPlan& p, const Weight& w, char* ws, hipStream_t stream) {
+  typedef Tiles<DT, false, false> Z;
+  typedef Tiles<DT, true, true> W;
+  typedef Tiles<DT, true, false> H;
+  loss_rows_kernel<true><<<dim3(1), dim3(1024), 0, stream>>>(a, (LossMeta*)ws, (int32_t*)(ws + p.index),
+                                                             (int32_t*)(ws + p.position));
+  if (a.rows > 0)
+    loss_pack_kernel<true><<<dim3((unsigned)min64(a.rows, 8192)), dim3(256), 0, stream>>>(
+        a, (const int32_t*)(ws + p.position), (uint16_t*)(ws + p.packed));
   for (int64_t i = 0; i < p.pieces; ++i) {
-    a.piece_from = (int32_t)(i * p.piece);
-    a.piece = (int32_t)min64(p.piece, a.vocab - a.piece_from);
+    take_piece(a, w, i * p.piece, p.piece, stream);
     a.first_piece = i == 0;
-    a.last_piece = i + 1 == p.pieces;
-    const unsigned tiles = (unsigned)((a.piece + kTile - 1) / kTile);
-    if (row_tiles > 0) loss_dz_general_kernel<DT><<<dim3(tiles, row_tiles), dim3(256), 0, stream>>>(a);
-    loss_dweight_general_kernel<DT><<<dim3(width_tiles, tiles), dim3(256), 0, stream>>>(a);
-    if (row_tiles > 0) loss_dhidden_general_kernel<DT><<<dim3(width_tiles, row_tiles), dim3(256), 0, stream>>>(a);
+    switch (p.tile) {
+      case kTile16: launch_piece<typename Z::T16, typename W::T256, typename H::T16, DT>(a, p, stream); break;
+      case kTile64: launch_piece<typename Z::T64, typename W::T256, typename H::T64, DT>(a, p, stream); break;
+      case kTile128: launch_piece<typename Z::T128, typename W::T256, typename H::T128, DT>(a, p, stream); break;
+      case kTile256: launch_piece<typename Z::T256, typename W::T256, typename H::T256, DT>(a, p, stream); break;
+    }
   }
+  if (a.sum && a.rows > 0)
+    loss_dhidden_kernel<DT><<<dim3((unsigned)min64(a.rows, 8192)), dim3(256), 0, stream>>>(a);
   return check_launch("cross entropy gradient kernel");
 }
 
@@ -286,9 +488,11 @@ using namespace hprms;
 
 extern "C" {
 
-int64_t hprms_linear_cross_entropy_workspace(int64_t rows, int64_t hidden, int64_t vocab) {
-  const int rc = check_sizes(rows, hidden, vocab);
-  return rc != HPRMS_OK ? rc : forward_plan(rows, vocab).total;
+int64_t hprms_linear_cross_entropy_workspace(int64_t rows, int64_t hidden_size, int64_t vocab, const void* weight,
+                                             int64_t weight_row_stride) {
+  const int rc = check_sizes(rows, hidden_size, vocab);
+  if (rc != HPRMS_OK) return rc;
+  return forward_plan(rows, hidden_size, vocab, weight_in_place(weight, weight_row_stride, hidden_size)).total;
 }
 
 int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, const void* weight, const int64_t* target,
@@ -300,18 +504,19 @@ int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, cons
   if (rows == 0) return HPRMS_OK;
   if (!loss || !lse || !aligned_to(loss, 4) || !aligned_to(lse, 4))
     return fail(HPRMS_E_INVALID, "null or misaligned tensor pointer (loss, lse)");
-  const ForwardPlan p = forward_plan(rows, vocab);
+  const bool in_place = weight_in_place(weight, weight_row_stride, hidden_size);
+  const ForwardPlan p = forward_plan(rows, hidden_size, vocab, in_place);
   rc = check_workspace(workspace, workspace_size, p.total);
   if (rc != HPRMS_OK) return rc;
   char* ws = (char*)workspace;
   LossArgs a = {};
   a.hidden = (const uint16_t*)hidden;
-  a.weight = (const uint16_t*)weight;
+  a.packed = (const uint16_t*)(ws + p.packed);
   a.target = target;
   a.meta = (const LossMeta*)ws;
   a.index = (const int32_t*)(ws + p.index);
   a.hidden_stride = hidden_row_stride;
-  a.weight_stride = weight_row_stride;
+  a.packed_width = (int32_t)packed_width_of(hidden_size);
   a.ignore_index = ignore_index;
   a.rows = (int32_t)rows;
   a.width = (int32_t)hidden_size;
@@ -320,14 +525,17 @@ int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, cons
   a.lse = lse;
   a.target_logit = (float*)(ws + p.target_logit);
   a.partial = (float2*)(ws + p.partial);
-  return dtype == HPRMS_DTYPE_BF16
-             ? run_forward<HPRMS_DTYPE_BF16>(a, p, (LossMeta*)ws, (int32_t*)(ws + p.index), stream)
-             : run_forward<HPRMS_DTYPE_FP16>(a, p, (LossMeta*)ws, (int32_t*)(ws + p.index), stream);
+  a.rows_at = (int32_t)p.rows_at;
+  const Weight w{(const uint16_t*)weight, weight_row_stride, in_place ? nullptr : (uint16_t*)(ws + p.weight)};
+  return dtype == HPRMS_DTYPE_BF16 ? run_forward<HPRMS_DTYPE_BF16>(a, p, w, ws, stream)
+                                   : run_forward<HPRMS_DTYPE_FP16>(a, p, w, ws, stream);
 }
 
-int64_t hprms_linear_cross_entropy_backward_workspace(int64_t rows, int64_t hidden, int64_t vocab) {
-  const int rc = check_sizes(rows, hidden, vocab);
-  return rc != HPRMS_OK ? rc : backward_plan(rows, hidden, vocab).total;
+int64_t hprms_linear_cross_entropy_backward_workspace(int64_t rows, int64_t hidden_size, int64_t vocab,
+                                                      const void* weight, int64_t weight_row_stride) {
+  const int rc = check_sizes(rows, hidden_size, vocab);
+  if (rc != HPRMS_OK) return rc;
+  return backward_plan(rows, hidden_size, vocab, weight_in_place(weight, weight_row_stride, hidden_size)).total;
 }
 
 int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const float* dloss, const void* hidden,
@@ -346,18 +554,19 @@ int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const floa
     return fail(HPRMS_E_INVALID, "null tensor pointer");
   if (!aligned_to(dweight, 2) || !aligned_to(dhidden, 2) || !aligned_to(dloss, 4) || !aligned_to(lse, 4))
     return fail(HPRMS_E_INVALID, "tensors must be aligned to their elements");
-  const BackwardPlan p = backward_plan(rows, hidden_size, vocab);
+  const bool in_place = weight_in_place(weight, weight_row_stride, hidden_size);
+  const BackwardPlan p = backward_plan(rows, hidden_size, vocab, in_place);
   rc = check_workspace(workspace, workspace_size, p.total);
   if (rc != HPRMS_OK) return rc;
   char* ws = (char*)workspace;
   LossArgs a = {};
   a.hidden = (const uint16_t*)hidden;
-  a.weight = (const uint16_t*)weight;
+  a.packed = (const uint16_t*)(ws + p.packed);
   a.target = target;
   a.meta = (const LossMeta*)ws;
   a.index = (const int32_t*)(ws + p.index);
   a.hidden_stride = hidden_row_stride;
-  a.weight_stride = weight_row_stride;
+  a.packed_width = (int32_t)packed_width_of(hidden_size);
   a.ignore_index = ignore_index;
   a.rows = (int32_t)rows;
   a.width = (int32_t)hidden_size;
@@ -365,15 +574,16 @@ int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const floa
   a.lse = const_cast<float*>(lse);
   a.dloss = dloss;
   a.dz = (uint16_t*)(ws + p.dz);
-  a.dz_stride = p.piece;
+  a.dz_stride = (int32_t)p.piece;
   a.dhidden = (uint16_t*)dhidden;
   a.dhidden_stride = dhidden_row_stride;
   a.dweight = (uint16_t*)dweight;
   a.dweight_stride = dweight_row_stride;
-  a.sum = (float*)(ws + p.sum);
-  return dtype == HPRMS_DTYPE_BF16
-             ? run_backward<HPRMS_DTYPE_BF16>(a, p, (LossMeta*)ws, (int32_t*)(ws + p.index), stream)
-             : run_backward<HPRMS_DTYPE_FP16>(a, p, (LossMeta*)ws, (int32_t*)(ws + p.index), stream);
+  a.sum = p.pieces * p.splits > 1 ? (float*)(ws + p.sum) : nullptr;
+  a.splits = (int32_t)p.splits;
+  const Weight w{(const uint16_t*)weight, weight_row_stride, in_place ? nullptr : (uint16_t*)(ws + p.weight)};
+  return dtype == HPRMS_DTYPE_BF16 ? run_backward<HPRMS_DTYPE_BF16>(a, p, w, ws, stream)
+                                   : run_backward<HPRMS_DTYPE_FP16>(a, p, w, ws, stream);
 }
 
 }  // extern "C"

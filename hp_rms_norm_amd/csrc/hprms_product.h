@@ -1,0 +1,200 @@
+// hprms_product.h - the tile product of the loss kernels: C = A . B^T over 16-bit
+// operands with binary32 sums, on the matrix cores.
+#pragma once
+
+#include "hprms_device.h"
+
+namespace hprms {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == HPRMS_DTYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+
+// One operand of a tile: `rows` of its first index (the tile's extent) over the
+// summed index k.
+//   KOUTER false: element (r, k) at base + r * stride + k (k contiguous)
+//   KOUTER true:  element (r, k) at base + k * stride + r (r contiguous)
+// `bytes` from base hold the operand: what lies past them reads as 0.
+struct Operand {
+  const uint16_t* base;
+  int64_t bytes;
+  int32_t stride;  // elements, a multiple of 8
+};
+
+typedef __attribute__((address_space(3))) uint16_t lds_u16;
+
+// A workgroup of WM x WN waves computes an MT x NT tile, each wave MI x NI
+// fragments of 16 x 16.  Slices of BK summed entries travel from memory to LDS
+// without registers (16 bytes a lane), ST slices deep; a slice's LDS rows are
+// swizzled through the addresses that the lanes load from, so that fragment
+// reads touch every bank once:
+//   k contiguous: LDS row r holds 2 * BK bytes, its 16-byte chunk p the row's
+//     chunk p ^ (r mod 8) (BK = 64) or p ^ (r / 2 mod 4) (BK = 32); a
+//     fragment is one 16-byte read a lane.
+//   k outer: LDS row k holds 2 * extent bytes, its 32-byte unit u the unit
+//     u ^ (k mod 4, or fewer units: mod the units); a fragment is two transposing 8-byte reads a lane, which give
+//     16 lanes 4 entries of 16 columns.
+template <int DT, int MT_, int NT_, int WM_, int WN_, int BK_, int ST_, bool AKO_, bool BKO_>
+struct Product {
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, BK = BK_, ST = ST_;
+  static constexpr bool AKO = AKO_, BKO = BKO_;
+  static constexpr int NW = WM * WN;
+  static constexpr int MI = MT / WM / 16, NI = NT / WN / 16;
+  static constexpr int ABYTES = MT * BK * 2, BBYTES = NT * BK * 2;
+  static constexpr int STAGE = ABYTES + BBYTES;
+  static constexpr int LA = (ABYTES / 1024 + NW - 1) / NW, LB = (BBYTES / 1024 + NW - 1) / NW;
+  static constexpr int LDS_BYTES = STAGE * ST;
+  static_assert(BK == 64 || BK == 32, "slice depth");
+  static_assert(MT % (WM * 16) == 0 && NT % (WN * 16) == 0, "wave tiles");
+  static_assert(ABYTES % 1024 == 0 && BBYTES % 1024 == 0, "whole loads");
+
+  // Byte offset, from the operand's base, of what lane `lane` loads in load j
+  // of a slice (1024 bytes of LDS), for an operand of EXT rows; *k: the slice's
+  // summed entry where the lane's 8 elements begin (k contiguous).
+  template <int EXT, bool KO>
+  __device__ static __forceinline__ uint32_t load_offset(int j, int lane, int32_t stride, int* k) {
+    const int at = j * 1024 + lane * 16;  // byte in the slice
+    if constexpr (!KO) {
+      constexpr int RB = BK * 2;
+      const int r = at / RB, p = at % RB / 16;
+      const int c = BK == 64 ? p ^ (r & 7) : p ^ ((r >> 1) & 3);
+      *k = c * 8;
+      return ((uint32_t)r * (uint32_t)stride + c * 8) * 2;
+    } else {
+      constexpr int RB = EXT * 2;
+      const int kr = at / RB, p = at % RB / 16;
+      const int u = (p >> 1) ^ swizzle_k<EXT>(kr);
+      *k = 0;
+      return ((uint32_t)kr * (uint32_t)stride + u * 16 + (p & 1) * 8) * 2;
+    }
+  }
+  template <int EXT>
+  __device__ static __forceinline__ int swizzle_k(int k) {
+    constexpr int UNITS = EXT / 16;
+    return (k & 3) & (UNITS - 1 < 3 ? UNITS - 1 : 3);
+  }
+
+  // The fragment of rows r0 ... r0 + 15 and entries kk * 32 ... + 31 of a slice.
+  template <int EXT, bool KO>
+  __device__ static __forceinline__ u32x4 fragment(lds_u16* slice, int r0, int kk, int lane) {
+    if constexpr (!KO) {
+      const int r = r0 + (lane & 15), c = kk * 4 + (lane >> 4);
+      const int p = BK == 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
+      return *(__attribute__((address_space(3))) u32x4*)(slice + r * BK + p * 8);
+    } else {
+      // 16 lanes read 4 rows of k (lane & 15) / 4, 4 columns each
+      const int k = kk * 32 + (lane >> 4) * 8 + ((lane & 15) >> 2);
+      const int u = (r0 / 16) ^ swizzle_k<EXT>(k);
+      lds_u16* p = slice + k * EXT + u * 16 + (lane & 3) * 4;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+      const s16x4 hi =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * EXT));
+      const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
+      return u32x4{l[0], l[1], h[0], h[1]};
+    }
+  }
+
+  // acc <- A . B^T over k in [0, depth).
+  __device__ static __forceinline__ void run(const Operand& a, const Operand& b, int32_t depth, uint16_t* lds_generic,
+                                             f32x4 (&acc)[MI][NI]) {
+    lds_u16* lds = (lds_u16*)lds_generic;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    uint32_t oa[LA], ob[LB];
+    int ka[LA], kb[LB];
+    int ja[LA], jb[LB];
+#pragma unroll
+    for (int i = 0; i < LA; ++i) {
+      // waves without a load of their own repeat the last one
+      ja[i] = i * NW + wave < ABYTES / 1024 ? i * NW + wave : ABYTES / 1024 - 1;
+      oa[i] = load_offset<MT, AKO>(ja[i], lane, a.stride, &ka[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+      jb[i] = i * NW + wave < BBYTES / 1024 ? i * NW + wave : BBYTES / 1024 - 1;
+      ob[i] = load_offset<NT, BKO>(jb[i], lane, b.stride, &kb[i]);
+    }
+    const int32_t slices = (depth + BK - 1) / BK;
+    const int64_t astep = AKO ? (int64_t)a.stride * BK * 2 : BK * 2;
+    const int64_t bstep = BKO ? (int64_t)b.stride * BK * 2 : BK * 2;
+    const char* abase = (const char*)a.base;
+    const char* bbase = (const char*)b.base;
+    int64_t abytes = a.bytes, bbytes = b.bytes;
+
+    // loads of slice t into LDS stage s; past the last slice nothing is in range
+    auto load = [&](int32_t t, int s) {
+      const bool in = t < slices;
+      const int64_t an = !in || abytes < 0 ? 0 : abytes > 0x7fffffff ? 0x7fffffff : abytes;
+      const int64_t bn = !in || bbytes < 0 ? 0 : bbytes > 0x7fffffff ? 0x7fffffff : bbytes;
+      const __amdgpu_buffer_rsrc_t ra = make_rsrc(abase, (uint32_t)an);
+      const __amdgpu_buffer_rsrc_t rb = make_rsrc(bbase, (uint32_t)bn);
+      lds_u16* stage = lds + s * (STAGE / 2);
+      const int left = depth - t * BK;  // entries of k from this slice on
+#pragma unroll
+      for (int i = 0; i < LA; ++i) {
+        const uint32_t off = !AKO && ka[i] >= left ? kOOB : oa[i];
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(stage + ja[i] * 512), 16,
+                                                 off, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < LB; ++i) {
+        const uint32_t off = !BKO && kb[i] >= left ? kOOB : ob[i];
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rb, (__attribute__((address_space(3))) void*)(stage + ABYTES / 2 + jb[i] * 512), 16, off, 0, 0, 0);
+      }
+      abase += astep;
+      abytes -= astep;
+      bbase += bstep;
+      bbytes -= bstep;
+    };
+
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) load(s, s);
+    int s = 0;
+    for (int32_t t = 0; t < slices; ++t) {
+      // this slice has landed (the ST - 2 later ones may be on their way) and
+      // every wave has the fragments of the last one in registers
+      constexpr int WAIT = (ST - 2) * (LA + LB);
+      __builtin_amdgcn_s_waitcnt((WAIT & 15) | (WAIT >> 4) << 14 | 0x70);  // vmcnt(WAIT) lgkmcnt(0)
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      load(t + ST - 1, s == 0 ? ST - 1 : s - 1);
+      lds_u16* as = lds + s * (STAGE / 2);
+      lds_u16* bs = as + ABYTES / 2;
+#pragma unroll
+      for (int kk = 0; kk < BK / 32; ++kk) {
+        u32x4 fa[MI], fb[NI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[i] = fragment<MT, AKO>(as, (wm * MI + i) * 16, kk, lane);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) fb[j] = fragment<NT, BKO>(bs, (wn * NI + j) * 16, kk, lane);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<DT>(fa[i], fb[j], acc[i][j]);
+      }
+      s = s + 1 == ST ? 0 : s + 1;
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0) lgkmcnt(0): LDS is free again behind the next barrier
+  }
+};
+
+}  // namespace hprms

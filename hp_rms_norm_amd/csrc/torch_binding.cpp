@@ -685,7 +685,8 @@ void linear_cross_entropy_hip(at::Tensor& loss, at::Tensor& lse, const at::Tenso
   if (s.rows == 0) return;
   c10::DeviceGuard guard(hidden.device());
   hipStream_t stream = c10::hip::getCurrentHIPStream(hidden.device().index()).stream();
-  const at::Tensor ws = workspace_of(hprms_linear_cross_entropy_workspace(s.rows, s.hidden, s.vocab), hidden);
+  const at::Tensor ws = workspace_of(
+      hprms_linear_cross_entropy_workspace(s.rows, s.hidden, s.vocab, weight.data_ptr(), s.weight_stride), hidden);
   check_status(hprms_linear_cross_entropy(loss.data_ptr<float>(), lse.data_ptr<float>(), hidden.data_ptr(),
                                           weight.data_ptr(), target.data_ptr<int64_t>(), ws.data_ptr(), ws.numel(),
                                           s.rows, s.hidden, s.vocab, s.hidden_stride, s.weight_stride, ignore_index,
@@ -733,8 +734,10 @@ void linear_cross_entropy_backward_hip(at::Tensor& dhidden, at::Tensor& dweight,
   const LossGradShape s = check_loss_backward(dhidden, dweight, dloss, hidden, weight, target, lse);
   c10::DeviceGuard guard(hidden.device());
   hipStream_t stream = c10::hip::getCurrentHIPStream(hidden.device().index()).stream();
-  const at::Tensor ws =
-      workspace_of(hprms_linear_cross_entropy_backward_workspace(s.f.rows, s.f.hidden, s.f.vocab), hidden);
+  const at::Tensor ws = workspace_of(
+      hprms_linear_cross_entropy_backward_workspace(s.f.rows, s.f.hidden, s.f.vocab, weight.data_ptr(),
+                                                    s.f.weight_stride),
+      hidden);
   check_status(hprms_linear_cross_entropy_backward(
       dhidden.data_ptr(), dweight.data_ptr(), dloss.data_ptr<float>(), hidden.data_ptr(), weight.data_ptr(),
       target.data_ptr<int64_t>(), lse.data_ptr<float>(), ws.data_ptr(), ws.numel(), s.f.rows, s.f.hidden, s.f.vocab,

@@ -403,10 +403,15 @@ int hprms_rmsnorm_backward(void* dinput, void* dweight, const void* dout, const 
  * ignore_index get loss 0 and lse 0 and are not read; any other target outside
  * [0, vocab) gives a NaN loss.  The workspace is as for
  * hprms_rmsnorm_backward(), 256-byte aligned, of
- * hprms_linear_cross_entropy_workspace() bytes.  rows == 0 is a no-op.  No
- * counterpart in the reference.
+ * hprms_linear_cross_entropy_workspace() bytes, which depends on the weight's
+ * address and row stride: rows that 16-byte loads cannot take in place (an
+ * address or stride off 16 bytes, hidden_size % 8 != 0, a stride above 2^21)
+ * are packed there, a piece of the vocabulary at a time.  rows == 0 is a no-op.
+ * rows, hidden_size and vocab go up to 2^22, 2^20 and 2^28.  No counterpart in
+ * the reference.
  */
-int64_t hprms_linear_cross_entropy_workspace(int64_t rows, int64_t hidden, int64_t vocab);
+int64_t hprms_linear_cross_entropy_workspace(int64_t rows, int64_t hidden_size, int64_t vocab, const void* weight,
+                                             int64_t weight_row_stride);
 int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, const void* weight, const int64_t* target,
                                void* workspace, int64_t workspace_size, int64_t rows, int64_t hidden_size,
                                int64_t vocab, int64_t hidden_row_stride, int64_t weight_row_stride,
@@ -425,7 +430,8 @@ int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, cons
  * hprms_linear_cross_entropy_backward_workspace() bytes, 256-byte aligned.  No
  * counterpart in the reference.
  */
-int64_t hprms_linear_cross_entropy_backward_workspace(int64_t rows, int64_t hidden, int64_t vocab);
+int64_t hprms_linear_cross_entropy_backward_workspace(int64_t rows, int64_t hidden_size, int64_t vocab,
+                                                      const void* weight, int64_t weight_row_stride);
 int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const float* dloss, const void* hidden,
                                         const void* weight, const int64_t* target, const float* lse, void* workspace,
                                         int64_t workspace_size, int64_t rows, int64_t hidden_size, int64_t vocab,
