@@ -41,10 +41,10 @@ namespace hprms {
 typedef u32x4 u32x4_u __attribute__((aligned(2)));
 typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(2)));
 
-// What the row list says, written by loss_rows_kernel.
+// What the row list says, written by loss_pack_kernel.
 struct LossMeta {
   int32_t count;   // listed rows
-  float scale;     // power of two applied to dloss
+  float scale;     // gradient: power of two applied to dloss
   float unscale;   // its inverse
   int32_t pad;
 };
@@ -83,8 +83,10 @@ struct LossArgs {
   int64_t dhidden_stride;
   uint16_t* dweight;
   int64_t dweight_stride;
-  float* sum;               // [splits, rows, packed_width] shares of dhidden, by list position; null: none
-  int32_t first_piece, splits;
+  float* sum;               // [splits, count, packed_width] shares of dhidden, by list position; null: none
+  int32_t first_piece;
+  int32_t piece_size, slots, most_splits;  // see splits_of
+  int32_t pack_rows;        // rows per workgroup of the packing kernel
 };
 
 // ---- epilogues ------------------------------------------------------------------------
@@ -190,6 +192,16 @@ __device__ __forceinline__ void dz_epilogue(const LossArgs& a, const f32x4 (&acc
   }
 }
 
+// 8 elements p[0 ... 7], of which the first n exist (n may be negative); the others read as 0
+__device__ __forceinline__ u32x4 load_some(const uint16_t* p, int n) {
+  if (n >= 8) return *(const u32x4_u*)p;
+  u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < n) v[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
+  return v;
+}
+
 template <int DT>
 __device__ __forceinline__ void store_four(uint16_t* p, const float* d, int n) {
   using F = Fmt<DT>;
@@ -241,7 +253,7 @@ __device__ __forceinline__ void dhidden_epilogue(const LossArgs& a, const f32x4 
       const int m = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4;
       if (a.sum) {
         if (m >= a.packed_width) continue;
-        f32x4* s = (f32x4*)(a.sum + ((int64_t)split * a.rows + n) * a.packed_width + m);
+        f32x4* s = (f32x4*)(a.sum + ((int64_t)split * count + n) * a.packed_width + m);
         *s = a.first_piece ? acc[mi][ni] : acc[mi][ni] + *s;
       } else if (m < a.width) {
         float d[4];

@@ -9,83 +9,70 @@ namespace hprms {
 namespace {
 
 // ---- the list of rows that carry a loss -----------------------------------------------
-// One workgroup: `index` gets the rows whose target is not ignore_index, in
-// order, and `position` each row's place among them (-1: none); with GRAD also the scale of dloss, from the largest of its finite
-// magnitudes.  Without GRAD the other rows' loss and lse are set to 0.
+// sums over the workgroup's 256 lanes
+__device__ __forceinline__ int block_count(int v, int* lds) {
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+// Lists the rows whose target is not ignore_index, in order, and packs their
+// hidden values side by side, zero up to packed_width: one operand layout for
+// any width, stride and alignment, and no ignored rows in the products.  Each
+// workgroup takes a.pack_rows rows, whose places it knows from counting the
+// rows before them itself (at most 512 workgroups, so that those 8 bytes a row
+// stay few).  The other rows get loss and lse 0, or (GRAD) a zero dhidden.
+// With GRAD the first workgroup also scales dloss, by the largest of its
+// finite magnitudes.
 template <bool GRAD>
-__global__ __launch_bounds__(1024) void loss_rows_kernel(LossArgs a, LossMeta* meta, int32_t* index,
-                                                         int32_t* position) {
-  __shared__ int32_t waves[16];
-  __shared__ float tops[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int32_t count = 0;
-  float top = 0.0f;
-  for (int32_t r0 = 0; r0 < a.rows; r0 += 1024) {
-    const int32_t row = r0 + threadIdx.x;
-    const bool in = row < a.rows;
-    const bool keep = in && a.target[row] != a.ignore_index;
-    const uint64_t mask = __ballot(keep);
-    if (lane == 0) waves[wave] = __popcll(mask);
-    __syncthreads();
-    int32_t before = count;
-    for (int i = 0; i < 16; ++i) {
-      if (i < wave) before += waves[i];
-      count += waves[i];
-    }
-    const int32_t at = before + __popcll(mask & ((uint64_t(1) << lane) - 1));
-    if (keep) index[at] = row;
-    if (in) position[row] = keep ? at : -1;
-    if constexpr (GRAD) {
-      if (keep) {
-        const float g = fabsf(a.dloss[row]);
-        if (g < __builtin_inff()) top = fmaxf(top, g);
+__global__ __launch_bounds__(256) void loss_pack_kernel(LossArgs a, LossMeta* meta, int32_t* index, uint16_t* packed) {
+  __shared__ int lds[4];
+  const int32_t r0 = blockIdx.x * a.pack_rows, r1 = min(r0 + a.pack_rows, a.rows);
+  int n = 0;
+  for (int32_t r = threadIdx.x; r < r0; r += 256) n += a.target[r] != a.ignore_index;
+  int32_t at = block_count(n, lds);
+  for (int32_t row = r0; row < r1; ++row) {
+    if (a.target[row] == a.ignore_index) {
+      if constexpr (GRAD) {
+        for (int32_t i = threadIdx.x; i < a.width; i += 256) a.dhidden[(int64_t)row * a.dhidden_stride + i] = 0;
+      } else if (threadIdx.x == 0) {
+        a.loss[row] = 0.0f;
+        a.lse[row] = 0.0f;
       }
-    } else if (in && !keep) {
-      a.loss[row] = 0.0f;
-      a.lse[row] = 0.0f;
+      continue;
     }
-    __syncthreads();
+    if (threadIdx.x == 0) index[at] = row;
+    const uint16_t* from = a.hidden + (int64_t)row * a.hidden_stride;
+    uint16_t* to = packed + (int64_t)at * a.packed_width;
+    for (int32_t i = threadIdx.x * 8; i < a.packed_width; i += 256 * 8) *(u32x4*)(to + i) = load_some(from + i, a.width - i);
+    ++at;
   }
-  float scale = 1.0f;
+  if (r1 == a.rows && threadIdx.x == 0) meta->count = at;
   if constexpr (GRAD) {
+    if (blockIdx.x != 0) return;
+    float top = 0.0f;
+#pragma unroll 4
+    for (int32_t r = threadIdx.x; r < a.rows; r += 256) {
+      const float g = fabsf(a.dloss[r]);
+      if (g < __builtin_inff() && a.target[r] != a.ignore_index) top = fmaxf(top, g);
+    }
     for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-    if (lane == 0) tops[wave] = top;
     __syncthreads();
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, tops[i]);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = __float_as_int(top);
+    __syncthreads();
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, __int_as_float(lds[i]));
     // 2^e <= top < 2^(e + 1); the scale brings it to [2^14, 2^15)
+    float scale = 1.0f;
     if (top > 0.0f) {
-      int e = (int)(__float_as_uint(top) >> 23) - 127;  // subnormals count as 2^-127
-      e = 14 - e;
+      int e = 14 - ((int)(__float_as_uint(top) >> 23) - 127);  // subnormals count as 2^-127
       e = e > 126 ? 126 : e < -112 ? -112 : e;
       scale = __uint_as_float((uint32_t)(e + 127) << 23);
     }
-  }
-  if (threadIdx.x == 0) *meta = LossMeta{count, scale, 1.0f / scale, 0};
-}
-
-// The listed rows' hidden values side by side, zero up to packed_width: one
-// operand layout for any width, stride and alignment, and no ignored rows in
-// the products.  With GRAD the other rows' dhidden is set to 0.
-template <bool GRAD>
-__global__ __launch_bounds__(256) void loss_pack_kernel(LossArgs a, const int32_t* position, uint16_t* packed) {
-  for (int32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const int32_t at = position[row];
-    if (at < 0) {
-      if constexpr (GRAD)
-        for (int32_t i = threadIdx.x; i < a.width; i += 256) a.dhidden[(int64_t)row * a.dhidden_stride + i] = 0;
-      continue;
-    }
-    const uint16_t* from = a.hidden + (int64_t)row * a.hidden_stride;
-    uint16_t* to = packed + (int64_t)at * a.packed_width;
-    for (int32_t i = threadIdx.x * 8; i < a.packed_width; i += 256 * 8) {
-      u32x4 v = {0, 0, 0, 0};
-      if (i + 8 <= a.width) {
-        v = *(const u32x4_u*)(from + i);
-      } else {
-        for (int j = 0; j < 8; ++j)
-          if (i + j < a.width) v[j / 2] |= (uint32_t)from[i + j] << (16 * (j & 1));
-      }
-      *(u32x4*)(to + i) = v;
+    if (threadIdx.x == 0) {
+      meta->scale = scale;
+      meta->unscale = 1.0f / scale;
     }
   }
 }
@@ -98,16 +85,7 @@ __global__ __launch_bounds__(256) void loss_pack_weight_kernel(const uint16_t* w
   for (int32_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const uint16_t* from = weight + (int64_t)row * stride;
     uint16_t* to = packed + (int64_t)row * packed_width;
-    for (int32_t i = threadIdx.x * 8; i < packed_width; i += 256 * 8) {
-      u32x4 v = {0, 0, 0, 0};
-      if (i + 8 <= width) {
-        v = *(const u32x4_u*)(from + i);
-      } else {
-        for (int j = 0; j < 8; ++j)
-          if (i + j < width) v[j / 2] |= (uint32_t)from[i + j] << (16 * (j & 1));
-      }
-      *(u32x4*)(to + i) = v;
-    }
+    for (int32_t i = threadIdx.x * 8; i < packed_width; i += 256 * 8) *(u32x4*)(to + i) = load_some(from + i, width - i);
   }
 }
 
@@ -151,35 +129,47 @@ __global__ __launch_bounds__(P::NW * 64) void loss_forward_kernel(LossArgs a, in
                                                min(count, a.row_from + a.rows_at), a.tile_from + m, (float2*)lds);
 }
 
-// Joins the tiles of RPB rows: 256 / RPB lanes per row, each over tiles in order.
+// Two maxima with their sums of exponentials relative to them, as one.
+__device__ __forceinline__ float2 join(float2 s, float2 o) {
+  const float top = fmaxf(s.x, o.x);
+  const float at = top == -__builtin_inff() ? 0.0f : top;
+  return {top, s.y * exp_neg(s.x - at) + o.y * exp_neg(o.x - at)};
+}
+
+// Joins the tiles of RPB rows: 256 / RPB lanes a row, each over every so many
+// tiles, then the lanes.
 template <int RPB>
 __global__ __launch_bounds__(256) void loss_join_kernel(LossArgs a, int32_t tiles) {
-  constexpr int S = 256 / RPB;
-  __shared__ float2 lds[S][RPB];
+  constexpr int S = 256 / RPB, U = 8;
+  __shared__ float2 lds[4][RPB];
   const int c = threadIdx.x % RPB, s = threadIdx.x / RPB;
   const int at = blockIdx.x * RPB + c;  // list position from row_from on
-  const int count = a.meta->count - a.row_from;
-  float top = -__builtin_inff(), sum = 0.0f;
-  if (at < count) {
-    for (int t = s; t < tiles; t += S) {
-      const float2 o = a.partial[(int64_t)t * a.rows_at + at];
-      const float m = fmaxf(top, o.x);
-      const float z = m == -__builtin_inff() ? 0.0f : m;
-      sum = sum * exp_neg(top - z) + o.y * exp_neg(o.x - z);
-      top = m;
-    }
+  const bool live = at < a.meta->count - a.row_from;
+  const float2 none = {-__builtin_inff(), 0.0f};
+  float2 all = none;
+  for (int t = s; t < tiles; t += S * U) {
+    float2 o[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      o[i] = live && t + i * S < tiles ? a.partial[(int64_t)(t + i * S) * a.rows_at + at] : none;
+    float top = all.x;
+#pragma unroll
+    for (int i = 0; i < U; ++i) top = fmaxf(top, o[i].x);
+    const float z = top == -__builtin_inff() ? 0.0f : top;
+    float sum = all.y * exp_neg(all.x - z);
+#pragma unroll
+    for (int i = 0; i < U; ++i) sum += o[i].y * exp_neg(o[i].x - z);
+    all = {top, sum};
   }
-  lds[s][c] = float2{top, sum};
+#pragma unroll
+  for (int m = RPB; m < 64; m <<= 1) all = join(all, {__shfl_xor(all.x, m), __shfl_xor(all.y, m)});
+  if ((threadIdx.x & 63) < RPB) lds[threadIdx.x >> 6][c] = all;
   __syncthreads();
-  if (s != 0 || at >= count) return;
-  float all = top;
-  for (int i = 1; i < S; ++i) all = fmaxf(all, lds[i][c].x);
-  const float z = all == -__builtin_inff() ? 0.0f : all;
-  float total = 0.0f;
-  for (int i = 0; i < S; ++i) total += lds[i][c].y * exp_neg(lds[i][c].x - z);
+  if (s != 0 || !live) return;
+  for (int i = 1; i < 4; ++i) all = join(all, lds[i][c]);
   const int row = a.index[a.row_from + at];
   const int64_t t = a.target[row];
-  const float lse = all + logf(total);
+  const float lse = all.x + logf(all.y);
   a.lse[row] = lse;
   a.loss[row] = t >= 0 && t < a.vocab ? lse - a.target_logit[a.row_from + at] : __builtin_nanf("");
 }
@@ -211,33 +201,53 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dweight_kernel(LossArgs a, in
   dweight_epilogue<DT, P::MI, P::NI>(a, acc, m0, n0, wave / P::WN, wave % P::WN);
 }
 
-// blockIdx.y: the split of the piece's vocabulary, `span` entries each
+// Splits of a piece's vocabulary over workgroups, where dhidden has fewer tiles
+// than `slots` (the workgroups that run at once): as many as fill them, of at
+// least 512 entries each, and `most` at the most.  The count of listed rows is
+// known on the device alone, so kernels and host compute this where they are.
+struct Splits {
+  int32_t count, span;
+};
+__host__ __device__ inline Splits splits_of(int32_t tiles, int32_t slots, int32_t piece, int32_t most) {
+  int32_t n = slots / (tiles > 0 ? tiles : 1);
+  if (n > piece / 512) n = piece / 512;
+  if (n > most) n = most;
+  if (n < 1) n = 1;
+  const int32_t span = ((piece + n - 1) / n + 63) / 64 * 64;
+  return {(piece + span - 1) / span, span};
+}
+
 template <class P, int DT>
-__global__ __launch_bounds__(P::NW * 64) void loss_dhidden_product_kernel(LossArgs a, int group, int span) {
+__global__ __launch_bounds__(P::NW * 64) void loss_dhidden_product_kernel(LossArgs a, int group) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[P::LDS_BYTES / 2];
   const int count = a.meta->count;
-  int m, n;
-  if (!tile_of(blockIdx.x, a.width_tiles, (count + P::NT - 1) / P::NT, group, &m, &n)) return;
+  const int row_tiles = (count + P::NT - 1) / P::NT;
+  const Splits sp = splits_of(a.width_tiles * row_tiles, a.slots, a.piece_size, a.most_splits);
+  int m, ns;
+  if (!tile_of(blockIdx.x, a.width_tiles, row_tiles * sp.count, group, &m, &ns)) return;
+  const int n = ns % row_tiles, split = ns / row_tiles, span = sp.span;
   const int m0 = m * P::MT, n0 = n * P::NT;
-  const int from = blockIdx.y * span;
+  const int from = split * span;
   // dz holds zeros past the piece up to a tile's end, so the depth may be rounded up to whole chunks
   const int depth = max(0, min(span, (a.piece - from + 7) & ~7));
   f32x4 acc[P::MI][P::NI];
   P::run(weight_columns(a, from, m0), dz_rows(a, n0, from, count), depth, lds, acc);
   const int wave = threadIdx.x >> 6;
-  dhidden_epilogue<DT, P::MI, P::NI>(a, acc, m0, n0, wave / P::WN, wave % P::WN, count, blockIdx.y);
+  dhidden_epilogue<DT, P::MI, P::NI>(a, acc, m0, n0, wave / P::WN, wave % P::WN, count, split);
 }
 
 // dhidden from its shares
 template <int DT>
-__global__ __launch_bounds__(256) void loss_dhidden_kernel(LossArgs a) {
+__global__ __launch_bounds__(256) void loss_dhidden_kernel(LossArgs a, int tile_rows) {
   const int count = a.meta->count;
+  const int splits = splits_of(a.width_tiles * ((count + tile_rows - 1) / tile_rows), a.slots, a.piece_size,
+                               a.most_splits).count;
   const float unscale = a.meta->unscale;
   for (int32_t n = blockIdx.x; n < count; n += gridDim.x) {
     uint16_t* to = a.dhidden + (int64_t)a.index[n] * a.dhidden_stride;
     for (int32_t i = threadIdx.x * 4; i < a.width; i += 256 * 4) {
       f32x4 d = {0, 0, 0, 0};
-      for (int s = 0; s < a.splits; ++s) d += *(const f32x4*)(a.sum + ((int64_t)s * a.rows + n) * a.packed_width + i);
+      for (int s = 0; s < splits; ++s) d += *(const f32x4*)(a.sum + ((int64_t)s * count + n) * a.packed_width + i);
       const float o[4] = {d[0] * unscale, d[1] * unscale, d[2] * unscale, d[3] * unscale};
       store_four<DT>(to + i, o, a.width - i);
     }
@@ -290,11 +300,13 @@ LogitTile logit_tile(int64_t rows) {
   return rows <= 16 ? kTile16 : rows <= 64 ? kTile64 : rows <= 128 ? kTile128 : kTile256;
 }
 int64_t logit_vocab_rows(LogitTile t) { return t <= kTile64 ? 128 : 256; }
+// hidden elements of a dhidden tile
+int64_t hidden_tile_width(LogitTile t) { return t <= kTile64 ? 128 : 256; }
 int64_t logit_rows(LogitTile t) { return t == kTile16 ? 16 : t == kTile64 ? 64 : t == kTile128 ? 128 : 256; }
 
 // Offsets of the workspace's parts, bytes.
 struct ForwardPlan {
-  int64_t index, position, target_logit, packed, weight, partial, total;
+  int64_t index, target_logit, packed, weight, partial, total;
   int64_t rows_at, tiles, piece;
   LogitTile tile;
 };
@@ -306,8 +318,7 @@ ForwardPlan forward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_pla
   p.piece = in_place ? round_up(vocab, kPieceUnit) : packed_piece(width, vocab);
   p.tiles = ceil_div(vocab, logit_vocab_rows(p.tile));
   p.index = 256;
-  p.position = p.index + round_up(rows * 4, 256);
-  p.target_logit = p.position + round_up(rows * 4, 256);
+  p.target_logit = p.index + round_up(rows * 4, 256);
   p.packed = p.target_logit + round_up(rows * 4, 256);
   p.weight = p.packed + rows * packed_width_of(width) * 2;
   p.partial = p.weight + (in_place ? 0 : p.piece * packed_width_of(width) * 2);
@@ -316,8 +327,9 @@ ForwardPlan forward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_pla
 }
 
 struct BackwardPlan {
-  int64_t index, position, packed, weight, dz, sum, total;
-  int64_t piece, pieces, dz_rows, splits, span;
+  int64_t index, packed, weight, dz, sum, total;
+  int64_t piece, pieces, dz_rows, row_tiles, width_tiles, slots, most_splits;
+  bool shares;
   LogitTile tile;
 };
 
@@ -329,20 +341,22 @@ BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_p
   p.piece = min64(p.piece, round_up(vocab, kPieceUnit));
   if (!in_place) p.piece = min64(p.piece, packed_piece(width, vocab));
   p.pieces = ceil_div(vocab, p.piece);
-  // splits of a piece's vocabulary where dhidden has fewer tiles than the GPU
-  // CUs, of at least 512 entries
-  const int64_t tiles = ceil_div(width, p.tile <= kTile64 ? 128 : 256) * ceil_div(max64(rows, 1), logit_rows(p.tile));
-  const int64_t slots = (int64_t)current_cus() * (p.tile <= kTile64 ? 2 : 1);
-  p.splits = max64(1, min64(slots / tiles, p.piece / 512));
-  p.span = round_up(ceil_div(p.piece, p.splits), 64);
-  p.splits = ceil_div(p.piece, p.span);
+  p.width_tiles = ceil_div(width, hidden_tile_width(p.tile));
+  const int64_t row_tiles = ceil_div(max64(rows, 1), logit_rows(p.tile));
+  p.slots = (int64_t)current_cus() * (p.tile == kTile256 ? 1 : 2);
+  // with fewer listed rows there are more splits, of fewer rows: count * splits
+  // stays within what a slot's tile holds each, or within one share of all rows
+  p.most_splits = max64(1, min64(p.slots / p.width_tiles, p.piece / 512));
+  const int64_t sum_rows = max64(rows, p.most_splits > 1 ? p.slots / p.width_tiles * logit_rows(p.tile) : 0);
+  const bool shares = p.pieces > 1 || p.most_splits > 1;
   p.index = 256;
-  p.position = p.index + round_up(rows * 4, 256);
-  p.packed = p.position + round_up(rows * 4, 256);
+  p.packed = p.index + round_up(rows * 4, 256);
   p.weight = p.packed + rows * packed_width_of(width) * 2;
   p.dz = p.weight + (in_place ? 0 : p.piece * packed_width_of(width) * 2);
   p.sum = p.dz + p.dz_rows * p.piece * 2;
-  p.total = p.sum + (p.pieces * p.splits > 1 ? p.splits * rows * packed_width_of(width) * 4 : 0);
+  p.total = p.sum + (shares ? sum_rows * packed_width_of(width) * 4 : 0);
+  p.row_tiles = row_tiles;
+  p.shares = shares;
   return p;
 }
 
@@ -374,7 +388,7 @@ struct Tiles {
   typedef Product<DT, 128, 16, 4, 1, 64, 4, AKO, BKO> T16;
   typedef Product<DT, 128, 64, 4, 1, 64, 3, AKO, BKO> T64;
   typedef Product<DT, 256, 128, 4, 2, 32, 3, AKO, BKO> T128;
-  typedef Product<DT, 256, 256, 2, 4, 64, 2, AKO, BKO> T256;
+  typedef Product<DT, 256, 256, 4, 2, 32, 4, AKO, BKO> T256;
 };
 
 // workgroups of `tiles` tiles, for tile_of
@@ -411,13 +425,18 @@ void take_piece(LossArgs& a, const Weight& w, int64_t from, int64_t piece, hipSt
   a.weight_width = a.packed_width;
 }
 
+template <bool GRAD>
+void launch_pack(LossArgs& a, char* ws, int64_t index, int64_t packed, hipStream_t stream) {
+  a.pack_rows = (int32_t)ceil_div(max64(a.rows, 1), 512);
+  const unsigned grid = (unsigned)ceil_div(max64(a.rows, 1), a.pack_rows);
+  loss_pack_kernel<GRAD><<<dim3(grid), dim3(256), 0, stream>>>(a, (LossMeta*)ws, (int32_t*)(ws + index),
+                                                              (uint16_t*)(ws + packed));
+}
+
 template <int DT>
 int run_forward(LossArgs a, const ForwardPlan& p, const Weight& w, char* ws, hipStream_t stream) {
   typedef Tiles<DT, false, false> T;
-  loss_rows_kernel<false><<<dim3(1), dim3(1024), 0, stream>>>(a, (LossMeta*)ws, (int32_t*)(ws + p.index),
-                                                              (int32_t*)(ws + p.position));
-  loss_pack_kernel<false><<<dim3((unsigned)min64(a.rows, 8192)), dim3(256), 0, stream>>>(
-      a, (const int32_t*)(ws + p.position), (uint16_t*)(ws + p.packed));
+  launch_pack<false>(a, ws, p.index, p.packed, stream);
   for (int64_t from = 0; from < a.rows; from += p.rows_at) {
     a.row_from = (int32_t)from;
     const int64_t here = min64(p.rows_at, a.rows - from);
@@ -450,10 +469,12 @@ void launch_piece(LossArgs a, const BackwardPlan& p, hipStream_t stream) {
   a.width_tiles = (int32_t)ceil_div(a.width, PW::MT);
   loss_dweight_kernel<PW, DT><<<dim3(grid_of((int64_t)a.vocab_tiles * a.width_tiles)), dim3(PW::NW * 64), 0, stream>>>(
       a, 8);
-  a.width_tiles = (int32_t)ceil_div(a.width, PH::MT);
+  a.width_tiles = (int32_t)p.width_tiles;
+  static_assert(PH::NT == PZ::NT, "one number of rows a tile");
+  // at most max(slots, tiles) workgroups, whatever the count of listed rows
   if (a.rows > 0)
-    loss_dhidden_product_kernel<PH, DT><<<dim3(grid_of(a.width_tiles * ceil_div(a.rows, PH::NT)), (unsigned)p.splits),
-                                          dim3(PH::NW * 64), 0, stream>>>(a, 4, (int)p.span);
+    loss_dhidden_product_kernel<PH, DT><<<dim3(grid_of(max64(p.width_tiles * p.row_tiles, p.slots))),
+                                          dim3(PH::NW * 64), 0, stream>>>(a, 4);
 }
 
 template <int DT>
@@ -461,11 +482,7 @@ int run_backward(LossArgs a, const BackwardPlan& p, const Weight& w, char* ws, h
   typedef Tiles<DT, false, false> Z;
   typedef Tiles<DT, true, true> W;
   typedef Tiles<DT, true, false> H;
-  loss_rows_kernel<true><<<dim3(1), dim3(1024), 0, stream>>>(a, (LossMeta*)ws, (int32_t*)(ws + p.index),
-                                                             (int32_t*)(ws + p.position));
-  if (a.rows > 0)
-    loss_pack_kernel<true><<<dim3((unsigned)min64(a.rows, 8192)), dim3(256), 0, stream>>>(
-        a, (const int32_t*)(ws + p.position), (uint16_t*)(ws + p.packed));
+  launch_pack<true>(a, ws, p.index, p.packed, stream);
   for (int64_t i = 0; i < p.pieces; ++i) {
     take_piece(a, w, i * p.piece, p.piece, stream);
     a.first_piece = i == 0;
@@ -477,7 +494,7 @@ int run_backward(LossArgs a, const BackwardPlan& p, const Weight& w, char* ws, h
     }
   }
   if (a.sum && a.rows > 0)
-    loss_dhidden_kernel<DT><<<dim3((unsigned)min64(a.rows, 8192)), dim3(256), 0, stream>>>(a);
+    loss_dhidden_kernel<DT><<<dim3((unsigned)min64(a.rows, 8192)), dim3(256), 0, stream>>>(a, (int)logit_rows(p.tile));
   return check_launch("cross entropy gradient kernel");
 }
 
@@ -579,8 +596,11 @@ int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const floa
   a.dhidden_stride = dhidden_row_stride;
   a.dweight = (uint16_t*)dweight;
   a.dweight_stride = dweight_row_stride;
-  a.sum = p.pieces * p.splits > 1 ? (float*)(ws + p.sum) : nullptr;
-  a.splits = (int32_t)p.splits;
+  a.sum = p.shares ? (float*)(ws + p.sum) : nullptr;
+  a.piece_size = (int32_t)p.piece;
+  a.width_tiles = (int32_t)p.width_tiles;
+  a.slots = (int32_t)p.slots;
+  a.most_splits = (int32_t)p.most_splits;
   const Weight w{(const uint16_t*)weight, weight_row_stride, in_place ? nullptr : (uint16_t*)(ws + p.weight)};
   return dtype == HPRMS_DTYPE_BF16 ? run_backward<HPRMS_DTYPE_BF16>(a, p, w, ws, stream)
                                    : run_backward<HPRMS_DTYPE_FP16>(a, p, w, ws, stream);
