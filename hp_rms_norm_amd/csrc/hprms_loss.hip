@@ -29,25 +29,54 @@ __device__ __forceinline__ int block_count(int v, int* lds) {
 template <bool GRAD>
 __global__ __launch_bounds__(256) void loss_pack_kernel(LossArgs a, LossMeta* meta, int32_t* index, uint16_t* packed) {
   __shared__ int lds[4];
+  __shared__ int64_t list[256];
   const int32_t r0 = blockIdx.x * a.pack_rows, r1 = min(r0 + a.pack_rows, a.rows);
   int n = 0;
   for (int32_t r = threadIdx.x; r < r0; r += 256) n += a.target[r] != a.ignore_index;
   int32_t at = block_count(n, lds);
-  for (int32_t row = r0; row < r1; ++row) {
-    if (a.target[row] == a.ignore_index) {
-      if constexpr (GRAD) {
-        for (int32_t i = threadIdx.x; i < a.width; i += 256) a.dhidden[(int64_t)row * a.dhidden_stride + i] = 0;
-      } else if (threadIdx.x == 0) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int32_t chunks = a.packed_width / 8;
+  // up to 256 rows at a time: their places, then their 16-byte chunks in one run
+  for (int32_t first = r0; first < r1; first += 256) {
+    const int32_t row = first + threadIdx.x, some = min(256, r1 - first);
+    const bool in = threadIdx.x < some;
+    const bool keep = in && a.target[row] != a.ignore_index;
+    const uint64_t mask = __ballot(keep);
+    if (lane == 0) lds[wave] = __popcll(mask);
+    __syncthreads();
+    int before = __popcll(mask & ((uint64_t(1) << lane) - 1)), kept = 0;
+    for (int i = 0; i < 4; ++i) {
+      if (i < wave) before += lds[i];
+      kept += lds[i];
+    }
+    if (keep) {
+      list[before] = row;
+      index[at + before] = row;
+    } else if (in) {
+      list[some - 1 - (threadIdx.x - before)] = row;  // the others from the end
+      if constexpr (!GRAD) {
         a.loss[row] = 0.0f;
         a.lse[row] = 0.0f;
       }
-      continue;
     }
-    if (threadIdx.x == 0) index[at] = row;
-    const uint16_t* from = a.hidden + (int64_t)row * a.hidden_stride;
-    uint16_t* to = packed + (int64_t)at * a.packed_width;
-    for (int32_t i = threadIdx.x * 8; i < a.packed_width; i += 256 * 8) *(u32x4*)(to + i) = load_some(from + i, a.width - i);
-    ++at;
+    __syncthreads();
+    constexpr int U = 8;  // loads on their way at once
+    for (int32_t e = threadIdx.x; e < kept * chunks; e += 256 * U) {
+      u32x4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int32_t x = min(e + u * 256, kept * chunks - 1), r = x / chunks, i = (x - r * chunks) * 8;
+        v[u] = load_some(a.hidden + list[r] * a.hidden_stride + i, a.width - i);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)  // the listed rows lie side by side
+        if (e + u * 256 < kept * chunks) *(u32x4*)(packed + (int64_t)at * a.packed_width + (e + u * 256) * 8) = v[u];
+    }
+    if constexpr (GRAD)
+      for (int32_t r = kept; r < some; ++r)
+        for (int32_t i = threadIdx.x; i < a.width; i += 256) a.dhidden[list[r] * a.dhidden_stride + i] = 0;
+    at += kept;
+    __syncthreads();
   }
   if (r1 == a.rows && threadIdx.x == 0) meta->count = at;
   if constexpr (GRAD) {
@@ -63,16 +92,18 @@ __global__ __launch_bounds__(256) void loss_pack_kernel(LossArgs a, LossMeta* me
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = __float_as_int(top);
     __syncthreads();
     for (int i = 0; i < 4; ++i) top = fmaxf(top, __int_as_float(lds[i]));
-    // 2^e <= top < 2^(e + 1); the scale brings it to [2^14, 2^15)
-    float scale = 1.0f;
+    // top = m 2^e: the scale is 2^(14 - e) / m (the exponent up to 126, so that it is finite)
+    float scale = 1.0f, unscale = 1.0f;
     if (top > 0.0f) {
-      int e = 14 - ((int)(__float_as_uint(top) >> 23) - 127);  // subnormals count as 2^-127
-      e = e > 126 ? 126 : e < -112 ? -112 : e;
-      scale = __uint_as_float((uint32_t)(e + 127) << 23);
+      const uint32_t bits = __float_as_uint(top);
+      const float m = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+      const int e = max((int)(bits >> 23) - 127, -112);
+      scale = ldexpf(1.0f / m, 14 - e);
+      unscale = ldexpf(m, e - 14);
     }
     if (threadIdx.x == 0) {
       meta->scale = scale;
-      meta->unscale = 1.0f / scale;
+      meta->unscale = unscale;
     }
   }
 }
@@ -388,7 +419,7 @@ struct Tiles {
   typedef Product<DT, 128, 16, 4, 1, 64, 4, AKO, BKO> T16;
   typedef Product<DT, 128, 64, 4, 1, 64, 3, AKO, BKO> T64;
   typedef Product<DT, 256, 128, 4, 2, 32, 3, AKO, BKO> T128;
-  typedef Product<DT, 256, 256, 4, 2, 32, 4, AKO, BKO> T256;
+  typedef RingProduct<DT, AKO, BKO> T256;
 };
 
 // workgroups of `tiles` tiles, for tile_of

@@ -250,4 +250,157 @@ struct Product {
   }
 };
 
+// The 256 x 256 tile of 8 waves (4 x 2, 64 x 128 each).
+//
+// LDS holds 10 chunks of 16 KB.  A slice of 64 summed entries is 4 of them, two
+// of A and two of B: 128 rows of 64 entries each (k contiguous) or all 256
+// rows' 32 entries (k outer), so that a load instruction takes whole 128-byte
+// lines (8 rows of 128 bytes, or 2 of 512).  Chunk c of the product lies at
+// place c mod 10: while slice t is in use, the four places that slice t - 1
+// left take B of slice t + 1 and A of slice t + 2.
+//
+// The waves of the second half (w + 4 shares a SIMD with w) run one phase
+// behind those of the first; the workgroup's barrier ends every phase, and a
+// phase is either the fragment reads of half a slice and 4 loads, or that
+// half's products, so each SIMD's matrix core works for one wave while the
+// other's fragments arrive.
+template <int DT, bool AKO_, bool BKO_>
+struct RingProduct {
+  static constexpr int MT = 256, NT = 256, WM = 4, WN = 2, NW = 8, MI = 4, NI = 8;
+  static constexpr bool AKO = AKO_, BKO = BKO_;
+  static constexpr int CHUNK = 16384, PLACES = 10;
+  static constexpr int LDS_BYTES = CHUNK * PLACES;
+
+  // Byte offset from the operand's slice of what lane `lane` loads in load j (0
+  // ... 15) of chunk q (0, 1); *k: the first of its entries (k contiguous).
+  template <bool KO>
+  __device__ static __forceinline__ uint32_t load_offset(int q, int j, int lane, int32_t stride, int* k) {
+    if constexpr (!KO) {
+      const int r = j * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
+      *k = c * 8;
+      return ((uint32_t)(q * 128 + r) * (uint32_t)stride + c * 8) * 2;
+    } else {
+      const int kr = j * 2 + (lane >> 5), p = lane & 31;
+      const int u = (p >> 1) ^ ((kr & 3) | (kr >> 1 & 4));
+      *k = 0;
+      return ((uint32_t)(q * 32 + kr) * (uint32_t)stride + u * 16 + (p & 1) * 8) * 2;
+    }
+  }
+
+  // The fragment of rows r0 ... r0 + 15 (of the tile) and entries kk * 32 ... +
+  // 31 of a slice whose first chunk of the operand lies at place `at`.
+  template <bool KO>
+  __device__ static __forceinline__ u32x4 fragment(lds_u16* chunk, int r0, int kk, int lane) {
+    if constexpr (!KO) {
+      const int r = (r0 & 127) + (lane & 15), c = kk * 4 + (lane >> 4);
+      return *(__attribute__((address_space(3))) u32x4*)(chunk + r * 64 + (c ^ (r & 7)) * 8);
+    } else {
+      const int k = (lane >> 4) * 8 + ((lane & 15) >> 2);
+      const int u = (r0 / 16) ^ ((k & 3) | (k >> 1 & 4));
+      lds_u16* p = chunk + k * 256 + u * 16 + (lane & 3) * 4;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * 256));
+      const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
+      return u32x4{l[0], l[1], h[0], h[1]};
+    }
+  }
+
+  static constexpr int wait_code(int vm) { return (vm & 15) | (vm >> 4) << 14 | 0x70; }  // vmcnt(vm) lgkmcnt(0)
+
+  __device__ static __forceinline__ void phase_end() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+  }
+
+  // one operand's way through its slices
+  template <bool KO>
+  struct Stream {
+    const char* base;
+    int64_t bytes, step;
+    int32_t left;  // entries of k from the next slice on
+    uint32_t off[4];
+    int k[4];
+    __device__ __forceinline__ Stream(const Operand& o, int32_t depth, int wave, int lane)
+        : base((const char*)o.base), bytes(o.bytes), step(KO ? (int64_t)o.stride * 128 : 128), left(depth) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) off[i] = load_offset<KO>(i >> 1, (i & 1) * 8 + wave, lane, o.stride, &k[i]);
+    }
+    // the next slice's two chunks to places p and p + 1; past the last slice nothing is in range
+    __device__ __forceinline__ void load(lds_u16* lds, int p, int wave) {
+      const int64_t n = left <= 0 || bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes;
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(base, (uint32_t)n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (__attribute__((address_space(3))) void*)(lds + (p + (i >> 1)) * (CHUNK / 2) + ((i & 1) * 8 + wave) * 512),
+            16, !KO && k[i] >= left ? kOOB : off[i], 0, 0, 0);
+      base += step;
+      bytes -= step;
+      left -= 64;
+    }
+  };
+
+  // acc <- A . B^T over k in [0, depth).
+  __device__ static __forceinline__ void run(const Operand& a, const Operand& b, int32_t depth, uint16_t* lds_generic,
+                                             f32x4 (&acc)[MI][NI]) {
+    lds_u16* lds = (lds_u16*)lds_generic;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const bool late = wave >= NW / 2;
+    Stream<AKO> sa(a, depth, wave, lane);
+    Stream<BKO> sb(b, depth, wave, lane);
+    const int32_t slices = (depth + 63) / 64;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    sa.load(lds, 0, wave);
+    sb.load(lds, 2, wave);
+    sa.load(lds, 4, wave);
+    __builtin_amdgcn_s_waitcnt(wait_code(4));
+    phase_end();
+    if (late) phase_end();
+    int p = 0;  // place of the slice's first chunk: always even, and its 4 chunks wrap in pairs
+    for (int32_t t = 0; t < slices; ++t) {
+      const int pb = p + 2 >= PLACES ? p + 2 - PLACES : p + 2;
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        u32x4 fa[MI], fb[NI];
+        lds_u16* ca = lds + (p + (AKO ? kk : wm >> 1)) * (CHUNK / 2);
+        lds_u16* cb = lds + (pb + (BKO ? kk : wn)) * (CHUNK / 2);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[i] = fragment<AKO>(ca, (wm * MI + i) * 16, kk, lane);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) fb[j] = fragment<BKO>(cb, (wn * NI + j) * 16, kk, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        if (kk == 0) {
+          sb.load(lds, p + 6 >= PLACES ? p + 6 - PLACES : p + 6, wave);
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the fragments are here
+        } else {
+          sa.load(lds, p + 8 >= PLACES ? p + 8 - PLACES : p + 8, wave);
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_s_waitcnt(wait_code(4));  // ... and all of slice t + 1
+        }
+        phase_end();
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<DT>(fa[i], fb[j], acc[i][j]);
+        __builtin_amdgcn_s_setprio(0);
+        phase_end();
+      }
+      p = p + 4 >= PLACES ? p + 4 - PLACES : p + 4;
+    }
+    if (!late) phase_end();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(wait_code(0));  // LDS is free again behind the next barrier
+  }
+};
+
 }  // namespace hprms

@@ -11,7 +11,7 @@ K(n) = 2 (n / 32 + 32).
         exponentials (3 e each for the exponential and the sum's step)
   loss  the two together
   gradient entries, exactly d = (p - onehot) g: rounding to 16 bits u |d|; p's
-        own error p (2 dz + 2^-16); with the largest |g| scaled into [2^14, 2^15),
+        own error p (2 dz + 2^-16); with the largest |g| scaled to 2^14,
         in float16 half the smallest subnormal, 2^-25 2^-14 max|g|; and 2^-126 |g|
         where p lies below binary32's normal numbers (its exponential may be 0:
         at a logit 88 under the row's lse p is 2^-127, and exact p goes down to
