@@ -24,9 +24,18 @@ namespace {
 
 // 16 bytes at any 2-byte boundary (gfx950 runs global accesses unaligned)
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ u32x4 load_vec(const uint16_t* p) { return *(const u32x4_a2*)p; }
-__device__ __forceinline__ void store_vec(uint16_t* p, u32x4 v) { *(u32x4_a2*)p = v; }
+// the row tensors are touched once
+template <bool NT>
+__device__ __forceinline__ u32x4 load_once(const uint16_t* p) {
+  if constexpr (NT)
+    return __builtin_nontemporal_load((const u32x4_a2*)p);
+  else
+    return load_vec(p);
+}
+__device__ __forceinline__ void store_once(uint16_t* p, u32x4 v) { __builtin_nontemporal_store(v, (u32x4_a2*)p); }
 
 struct NormGradArgs {
   uint16_t* dinput;
@@ -70,7 +79,7 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float* lds) {
 // last whole vector holds the row's last 8 elements, of which only those that
 // no whole vector holds count in the sums (the others are stored twice, with
 // the same bits).
-template <int DT, int LPR, int VPL, int BLOCK, bool RES>
+template <int DT, int LPR, int VPL, int BLOCK, bool AHEAD, bool RES, bool NT>
 __global__ __launch_bounds__(BLOCK) void norm_grad_kernel(NormGradArgs a) {
   using F = Fmt<DT>;
   constexpr int RPB = BLOCK / LPR;
@@ -82,9 +91,14 @@ __global__ __launch_bounds__(BLOCK) void norm_grad_kernel(NormGradArgs a) {
   int off[VPL];
   bool on[VPL];
   u32x4 w[VPL];
+  // at 4 vectors a lane of 1024 the registers do not hold the sums as well (74-92
+  // spilled): they lie in LDS, each lane's own
+  constexpr bool LACC = VPL >= 4;
+  __shared__ f32x4 lacc[LACC ? VPL * 2 : 1][LACC ? BLOCK : 1];
   float acc[VPL][8];
 #pragma unroll
   for (int k = 0; k < VPL; ++k) {
+    if constexpr (LACC) lacc[2 * k][threadIdx.x] = lacc[2 * k + 1][threadIdx.x] = f32x4{0, 0, 0, 0};
     const int v = k * LPR + lane;
     on[k] = v < slots;
     off[k] = v < nvec ? v * 8 : a.hidden - 8;
@@ -94,21 +108,34 @@ __global__ __launch_bounds__(BLOCK) void norm_grad_kernel(NormGradArgs a) {
   }
   // this lane's last slot is the row's tail vector: its first `dup` elements are a whole vector's too
   const int dup = tail ? 8 - tail : 0;
+  // the next rows' loads are issued before this row's sums are joined
+  u32x4 nx[VPL], nd[VPL], nr[VPL];
+  auto load_row = [&](int64_t row) {
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      nx[k] = nd[k] = nr[k] = u32x4{0, 0, 0, 0};
+      if (row < a.rows && on[k]) {
+        nx[k] = load_once<NT>(a.input + row * a.input_stride + off[k]);
+        nd[k] = load_once<NT>(a.dout + row * a.dout_stride + off[k]);
+        if constexpr (RES) nr[k] = load_once<NT>(a.dresidual + row * a.dresidual_stride + off[k]);
+      }
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  load_row((int64_t)blockIdx.x * RPB + sub);
   int phase = 0;
-  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.rows; row0 += (int64_t)gridDim.x * RPB) {
+  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.rows; row0 += step) {
     const int64_t row = row0 + sub;
     const bool live = RPB == 1 || row < a.rows;
     u32x4 x[VPL], d[VPL], r[VPL];
     float ss = 0.0f, gs = 0.0f;
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
-      x[k] = d[k] = r[k] = u32x4{0, 0, 0, 0};
-      if (live && on[k]) {
-        x[k] = load_vec(a.input + row * a.input_stride + off[k]);
-        d[k] = load_vec(a.dout + row * a.dout_stride + off[k]);
-        if constexpr (RES) r[k] = load_vec(a.dresidual + row * a.dresidual_stride + off[k]);
-      }
+      x[k] = nx[k];
+      d[k] = nd[k];
+      r[k] = nr[k];
     }
+    if constexpr (AHEAD) load_row(row + step);
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
       const int skip = tail && k * LPR + lane == nvec ? dup : 0;
@@ -127,22 +154,33 @@ __global__ __launch_bounds__(BLOCK) void norm_grad_kernel(NormGradArgs a) {
     phase ^= 1;
     const float rstd = 1.0f / sqrtf(ss / (float)a.hidden + a.eps);
     const float c = rstd * rstd * (rstd * (gs / (float)a.hidden));
+    // unpacked again below: the compiler would keep 24 floats a vector over the sums otherwise
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) asm volatile("" : "+v"(x[k]), "+v"(d[k]), "+v"(w[k]));
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
-      float o[8];
+      float o[8], dn[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float xf = j & 1 ? F::hi(x[k][j / 2]) : F::lo(x[k][j / 2]);
         const float df = j & 1 ? F::hi(d[k][j / 2]) : F::lo(d[k][j / 2]);
         const float wf = j & 1 ? F::hi(w[k][j / 2]) : F::lo(w[k][j / 2]);
-        if (live) acc[k][j] += df * (xf * rstd);
+        dn[j] = live ? df * (xf * rstd) : 0.0f;
         o[j] = rstd * (df * wf) - xf * c;
         if constexpr (RES) o[j] += j & 1 ? F::hi(r[k][j / 2]) : F::lo(r[k][j / 2]);
       }
+      if constexpr (LACC) {
+        lacc[2 * k][threadIdx.x] += f32x4{dn[0], dn[1], dn[2], dn[3]};
+        lacc[2 * k + 1][threadIdx.x] += f32x4{dn[4], dn[5], dn[6], dn[7]};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[k][j] += dn[j];
+      }
       if (live && on[k])
-        store_vec(a.dinput + row * a.dinput_stride + off[k],
-                  u32x4{F::pack(o[0], o[1]), F::pack(o[2], o[3]), F::pack(o[4], o[5]), F::pack(o[6], o[7])});
+        store_once(a.dinput + row * a.dinput_stride + off[k],
+                   u32x4{F::pack(o[0], o[1]), F::pack(o[2], o[3]), F::pack(o[4], o[5]), F::pack(o[6], o[7])});
     }
+    if constexpr (!AHEAD) load_row(row + step);
   }
   // one row of partial sums per workgroup; the row groups' columns are added through LDS
   __shared__ float cols[RPB > 1 ? RPB * LPR * 8 : 1];
@@ -158,6 +196,10 @@ __global__ __launch_bounds__(BLOCK) void norm_grad_kernel(NormGradArgs a) {
         for (int j = 0; j < 8; ++j)
           for (int i = 1; i < RPB; ++i) acc[k][j] += cols[(i * LPR + lane) * 8 + j];
       }
+    }
+    if constexpr (LACC) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[k][j] = lacc[2 * k + j / 4][threadIdx.x][j % 4];
     }
     const int skip = tail && k * LPR + lane == nvec ? dup : 0;
     if (sub == 0 && on[k]) {
@@ -225,8 +267,18 @@ __global__ __launch_bounds__(1024) void norm_grad_weight_kernel(const float* par
   const int c = threadIdx.x & 31, p = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 32 + c;
   float acc = 0.0f;
-  if (col < hidden)
-    for (int64_t i = p; i < parts; i += 32) acc += partial[i * hidden + col];
+  if (col < hidden) {
+    constexpr int U = 8;  // loads on their way at once
+    int64_t i = p;
+    for (; i + 32 * (U - 1) < parts; i += 32 * U) {
+      float v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = partial[(i + 32 * u) * hidden + col];
+#pragma unroll
+      for (int u = 0; u < U; ++u) acc += v[u];
+    }
+    for (; i < parts; i += 32) acc += partial[i * hidden + col];
+  }
   lds[p][c] = acc;
   __syncthreads();
   if (p == 0 && col < hidden) {
@@ -243,23 +295,30 @@ __global__ __launch_bounds__(1024) void norm_grad_weight_kernel(const float* par
 constexpr int64_t kMaxGradHidden = int64_t(1) << 24;
 constexpr int64_t kVectorHidden = 32768;  // the register-resident kernels' widest rows
 
+// Shapes by width.  One workgroup of 512 lanes per CU with the next rows' loads
+// ahead measured best from 1K to 8K: each further workgroup adds a row of
+// partial sums, which is written and read again (8192 x 4096 bf16 with
+// dresidual: 256 x 2 lanes x vectors at one workgroup of 512 per CU 48.1 us, at
+// two of 256 50.6, at four 60; 2999 x 4097 fp16: 256 x 3 20.4, at two of 256
+// 22.6).  Narrow rows have little to sum and take four of 256 (131072 x 128:
+// 20.4 us).  From 8K the registers do not hold a second row (2048 x 16384: 61.7
+// us, with the loads ahead 69).
 struct Shape {
-  int lpr, vpl, block;
+  int lpr, vpl, block, per_cu;
 };
 
-// Lanes and vectors per lane by width.
 Shape shape_of(int64_t hidden) {
   const int64_t slots = (hidden + 7) / 8;
-  if (slots <= 16) return {16, 1, 256};
-  if (slots <= 32) return {32, 1, 256};
-  if (slots <= 64) return {64, 1, 256};
-  if (slots <= 128) return {64, 2, 256};
-  if (slots <= 256) return {128, 2, 256};
-  if (slots <= 512) return {256, 2, 256};
-  if (slots <= 768) return {256, 3, 256};
-  if (slots <= 1024) return {512, 2, 512};
-  if (slots <= 2048) return {1024, 2, 1024};
-  return {1024, 4, 1024};
+  if (slots <= 16) return {16, 1, 256, 4};
+  if (slots <= 32) return {32, 1, 256, 4};
+  if (slots <= 64) return {64, 1, 256, 4};
+  if (slots <= 128) return {64, 2, 512, 1};
+  if (slots <= 256) return {128, 2, 512, 1};
+  if (slots <= 512) return {256, 2, 512, 1};
+  if (slots <= 768) return {256, 3, 512, 1};
+  if (slots <= 1024) return {512, 2, 512, 1};
+  if (slots <= 2048) return {1024, 2, 1024, 1};
+  return {1024, 4, 1024, 1};
 }
 
 bool is_general(int64_t hidden) { return hidden < 8 || hidden > kVectorHidden; }
@@ -270,7 +329,7 @@ int64_t grid_of(int64_t rows, int64_t hidden) {
   const Shape s = shape_of(hidden);
   const int64_t rpb = s.block / s.lpr;
   const int64_t groups = (rows + rpb - 1) / rpb;
-  const int64_t most = (int64_t)current_cus() * (1024 / s.block);
+  const int64_t most = (int64_t)current_cus() * s.per_cu;
   return groups < most ? groups : most;
 }
 
@@ -280,12 +339,26 @@ int64_t workspace_bytes(int64_t rows, int64_t hidden) {
   return n;
 }
 
-template <int DT, int LPR, int VPL, int BLOCK>
+// Past 2^24 elements the row tensors exceed what the caches keep between
+// operators, and non-temporal loads measured faster (8192 x 4096: 48.1 us
+// against 52.8 with plain ones); below, plain ones (2999 x 4096: 19.8 against
+// 21.5).  Stores are non-temporal throughout (0-10% faster).
+constexpr int64_t kCachedElements = int64_t(1) << 24;
+
+template <int DT, int LPR, int VPL, int BLOCK, bool AHEAD = true>
 void launch_rows(const NormGradArgs& a, int64_t grid, hipStream_t stream) {
-  if (a.dresidual)
-    norm_grad_kernel<DT, LPR, VPL, BLOCK, true><<<dim3((unsigned)grid), dim3(BLOCK), 0, stream>>>(a);
-  else
-    norm_grad_kernel<DT, LPR, VPL, BLOCK, false><<<dim3((unsigned)grid), dim3(BLOCK), 0, stream>>>(a);
+  const dim3 g((unsigned)grid), b(BLOCK);
+  if (a.rows > kCachedElements / a.hidden) {
+    if (a.dresidual)
+      norm_grad_kernel<DT, LPR, VPL, BLOCK, AHEAD, true, true><<<g, b, 0, stream>>>(a);
+    else
+      norm_grad_kernel<DT, LPR, VPL, BLOCK, AHEAD, false, true><<<g, b, 0, stream>>>(a);
+  } else {
+    if (a.dresidual)
+      norm_grad_kernel<DT, LPR, VPL, BLOCK, AHEAD, true, false><<<g, b, 0, stream>>>(a);
+    else
+      norm_grad_kernel<DT, LPR, VPL, BLOCK, AHEAD, false, false><<<g, b, 0, stream>>>(a);
+  }
 }
 
 template <int DT>
@@ -304,13 +377,13 @@ int launch_all(const NormGradArgs& a, int64_t grid, void* dweight, int dweight_d
       case 16 * 8 + 1: launch_rows<DT, 16, 1, 256>(a, grid, stream); break;
       case 32 * 8 + 1: launch_rows<DT, 32, 1, 256>(a, grid, stream); break;
       case 64 * 8 + 1: launch_rows<DT, 64, 1, 256>(a, grid, stream); break;
-      case 64 * 8 + 2: launch_rows<DT, 64, 2, 256>(a, grid, stream); break;
-      case 128 * 8 + 2: launch_rows<DT, 128, 2, 256>(a, grid, stream); break;
-      case 256 * 8 + 2: launch_rows<DT, 256, 2, 256>(a, grid, stream); break;
-      case 256 * 8 + 3: launch_rows<DT, 256, 3, 256>(a, grid, stream); break;
+      case 64 * 8 + 2: launch_rows<DT, 64, 2, 512>(a, grid, stream); break;
+      case 128 * 8 + 2: launch_rows<DT, 128, 2, 512>(a, grid, stream); break;
+      case 256 * 8 + 2: launch_rows<DT, 256, 2, 512>(a, grid, stream); break;
+      case 256 * 8 + 3: launch_rows<DT, 256, 3, 512>(a, grid, stream); break;
       case 512 * 8 + 2: launch_rows<DT, 512, 2, 512>(a, grid, stream); break;
-      case 1024 * 8 + 2: launch_rows<DT, 1024, 2, 1024>(a, grid, stream); break;
-      default: launch_rows<DT, 1024, 4, 1024>(a, grid, stream); break;
+      case 1024 * 8 + 2: launch_rows<DT, 1024, 2, 1024, false>(a, grid, stream); break;
+      default: launch_rows<DT, 1024, 4, 1024, false>(a, grid, stream); break;
     }
   }
   const dim3 wgrid((unsigned)((a.hidden + 31) / 32));
