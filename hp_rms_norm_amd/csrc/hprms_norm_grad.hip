@@ -295,14 +295,16 @@ __global__ __launch_bounds__(1024) void norm_grad_weight_kernel(const float* par
 constexpr int64_t kMaxGradHidden = int64_t(1) << 24;
 constexpr int64_t kVectorHidden = 32768;  // the register-resident kernels' widest rows
 
-// Shapes by width.  One workgroup of 512 lanes per CU with the next rows' loads
-// ahead measured best from 1K to 8K: each further workgroup adds a row of
-// partial sums, which is written and read again (8192 x 4096 bf16 with
-// dresidual: 256 x 2 lanes x vectors at one workgroup of 512 per CU 48.1 us, at
-// two of 256 50.6, at four 60; 2999 x 4097 fp16: 256 x 3 20.4, at two of 256
-// 22.6).  Narrow rows have little to sum and take four of 256 (131072 x 128:
-// 20.4 us).  From 8K the registers do not hold a second row (2048 x 16384: 61.7
-// us, with the loads ahead 69).
+// Shapes by width, with the next rows' loads ahead up to 8K.  Few workgroups a
+// CU measured best: each adds a row of partial sums, which is written and read
+// again.  Times of the row kernel on bf16 rows with dresidual, lanes x vectors
+// x workgroup x workgroups per CU (268 MB each): 8192 x 4096 512 x 1 x 512 x 2
+// 52.5 us, 256 x 2 x 512 x 1 57.4, 256 x 2 x 256 x 3 56.4; 16384 x 2048 128 x 2
+// x 256 x 2 48.9, 128 x 2 x 512 x 1 57.0; 32768 x 1024 64 x 2 x 512 x 1 49.5,
+// 64 x 2 x 256 x 4 51.6; 4096 x 8192 512 x 2 x 512 x 1 59.4, two of them 60.3.
+// Odd rows of 4097 and rows of 128 are within 2% between their candidates.  From
+// 8K the registers do not hold a second row (2048 x 16384: 61.1 us, 62.9 with
+// the loads ahead).
 struct Shape {
   int lpr, vpl, block, per_cu;
 };
@@ -313,8 +315,8 @@ Shape shape_of(int64_t hidden) {
   if (slots <= 32) return {32, 1, 256, 4};
   if (slots <= 64) return {64, 1, 256, 4};
   if (slots <= 128) return {64, 2, 512, 1};
-  if (slots <= 256) return {128, 2, 512, 1};
-  if (slots <= 512) return {256, 2, 512, 1};
+  if (slots <= 256) return {128, 2, 256, 2};
+  if (slots <= 512) return {512, 1, 512, 2};
   if (slots <= 768) return {256, 3, 512, 1};
   if (slots <= 1024) return {512, 2, 512, 1};
   if (slots <= 2048) return {1024, 2, 1024, 1};
@@ -378,8 +380,8 @@ int launch_all(const NormGradArgs& a, int64_t grid, void* dweight, int dweight_d
       case 32 * 8 + 1: launch_rows<DT, 32, 1, 256>(a, grid, stream); break;
       case 64 * 8 + 1: launch_rows<DT, 64, 1, 256>(a, grid, stream); break;
       case 64 * 8 + 2: launch_rows<DT, 64, 2, 512>(a, grid, stream); break;
-      case 128 * 8 + 2: launch_rows<DT, 128, 2, 512>(a, grid, stream); break;
-      case 256 * 8 + 2: launch_rows<DT, 256, 2, 512>(a, grid, stream); break;
+      case 128 * 8 + 2: launch_rows<DT, 128, 2, 256>(a, grid, stream); break;
+      case 512 * 8 + 1: launch_rows<DT, 512, 1, 512>(a, grid, stream); break;
       case 256 * 8 + 3: launch_rows<DT, 256, 3, 512>(a, grid, stream); break;
       case 512 * 8 + 2: launch_rows<DT, 512, 2, 512>(a, grid, stream); break;
       case 1024 * 8 + 2: launch_rows<DT, 1024, 2, 1024, false>(a, grid, stream); break;
