@@ -47,9 +47,14 @@ void rows_of(const at::Tensor& t, int64_t hidden, int64_t* rows, int64_t* stride
     *stride = 0;
     return;
   }
-  at::Tensor flat = t.view({-1, hidden});
-  *rows = flat.size(0);
-  *stride = *rows <= 1 ? hidden : flat.stride(0);
+  if (t.dim() == 2) {  // nothing to flatten
+    *rows = t.size(0);
+    *stride = *rows <= 1 ? hidden : t.stride(0);
+  } else {
+    const at::Tensor flat = t.view({-1, hidden});
+    *rows = flat.size(0);
+    *stride = *rows <= 1 ? hidden : flat.stride(0);
+  }
   TORCH_CHECK(*stride >= hidden, "rows of the tensor overlap (row stride ", *stride, " < hidden ", hidden, ")");
 }
 
@@ -797,6 +802,7 @@ void check_outs(at::TensorList outs, at::TensorList grads) {
 // gradient other than its own (which it must then be, exactly).
 void check_out_spans(const at::Tensor& norm, at::TensorList outs, at::TensorList grads) {
   std::vector<Span> spans;
+  spans.reserve(outs.size());
   for (size_t i = 0; i < outs.size(); ++i)
     if (outs[i].numel() > 0) spans.push_back(span_of(outs[i], i));
   std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.first < b.first; });
@@ -824,6 +830,11 @@ struct GradArrays {
 
 GradArrays grad_arrays(at::TensorList outs, at::TensorList grads) {
   GradArrays a;
+  a.outs.reserve(outs.size());
+  a.out_dtypes.reserve(outs.size());
+  a.grads.reserve(grads.size());
+  a.dtypes.reserve(grads.size());
+  a.counts.reserve(grads.size());
   for (const at::Tensor& t : outs) {
     a.outs.push_back(t.data_ptr());
     a.out_dtypes.push_back(grad_dtype_code(t));

@@ -151,7 +151,7 @@ def test_workspace_sizes():
                  lambda: abi.linear_cross_entropy_workspace((1 << 22) + 1, 64, 64),
                  lambda: abi.linear_cross_entropy_backward_workspace(1, 64, 0),
                  lambda: abi.linear_cross_entropy_backward_workspace(1, 64, (1 << 28) + 1),
-                 lambda: abi.grad_norm_workspace([-1]), lambda: abi.grad_norm_workspace([1 << 49])):
+                 lambda: abi.grad_norm_workspace([-1]), lambda: abi.grad_norm_workspace([1 << 43])):
         with pytest.raises(abi.HprmsError):
             call()
 
