@@ -61,11 +61,13 @@ struct LossArgs {
   const LossMeta* meta;
   const int32_t* index;     // the row of each list position
   const uint16_t* packed;   // the listed rows' hidden values, [rows, packed_width], zeros past width
+  const uint16_t* turned;   // gradient: packed transposed, [packed_width, turned_stride], zeros from count to a multiple of 64
   int64_t hidden_stride;
   int64_t ignore_index;
   int32_t weight_stride;    // elements, a multiple of 8
   int32_t weight_width;     // readable elements of a weight row, a multiple of 8
   int32_t packed_width;     // a multiple of 64
+  int32_t turned_stride;    // rows rounded up to a multiple of 64
   int32_t rows;             // of the call
   int32_t width;            // elements of a hidden row
   int32_t vocab;

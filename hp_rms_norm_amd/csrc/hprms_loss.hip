@@ -108,8 +108,36 @@ __global__ __launch_bounds__(256) void loss_pack_kernel(LossArgs a, LossMeta* me
   }
 }
 
-// The same for a piece of a weight whose rows the products cannot read in
-// place (an odd width, stride or alignment).
+// The packed rows transposed, for dweight: its products sum over the rows, and
+// of two operands that lie across the sum (k outer) one costs the matrix cores
+// 7% (4096 x 32768 x 4096 tiles: 1340 TFLOP/s with hidden k contiguous, 1250
+// with both k outer).  One workgroup turns 64 x 64.
+__global__ __launch_bounds__(256) void loss_turn_kernel(LossArgs a, uint16_t* turned) {
+  __shared__ uint16_t tile[64][66];  // 33 banks a row
+  const int count = a.meta->count;
+  const int n0 = blockIdx.x * 64, w0 = blockIdx.y * 64;
+  if (n0 >= count) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = threadIdx.x + i * 256, n = e >> 3, w = (e & 7) * 8;
+    u32x4 v = {0, 0, 0, 0};
+    if (n0 + n < count) v = *(const u32x4*)(a.packed + (int64_t)(n0 + n) * a.packed_width + w0 + w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *(uint32_t*)&tile[n][w + 2 * j] = v[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = threadIdx.x + i * 256, w = e >> 3, n = (e & 7) * 8;
+    u32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = tile[n + 2 * j][w] | (uint32_t)tile[n + 2 * j + 1][w] << 16;
+    *(u32x4*)(turned + (int64_t)(w0 + w) * a.turned_stride + n0 + n) = v;
+  }
+}
+
+// A piece of a weight whose rows the products cannot read in place (an odd
+// width, stride or alignment), packed likewise.
 __global__ __launch_bounds__(256) void loss_pack_weight_kernel(const uint16_t* weight, int64_t stride, int32_t rows,
                                                                int32_t width, int32_t packed_width,
                                                                uint16_t* packed) {
@@ -134,8 +162,9 @@ __device__ __forceinline__ Operand weight_columns(const LossArgs& a, int k, int 
 __device__ __forceinline__ Operand packed_rows(const LossArgs& a, int n, int count) {
   return {a.packed + (int64_t)n * a.packed_width, (int64_t)(count - n) * a.packed_width * 2, a.packed_width};
 }
-__device__ __forceinline__ Operand packed_columns(const LossArgs& a, int m, int count) {
-  return {a.packed + m, ((int64_t)count * a.packed_width - m) * 2, a.packed_width};
+__device__ __forceinline__ Operand turned_rows(const LossArgs& a, int m) {
+  return {a.turned + (int64_t)m * a.turned_stride, (int64_t)(a.packed_width - m) * a.turned_stride * 2,
+          a.turned_stride};
 }
 __device__ __forceinline__ Operand dz_rows(const LossArgs& a, int n, int v, int count) {
   return {a.dz + (int64_t)n * a.dz_stride + v, ((int64_t)(count - n) * a.dz_stride - v) * 2, a.dz_stride};
@@ -227,7 +256,8 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dweight_kernel(LossArgs a, in
   if (!tile_of(blockIdx.x, a.width_tiles, a.vocab_tiles, group, &m, &n)) return;
   const int m0 = m * P::MT, n0 = n * P::NT;
   f32x4 acc[P::MI][P::NI];
-  P::run(packed_columns(a, m0, count), dz_columns(a, n0, count), count, lds, acc);
+  // `turned` holds zeros past the count, so the depth may be rounded up to whole chunks
+  P::run(turned_rows(a, m0), dz_columns(a, n0, count), (count + 7) & ~7, lds, acc);
   const int wave = threadIdx.x >> 6;
   dweight_epilogue<DT, P::MI, P::NI>(a, acc, m0, n0, wave / P::WN, wave % P::WN);
 }
@@ -358,7 +388,8 @@ ForwardPlan forward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_pla
 }
 
 struct BackwardPlan {
-  int64_t index, packed, weight, dz, sum, total;
+  int64_t index, packed, turned, weight, dz, sum, total;
+  int64_t turned_stride;
   int64_t piece, pieces, dz_rows, row_tiles, width_tiles, slots, most_splits;
   bool shares;
   LogitTile tile;
@@ -382,7 +413,9 @@ BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_p
   const bool shares = p.pieces > 1 || p.most_splits > 1;
   p.index = 256;
   p.packed = p.index + round_up(rows * 4, 256);
-  p.weight = p.packed + rows * packed_width_of(width) * 2;
+  p.turned_stride = round_up(rows, 64);
+  p.turned = p.packed + round_up(rows * packed_width_of(width) * 2, 256);
+  p.weight = p.turned + p.turned_stride * packed_width_of(width) * 2;
   p.dz = p.weight + (in_place ? 0 : p.piece * packed_width_of(width) * 2);
   p.sum = p.dz + p.dz_rows * p.piece * 2;
   p.total = p.sum + (shares ? sum_rows * packed_width_of(width) * 4 : 0);
@@ -414,12 +447,15 @@ int check_workspace(const void* workspace, int64_t size, int64_t need) {
   return HPRMS_OK;
 }
 
-template <int DT, bool AKO, bool BKO>
+// Tiles of the products over the hidden index (z: A and B k contiguous) and over
+// the vocabulary (dhidden: A k outer).  An operand that lies k outer takes more
+// LDS instructions a fragment, so its side of a wave's part is the short one.
+template <int DT, bool AKO>
 struct Tiles {
-  typedef Product<DT, 128, 16, 4, 1, 64, 4, AKO, BKO> T16;
-  typedef Product<DT, 128, 64, 4, 1, 64, 3, AKO, BKO> T64;
-  typedef Product<DT, 256, 128, 4, 2, 32, 3, AKO, BKO> T128;
-  typedef RingProduct<DT, AKO, BKO> T256;
+  typedef Product<DT, 128, 16, 4, 1, 64, 4, AKO, false> T16;
+  typedef Product<DT, 128, 64, 4, 1, 64, 3, AKO, false> T64;
+  typedef Product<DT, 256, 128, 4, 2, 32, 3, AKO, false> T128;
+  typedef RingProduct<DT, AKO, false, AKO ? 4 : 2> T256;
 };
 
 // workgroups of `tiles` tiles, for tile_of
@@ -466,7 +502,7 @@ void launch_pack(LossArgs& a, char* ws, int64_t index, int64_t packed, hipStream
 
 template <int DT>
 int run_forward(LossArgs a, const ForwardPlan& p, const Weight& w, char* ws, hipStream_t stream) {
-  typedef Tiles<DT, false, false> T;
+  typedef Tiles<DT, false> T;
   launch_pack<false>(a, ws, p.index, p.packed, stream);
   for (int64_t from = 0; from < a.rows; from += p.rows_at) {
     a.row_from = (int32_t)from;
@@ -510,18 +546,21 @@ void launch_piece(LossArgs a, const BackwardPlan& p, hipStream_t stream) {
 
 template <int DT>
 int run_backward(LossArgs a, const BackwardPlan& p, const Weight& w, char* ws, hipStream_t stream) {
-  typedef Tiles<DT, false, false> Z;
-  typedef Tiles<DT, true, true> W;
-  typedef Tiles<DT, true, false> H;
+  typedef Tiles<DT, false> Z;
+  typedef RingProduct<DT, false, true, 2> W;  // dweight
+  typedef Tiles<DT, true> H;
   launch_pack<true>(a, ws, p.index, p.packed, stream);
+  if (a.rows > 0)
+    loss_turn_kernel<<<dim3((unsigned)ceil_div(a.rows, 64), (unsigned)(a.packed_width / 64)), dim3(256), 0, stream>>>(
+        a, (uint16_t*)(ws + p.turned));
   for (int64_t i = 0; i < p.pieces; ++i) {
     take_piece(a, w, i * p.piece, p.piece, stream);
     a.first_piece = i == 0;
     switch (p.tile) {
-      case kTile16: launch_piece<typename Z::T16, typename W::T256, typename H::T16, DT>(a, p, stream); break;
-      case kTile64: launch_piece<typename Z::T64, typename W::T256, typename H::T64, DT>(a, p, stream); break;
-      case kTile128: launch_piece<typename Z::T128, typename W::T256, typename H::T128, DT>(a, p, stream); break;
-      case kTile256: launch_piece<typename Z::T256, typename W::T256, typename H::T256, DT>(a, p, stream); break;
+      case kTile16: launch_piece<typename Z::T16, W, typename H::T16, DT>(a, p, stream); break;
+      case kTile64: launch_piece<typename Z::T64, W, typename H::T64, DT>(a, p, stream); break;
+      case kTile128: launch_piece<typename Z::T128, W, typename H::T128, DT>(a, p, stream); break;
+      case kTile256: launch_piece<typename Z::T256, W, typename H::T256, DT>(a, p, stream); break;
     }
   }
   if (a.sum && a.rows > 0)
@@ -627,6 +666,8 @@ int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const floa
   a.dhidden_stride = dhidden_row_stride;
   a.dweight = (uint16_t*)dweight;
   a.dweight_stride = dweight_row_stride;
+  a.turned = (const uint16_t*)(ws + p.turned);
+  a.turned_stride = (int32_t)p.turned_stride;
   a.sum = p.shares ? (float*)(ws + p.sum) : nullptr;
   a.piece_size = (int32_t)p.piece;
   a.width_tiles = (int32_t)p.width_tiles;

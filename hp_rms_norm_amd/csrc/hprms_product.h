@@ -250,7 +250,7 @@ struct Product {
   }
 };
 
-// The 256 x 256 tile of 8 waves (4 x 2, 64 x 128 each).
+// The 256 x 256 tile of 8 waves: WM x 8 / WM, 64 x 128 or 128 x 64 each.
 //
 // LDS holds 10 chunks of 16 KB.  A slice of 64 summed entries is 4 of them, two
 // of A and two of B: 128 rows of 64 entries each (k contiguous) or all 256
@@ -264,9 +264,9 @@ struct Product {
 // phase is either the fragment reads of half a slice and 4 loads, or that
 // half's products, so each SIMD's matrix core works for one wave while the
 // other's fragments arrive.
-template <int DT, bool AKO_, bool BKO_>
+template <int DT, bool AKO_, bool BKO_, int WM_ = 4>
 struct RingProduct {
-  static constexpr int MT = 256, NT = 256, WM = 4, WN = 2, NW = 8, MI = 4, NI = 8;
+  static constexpr int MT = 256, NT = 256, NW = 8, WM = WM_, WN = NW / WM, MI = MT / WM / 16, NI = NT / WN / 16;
   static constexpr bool AKO = AKO_, BKO = BKO_;
   static constexpr int CHUNK = 16384, PLACES = 10;
   static constexpr int LDS_BYTES = CHUNK * PLACES;
@@ -370,8 +370,8 @@ struct RingProduct {
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         u32x4 fa[MI], fb[NI];
-        lds_u16* ca = lds + (p + (AKO ? kk : wm >> 1)) * (CHUNK / 2);
-        lds_u16* cb = lds + (pb + (BKO ? kk : wn)) * (CHUNK / 2);
+        lds_u16* ca = lds + (p + (AKO ? kk : wm * MI >> 3)) * (CHUNK / 2);
+        lds_u16* cb = lds + (pb + (BKO ? kk : wn * NI >> 3)) * (CHUNK / 2);
 #pragma unroll
         for (int i = 0; i < MI; ++i) fa[i] = fragment<AKO>(ca, (wm * MI + i) * 16, kk, lane);
 #pragma unroll
