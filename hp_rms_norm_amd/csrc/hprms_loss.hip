@@ -235,6 +235,10 @@ __global__ __launch_bounds__(256) void loss_join_kernel(LossArgs a, int32_t tile
 }
 
 // ---- gradient ---------------------------------------------------------------------------
+// LDS of a kernel whose tile leaves through it
+template <class P>
+constexpr int kLdsOut = P::LDS_BYTES > kTileOutBytes<P> ? P::LDS_BYTES : kTileOutBytes<P>;
+
 template <class P, int DT>
 __global__ __launch_bounds__(P::NW * 64) void loss_dz_kernel(LossArgs a, int group) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[P::LDS_BYTES / 2];
@@ -244,13 +248,12 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dz_kernel(LossArgs a, int gro
   const int m0 = m * P::MT, n0 = n * P::NT;
   f32x4 acc[P::MI][P::NI];
   P::run(weight_rows(a, m0), packed_rows(a, n0, count), a.width, lds, acc);
-  const int wave = threadIdx.x >> 6;
-  dz_epilogue<DT, P::MI, P::NI>(a, acc, m0, n0, wave / P::WN, wave % P::WN, count);
+  dz_epilogue<P, DT>(a, acc, m0, n0, count);
 }
 
 template <class P, int DT>
 __global__ __launch_bounds__(P::NW * 64) void loss_dweight_kernel(LossArgs a, int group) {
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[P::LDS_BYTES / 2];
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[kLdsOut<P> / 2];
   const int count = a.meta->count;
   int m, n;
   if (!tile_of(blockIdx.x, a.width_tiles, a.vocab_tiles, group, &m, &n)) return;
@@ -258,8 +261,7 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dweight_kernel(LossArgs a, in
   f32x4 acc[P::MI][P::NI];
   // `turned` holds zeros past the count, so the depth may be rounded up to whole chunks
   P::run(turned_rows(a, m0), dz_columns(a, n0, count), (count + 7) & ~7, lds, acc);
-  const int wave = threadIdx.x >> 6;
-  dweight_epilogue<DT, P::MI, P::NI>(a, acc, m0, n0, wave / P::WN, wave % P::WN);
+  dweight_epilogue<P, DT>(a, acc, m0, n0, lds);
 }
 
 // Splits of a piece's vocabulary over workgroups, where dhidden has fewer tiles
@@ -301,16 +303,27 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dhidden_product_kernel(LossAr
 template <int DT>
 __global__ __launch_bounds__(256) void loss_dhidden_kernel(LossArgs a, int tile_rows) {
   const int count = a.meta->count;
+
   const int splits = splits_of(a.width_tiles * ((count + tile_rows - 1) / tile_rows), a.slots, a.piece_size,
                                a.most_splits).count;
   const float unscale = a.meta->unscale;
+  const int64_t step = (int64_t)count * a.packed_width;
   for (int32_t n = blockIdx.x; n < count; n += gridDim.x) {
-    uint16_t* to = a.dhidden + (int64_t)a.index[n] * a.dhidden_stride;
-    for (int32_t i = threadIdx.x * 4; i < a.width; i += 256 * 4) {
+    for (int32_t i = (blockIdx.y * 256 + threadIdx.x) * 4; i < a.width; i += gridDim.y * 1024) {
+      const float* from = a.sum + (int64_t)n * a.packed_width + i;
       f32x4 d = {0, 0, 0, 0};
-      for (int s = 0; s < splits; ++s) d += *(const f32x4*)(a.sum + ((int64_t)s * count + n) * a.packed_width + i);
+      constexpr int U = 8;  // loads on their way at once
+      int s = 0;
+      for (; s + U <= splits; s += U) {
+        f32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = *(const f32x4*)(from + (s + u) * step);
+#pragma unroll
+        for (int u = 0; u < U; ++u) d += v[u];
+      }
+      for (; s < splits; ++s) d += *(const f32x4*)(from + s * step);
       const float o[4] = {d[0] * unscale, d[1] * unscale, d[2] * unscale, d[3] * unscale};
-      store_four<DT>(to + i, o, a.width - i);
+      store_four<DT>(a.dhidden + (int64_t)a.index[n] * a.dhidden_stride + i, o, a.width - i);
     }
   }
 }
@@ -321,6 +334,7 @@ constexpr int64_t kMaxLossWidth = int64_t(1) << 20;
 constexpr int64_t kMaxVocab = int64_t(1) << 28;
 constexpr int64_t kRowChunk = 16384;  // list positions per forward launch: bounds the partial sums
 constexpr int64_t kPieceElements = int64_t(1) << 27;  // of dz, and of a packed weight, per piece: 256 MiB
+constexpr int64_t kFewRows = 128;
 constexpr int64_t kPieceUnit = 256;   // pieces are whole tiles of every kernel
 // a tile's 256 rows at this stride stay within a buffer access's 31-bit offset
 constexpr int64_t kMaxWeightStride = int64_t(1) << 21;
@@ -362,7 +376,7 @@ LogitTile logit_tile(int64_t rows) {
 }
 int64_t logit_vocab_rows(LogitTile t) { return t <= kTile64 ? 128 : 256; }
 // hidden elements of a dhidden tile
-int64_t hidden_tile_width(LogitTile t) { return t <= kTile64 ? 128 : 256; }
+int64_t hidden_tile_width(LogitTile t) { return 256; }
 int64_t logit_rows(LogitTile t) { return t == kTile16 ? 16 : t == kTile64 ? 64 : t == kTile128 ? 128 : 256; }
 
 // Offsets of the workspace's parts, bytes.
@@ -452,8 +466,10 @@ int check_workspace(const void* workspace, int64_t size, int64_t need) {
 // LDS instructions a fragment, so its side of a wave's part is the short one.
 template <int DT, bool AKO>
 struct Tiles {
-  typedef Product<DT, 128, 16, 4, 1, 64, 4, AKO, false> T16;
-  typedef Product<DT, 128, 64, 4, 1, 64, 3, AKO, false> T64;
+  typedef std::conditional_t<AKO, Product<DT, 256, 16, 4, 1, 32, 4, true, false>,
+                             Product<DT, 128, 16, 4, 1, 64, 4, false, false>> T16;
+  typedef std::conditional_t<AKO, Product<DT, 256, 64, 4, 1, 32, 4, true, false>,
+                             Product<DT, 128, 64, 4, 1, 64, 3, false, false>> T64;
   typedef Product<DT, 256, 128, 4, 2, 32, 3, AKO, false> T128;
   typedef RingProduct<DT, AKO, false, AKO ? 4 : 2> T256;
 };
@@ -548,6 +564,7 @@ template <int DT>
 int run_backward(LossArgs a, const BackwardPlan& p, const Weight& w, char* ws, hipStream_t stream) {
   typedef Tiles<DT, false> Z;
   typedef RingProduct<DT, false, true, 2> W;  // dweight
+  typedef Product<DT, 128, 128, 2, 2, 32, 2, false, true> WS;  // ... of few rows
   typedef Tiles<DT, true> H;
   launch_pack<true>(a, ws, p.index, p.packed, stream);
   if (a.rows > 0)
@@ -557,14 +574,20 @@ int run_backward(LossArgs a, const BackwardPlan& p, const Weight& w, char* ws, h
     take_piece(a, w, i * p.piece, p.piece, stream);
     a.first_piece = i == 0;
     switch (p.tile) {
-      case kTile16: launch_piece<typename Z::T16, W, typename H::T16, DT>(a, p, stream); break;
-      case kTile64: launch_piece<typename Z::T64, W, typename H::T64, DT>(a, p, stream); break;
-      case kTile128: launch_piece<typename Z::T128, W, typename H::T128, DT>(a, p, stream); break;
-      case kTile256: launch_piece<typename Z::T256, W, typename H::T256, DT>(a, p, stream); break;
+      case kTile16: launch_piece<typename Z::T16, WS, typename H::T16, DT>(a, p, stream); break;
+      case kTile64: launch_piece<typename Z::T64, WS, typename H::T64, DT>(a, p, stream); break;
+      case kTile128: launch_piece<typename Z::T128, WS, typename H::T128, DT>(a, p, stream); break;
+      case kTile256:
+        if (a.rows <= kFewRows)
+          launch_piece<typename Z::T256, WS, typename H::T256, DT>(a, p, stream);
+        else
+          launch_piece<typename Z::T256, W, typename H::T256, DT>(a, p, stream);
+        break;
     }
   }
   if (a.sum && a.rows > 0)
-    loss_dhidden_kernel<DT><<<dim3((unsigned)min64(a.rows, 8192)), dim3(256), 0, stream>>>(a, (int)logit_rows(p.tile));
+    loss_dhidden_kernel<DT><<<dim3((unsigned)min64(a.rows, 4096), a.rows < 1024 ? (unsigned)ceil_div(a.width, 1024) : 1u),
+                              dim3(256), 0, stream>>>(a, (int)logit_rows(p.tile));
   return check_launch("cross entropy gradient kernel");
 }
 
