@@ -334,7 +334,7 @@ constexpr int64_t kMaxLossWidth = int64_t(1) << 20;
 constexpr int64_t kMaxVocab = int64_t(1) << 28;
 constexpr int64_t kRowChunk = 16384;  // list positions per forward launch: bounds the partial sums
 constexpr int64_t kPieceElements = int64_t(1) << 27;  // of dz, and of a packed weight, per piece: 256 MiB
-constexpr int64_t kFewRows = 128;
+constexpr int64_t kHiddenTile = 256;  // hidden elements of a dhidden tile
 constexpr int64_t kPieceUnit = 256;   // pieces are whole tiles of every kernel
 // a tile's 256 rows at this stride stay within a buffer access's 31-bit offset
 constexpr int64_t kMaxWeightStride = int64_t(1) << 21;
@@ -369,15 +369,18 @@ int64_t packed_piece(int64_t width, int64_t vocab) {
   return min64(p, round_up(vocab, kPieceUnit));
 }
 
-// Tiles of z by the number of rows: vocabulary rows and list positions.
-enum LogitTile { kTile16, kTile64, kTile128, kTile256 };
-LogitTile logit_tile(int64_t rows) {
-  return rows <= 16 ? kTile16 : rows <= 64 ? kTile64 : rows <= 128 ? kTile128 : kTile256;
+// Tiles of z, vocabulary rows x list positions, by the number of rows: 128 x 16
+// and 128 x 64 (the weight's bytes bound these: 131072 x 4096 in 185 us, 5.8
+// TB/s, up to 64 rows), 256 x 128, 256 x 256; and 128 x 128 where 256 x 256 would
+// leave half of the CUs without a tile.
+enum LogitTile { kTile16, kTile64, kTileSmall, kTile128, kTile256 };
+LogitTile logit_tile(int64_t rows, int64_t vocab) {
+  if (rows <= 64) return rows <= 16 ? kTile16 : kTile64;
+  if (2 * ceil_div(vocab, 256) * ceil_div(rows, 256) <= current_cus()) return kTileSmall;
+  return rows <= 128 ? kTile128 : kTile256;
 }
-int64_t logit_vocab_rows(LogitTile t) { return t <= kTile64 ? 128 : 256; }
-// hidden elements of a dhidden tile
-int64_t hidden_tile_width(LogitTile t) { return 256; }
-int64_t logit_rows(LogitTile t) { return t == kTile16 ? 16 : t == kTile64 ? 64 : t == kTile128 ? 128 : 256; }
+int64_t logit_vocab_rows(LogitTile t) { return t <= kTileSmall ? 128 : 256; }
+int64_t logit_rows(LogitTile t) { return t == kTile16 ? 16 : t == kTile64 ? 64 : t == kTile256 ? 256 : 128; }
 
 // Offsets of the workspace's parts, bytes.
 struct ForwardPlan {
@@ -388,7 +391,7 @@ struct ForwardPlan {
 
 ForwardPlan forward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_place) {
   ForwardPlan p;
-  p.tile = logit_tile(rows);
+  p.tile = logit_tile(rows, vocab);
   p.rows_at = min64(rows, kRowChunk);
   p.piece = in_place ? round_up(vocab, kPieceUnit) : packed_piece(width, vocab);
   p.tiles = ceil_div(vocab, logit_vocab_rows(p.tile));
@@ -411,13 +414,13 @@ struct BackwardPlan {
 
 BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_place) {
   BackwardPlan p;
-  p.tile = logit_tile(rows);
+  p.tile = logit_tile(rows, vocab);
   p.dz_rows = round_up(max64(rows, 1), logit_rows(p.tile));
   p.piece = max64(kPieceElements / max64(p.dz_rows, 256) / kPieceUnit * kPieceUnit, 4 * kPieceUnit);
   p.piece = min64(p.piece, round_up(vocab, kPieceUnit));
   if (!in_place) p.piece = min64(p.piece, packed_piece(width, vocab));
   p.pieces = ceil_div(vocab, p.piece);
-  p.width_tiles = ceil_div(width, hidden_tile_width(p.tile));
+  p.width_tiles = ceil_div(width, kHiddenTile);
   const int64_t row_tiles = ceil_div(max64(rows, 1), logit_rows(p.tile));
   p.slots = (int64_t)current_cus() * (p.tile == kTile256 ? 1 : 2);
   // with fewer listed rows there are more splits, of fewer rows: count * splits
@@ -470,6 +473,7 @@ struct Tiles {
                              Product<DT, 128, 16, 4, 1, 64, 4, false, false>> T16;
   typedef std::conditional_t<AKO, Product<DT, 256, 64, 4, 1, 32, 4, true, false>,
                              Product<DT, 128, 64, 4, 1, 64, 3, false, false>> T64;
+  typedef Product<DT, 128, 128, 2, 2, 64, 2, false, false> Small;
   typedef Product<DT, 256, 128, 4, 2, 32, 3, AKO, false> T128;
   typedef RingProduct<DT, AKO, false, AKO ? 4 : 2> T256;
 };
@@ -529,6 +533,7 @@ int run_forward(LossArgs a, const ForwardPlan& p, const Weight& w, char* ws, hip
       switch (p.tile) {
         case kTile16: launch_forward<typename T::T16, DT>(a, here, stream); break;
         case kTile64: launch_forward<typename T::T64, DT>(a, here, stream); break;
+        case kTileSmall: launch_forward<typename T::Small, DT>(a, here, stream); break;
         case kTile128: launch_forward<typename T::T128, DT>(a, here, stream); break;
         case kTile256: launch_forward<typename T::T256, DT>(a, here, stream); break;
       }
@@ -573,12 +578,22 @@ int run_backward(LossArgs a, const BackwardPlan& p, const Weight& w, char* ws, h
   for (int64_t i = 0; i < p.pieces; ++i) {
     take_piece(a, w, i * p.piece, p.piece, stream);
     a.first_piece = i == 0;
+    // dweight in tiles of 128 x 128, which run four to a CU, where the sums over
+    // the rows are short (128 rows of 131072 x 4096: 331 us, 256 x 256 430) or 256
+    // x 256 would leave CUs without a tile
+    const bool few = a.rows <= 128 || ceil_div(a.piece, 256) * ceil_div(a.width, 256) < current_cus();
     switch (p.tile) {
       case kTile16: launch_piece<typename Z::T16, WS, typename H::T16, DT>(a, p, stream); break;
       case kTile64: launch_piece<typename Z::T64, WS, typename H::T64, DT>(a, p, stream); break;
+      case kTileSmall:
+        if (few)
+          launch_piece<typename Z::Small, WS, typename H::T128, DT>(a, p, stream);
+        else
+          launch_piece<typename Z::Small, W, typename H::T128, DT>(a, p, stream);
+        break;
       case kTile128: launch_piece<typename Z::T128, WS, typename H::T128, DT>(a, p, stream); break;
       case kTile256:
-        if (a.rows <= kFewRows)
+        if (few)
           launch_piece<typename Z::T256, WS, typename H::T256, DT>(a, p, stream);
         else
           launch_piece<typename Z::T256, W, typename H::T256, DT>(a, p, stream);
