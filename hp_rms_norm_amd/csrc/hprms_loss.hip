@@ -372,9 +372,12 @@ int64_t packed_piece(int64_t width, int64_t vocab) {
 // Tiles of z, vocabulary rows x list positions, by the number of rows: 128 x 16
 // and 128 x 64 (the weight's bytes bound these: 131072 x 4096 in 185 us, 5.8
 // TB/s, up to 64 rows), 256 x 128, 256 x 256; and 128 x 128 where 256 x 256 would
-// leave half of the CUs without a tile.
+// leave half of the CUs without a tile.  In batch-invariant mode always 256 x
+// 256: a row's logits are summed alike in every shape, but its exponentials
+// tile by tile, so the shape shows in the last bits of its lse.
 enum LogitTile { kTile16, kTile64, kTileSmall, kTile128, kTile256 };
 LogitTile logit_tile(int64_t rows, int64_t vocab) {
+  if (hprms_batch_invariant()) return kTile256;
   if (rows <= 64) return rows <= 16 ? kTile16 : kTile64;
   if (2 * ceil_div(vocab, 256) * ceil_div(rows, 256) <= current_cus()) return kTileSmall;
   return rows <= 128 ? kTile128 : kTile256;
@@ -539,7 +542,7 @@ int run_forward(LossArgs a, const ForwardPlan& p, const Weight& w, char* ws, hip
       }
       a.tile_from += (int32_t)ceil_div(a.piece, logit_vocab_rows(p.tile));
     }
-    if (here < 256)
+    if (here < 256 && !hprms_batch_invariant())
       loss_join_kernel<1><<<dim3((unsigned)here), dim3(256), 0, stream>>>(a, (int32_t)p.tiles);
     else
       loss_join_kernel<16><<<dim3((unsigned)((here + 15) / 16)), dim3(256), 0, stream>>>(a, (int32_t)p.tiles);

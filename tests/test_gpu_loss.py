@@ -290,3 +290,49 @@ def test_two_streams_at_once(ops):
     torch.cuda.synchronize()
     for i, g in enumerate(got):
         assert all(torch.equal(x, y) for x, y in zip(g, want[i % 2]))
+
+
+def test_batch_invariant_mode_fixes_a_rows_bits(ops):
+    """With the mode on, a row's loss and lse are the same bits in calls of any
+    row count, at any place among the rows."""
+    h, w, t, _ = make(700, 192, 5000, torch.bfloat16, 17)
+    previous = ops.set_batch_invariant(True)
+    try:
+        loss, lse = ops.linear_cross_entropy(h, w, t)
+        check_forward(loss, lse, h, w, t)
+        for rows in (1, 5, 16, 17, 64, 65, 128, 129, 300):
+            for at in (0, 700 - rows):
+                a, b = ops.linear_cross_entropy(h[at:at + rows], w, t[at:at + rows])
+                assert torch.equal(a, loss[at:at + rows]) and torch.equal(b, lse[at:at + rows])
+        keep = torch.arange(700, device=DEV) % 3 == 0
+        a, b = ops.linear_cross_entropy(h, w, torch.where(keep, t, IGNORE))
+        assert torch.equal(a[keep], loss[keep]) and torch.equal(b[keep], lse[keep])
+    finally:
+        ops.set_batch_invariant(previous)
+
+
+SHAPES = [(12, 300, 700), (40, 512, 3000), (100, 264, 9000), (100, 128, 70000), (200, 128, 70000), (300, 384, 2000),
+          (900, 128, 70000)]
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", SHAPES)
+def test_every_tile_shape(ops, rows, hidden, vocab):
+    """Row counts and vocabularies on both sides of the tile rules, and counts
+    of listed rows below the call's rows (fewer row tiles, more splits)."""
+    for ignored in (0.0, 0.6):
+        run(ops, *make(rows, hidden, vocab, torch.bfloat16, rows + vocab, ignored))
+
+
+def test_weight_rows_in_a_wider_store_with_other_values_around(ops):
+    """What lies between and around the weight's rows is not part of it: NaN
+    there changes nothing (in place and packed)."""
+    for hidden, pad in ((96, 8), (104, 24), (64, 64), (100, 5)):
+        h, w, t, dloss = make(80, hidden, 513, torch.bfloat16, 18)
+        want = run(ops, h, w, t, dloss)
+        store = torch.full((515, hidden + pad), float("nan"), device=DEV, dtype=torch.bfloat16)
+        view = store[1:514, :hidden]
+        view.copy_(w)
+        loss, lse = ops.linear_cross_entropy(h, view, t)
+        dh, dw = ops.linear_cross_entropy_backward(dloss, h, view, t, lse)
+        assert torch.equal(loss, want[0]) and torch.equal(lse, want[1])
+        assert torch.equal(dh, want[2]) and torch.equal(dw, want[3])
