@@ -10,18 +10,22 @@
 
 namespace hprms {
 
+// Not exported: the product and the bench library, loaded into one process,
+// each keep their own.
+#define HPRMS_LOCAL __attribute__((visibility("hidden")))
+
 // A whole MI355X: what the row-count rules were measured on.
 constexpr int kRefCUs = 256;
 
 // Sets the calling thread's error text (hprms_last_error) and returns `code`.
-__attribute__((format(printf, 2, 3))) int fail(int code, const char* fmt, ...);
+HPRMS_LOCAL __attribute__((format(printf, 2, 3))) int fail(int code, const char* fmt, ...);
 
 // HPRMS_OK, or HPRMS_E_LAUNCH with the runtime's message about the last launch.
-int check_launch(const char* what);
+HPRMS_LOCAL int check_launch(const char* what);
 
 // CUs of the current device; 256 when there is no device to ask (a launch
 // would then fail and report why)
-int current_cus();
+HPRMS_LOCAL int current_cus();
 
 // No buffer on any GPU spans more bytes (virtual addresses have at most 57
 // bits), and under this bound the kernels' 64-bit row offsets cannot overflow.

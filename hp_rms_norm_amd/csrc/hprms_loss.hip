@@ -303,7 +303,6 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dhidden_product_kernel(LossAr
 template <int DT>
 __global__ __launch_bounds__(256) void loss_dhidden_kernel(LossArgs a, int tile_rows) {
   const int count = a.meta->count;
-
   const int splits = splits_of(a.width_tiles * ((count + tile_rows - 1) / tile_rows), a.slots, a.piece_size,
                                a.most_splits).count;
   const float unscale = a.meta->unscale;

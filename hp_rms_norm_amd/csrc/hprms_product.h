@@ -34,6 +34,18 @@ struct Operand {
 
 typedef __attribute__((address_space(3))) uint16_t lds_u16;
 
+// vmcnt(vm) lgkmcnt(0): all but the last vm loads and every LDS read are done
+constexpr int wait_code(int vm) { return (vm & 15) | (vm >> 4) << 14 | 0x70; }
+
+// The workgroup's barrier, which neither memory accesses nor products pass.
+__device__ __forceinline__ void phase_end() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
 // A workgroup of WM x WN waves computes an MT x NT tile, each wave MI x NI
 // fragments of 16 x 16.  Slices of BK summed entries travel from memory to LDS
 // without registers (16 bytes a lane), ST slices deep; a slice's LDS rows are
@@ -47,16 +59,9 @@ typedef __attribute__((address_space(3))) uint16_t lds_u16;
 //     fragment is two transposing 8-byte reads a lane, which give each 16 lanes
 //     4 entries of 16 columns.
 //
-// With 8 waves (two to a SIMD: w and w + 4) the waves of the second half run
-// one phase behind those of the first: a phase is either a slice's fragment
-// reads and the loads of a later slice, or its products, and the workgroup's
-// barrier ends every phase, so each SIMD's matrix core works for one wave
-// while the other's fragments arrive.  Without that both waves of a SIMD wait
-// for LDS at the same time.  256 x 256 x 4096 products measured 1240 against
-// 1080 TFLOP/s (k contiguous), 1240 against 920 (both k outer) and at
-// 256 x 256 x 32768 1330 against 960 (A k outer); the clock falls from 2.2 to
-// 1.9-2.0 GHz under it, and a loop of nothing but these instructions reaches
-// 2080 TFLOP/s at 2.06 GHz.
+// With 8 waves the two halves of the workgroup run one phase apart, as in
+// RingProduct below (256 x 128 x 4096 tiles, two workgroups a CU: 999 TFLOP/s
+// against 985 without).
 template <int DT, int MT_, int NT_, int WM_, int WN_, int BK_, int ST_, bool AKO_, bool BKO_>
 struct Product {
   static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, BK = BK_, ST = ST_;
@@ -115,16 +120,6 @@ struct Product {
       const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
       return u32x4{l[0], l[1], h[0], h[1]};
     }
-  }
-
-  static constexpr int wait_code(int vm) { return (vm & 15) | (vm >> 4) << 14 | 0x70; }  // vmcnt(vm) lgkmcnt(0)
-
-  __device__ static __forceinline__ void phase_end() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
   }
 
   // Behind it every wave's share of the oldest of the ST - 1 slices on their
@@ -263,7 +258,24 @@ struct Product {
 // behind those of the first; the workgroup's barrier ends every phase, and a
 // phase is either the fragment reads of half a slice and 4 loads, or that
 // half's products, so each SIMD's matrix core works for one wave while the
-// other's fragments arrive.
+// other's fragments arrive.  Without that both waves of a SIMD wait for LDS at
+// the same time.
+//
+// 1.1 TFLOP of each kind, tiles in XCD-contiguous order, TFLOP/s (a library
+// product of the same sizes: 1450, 1100 and 1370):
+//
+//                                  32768 x 4096    4096 x 32768    4096 x 4096
+//                                  x 4096          x 4096          x 32768
+//   k of both operands contiguous  1380-1410
+//   k of B outer (k of both)                       1340 (1250)
+//   k of A outer                                                   1420
+//   64-byte rows a slice, 4 slices 1240            1240 (both)     1330
+//   the same without the phases    1080            920 (both)      960
+//
+// At 1.4 PFLOP/s a slice of 32 takes 1160-1180 cycles, of which the matrix cores
+// work 1024, and the clock falls from 2.4 to 1.7 GHz: power bounds it (a loop
+// of nothing but these instructions on random values reaches 2080 TFLOP/s at
+// 2.06 GHz; zeros run at 2.4 GHz).
 template <int DT, bool AKO_, bool BKO_, int WM_ = 4>
 struct RingProduct {
   static constexpr int MT = 256, NT = 256, NW = 8, WM = WM_, WN = NW / WM, MI = MT / WM / 16, NI = NT / WN / 16;
@@ -303,16 +315,6 @@ struct RingProduct {
       const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
       return u32x4{l[0], l[1], h[0], h[1]};
     }
-  }
-
-  static constexpr int wait_code(int vm) { return (vm & 15) | (vm >> 4) << 14 | 0x70; }  // vmcnt(vm) lgkmcnt(0)
-
-  __device__ static __forceinline__ void phase_end() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
   }
 
   // one operand's way through its slices

@@ -103,6 +103,44 @@ def test_large_and_tiny_values(ops):
     check_clipped(outs, grads, 1.0)
 
 
+def test_tensors_without_elements(ops):
+    empty = [torch.empty(0, device=DEV), torch.empty((3, 0), device=DEV, dtype=torch.bfloat16)]
+    assert float(ops.grad_norm(empty)) == 0.0 and float(ops.clip_grad_norm_(empty, 1.0)) == 0.0
+    grads = empty + make([10], [torch.float32], 2)
+    check_norm(ops.grad_norm(grads), grads)
+
+
+def test_shared_memory_is_refused_before_anything_is_written(ops):
+    base = make([100], [torch.float32], 2)[0]
+    before = base.clone()
+    for call in (lambda: ops.clip_grad_norm_([base, base], 0.1),
+                 lambda: ops.clip_grad_norm_([base[:60], base[40:]], 0.1),
+                 lambda: ops.clip_grad_norm_out([base[:50], torch.empty(50, device=DEV)], [base[50:], base[:50]], 0.1),
+                 lambda: ops.clip_grad_norm_out([base[1:51]], [base[:50]], 0.1)):
+        with pytest.raises(RuntimeError, match="share"):
+            call()
+    assert torch.equal(base, before)
+    # reading one tensor twice, into two others, is fine
+    outs = [torch.empty(100, device=DEV), torch.empty(100, device=DEV)]
+    ops.clip_grad_norm_out(outs, [base, base], 0.1)
+    check_clipped(outs, [base, base], 0.1)
+
+
+def test_a_list_past_the_folded_sums(ops):
+    """More than 2^25 elements: longer units, and the sums added by a kernel of
+    their own; in place and into other tensors, clipped and not."""
+    grads = make([(1 << 25) + 77, 12345, 1 << 20], [torch.bfloat16, torch.float32], 20)
+    norm = exact_norm(grads)
+    outs = [torch.empty_like(t) for t in grads]
+    check_norm(ops.clip_grad_norm_out(outs, grads, 0.25 * norm), grads)
+    check_clipped(outs, grads, 0.25 * norm)
+    before = [t.clone() for t in grads]
+    ops.clip_grad_norm_(grads, 2 * norm)
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    ops.clip_grad_norm_(grads, 0.25 * norm)
+    assert all(torch.equal(a, b) for a, b in zip(grads, outs))
+
+
 def test_not_finite(ops):
     for bad, factor in ((float("nan"), float("nan")), (float("inf"), 0.0)):
         grads = make([100, 100], [torch.float32], 8)

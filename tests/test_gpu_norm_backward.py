@@ -99,6 +99,33 @@ def test_strided_and_misaligned_rows(ops, hidden, pad, offset):
         assert not bool(store[:-1, hidden:].any())
 
 
+def test_another_stream_and_misplaced_outputs(ops):
+    x, dout, dres, w = make(300, 2048, torch.bfloat16, 4)
+    want = ops.rms_norm_backward(dout, x, w, EPS, dresidual=dres)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = ops.rms_norm_backward(dout, x, w, EPS, dresidual=dres)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    store = torch.zeros(300 * 2048 + 1, device=DEV, dtype=torch.bfloat16)
+    for dx, dw in ((store[1:].view(300, 2048), store[:2048]), (x, x[0]), (dout, w)):
+        with pytest.raises(RuntimeError):
+            ops.rms_norm_backward_out(dx, dw, dout, x, w, EPS)
+    shifted = torch.as_strided(dout, (299, 2048), (2048, 1), 2048)   # dout's rows, one further
+    with pytest.raises(RuntimeError):
+        ops.rms_norm_backward_out(shifted, torch.empty_like(w), dout[:299], x[:299], w, EPS)
+
+
+def test_past_the_cached_size(ops):
+    """More than 2^24 elements take the non-temporal loads: the same bits row by row."""
+    x, dout, dres, w = make(4200, 4096, torch.bfloat16, 6)
+    dx, dw = ops.rms_norm_backward(dout, x, w, EPS, dresidual=dres)
+    check(dx, dw, x, dout, dres, w)
+    part, _ = ops.rms_norm_backward(dout[4000:], x[4000:], w, EPS, dresidual=dres[4000:])
+    assert torch.equal(part, dx[4000:])
+
+
 @pytest.mark.parametrize("hidden", [9, 128, 4096, 4097, 40000])
 def test_in_place_on_each_row_tensor(ops, hidden):
     x, dout, dres, w = make(50, hidden, torch.bfloat16, 3)
