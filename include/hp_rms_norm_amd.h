@@ -383,9 +383,9 @@ int hprms_batch_invariant(void);
  * exactly; dweight is of dweight_dtype (dtype or HPRMS_DTYPE_FP32) and is
  * written, not added to (rows == 0 writes zeros).  The sums' order is fixed for
  * given sizes and CU count.  `workspace`: hprms_rmsnorm_backward_workspace()
- * bytes (a negative status for bad sizes) on the device, 16-byte aligned, free
- * again when the call has run on `stream`; calls that may run at the same time
- * need one each.  No counterpart in the reference, which has no gradients.
+ * bytes (a negative status for bad sizes; asked for with the same device
+ * current) on the device, 16-byte aligned, free again when the call has run on
+ * `stream`; calls that may run at the same time need one each.  No counterpart in the reference, which has no gradients.
  */
 int64_t hprms_rmsnorm_backward_workspace(int64_t rows, int64_t hidden);
 int hprms_rmsnorm_backward(void* dinput, void* dweight, const void* dout, const void* input, const void* weight,
