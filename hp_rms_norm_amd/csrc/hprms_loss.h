@@ -91,6 +91,8 @@ struct LossArgs {
   float* sum;               // [splits, count, packed_width] shares of dhidden, by list position; null: none
   int32_t first_piece;
   int32_t piece_size, slots, most_splits;  // see splits_of
+  float* weight_sum;        // [splits, piece rounded up to 128, packed_width] shares of dweight; null: none
+  int32_t weight_most;      // splits of dweight at most
   int32_t pack_rows;        // rows per workgroup of the packing kernel
 };
 
@@ -110,17 +112,27 @@ __device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2
 // vocabulary rows and the sum of exponentials relative to it.  A wave's 4 lanes
 // of a column join by swizzles, the WM waves stacked over the column through
 // LDS.  NaN logits leave the maximum and make the sum NaN.
+// `t`: the targets of this lane's columns, in the piece, or -1 (loaded before
+// the tile loop: two dependent loads that would stand at its end).
+template <int NI>
+__device__ __forceinline__ void load_targets(const LossArgs& a, int n0, int wn, int count, int (&t)[NI]) {
+#pragma unroll
+  for (int ni = 0; ni < NI; ++ni) {
+    const int n = n0 + (wn * NI + ni) * 16 + (threadIdx.x & 15);
+    const int64_t in = n < count ? a.target[a.index[n]] - a.piece_from : -1;
+    t[ni] = in >= 0 && in < a.piece ? (int)in : -1;
+  }
+}
+
 template <int MI, int NI, int WM, int WN>
-__device__ __forceinline__ void forward_epilogue(const LossArgs& a, const f32x4 (&acc)[MI][NI], int m0, int n0, int wm,
-                                                 int wn, int count, int tile, float2* lds) {
+__device__ __forceinline__ void forward_epilogue(const LossArgs& a, const f32x4 (&acc)[MI][NI], const int (&t)[NI],
+                                                 int m0, int n0, int wm, int wn, int count, int tile, float2* lds) {
   const int lane = threadIdx.x & 63;
   __syncthreads();  // the tile loop's LDS reads are over
 #pragma unroll
   for (int ni = 0; ni < NI; ++ni) {
     const int col = wn * NI * 16 + ni * 16 + (lane & 15);
     const int n = n0 + col;
-    const bool live = n < count;
-    const int64_t t = live ? a.target[a.index[n]] - a.piece_from : -1;  // in the piece
     float top = -__builtin_inff();
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi)
@@ -128,7 +140,7 @@ __device__ __forceinline__ void forward_epilogue(const LossArgs& a, const f32x4 
       for (int i = 0; i < 4; ++i) {
         const int v = m0 + (wm * MI + mi) * 16 + (lane >> 4) * 4 + i;  // in the piece
         if (v < a.piece) top = fmaxf(top, acc[mi][ni][i]);
-        if (v == t && v < a.piece) a.target_logit[n] = acc[mi][ni][i];
+        if (v == t[ni]) a.target_logit[n] = acc[mi][ni][i];
       }
     top = fmaxf(top, xor16(top));
     top = fmaxf(top, xor32(top));
@@ -199,28 +211,34 @@ __device__ __forceinline__ void tile_out(uint16_t* lds, int left, From&& from, T
 
 // The piece's dz of the tile, 0 where there is no row or no vocabulary entry.
 // A target outside [0, vocab) gives NaN.
-template <class P, int DT>
-__device__ __forceinline__ void dz_epilogue(const LossArgs& a, const f32x4 (&acc)[P::MI][P::NI], int m0, int n0,
-                                            int count) {
-  using F = Fmt<DT>;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / P::WN, wn = wave % P::WN;
-  const float scale = a.meta->scale;
+template <class P>
+struct DzColumns {  // of this lane's columns; loaded before the tile loop, as in the forward kernel
   float lse[P::NI], g[P::NI];
   int t[P::NI];  // the target in the piece, or -1
+  __device__ __forceinline__ void load(const LossArgs& a, int n0, int wn, int count) {
+    const float scale = a.meta->scale;
 #pragma unroll
-  for (int ni = 0; ni < P::NI; ++ni) {
-    const int n = n0 + (wn * P::NI + ni) * 16 + (lane & 15);
-    lse[ni] = g[ni] = 0.0f;
-    t[ni] = -1;
-    if (n < count) {
-      const int row = a.index[n];
-      const int64_t target = a.target[row];
-      lse[ni] = a.lse[row];
-      g[ni] = target >= 0 && target < a.vocab ? a.dloss[row] * scale : __builtin_nanf("");
-      const int64_t in = target - a.piece_from;
-      t[ni] = in >= 0 && in < a.piece ? (int)in : -1;
+    for (int ni = 0; ni < P::NI; ++ni) {
+      const int n = n0 + (wn * P::NI + ni) * 16 + (threadIdx.x & 15);
+      lse[ni] = g[ni] = 0.0f;
+      t[ni] = -1;
+      if (n < count) {
+        const int row = a.index[n];
+        const int64_t target = a.target[row];
+        lse[ni] = a.lse[row];
+        g[ni] = target >= 0 && target < a.vocab ? a.dloss[row] * scale : __builtin_nanf("");
+        const int64_t in = target - a.piece_from;
+        t[ni] = in >= 0 && in < a.piece ? (int)in : -1;
+      }
     }
   }
+};
+
+template <class P, int DT>
+__device__ __forceinline__ void dz_epilogue(const LossArgs& a, const f32x4 (&acc)[P::MI][P::NI], const DzColumns<P>& c,
+                                            int m0, int n0, int count) {
+  using F = Fmt<DT>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / P::WN, wn = wave % P::WN;
   // (through tile_out measured 3% slower here: 827 us against 802 for 4096 x 32768 x 4096)
 #pragma unroll
   for (int ni = 0; ni < P::NI; ++ni) {
@@ -232,8 +250,8 @@ __device__ __forceinline__ void dz_epilogue(const LossArgs& a, const f32x4 (&acc
       float d[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = exp_neg(acc[mi][ni][i] - lse[ni]);
-        d[i] = n < count && m + i < a.piece ? (m + i == t[ni] ? p - 1.0f : p) * g[ni] : 0.0f;
+        const float p = exp_neg(acc[mi][ni][i] - c.lse[ni]);
+        d[i] = n < count && m + i < a.piece ? (m + i == c.t[ni] ? p - 1.0f : p) * c.g[ni] : 0.0f;
       }
       *(u32x2*)(to + m) = u32x2{F::pack(d[0], d[1]), F::pack(d[2], d[3])};
     }

@@ -162,15 +162,15 @@ __device__ __forceinline__ Operand weight_columns(const LossArgs& a, int k, int 
 __device__ __forceinline__ Operand packed_rows(const LossArgs& a, int n, int count) {
   return {a.packed + (int64_t)n * a.packed_width, (int64_t)(count - n) * a.packed_width * 2, a.packed_width};
 }
-__device__ __forceinline__ Operand turned_rows(const LossArgs& a, int m) {
-  return {a.turned + (int64_t)m * a.turned_stride, (int64_t)(a.packed_width - m) * a.turned_stride * 2,
+__device__ __forceinline__ Operand turned_rows(const LossArgs& a, int m, int k) {
+  return {a.turned + (int64_t)m * a.turned_stride + k, ((int64_t)(a.packed_width - m) * a.turned_stride - k) * 2,
           a.turned_stride};
 }
 __device__ __forceinline__ Operand dz_rows(const LossArgs& a, int n, int v, int count) {
   return {a.dz + (int64_t)n * a.dz_stride + v, ((int64_t)(count - n) * a.dz_stride - v) * 2, a.dz_stride};
 }
-__device__ __forceinline__ Operand dz_columns(const LossArgs& a, int v, int count) {
-  return {a.dz + v, ((int64_t)count * a.dz_stride - v) * 2, a.dz_stride};
+__device__ __forceinline__ Operand dz_columns(const LossArgs& a, int v, int k, int count) {
+  return {a.dz + (int64_t)k * a.dz_stride + v, ((int64_t)(count - k) * a.dz_stride - v) * 2, a.dz_stride};
 }
 
 // ---- forward ----------------------------------------------------------------------------
@@ -182,11 +182,13 @@ __global__ __launch_bounds__(P::NW * 64) void loss_forward_kernel(LossArgs a, in
   int m, n;
   if (here <= 0 || !tile_of(blockIdx.x, a.vocab_tiles, (here + P::NT - 1) / P::NT, group, &m, &n)) return;
   const int m0 = m * P::MT, n0 = a.row_from + n * P::NT;
+  const int wave = threadIdx.x >> 6, end = min(count, a.row_from + a.rows_at);
+  int t[P::NI];
+  load_targets<P::NI>(a, n0, wave % P::WN, end, t);
   f32x4 acc[P::MI][P::NI];
   P::run(weight_rows(a, m0), packed_rows(a, n0, count), a.width, lds, acc);
-  const int wave = threadIdx.x >> 6;
-  forward_epilogue<P::MI, P::NI, P::WM, P::WN>(a, acc, m0, n0, wave / P::WN, wave % P::WN,
-                                               min(count, a.row_from + a.rows_at), a.tile_from + m, (float2*)lds);
+  forward_epilogue<P::MI, P::NI, P::WM, P::WN>(a, acc, t, m0, n0, wave / P::WN, wave % P::WN, end, a.tile_from + m,
+                                               (float2*)lds);
 }
 
 // Two maxima with their sums of exponentials relative to them, as one.
@@ -246,38 +248,92 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dz_kernel(LossArgs a, int gro
   int m, n;
   if (!tile_of(blockIdx.x, a.vocab_tiles, (count + P::NT - 1) / P::NT, group, &m, &n)) return;
   const int m0 = m * P::MT, n0 = n * P::NT;
+  DzColumns<P> columns;
+  columns.load(a, n0, (threadIdx.x >> 6) % P::WN, count);
   f32x4 acc[P::MI][P::NI];
   P::run(weight_rows(a, m0), packed_rows(a, n0, count), a.width, lds, acc);
-  dz_epilogue<P, DT>(a, acc, m0, n0, count);
+  dz_epilogue<P, DT>(a, acc, columns, m0, n0, count);
+}
+
+// Splits of a product's summed entries over workgroups, where it has fewer tiles
+// than `slots` (the workgroups that run at once): as many as fill them, of at
+// least 256 entries each, and `most` at the most.  The count of listed rows is
+// known on the device alone, so kernels and host compute this where they are.
+struct Splits {
+  int32_t count, span;
+};
+__host__ __device__ inline Splits splits_of(int32_t tiles, int32_t slots, int32_t depth, int32_t most) {
+  int32_t n = slots / (tiles > 0 ? tiles : 1);
+  if (n > depth / 256) n = depth / 256;
+  if (n > most) n = most;
+  if (n < 1) n = 1;
+  const int32_t span = ((depth + n - 1) / n + 63) / 64 * 64;
+  return {span > 0 ? (depth + span - 1) / span : 1, span > 0 ? span : 64};
+}
+
+__device__ __forceinline__ Splits weight_splits(const LossArgs& a, int count) {
+  const Splits sp = splits_of(((a.piece + 127) / 128) * ((a.width + 127) / 128), a.slots, count, a.weight_most);
+  return {sp.count > 0 ? sp.count : 1, sp.span};
 }
 
 template <class P, int DT>
 __global__ __launch_bounds__(P::NW * 64) void loss_dweight_kernel(LossArgs a, int group) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[kLdsOut<P> / 2];
   const int count = a.meta->count;
-  int m, n;
-  if (!tile_of(blockIdx.x, a.width_tiles, a.vocab_tiles, group, &m, &n)) return;
+  const Splits sp = a.weight_sum ? weight_splits(a, count) : Splits{1, (count + 63) & ~63};
+  int m, ns;
+  if (!tile_of(blockIdx.x, a.width_tiles, a.vocab_tiles * sp.count, group, &m, &ns)) return;
+  const int n = ns % a.vocab_tiles, split = ns / a.vocab_tiles, from = split * sp.span;
   const int m0 = m * P::MT, n0 = n * P::NT;
   f32x4 acc[P::MI][P::NI];
   // `turned` holds zeros past the count, so the depth may be rounded up to whole chunks
-  P::run(turned_rows(a, m0), dz_columns(a, n0, count), (count + 7) & ~7, lds, acc);
-  dweight_epilogue<P, DT>(a, acc, m0, n0, lds);
+  P::run(turned_rows(a, m0, from), dz_columns(a, n0, from, count), max(0, min(sp.span, (count - from + 7) & ~7)), lds,
+         acc);
+  if (sp.count == 1) {
+    dweight_epilogue<P, DT>(a, acc, m0, n0, lds);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / P::WN, wn = wave % P::WN;
+  float* to = a.weight_sum + (int64_t)split * ((a.piece + 127) & ~127) * a.packed_width;
+#pragma unroll
+  for (int ni = 0; ni < P::NI; ++ni)
+#pragma unroll
+    for (int mi = 0; mi < P::MI; ++mi) {
+      const int v = n0 + (wn * P::NI + ni) * 16 + (lane & 15), i = m0 + (wm * P::MI + mi) * 16 + (lane >> 4) * 4;
+      if (v < a.piece && i < a.packed_width) *(f32x4*)(to + (int64_t)v * a.packed_width + i) = acc[mi][ni];
+    }
 }
 
-// Splits of a piece's vocabulary over workgroups, where dhidden has fewer tiles
-// than `slots` (the workgroups that run at once): as many as fill them, of at
-// least 512 entries each, and `most` at the most.  The count of listed rows is
-// known on the device alone, so kernels and host compute this where they are.
-struct Splits {
-  int32_t count, span;
-};
-__host__ __device__ inline Splits splits_of(int32_t tiles, int32_t slots, int32_t piece, int32_t most) {
-  int32_t n = slots / (tiles > 0 ? tiles : 1);
-  if (n > piece / 512) n = piece / 512;
-  if (n > most) n = most;
-  if (n < 1) n = 1;
-  const int32_t span = ((piece + n - 1) / n + 63) / 64 * 64;
-  return {(piece + span - 1) / span, span};
+// One row's sum of its shares, scaled back and rounded: elements i ... i + 3.
+template <int DT>
+__device__ __forceinline__ void sum_shares(const float* from, int64_t step, int splits, float unscale, uint16_t* to,
+                                           int left) {
+  f32x4 d = {0, 0, 0, 0};
+  constexpr int U = 8;  // loads on their way at once
+  int s = 0;
+  for (; s + U <= splits; s += U) {
+    f32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = *(const f32x4*)(from + (s + u) * step);
+#pragma unroll
+    for (int u = 0; u < U; ++u) d += v[u];
+  }
+  for (; s < splits; ++s) d += *(const f32x4*)(from + s * step);
+  const float o[4] = {d[0] * unscale, d[1] * unscale, d[2] * unscale, d[3] * unscale};
+  store_four<DT>(to, o, left);
+}
+
+// dweight from its shares, if it has any
+template <int DT>
+__global__ __launch_bounds__(256) void loss_dweight_sum_kernel(LossArgs a) {
+  const int splits = weight_splits(a, a.meta->count).count;
+  if (splits == 1) return;
+  const float unscale = a.meta->unscale;
+  const int64_t step = (int64_t)((a.piece + 127) & ~127) * a.packed_width;
+  for (int32_t v = blockIdx.x; v < a.piece; v += gridDim.x)
+    for (int32_t i = threadIdx.x * 4; i < a.width; i += 1024)
+      sum_shares<DT>(a.weight_sum + (int64_t)v * a.packed_width + i, step, splits, unscale,
+                     a.dweight + ((int64_t)a.piece_from + v) * a.dweight_stride + i, a.width - i);
 }
 
 template <class P, int DT>
@@ -308,22 +364,9 @@ __global__ __launch_bounds__(256) void loss_dhidden_kernel(LossArgs a, int tile_
   const float unscale = a.meta->unscale;
   const int64_t step = (int64_t)count * a.packed_width;
   for (int32_t n = blockIdx.x; n < count; n += gridDim.x) {
-    for (int32_t i = (blockIdx.y * 256 + threadIdx.x) * 4; i < a.width; i += gridDim.y * 1024) {
-      const float* from = a.sum + (int64_t)n * a.packed_width + i;
-      f32x4 d = {0, 0, 0, 0};
-      constexpr int U = 8;  // loads on their way at once
-      int s = 0;
-      for (; s + U <= splits; s += U) {
-        f32x4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = *(const f32x4*)(from + (s + u) * step);
-#pragma unroll
-        for (int u = 0; u < U; ++u) d += v[u];
-      }
-      for (; s < splits; ++s) d += *(const f32x4*)(from + s * step);
-      const float o[4] = {d[0] * unscale, d[1] * unscale, d[2] * unscale, d[3] * unscale};
-      store_four<DT>(a.dhidden + (int64_t)a.index[n] * a.dhidden_stride + i, o, a.width - i);
-    }
+    for (int32_t i = (blockIdx.y * 256 + threadIdx.x) * 4; i < a.width; i += gridDim.y * 1024)
+      sum_shares<DT>(a.sum + (int64_t)n * a.packed_width + i, step, splits, unscale,
+                     a.dhidden + (int64_t)a.index[n] * a.dhidden_stride + i, a.width - i);
   }
 }
 
@@ -370,19 +413,29 @@ int64_t packed_piece(int64_t width, int64_t vocab) {
 
 // Tiles of z, vocabulary rows x list positions, by the number of rows: 128 x 16
 // and 128 x 64 (the weight's bytes bound these: 131072 x 4096 in 185 us, 5.8
-// TB/s, up to 64 rows), 256 x 128, 256 x 256; and 128 x 128 where 256 x 256 would
-// leave half of the CUs without a tile.  In batch-invariant mode always 256 x
-// 256: a row's logits are summed alike in every shape, but its exponentials
-// tile by tile, so the shape shows in the last bits of its lse.
-enum LogitTile { kTile16, kTile64, kTileSmall, kTile128, kTile256 };
+// TB/s, up to 64 rows), 256 x 128, 256 x 256; 64 x 16 and 64 x 64 where 128
+// vocabulary rows would leave a CU fewer than two workgroups (14814 x 6656, 23
+// rows: 55 us with them); and 128 x 128 where 256 x 256 would leave half of the
+// CUs without a tile.  In batch-invariant mode always 256 x 256: a row's logits
+// are summed alike in every shape, but its exponentials tile by tile, so the
+// shape shows in the last bits of its lse.
+enum LogitTile { kTile16Short, kTile64Short, kTile16, kTile64, kTileSmall, kTile128, kTile256 };
 LogitTile logit_tile(int64_t rows, int64_t vocab) {
   if (hprms_batch_invariant()) return kTile256;
-  if (rows <= 64) return rows <= 16 ? kTile16 : kTile64;
+  if (rows <= 64) {
+    if (ceil_div(vocab, 128) < 2 * (int64_t)current_cus()) return rows <= 16 ? kTile16Short : kTile64Short;
+    return rows <= 16 ? kTile16 : kTile64;
+  }
   if (2 * ceil_div(vocab, 256) * ceil_div(rows, 256) <= current_cus()) return kTileSmall;
   return rows <= 128 ? kTile128 : kTile256;
 }
-int64_t logit_vocab_rows(LogitTile t) { return t <= kTileSmall ? 128 : 256; }
-int64_t logit_rows(LogitTile t) { return t == kTile16 ? 16 : t == kTile64 ? 64 : t == kTile256 ? 256 : 128; }
+int64_t logit_vocab_rows(LogitTile t) { return t <= kTile64Short ? 64 : t <= kTileSmall ? 128 : 256; }
+int64_t logit_rows(LogitTile t) {
+  return t == kTile16Short || t == kTile16   ? 16
+         : t == kTile64Short || t == kTile64 ? 64
+         : t == kTile256                     ? 256
+                                             : 128;
+}
 
 // Offsets of the workspace's parts, bytes.
 struct ForwardPlan {
@@ -410,7 +463,8 @@ struct BackwardPlan {
   int64_t index, packed, turned, weight, dz, sum, total;
   int64_t turned_stride;
   int64_t piece, pieces, dz_rows, row_tiles, width_tiles, slots, most_splits;
-  bool shares;
+  int64_t weight_sum, weight_most;
+  bool shares, few;
   LogitTile tile;
 };
 
@@ -427,7 +481,7 @@ BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_p
   p.slots = (int64_t)current_cus() * (p.tile == kTile256 ? 1 : 2);
   // with fewer listed rows there are more splits, of fewer rows: count * splits
   // stays within what a slot's tile holds each, or within one share of all rows
-  p.most_splits = max64(1, min64(p.slots / p.width_tiles, p.piece / 512));
+  p.most_splits = max64(1, min64(p.slots / p.width_tiles, p.piece / 256));
   const int64_t sum_rows = max64(rows, p.most_splits > 1 ? p.slots / p.width_tiles * logit_rows(p.tile) : 0);
   const bool shares = p.pieces > 1 || p.most_splits > 1;
   p.index = 256;
@@ -440,6 +494,15 @@ BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_p
   p.total = p.sum + (shares ? sum_rows * packed_width_of(width) * 4 : 0);
   p.row_tiles = row_tiles;
   p.shares = shares;
+  // dweight in tiles of 128 x 128, which run four to a CU, where the sums over
+  // the rows are short (128 rows of 131072 x 4096: 331 us, 256 x 256 430) or 256 x
+  // 256 would leave CUs without a tile; where even these do, the rows are split
+  p.few = rows <= 128 || ceil_div(p.piece, 256) * ceil_div(width, 256) < current_cus();
+  p.weight_most = 1;
+  if (p.few && p.pieces == 1)
+    p.weight_most = max64(1, min64(p.slots / (ceil_div(vocab, 128) * ceil_div(width, 128)), rows / 256));
+  p.weight_sum = round_up(p.total, 256);
+  if (p.weight_most > 1) p.total = p.weight_sum + p.weight_most * round_up(vocab, 128) * packed_width_of(width) * 4;
   return p;
 }
 
@@ -475,6 +538,8 @@ struct Tiles {
                              Product<DT, 128, 16, 4, 1, 64, 4, false, false>> T16;
   typedef std::conditional_t<AKO, Product<DT, 256, 64, 4, 1, 32, 4, true, false>,
                              Product<DT, 128, 64, 4, 1, 64, 3, false, false>> T64;
+  typedef Product<DT, 64, 16, 4, 1, 64, 6, false, false> T16Short;
+  typedef Product<DT, 64, 64, 4, 1, 64, 5, false, false> T64Short;
   typedef Product<DT, 128, 128, 2, 2, 64, 2, false, false> Small;
   typedef Product<DT, 256, 128, 4, 2, 32, 3, AKO, false> T128;
   typedef RingProduct<DT, AKO, false, AKO ? 4 : 2> T256;
@@ -533,6 +598,8 @@ int run_forward(LossArgs a, const ForwardPlan& p, const Weight& w, char* ws, hip
     for (int64_t v = 0; v < a.vocab; v += p.piece) {
       take_piece(a, w, v, p.piece, stream);
       switch (p.tile) {
+        case kTile16Short: launch_forward<typename T::T16Short, DT>(a, here, stream); break;
+        case kTile64Short: launch_forward<typename T::T64Short, DT>(a, here, stream); break;
         case kTile16: launch_forward<typename T::T16, DT>(a, here, stream); break;
         case kTile64: launch_forward<typename T::T64, DT>(a, here, stream); break;
         case kTileSmall: launch_forward<typename T::Small, DT>(a, here, stream); break;
@@ -557,8 +624,10 @@ void launch_piece(LossArgs a, const BackwardPlan& p, hipStream_t stream) {
         a, 4);
   a.vocab_tiles = (int32_t)ceil_div(a.piece, PW::NT);
   a.width_tiles = (int32_t)ceil_div(a.width, PW::MT);
-  loss_dweight_kernel<PW, DT><<<dim3(grid_of((int64_t)a.vocab_tiles * a.width_tiles)), dim3(PW::NW * 64), 0, stream>>>(
-      a, 8);
+  loss_dweight_kernel<PW, DT><<<dim3(grid_of(max64((int64_t)a.vocab_tiles * a.width_tiles, a.weight_sum ? p.slots : 0))),
+                                dim3(PW::NW * 64), 0, stream>>>(a, 8);
+  if (a.weight_sum)
+    loss_dweight_sum_kernel<DT><<<dim3((unsigned)min64(a.piece, 8192)), dim3(256), 0, stream>>>(a);
   a.width_tiles = (int32_t)p.width_tiles;
   static_assert(PH::NT == PZ::NT, "one number of rows a tile");
   // at most max(slots, tiles) workgroups, whatever the count of listed rows
@@ -580,22 +649,20 @@ int run_backward(LossArgs a, const BackwardPlan& p, const Weight& w, char* ws, h
   for (int64_t i = 0; i < p.pieces; ++i) {
     take_piece(a, w, i * p.piece, p.piece, stream);
     a.first_piece = i == 0;
-    // dweight in tiles of 128 x 128, which run four to a CU, where the sums over
-    // the rows are short (128 rows of 131072 x 4096: 331 us, 256 x 256 430) or 256
-    // x 256 would leave CUs without a tile
-    const bool few = a.rows <= 128 || ceil_div(a.piece, 256) * ceil_div(a.width, 256) < current_cus();
     switch (p.tile) {
+      case kTile16Short: launch_piece<typename Z::T16Short, WS, typename H::T16, DT>(a, p, stream); break;
+      case kTile64Short: launch_piece<typename Z::T64Short, WS, typename H::T64, DT>(a, p, stream); break;
       case kTile16: launch_piece<typename Z::T16, WS, typename H::T16, DT>(a, p, stream); break;
       case kTile64: launch_piece<typename Z::T64, WS, typename H::T64, DT>(a, p, stream); break;
       case kTileSmall:
-        if (few)
+        if (p.few)
           launch_piece<typename Z::Small, WS, typename H::T128, DT>(a, p, stream);
         else
           launch_piece<typename Z::Small, W, typename H::T128, DT>(a, p, stream);
         break;
       case kTile128: launch_piece<typename Z::T128, WS, typename H::T128, DT>(a, p, stream); break;
       case kTile256:
-        if (few)
+        if (p.few)
           launch_piece<typename Z::T256, WS, typename H::T256, DT>(a, p, stream);
         else
           launch_piece<typename Z::T256, W, typename H::T256, DT>(a, p, stream);
@@ -713,6 +780,8 @@ int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const floa
   a.width_tiles = (int32_t)p.width_tiles;
   a.slots = (int32_t)p.slots;
   a.most_splits = (int32_t)p.most_splits;
+  a.weight_sum = p.weight_most > 1 ? (float*)(ws + p.weight_sum) : nullptr;
+  a.weight_most = (int32_t)p.weight_most;
   const Weight w{(const uint16_t*)weight, weight_row_stride, in_place ? nullptr : (uint16_t*)(ws + p.weight)};
   return dtype == HPRMS_DTYPE_BF16 ? run_backward<HPRMS_DTYPE_BF16>(a, p, w, ws, stream)
                                    : run_backward<HPRMS_DTYPE_FP16>(a, p, w, ws, stream);

@@ -312,7 +312,7 @@ def test_batch_invariant_mode_fixes_a_rows_bits(ops):
 
 
 SHAPES = [(12, 300, 700), (40, 512, 3000), (100, 264, 9000), (100, 128, 70000), (200, 128, 70000), (300, 384, 2000),
-          (900, 128, 70000)]
+          (900, 128, 70000), (1500, 64, 200), (2000, 200, 1100), (700, 520, 300)]
 
 
 @pytest.mark.parametrize("rows,hidden,vocab", SHAPES)
