@@ -352,6 +352,8 @@ int run_norm(float* norm, void* const* outs, const int* out_dtypes, const void* 
                   out_dtypes[i]);
     if (counts[i] == 0) continue;
     if (!grads[i] || (outs && !outs[i])) return fail(HPRMS_E_INVALID, "null tensor pointer (tensor %d)", i);
+    if (outs && outs[i] == grads[i] && out_dtypes[i] != dtypes[i])
+      return fail(HPRMS_E_INVALID, "output %d lies on its gradient but has another dtype", i);
     if (((uintptr_t)grads[i] & (dtypes[i] == HPRMS_DTYPE_FP32 ? 3 : 1)) != 0 ||
         (outs && ((uintptr_t)outs[i] & (out_dtypes[i] == HPRMS_DTYPE_FP32 ? 3 : 1)) != 0))
       return fail(HPRMS_E_INVALID, "tensor %d is not aligned to its elements", i);

@@ -247,3 +247,10 @@ def test_clip_abi_refuses():
     n = (ctypes.c_int64 * 1)(4)
     assert L.hprms_clip_grad_norm(0x100, None, None, None, None, n, 1, 1.0, 0x10000, 1 << 20, None) == \
         abi.HPRMS_E_INVALID
+
+
+def test_clip_abi_refuses_an_output_of_another_dtype_on_its_gradient():
+    for dtype in (0, 1):
+        with pytest.raises(abi.HprmsError, match="output 1 lies on its gradient"):
+            abi.clip_grad_norm(0x100, [0x3000, 0x1000], [2, 2], [0x2000, 0x1000], [dtype] * 2, [4, 4], 1.0, 0x10000,
+                               1 << 20)
