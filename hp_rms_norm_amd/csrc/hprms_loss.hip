@@ -415,7 +415,7 @@ int64_t packed_piece(int64_t width, int64_t vocab) {
 // and 128 x 64 (the weight's bytes bound these: 131072 x 4096 in 185 us, 5.8
 // TB/s, up to 64 rows), 256 x 128, 256 x 256; 64 x 16 and 64 x 64 where 128
 // vocabulary rows would leave a CU fewer than two workgroups (14814 x 6656, 23
-// rows: 55 us with them); and 128 x 128 where 256 x 256 would leave half of the
+// rows: 45 us, 55 with 128 x 64); and 128 x 128 where 256 x 256 would leave half of the
 // CUs without a tile.  In batch-invariant mode always 256 x 256: a row's logits
 // are summed alike in every shape, but its exponentials tile by tile, so the
 // shape shows in the last bits of its lse.
@@ -782,7 +782,9 @@ int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const floa
   a.most_splits = (int32_t)p.most_splits;
   a.weight_sum = p.weight_most > 1 ? (float*)(ws + p.weight_sum) : nullptr;
   a.weight_most = (int32_t)p.weight_most;
-  const Weight w{(const uint16_t*)weight, weight_row_stride, in_place ? nullptr : (uint16_t*)(ws + p.weight)};
+  // without rows nothing reads the weight, which may then be null
+  const Weight w{(const uint16_t*)weight, weight_row_stride,
+                 in_place || rows == 0 ? nullptr : (uint16_t*)(ws + p.weight)};
   return dtype == HPRMS_DTYPE_BF16 ? run_backward<HPRMS_DTYPE_BF16>(a, p, w, ws, stream)
                                    : run_backward<HPRMS_DTYPE_FP16>(a, p, w, ws, stream);
 }

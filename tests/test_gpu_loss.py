@@ -22,6 +22,8 @@ K(n) = 2 (n / 32 + 32).
 import pytest
 import torch
 
+from hp_rms_norm_amd import abi
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
@@ -138,6 +140,17 @@ def test_all_rows_ignored_and_no_rows(ops):
     assert loss.shape == (0,) and lse.shape == (0,)
     dh, dw = ops.linear_cross_entropy_backward(dloss[:0], h[:0], w, t[:0], lse)
     assert dh.shape == (0, 64) and not bool(dw.any())
+
+
+@pytest.mark.parametrize("hidden", [64, 65])
+def test_no_rows_need_no_tensors_but_dweight(ops, hidden):
+    dw = torch.ones((300, hidden), dtype=torch.bfloat16, device="cuda")
+    size = abi.linear_cross_entropy_backward_workspace(0, hidden, 300)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    abi.linear_cross_entropy_backward(0, dw.data_ptr(), 0, 0, 0, 0, 0, ws.data_ptr(), size, 0, hidden, 300, hidden,
+                                      hidden, hidden, hidden, IGNORE, abi.DTYPE_BF16,
+                                      torch.cuda.current_stream().cuda_stream)
+    assert not bool(dw.any())
 
 
 def test_other_ignore_index_and_targets_out_of_range(ops):
