@@ -108,12 +108,8 @@ __device__ __forceinline__ float xor32(float v) { return __shfl_xor(v, 32); }
 // exp(x) as 2^(x log2 e); the argument is at most 0 in every use but for NaN
 __device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 
-// Per column (list position) of the workgroup's tile: the maximum over its
-// vocabulary rows and the sum of exponentials relative to it.  A wave's 4 lanes
-// of a column join by swizzles, the WM waves stacked over the column through
-// LDS.  NaN logits leave the maximum and make the sum NaN.
-// `t`: the targets of this lane's columns, in the piece, or -1 (loaded before
-// the tile loop: two dependent loads that would stand at its end).
+// The targets of this lane's columns, in the piece, or -1 (loaded before the
+// tile loop: two dependent loads that would stand at its end).
 template <int NI>
 __device__ __forceinline__ void load_targets(const LossArgs& a, int n0, int wn, int count, int (&t)[NI]) {
 #pragma unroll
@@ -124,6 +120,11 @@ __device__ __forceinline__ void load_targets(const LossArgs& a, int n0, int wn, 
   }
 }
 
+// Per column (list position) of the workgroup's tile: the maximum over its
+// vocabulary rows and the sum of exponentials relative to it.  A wave's 4 lanes
+// of a column join by swizzles, the WM waves stacked over the column through
+// LDS.  NaN logits leave the maximum and make the sum NaN.
+// `t` is load_targets's.
 template <int MI, int NI, int WM, int WN>
 __device__ __forceinline__ void forward_epilogue(const LossArgs& a, const f32x4 (&acc)[MI][NI], const int (&t)[NI],
                                                  int m0, int n0, int wm, int wn, int count, int tile, float2* lds) {
@@ -175,8 +176,8 @@ __device__ __forceinline__ void forward_epilogue(const LossArgs& a, const f32x4 
 // A tile of 16-bit values on its way out: the fragments hold 4 neighbours of a
 // row (of the output: a column of the product) a lane, which would store 32
 // bytes of 16 rows at a time; through LDS whole rows of the tile go out, 16
-// bytes a lane (dweight of one row, 131072 x 4096: 311 us with the fragments'
-// own stores).  `from(mi, ni)` gives a fragment's 4 values as 8 bytes; `to(row)`
+// bytes a lane (dweight of one row, 131072 x 4096: 197 us, 311 with the
+// fragments' own stores).  `from(mi, ni)` gives a fragment's 4 values as 8 bytes; `to(row)`
 // is where a row of the tile begins, null if it does not exist, and `left` the
 // elements from there on that do.
 template <class P>
