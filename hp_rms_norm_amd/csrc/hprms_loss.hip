@@ -162,6 +162,9 @@ __device__ __forceinline__ Operand weight_columns(const LossArgs& a, int k, int 
 __device__ __forceinline__ Operand packed_rows(const LossArgs& a, int n, int count) {
   return {a.packed + (int64_t)n * a.packed_width, (int64_t)(count - n) * a.packed_width * 2, a.packed_width};
 }
+__device__ __forceinline__ Operand packed_columns(const LossArgs& a, int k, int m, int count) {
+  return {a.packed + (int64_t)k * a.packed_width + m, ((int64_t)(count - k) * a.packed_width - m) * 2, a.packed_width};
+}
 __device__ __forceinline__ Operand turned_rows(const LossArgs& a, int m, int k) {
   return {a.turned + (int64_t)m * a.turned_stride + k, ((int64_t)(a.packed_width - m) * a.turned_stride - k) * 2,
           a.turned_stride};
@@ -187,8 +190,9 @@ __global__ __launch_bounds__(P::NW * 64) void loss_forward_kernel(LossArgs a, in
   load_targets<P::NI>(a, n0, wave % P::WN, end, t);
   f32x4 acc[P::MI][P::NI];
   P::run(weight_rows(a, m0), packed_rows(a, n0, count), a.width, lds, acc);
-  forward_epilogue<P::MI, P::NI, P::WM, P::WN>(a, acc, t, m0, n0, wave / P::WN, wave % P::WN, end, a.tile_from + m,
-                                               (float2*)lds);
+  // (a SumProduct's waves all hold the whole tile, and all do the same)
+  forward_epilogue<P::MI, P::NI, P::WM, P::WN>(a, acc, t, m0, n0, wave / P::WN % P::WM, wave % P::WN, end,
+                                               a.tile_from + m, (float2*)lds);
 }
 
 // Two maxima with their sums of exponentials relative to them, as one.
@@ -252,6 +256,7 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dz_kernel(LossArgs a, int gro
   columns.load(a, n0, (threadIdx.x >> 6) % P::WN, count);
   f32x4 acc[P::MI][P::NI];
   P::run(weight_rows(a, m0), packed_rows(a, n0, count), a.width, lds, acc);
+  if (P::NW > P::WM * P::WN && threadIdx.x >= P::WM * P::WN * 64) return;  // a SumProduct's first wave has it all
   dz_epilogue<P, DT>(a, acc, columns, m0, n0, count);
 }
 
@@ -286,9 +291,13 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dweight_kernel(LossArgs a, in
   const int n = ns % a.vocab_tiles, split = ns / a.vocab_tiles, from = split * sp.span;
   const int m0 = m * P::MT, n0 = n * P::NT;
   f32x4 acc[P::MI][P::NI];
-  // `turned` holds zeros past the count, so the depth may be rounded up to whole chunks
-  P::run(turned_rows(a, m0, from), dz_columns(a, n0, from, count), max(0, min(sp.span, (count - from + 7) & ~7)), lds,
-         acc);
+  // rows past the count are out of range or, in `turned`, zeros, so the depth may be rounded up to whole chunks
+  Operand hidden;
+  if constexpr (P::AKO)
+    hidden = packed_columns(a, from, m0, count);
+  else
+    hidden = turned_rows(a, m0, from);
+  P::run(hidden, dz_columns(a, n0, from, count), max(0, min(sp.span, (count - from + 7) & ~7)), lds, acc);
   if (sp.count == 1) {
     dweight_epilogue<P, DT>(a, acc, m0, n0, lds);
     return;
@@ -415,23 +424,28 @@ int64_t packed_piece(int64_t width, int64_t vocab) {
 // and 128 x 64 (the weight's bytes bound these: 131072 x 4096 in 185 us, 5.8
 // TB/s, up to 64 rows), 256 x 128, 256 x 256; 64 x 16 and 64 x 64 where 128
 // vocabulary rows would leave a CU fewer than two workgroups (14814 x 6656, 23
-// rows: 45 us, 55 with 128 x 64); and 128 x 128 where 256 x 256 would leave half of the
-// CUs without a tile.  In batch-invariant mode always 256 x 256: a row's logits
-// are summed alike in every shape, but its exponentials tile by tile, so the
-// shape shows in the last bits of its lse.
-enum LogitTile { kTile16Short, kTile64Short, kTile16, kTile64, kTileSmall, kTile128, kTile256 };
+// rows: 45 us, 55 with 128 x 64); 16 x 16, whose waves share the sum, up to one
+// workgroup a CU (1361 x 4544, 1 row: 9.0 us, 64 x 16 21; beyond, 17839 x 768, 6
+// rows, 14.4 against 8.5); and 128 x 128 where 256 x 256 would leave half of the
+// CUs without a tile.  In batch-invariant mode always 256 x 256: the shapes sum a
+// row's exponentials, and 16 x 16 its logits, in other orders, which shows in the
+// last bits of its lse.
+enum LogitTile { kTile16Sum, kTile16Short, kTile64Short, kTile16, kTile64, kTileSmall, kTile128, kTile256 };
 LogitTile logit_tile(int64_t rows, int64_t vocab) {
   if (hprms_batch_invariant()) return kTile256;
   if (rows <= 64) {
+    if (rows <= 16 && ceil_div(vocab, 16) <= current_cus()) return kTile16Sum;
     if (ceil_div(vocab, 128) < 2 * (int64_t)current_cus()) return rows <= 16 ? kTile16Short : kTile64Short;
     return rows <= 16 ? kTile16 : kTile64;
   }
   if (2 * ceil_div(vocab, 256) * ceil_div(rows, 256) <= current_cus()) return kTileSmall;
   return rows <= 128 ? kTile128 : kTile256;
 }
-int64_t logit_vocab_rows(LogitTile t) { return t <= kTile64Short ? 64 : t <= kTileSmall ? 128 : 256; }
+int64_t logit_vocab_rows(LogitTile t) {
+  return t == kTile16Sum ? 16 : t <= kTile64Short ? 64 : t <= kTileSmall ? 128 : 256;
+}
 int64_t logit_rows(LogitTile t) {
-  return t == kTile16Short || t == kTile16   ? 16
+  return t <= kTile16Short || t == kTile16   ? 16
          : t == kTile64Short || t == kTile64 ? 64
          : t == kTile256                     ? 256
                                              : 128;
@@ -484,20 +498,20 @@ BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_p
   p.most_splits = max64(1, min64(p.slots / p.width_tiles, p.piece / 256));
   const int64_t sum_rows = max64(rows, p.most_splits > 1 ? p.slots / p.width_tiles * logit_rows(p.tile) : 0);
   const bool shares = p.pieces > 1 || p.most_splits > 1;
+  // dweight in tiles of 128 x 128, which run four to a CU, where the sums over
+  // the rows are short (128 rows of 131072 x 4096: 331 us, 256 x 256 430) or 256 x
+  // 256 would leave CUs without a tile; where even these do, the rows are split
+  p.few = rows <= 128 || ceil_div(p.piece, 256) * ceil_div(width, 256) < current_cus();
   p.index = 256;
   p.packed = p.index + round_up(rows * 4, 256);
   p.turned_stride = round_up(rows, 64);
   p.turned = p.packed + round_up(rows * packed_width_of(width) * 2, 256);
-  p.weight = p.turned + p.turned_stride * packed_width_of(width) * 2;
+  p.weight = p.turned + (p.few ? 0 : p.turned_stride * packed_width_of(width) * 2);
   p.dz = p.weight + (in_place ? 0 : p.piece * packed_width_of(width) * 2);
   p.sum = p.dz + p.dz_rows * p.piece * 2;
   p.total = p.sum + (shares ? sum_rows * packed_width_of(width) * 4 : 0);
   p.row_tiles = row_tiles;
   p.shares = shares;
-  // dweight in tiles of 128 x 128, which run four to a CU, where the sums over
-  // the rows are short (128 rows of 131072 x 4096: 331 us, 256 x 256 430) or 256 x
-  // 256 would leave CUs without a tile; where even these do, the rows are split
-  p.few = rows <= 128 || ceil_div(p.piece, 256) * ceil_div(width, 256) < current_cus();
   p.weight_most = 1;
   if (p.few && p.pieces == 1)
     p.weight_most = max64(1, min64(p.slots / (ceil_div(vocab, 128) * ceil_div(width, 128)), rows / 256));
@@ -538,6 +552,7 @@ struct Tiles {
                              Product<DT, 128, 16, 4, 1, 64, 4, false, false>> T16;
   typedef std::conditional_t<AKO, Product<DT, 256, 64, 4, 1, 32, 4, true, false>,
                              Product<DT, 128, 64, 4, 1, 64, 3, false, false>> T64;
+  typedef SumProduct<DT, 1, 1, 4, 6> T16Sum;
   typedef Product<DT, 64, 16, 4, 1, 64, 6, false, false> T16Short;
   typedef Product<DT, 64, 64, 4, 1, 64, 5, false, false> T64Short;
   typedef Product<DT, 128, 128, 2, 2, 64, 2, false, false> Small;
@@ -598,6 +613,7 @@ int run_forward(LossArgs a, const ForwardPlan& p, const Weight& w, char* ws, hip
     for (int64_t v = 0; v < a.vocab; v += p.piece) {
       take_piece(a, w, v, p.piece, stream);
       switch (p.tile) {
+        case kTile16Sum: launch_forward<typename T::T16Sum, DT>(a, here, stream); break;
         case kTile16Short: launch_forward<typename T::T16Short, DT>(a, here, stream); break;
         case kTile64Short: launch_forward<typename T::T64Short, DT>(a, here, stream); break;
         case kTile16: launch_forward<typename T::T16, DT>(a, here, stream); break;
@@ -640,16 +656,17 @@ template <int DT>
 int run_backward(LossArgs a, const BackwardPlan& p, const Weight& w, char* ws, hipStream_t stream) {
   typedef Tiles<DT, false> Z;
   typedef RingProduct<DT, false, true, 2> W;  // dweight
-  typedef Product<DT, 128, 128, 2, 2, 32, 2, false, true> WS;  // ... of few rows
+  typedef Product<DT, 128, 128, 2, 2, 32, 2, true, true> WS;  // ... of few rows: not worth a launch that turns them
   typedef Tiles<DT, true> H;
   launch_pack<true>(a, ws, p.index, p.packed, stream);
-  if (a.rows > 0)
+  if (!p.few)
     loss_turn_kernel<<<dim3((unsigned)ceil_div(a.rows, 64), (unsigned)(a.packed_width / 64)), dim3(256), 0, stream>>>(
         a, (uint16_t*)(ws + p.turned));
   for (int64_t i = 0; i < p.pieces; ++i) {
     take_piece(a, w, i * p.piece, p.piece, stream);
     a.first_piece = i == 0;
     switch (p.tile) {
+      case kTile16Sum: launch_piece<typename Z::T16Sum, WS, typename H::T16, DT>(a, p, stream); break;
       case kTile16Short: launch_piece<typename Z::T16Short, WS, typename H::T16, DT>(a, p, stream); break;
       case kTile64Short: launch_piece<typename Z::T64Short, WS, typename H::T64, DT>(a, p, stream); break;
       case kTile16: launch_piece<typename Z::T16, WS, typename H::T16, DT>(a, p, stream); break;

@@ -245,6 +245,83 @@ struct Product {
   }
 };
 
+// Few tiles over a long sum: the waves of a workgroup share one tile of MI x NI
+// fragments and take the summed entries in turn, 64 at a time, from memory
+// straight to registers, D of their turns ahead; both operands k contiguous.  The
+// waves' sums are joined through LDS in a fixed order, and every wave holds the
+// whole tile afterwards (WM = WN = 1).  A tile's time is its latency: a slice of
+// Product above costs a workgroup that is alone on its CU 0.3 us, its barrier
+// and its way through LDS, however many slices are on their way (71 slices: 21
+// us with 6 or 15 stages), while here 4 waves go through them at 9.0 us.  With
+// many tiles loads of half lines tell (16 rows of 60000 x 4096: 3.7 TB/s, 6 there).
+template <int DT, int MI_, int NI_, int NW_, int D>
+struct SumProduct {
+  static constexpr int MI = MI_, NI = NI_, MT = MI * 16, NT = NI * 16, NW = NW_, WM = 1, WN = 1;
+  static constexpr int LDS_BYTES = NW * MI * NI * 1024;
+
+  __device__ static __forceinline__ void run(const Operand& a, const Operand& b, int32_t depth, uint16_t* lds_generic,
+                                             f32x4 (&acc)[MI][NI]) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, k0 = (lane >> 4) * 8;
+    const __amdgpu_buffer_rsrc_t ra = make_rsrc(a.base, a.bytes < 0x7fffffff ? (uint32_t)a.bytes : 0x7fffffffu);
+    const __amdgpu_buffer_rsrc_t rb = make_rsrc(b.base, b.bytes < 0x7fffffff ? (uint32_t)b.bytes : 0x7fffffffu);
+    uint32_t oa[MI], ob[NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) oa[i] = ((uint32_t)(i * 16 + r) * (uint32_t)a.stride + k0) * 2;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) ob[j] = ((uint32_t)(j * 16 + r) * (uint32_t)b.stride + k0) * 2;
+    u32x4 fa[D][2][MI], fb[D][2][NI];
+    // the two steps of slice t; past the depth nothing is in range
+    auto load = [&](int t, u32x4 (&va)[2][MI], u32x4 (&vb)[2][NI]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = t * 64 + h * 32;
+        const bool in = k + k0 < depth;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+          va[h][i] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? oa[i] + k * 2 : kOOB, 0, 0);
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+          vb[h][j] = __builtin_amdgcn_raw_buffer_load_b128(rb, in ? ob[j] + k * 2 : kOOB, 0, 0);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(wave + d * NW, fa[d], fb[d]);
+    const int32_t slices = (depth + 63) / 64;
+    for (int32_t t = wave; t < slices; t += D * NW) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = mfma16<DT>(fa[d][h][i], fb[d][h][j], acc[i][j]);
+        load(t + (d + D) * NW, fa[d], fb[d]);
+      }
+    }
+    f32x4* lds = (f32x4*)lds_generic;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) lds[((wave * MI + i) * NI + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        acc[i][j] = lds[(i * NI + j) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) acc[i][j] += lds[((w * MI + i) * NI + j) * 64 + lane];
+      }
+  }
+};
+
 // The 256 x 256 tile of 8 waves: WM x 8 / WM, 64 x 128 or 128 x 64 each.
 //
 // LDS holds 10 chunks of 16 KB.  A slice of 64 summed entries is 4 of them, two
