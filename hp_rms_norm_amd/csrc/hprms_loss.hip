@@ -336,21 +336,26 @@ __global__ __launch_bounds__(P::NW * 64) void loss_dweight_kernel(LossArgs a, in
     }
 }
 
-// One row's sum of its shares, scaled back and rounded: elements i ... i + 3.
-template <int DT>
-__device__ __forceinline__ void sum_shares(const float* from, int64_t step, int splits, float unscale, uint16_t* to,
-                                           int left) {
+// A row's sum of its shares, elements i ... i + 3.
+__device__ __forceinline__ f32x4 sum_shares(const float* from, int64_t step, int splits) {
   f32x4 d = {0, 0, 0, 0};
   constexpr int U = 8;  // loads on their way at once
-  int s = 0;
-  for (; s + U <= splits; s += U) {
+  for (int s = 0; s < splits; s += U) {
     f32x4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = *(const f32x4*)(from + (s + u) * step);
+    for (int u = 0; u < U; ++u) {
+      v[u] = f32x4{0, 0, 0, 0};
+      if (s + u < splits) v[u] = *(const f32x4*)(from + (s + u) * step);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) d += v[u];
   }
-  for (; s < splits; ++s) d += *(const f32x4*)(from + s * step);
+  return d;
+}
+
+// ... scaled back and rounded, the first `left` of the four
+template <int DT>
+__device__ __forceinline__ void store_sum(uint16_t* to, f32x4 d, float unscale, int left) {
   const float o[4] = {d[0] * unscale, d[1] * unscale, d[2] * unscale, d[3] * unscale};
   store_four<DT>(to, o, left);
 }
@@ -364,8 +369,8 @@ __global__ __launch_bounds__(256) void loss_dweight_sum_kernel(LossArgs a) {
   const int64_t step = (int64_t)((a.piece + 127) & ~127) * a.packed_width;
   for (int32_t v = blockIdx.x; v < a.piece; v += gridDim.x)
     for (int32_t i = threadIdx.x * 4; i < a.width; i += 1024)
-      sum_shares<DT>(a.weight_sum + (int64_t)v * a.packed_width + i, step, splits, unscale,
-                     a.dweight + ((int64_t)a.piece_from + v) * a.dweight_stride + i, a.width - i);
+      store_sum<DT>(a.dweight + ((int64_t)a.piece_from + v) * a.dweight_stride + i,
+                    sum_shares(a.weight_sum + (int64_t)v * a.packed_width + i, step, splits), unscale, a.width - i);
 }
 
 template <class P, int DT>
@@ -396,9 +401,10 @@ __global__ __launch_bounds__(256) void loss_dhidden_kernel(LossArgs a, int tile_
   const float unscale = a.meta->unscale;
   const int64_t step = (int64_t)count * a.packed_width;
   for (int32_t n = blockIdx.x; n < count; n += gridDim.x) {
+    const int32_t row = a.index[n];
     for (int32_t i = (blockIdx.y * 256 + threadIdx.x) * 4; i < a.width; i += gridDim.y * 1024)
-      sum_shares<DT>(a.sum + (int64_t)n * a.packed_width + i, step, splits, unscale,
-                     a.dhidden + (int64_t)a.index[n] * a.dhidden_stride + i, a.width - i);
+      store_sum<DT>(a.dhidden + (int64_t)row * a.dhidden_stride + i,
+                    sum_shares(a.sum + (int64_t)n * a.packed_width + i, step, splits), unscale, a.width - i);
   }
 }
 
