@@ -336,6 +336,19 @@ def test_every_tile_shape(ops, rows, hidden, vocab):
         run(ops, *make(rows, hidden, vocab, torch.bfloat16, rows + vocab, ignored))
 
 
+FEW = [(1, 2600, 1000), (16, 6400, 4096), (7, 1537, 333), (3, 64, 4096), (9, 72, 4097), (5, 264, 5000),
+       (16, 1600, 30001), (16, 128, 70000), (17, 1600, 500), (40, 128, 70000)]
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", FEW)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_few_rows(ops, rows, hidden, vocab, dtype):
+    """Up to 64 rows: the tiles whose waves share the sum (whole turns, ends
+    inside a turn, fewer slices than waves) and their neighbours."""
+    for ignored in (0.0, 0.6):
+        run(ops, *make(rows, hidden, vocab, dtype, rows + hidden, ignored))
+
+
 def test_weight_rows_in_a_wider_store_with_other_values_around(ops):
     """What lies between and around the weight's rows is not part of it: NaN
     there changes nothing (in place and packed)."""
