@@ -36,65 +36,13 @@
 // the hidden index for both gradients.  The tile loop: hprms_product.h.
 #pragma once
 
+#include "hprms_loss_rows.h"
 #include "hprms_product.h"
 
 namespace hprms {
 
-// 8 and 16 bytes at any 2-byte boundary
-typedef u32x4 u32x4_u __attribute__((aligned(2)));
+// 8 bytes at any 2-byte boundary
 typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(2)));
-
-// What the row list says, written by loss_pack_kernel.
-struct LossMeta {
-  int32_t count;   // listed rows
-  float scale;     // gradient: applied to dloss
-  float unscale;   // its inverse
-  int32_t pad;
-};
-
-// The arguments of every loss kernel.  Listed rows are numbered by their
-// position in the list ("list position").
-struct LossArgs {
-  const uint16_t* hidden;
-  const uint16_t* weight;   // the piece's first row (the caller's, or packed)
-  const int64_t* target;
-  const LossMeta* meta;
-  const int32_t* index;     // the row of each list position
-  const uint16_t* packed;   // the listed rows' hidden values, [rows, packed_width], zeros past width
-  const uint16_t* turned;   // gradient: packed transposed, [packed_width, turned_stride], zeros from count to a multiple of 64
-  int64_t hidden_stride;
-  int64_t ignore_index;
-  int32_t weight_stride;    // elements, a multiple of 8
-  int32_t weight_width;     // readable elements of a weight row, a multiple of 8
-  int32_t packed_width;     // a multiple of 64
-  int32_t turned_stride;    // rows rounded up to a multiple of 64
-  int32_t rows;             // of the call
-  int32_t width;            // elements of a hidden row
-  int32_t vocab;
-  int32_t piece_from, piece;  // vocabulary rows of this launch
-  int32_t vocab_tiles, width_tiles;  // tiles of this launch
-  // forward
-  float* loss;
-  float* lse;               // gradient: read
-  float* target_logit;      // [rows], by list position
-  float2* partial;          // [vocabulary tiles, rows_at]: maximum and sum of exponentials
-  int32_t row_from, rows_at;  // list positions of this launch: [row_from, row_from + rows_at)
-  int32_t tile_from;        // vocabulary tiles before this piece
-  // gradient
-  int32_t dz_stride;
-  const float* dloss;
-  uint16_t* dz;             // [rows rounded up, dz_stride], by list position
-  uint16_t* dhidden;
-  int64_t dhidden_stride;
-  uint16_t* dweight;
-  int64_t dweight_stride;
-  float* sum;               // [splits, count, packed_width] shares of dhidden, by list position; null: none
-  int32_t first_piece;
-  int32_t piece_size, slots, most_splits;  // see splits_of
-  float* weight_sum;        // [splits, piece rounded up to 128, packed_width] shares of dweight; null: none
-  int32_t weight_most;      // splits of dweight at most
-  int32_t pack_rows;        // rows per workgroup of the packing kernel
-};
 
 // ---- epilogues ------------------------------------------------------------------------
 // Each sees a wave's tile of MI x NI fragments whose first row and column are
@@ -257,16 +205,6 @@ __device__ __forceinline__ void dz_epilogue(const LossArgs& a, const f32x4 (&acc
       *(u32x2*)(to + m) = u32x2{F::pack(d[0], d[1]), F::pack(d[2], d[3])};
     }
   }
-}
-
-// 8 elements p[0 ... 7], of which the first n exist (n may be negative); the others read as 0
-__device__ __forceinline__ u32x4 load_some(const uint16_t* p, int n) {
-  if (n >= 8) return *(const u32x4_u*)p;
-  u32x4 v = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < n) v[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
-  return v;
 }
 
 template <int DT>
