@@ -337,8 +337,8 @@ int64_t packed_piece(int64_t width, int64_t vocab) {
 // row's exponentials, and 16 x 16 its logits, in other orders, which shows in the
 // last bits of its lse.
 enum LogitTile { kTile16Sum, kTile16Short, kTile64Short, kTile16, kTile64, kTileSmall, kTile128, kTile256 };
-LogitTile logit_tile(int64_t rows, int64_t vocab) {
-  if (hprms_batch_invariant()) return kTile256;
+LogitTile logit_tile(int64_t rows, int64_t vocab, bool invariant) {
+  if (invariant) return kTile256;
   if (rows <= 64) {
     if (rows <= 16 && ceil_div(vocab, 16) <= current_cus()) return kTile16Sum;
     if (ceil_div(vocab, 128) < 2 * (int64_t)current_cus()) return rows <= 16 ? kTile16Short : kTile64Short;
@@ -357,16 +357,19 @@ int64_t logit_rows(LogitTile t) {
                                              : 128;
 }
 
-// Offsets of the workspace's parts, bytes.
+// Offsets of the workspace's parts, bytes.  A call reads the batch-invariant
+// mode once, into its plan.
 struct ForwardPlan {
   int64_t index, target_logit, packed, weight, partial, total;
   int64_t rows_at, tiles, piece;
   LogitTile tile;
+  bool invariant;
 };
 
-ForwardPlan forward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_place) {
+ForwardPlan forward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_place, bool invariant) {
   ForwardPlan p;
-  p.tile = logit_tile(rows, vocab);
+  p.invariant = invariant;
+  p.tile = logit_tile(rows, vocab, invariant);
   p.rows_at = min64(rows, kRowChunk);
   p.piece = in_place ? round_up(vocab, kPieceUnit) : packed_piece(width, vocab);
   p.tiles = ceil_div(vocab, logit_vocab_rows(p.tile));
@@ -388,9 +391,9 @@ struct BackwardPlan {
   LogitTile tile;
 };
 
-BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_place) {
+BackwardPlan backward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_place, bool invariant) {
   BackwardPlan p;
-  p.tile = logit_tile(rows, vocab);
+  p.tile = logit_tile(rows, vocab, invariant);
   p.dz_rows = round_up(max64(rows, 1), logit_rows(p.tile));
   p.piece = max64(kPieceElements / max64(p.dz_rows, 256) / kPieceUnit * kPieceUnit, 4 * kPieceUnit);
   p.piece = min64(p.piece, round_up(vocab, kPieceUnit));
@@ -530,7 +533,7 @@ int run_forward(LossArgs a, const ForwardPlan& p, const Weight& w, char* ws, hip
       }
       a.tile_from += (int32_t)ceil_div(a.piece, logit_vocab_rows(p.tile));
     }
-    if (here < 256 && !hprms_batch_invariant())
+    if (here < 256 && !p.invariant)
       loss_join_kernel<1><<<dim3((unsigned)here), dim3(256), 0, stream>>>(a, (int32_t)p.tiles);
     else
       loss_join_kernel<16><<<dim3((unsigned)((here + 15) / 16)), dim3(256), 0, stream>>>(a, (int32_t)p.tiles);
@@ -605,11 +608,14 @@ using namespace hprms;
 
 extern "C" {
 
+// Enough for either mode: the mode may change between the query and the call.
 int64_t hprms_linear_cross_entropy_workspace(int64_t rows, int64_t hidden_size, int64_t vocab, const void* weight,
                                              int64_t weight_row_stride) {
   const int rc = check_sizes(rows, hidden_size, vocab);
   if (rc != HPRMS_OK) return rc;
-  return forward_plan(rows, hidden_size, vocab, weight_in_place(weight, weight_row_stride, hidden_size)).total;
+  const bool in_place = weight_in_place(weight, weight_row_stride, hidden_size);
+  return max64(forward_plan(rows, hidden_size, vocab, in_place, false).total,
+               forward_plan(rows, hidden_size, vocab, in_place, true).total);
 }
 
 int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, const void* weight, const int64_t* target,
@@ -622,7 +628,7 @@ int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, cons
   if (!loss || !lse || !aligned_to(loss, 4) || !aligned_to(lse, 4))
     return fail(HPRMS_E_INVALID, "null or misaligned tensor pointer (loss, lse)");
   const bool in_place = weight_in_place(weight, weight_row_stride, hidden_size);
-  const ForwardPlan p = forward_plan(rows, hidden_size, vocab, in_place);
+  const ForwardPlan p = forward_plan(rows, hidden_size, vocab, in_place, hprms_batch_invariant() != 0);
   rc = check_workspace(workspace, workspace_size, p.total);
   if (rc != HPRMS_OK) return rc;
   char* ws = (char*)workspace;
@@ -652,7 +658,9 @@ int64_t hprms_linear_cross_entropy_backward_workspace(int64_t rows, int64_t hidd
                                                       const void* weight, int64_t weight_row_stride) {
   const int rc = check_sizes(rows, hidden_size, vocab);
   if (rc != HPRMS_OK) return rc;
-  return backward_plan(rows, hidden_size, vocab, weight_in_place(weight, weight_row_stride, hidden_size)).total;
+  const bool in_place = weight_in_place(weight, weight_row_stride, hidden_size);
+  return max64(backward_plan(rows, hidden_size, vocab, in_place, false).total,
+               backward_plan(rows, hidden_size, vocab, in_place, true).total);
 }
 
 int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const float* dloss, const void* hidden,
@@ -672,7 +680,7 @@ int hprms_linear_cross_entropy_backward(void* dhidden, void* dweight, const floa
   if (!aligned_to(dweight, 2) || !aligned_to(dhidden, 2) || !aligned_to(dloss, 4) || !aligned_to(lse, 4))
     return fail(HPRMS_E_INVALID, "tensors must be aligned to their elements");
   const bool in_place = weight_in_place(weight, weight_row_stride, hidden_size);
-  const BackwardPlan p = backward_plan(rows, hidden_size, vocab, in_place);
+  const BackwardPlan p = backward_plan(rows, hidden_size, vocab, in_place, hprms_batch_invariant() != 0);
   rc = check_workspace(workspace, workspace_size, p.total);
   if (rc != HPRMS_OK) return rc;
   char* ws = (char*)workspace;

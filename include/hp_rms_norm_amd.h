@@ -404,7 +404,7 @@ int hprms_rmsnorm_backward(void* dinput, void* dweight, const void* dout, const 
  * [0, vocab) gives a NaN loss.  The workspace is as for
  * hprms_rmsnorm_backward(), 256-byte aligned, of
  * hprms_linear_cross_entropy_workspace() bytes, which depends on the weight's
- * address and row stride: rows that 16-byte loads cannot take in place (an
+ * address and row stride, and is enough in either batch-invariant mode: rows that 16-byte loads cannot take in place (an
  * address or stride off 16 bytes, hidden_size % 8 != 0, a stride above 2^21)
  * are packed there, a piece of the vocabulary at a time.  rows == 0 is a no-op.
  * rows, hidden_size and vocab go up to 2^22, 2^20 and 2^28.  No counterpart in
@@ -427,8 +427,8 @@ int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, cons
  * dhidden and no part in dweight, whatever their hidden values and dloss are; an
  * out-of-range target gives NaN gradients.  Both outputs are written, not added
  * to (rows == 0 zeroes dweight), and overlap none of the inputs.  Workspace:
- * hprms_linear_cross_entropy_backward_workspace() bytes, 256-byte aligned.  No
- * counterpart in the reference.
+ * hprms_linear_cross_entropy_backward_workspace() bytes, 256-byte aligned,
+ * enough in either batch-invariant mode.  No counterpart in the reference.
  */
 int64_t hprms_linear_cross_entropy_backward_workspace(int64_t rows, int64_t hidden_size, int64_t vocab,
                                                       const void* weight, int64_t weight_row_stride);
