@@ -216,10 +216,26 @@ def rms_norm_backward_out(dinput, dweight, dout, input, weight, eps, dresidual=N
     torch.ops.hp_rms_norm.rms_norm_backward.default(dinput, dweight, dout, input, weight, dresidual, eps)
 
 
+def _rows(t):
+    """``t`` if its rows can be read in place, else a contiguous copy."""
+    if t.is_contiguous():
+        return t
+    if t.dim() >= 2 and t.stride(-1) == 1 and t.stride(-2) >= t.size(-1) and all(
+            t.stride(i) == t.stride(i + 1) * t.size(i + 1) for i in range(t.dim() - 2)):
+        return t
+    return t.contiguous()
+
+
 def rms_norm_backward(dout, input, weight, eps, dresidual=None):
     """Allocating form of ``rms_norm_backward_out``: returns ``(dinput,
-    dweight)`` in the dtypes of ``input`` and ``weight``."""
-    dinput, dweight = torch.empty_like(dout), torch.empty_like(weight)
+    dweight)`` in the shapes and dtypes of ``input`` and ``weight``.  ``dout``
+    and ``dresidual`` may have any strides, as torch's engine hands them on
+    (expanded by a sum, permuted by a consumer): rows that cannot be read in
+    place are copied first."""
+    dout = _rows(dout)
+    if dresidual is not None:
+        dresidual = _rows(dresidual)
+    dinput, dweight = torch.empty_like(input), torch.empty_like(weight)
     torch.ops.hp_rms_norm.rms_norm_backward.default(dinput, dweight, dout, input, weight, dresidual, eps)
     return dinput, dweight
 

@@ -1,11 +1,13 @@
 """Calls of the training operators that their documentation allows, beside
 the ordinary ones: the mode that changes between a workspace's query and the
-call.  Bounds: tests/test_gpu_loss.py."""
+call, and gradients in the layouts that torch's engine hands on.  Bounds:
+tests/test_gpu_loss.py, tests/test_gpu_norm_backward.py."""
 import pytest
 import torch
 
 from hp_rms_norm_amd import abi
 from test_gpu_loss import check_backward, check_forward, make
+from test_gpu_norm_backward import check as check_norm_backward
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -45,3 +47,47 @@ def test_the_mode_changes_between_a_workspace_and_its_call(ops, rows, hidden, vo
             assert torch.equal(loss, want[0]) and torch.equal(lse, want[1])
     finally:
         ops.set_batch_invariant(previous)
+
+
+class AddNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ops, x, r, w):
+        n, s = ops.fused_add_rms_norm(x, r, w, 1e-6)
+        ctx.ops = ops
+        ctx.save_for_backward(s, w)
+        return n, s
+
+    @staticmethod
+    def backward(ctx, dn, ds):
+        s, w = ctx.saved_tensors
+        ctx.ops.seen.append((dn, ds))
+        d, dw = ctx.ops.rms_norm_backward(dn, s, w, 1e-6, dresidual=ds)
+        return None, d, d, dw
+
+
+class Recorder:
+    def __init__(self, ops):
+        self.seen = []
+        self.fused_add_rms_norm, self.rms_norm_backward = ops.fused_add_rms_norm, ops.rms_norm_backward
+
+
+@pytest.mark.parametrize("hidden", [64, 96, 1000])
+def test_gradients_as_the_engine_hands_them_on(ops, hidden):
+    """Expanded gradients (of a sum) and permuted ones (of a consumer that
+    transposed the output) of both outputs, against the formula with the same
+    gradients written out; and nothing of what the engine holds is changed."""
+    g = torch.Generator(device=DEV).manual_seed(hidden)
+    x, r = (torch.randn((6, 10, hidden), generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    w = (1 + 0.1 * torch.randn(hidden, generator=g, device=DEV)).to(torch.bfloat16)
+    c = torch.randn((10, 6, hidden), generator=g, device=DEV).to(torch.bfloat16)
+    for value in (lambda n, s: n.sum() + s.sum(),
+                  lambda n, s: (n.transpose(0, 1) * c).sum() + s.sum(),
+                  lambda n, s: n[:, :, :1].sum() + (s.permute(2, 1, 0) * c.permute(2, 0, 1)).sum()):
+        rec = Recorder(ops)
+        leaves = [v.clone().requires_grad_() for v in (x, r, w)]
+        n, s = AddNorm.apply(rec, *leaves)
+        value(n, s).backward()
+        ((dn, ds),) = rec.seen
+        flat = [v.detach().contiguous().view(60, hidden) for v in (s, dn, ds)]
+        check_norm_backward(leaves[0].grad.view(60, hidden), leaves[2].grad, flat[0], flat[1], flat[2], w)
+        assert torch.equal(leaves[0].grad, leaves[1].grad)
