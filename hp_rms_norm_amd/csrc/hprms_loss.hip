@@ -290,6 +290,9 @@ constexpr int64_t kMaxLossRows = int64_t(1) << 22;
 constexpr int64_t kMaxLossWidth = int64_t(1) << 20;
 constexpr int64_t kMaxVocab = int64_t(1) << 28;
 constexpr int64_t kRowChunk = 16384;  // list positions per forward launch: bounds the partial sums
+// tiles per forward launch, a multiple of 8: with up to 512 lanes each they stay
+// below the 2^32 work-items that a launch may hold
+constexpr int64_t kForwardTiles = (int64_t(1) << 23) - 8;
 constexpr int64_t kPieceElements = int64_t(1) << 27;  // of dz, and of a packed weight, per piece: 256 MiB
 constexpr int64_t kHiddenTile = 256;  // hidden elements of a dhidden tile
 constexpr int64_t kPieceUnit = 256;   // pieces are whole tiles of every kernel
@@ -370,9 +373,9 @@ ForwardPlan forward_plan(int64_t rows, int64_t width, int64_t vocab, bool in_pla
   ForwardPlan p;
   p.invariant = invariant;
   p.tile = logit_tile(rows, vocab, invariant);
-  p.rows_at = min64(rows, kRowChunk);
   p.piece = in_place ? round_up(vocab, kPieceUnit) : packed_piece(width, vocab);
   p.tiles = ceil_div(vocab, logit_vocab_rows(p.tile));
+  p.rows_at = min64(min64(rows, kRowChunk), kForwardTiles / p.tiles * logit_rows(p.tile));
   p.index = 256;
   p.target_logit = p.index + round_up(rows * 4, 256);
   p.packed = p.target_logit + round_up(rows * 4, 256);

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from hp_rms_norm_amd import abi
-from test_gpu_loss import check_backward, check_forward, make
+from test_gpu_loss import E, check_backward, check_forward, k_of, make
 from test_gpu_norm_backward import check as check_norm_backward
 
 pytestmark = pytest.mark.gpu
@@ -91,3 +91,29 @@ def test_gradients_as_the_engine_hands_them_on(ops, hidden):
         flat = [v.detach().contiguous().view(60, hidden) for v in (s, dn, ds)]
         check_norm_backward(leaves[0].grad.view(60, hidden), leaves[2].grad, flat[0], flat[1], flat[2], w)
         assert torch.equal(leaves[0].grad, leaves[1].grad)
+
+
+def test_more_tiles_than_one_launch_holds(ops):
+    """16384 rows of 2^25 + 1 vocabulary entries are 2^23 tiles of 512 lanes and
+    more: 2^32 work-items.  A row's sum joins 131073 tiles, 16 lanes apart, each
+    addition off by at most 3 e (its exponential and its step), besides what
+    test_gpu_loss.py's bound counts."""
+    rows, hidden, vocab = 16384, 64, (1 << 25) + 1
+    g = torch.Generator(device=DEV).manual_seed(5)
+    w = torch.randn((vocab, hidden), generator=g, device=DEV, dtype=torch.bfloat16) * 0.25
+    h = torch.randn((rows, hidden), generator=g, device=DEV, dtype=torch.bfloat16)
+    t = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+    t[-2], t[5] = vocab - 1, -100
+    loss, lse = ops.linear_cross_entropy(h, w, t)
+    at = torch.tensor([0, 1, 5, 300, 16127, 16128, 16129, rows - 2, rows - 1], device=DEV)
+    total, size = (torch.zeros(len(at), device=DEV, dtype=torch.float64) for _ in range(2))
+    for part in w.split(1 << 22):
+        total += torch.exp(h[at].double() @ part.double().t()).sum(1)
+        size = torch.maximum(size, (h[at].double().abs() @ part.double().abs().t()).amax(1))
+    want = torch.where(t[at] == -100, 0.0, total.log())
+    bound = k_of(hidden) * E * size + 2.0 ** -16 + (131073 / 16 + 128) * 3 * E + E * want.abs()
+    assert bool(((lse[at].double() - want).abs() <= bound).all())
+    z = (h[at].double() * w[t[at].clamp(min=0)].double()).sum(1)
+    want = torch.where(t[at] == -100, 0.0, want - z)
+    assert bool(((loss[at].double() - want).abs() <= 2 * bound + E * want.abs()).all())
+    assert bool(torch.isfinite(loss).all())
