@@ -117,3 +117,65 @@ def test_more_tiles_than_one_launch_holds(ops):
     want = torch.where(t[at] == -100, 0.0, want - z)
     assert bool(((loss[at].double() - want).abs() <= 2 * bound + E * want.abs()).all())
     assert bool(torch.isfinite(loss).all())
+
+
+def test_torch_compile_with_the_training_operators(ops):
+    """torch.compile (aot_eager: no codegen, fullgraph) traces the operators
+    through their Meta kernels and functionalises what they write, the list of
+    clip_grad_norm_ too: every output and every tensor written in place is the
+    eager call's, bit for bit."""
+    h, w, t, _ = make(40, 128, 300, torch.bfloat16, 30, 0.2)
+    g = torch.Generator(device=DEV).manual_seed(31)
+    r, dr = (torch.randn((40, 128), generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    nw = (1 + 0.1 * torch.randn(128, generator=g, device=DEV)).to(torch.bfloat16)
+    bias = torch.randn(77, generator=g, device=DEV)
+
+    def f(h, r, nw, w, t, dr, bias):
+        n, s = ops.fused_add_rms_norm(h, r, nw, 1e-6)
+        loss, lse = ops.linear_cross_entropy(n, w, t)
+        dn, dw = ops.linear_cross_entropy_backward(torch.full((), 0.03125, device=DEV), n, w, t, lse)
+        dx, dnw = ops.rms_norm_backward(dn, s, nw, 1e-6, dresidual=dr.expand(40, 128))
+        into, dnw32 = torch.empty_like(dn), torch.empty(128, device=DEV)
+        ops.rms_norm_backward_out(into, dnw32, dn, s, nw, 1e-6)
+        loss2, lse2 = torch.empty_like(loss), torch.empty_like(lse)
+        ops.linear_cross_entropy_out(loss2, lse2, n, w, t)
+        dn2, dw2 = torch.empty_like(dn), torch.empty_like(dw)
+        ops.linear_cross_entropy_backward_out(dn2, dw2, loss * 0.5, n, w, t, lse)
+        db = bias * 0.5
+        grads = [dw, dnw, db]
+        plain = ops.grad_norm(grads)
+        wide = [torch.empty(v.shape, device=DEV) for v in grads]
+        copied = ops.clip_grad_norm_out(wide, grads, 0.25)
+        clipped = ops.clip_grad_norm_(grads, 0.25)
+        again = ops.clip_grad_norm_([bias], 0.5)  # an input of the traced function, in place
+        return (loss, lse, dx, into, dnw32, loss2, lse2, dn2, dw2, plain, copied, clipped, again, *grads, *wide)
+
+    args = (h, r, nw, w, t, dr[:1])
+    b1, b2 = bias.clone(), bias.clone()
+    want = f(*args, b1)
+    got = torch.compile(f, backend="aot_eager", fullgraph=True)(*args, b2)
+    torch.cuda.synchronize()
+    assert torch.equal(b1, b2) and not torch.equal(b1, bias)
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert a.dtype == b.dtype and a.shape == b.shape, i
+        assert torch.equal(a, b), f"output {i} differs"
+
+
+def test_opcheck_of_the_training_operators(ops):
+    """torch's own check of schemas (what is written and what is not), Meta
+    kernels and functionalisation."""
+    h, w, t, dloss = make(12, 64, 100, torch.bfloat16, 32, 0.2)
+    loss, lse = ops.linear_cross_entropy(h, w, t)
+    nw = torch.ones(64, device=DEV, dtype=torch.bfloat16)
+    o = torch.ops.hp_rms_norm
+    grads = [torch.randn(5, device=DEV), torch.randn((3, 4), device=DEV).to(torch.float16)]
+    norm = torch.empty((), device=DEV)
+    for op, args in (
+            (o.rms_norm_backward, (torch.empty_like(h), torch.empty_like(nw), h.clone(), h, nw, None, 1e-6)),
+            (o.linear_cross_entropy, (loss.clone(), lse.clone(), h, w, t, -100)),
+            (o.linear_cross_entropy_backward,
+             (torch.empty_like(h), torch.empty_like(w), dloss, h, w, t, lse, -100)),
+            (o.grad_norm, (norm, grads)),
+            (o.clip_grad_norm_, (norm, [v.clone() for v in grads], 0.5)),
+            (o.clip_grad_norm_out, (norm, [torch.empty_like(v) for v in grads], grads, 0.5))):
+        torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor", "test_aot_dispatch_static"))
