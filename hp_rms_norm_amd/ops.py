@@ -267,7 +267,10 @@ def linear_cross_entropy_backward_out(dhidden, dweight, dloss, hidden, weight, t
     ``dweight <- dz.T @ hidden``.  ``lse`` is the forward call's, ``dloss``
     the gradient of each row's loss (float32 like ``target``; for a mean over
     n rows, 1 / n each).  The logits are computed again, a piece of the
-    vocabulary at a time; ``dz`` is rounded to the tensors' dtype, sums are
+    vocabulary at a time; ``dz`` is rounded to the tensors' dtype (in fp16 its
+    entries are off by half a step or by 2^-39 of the call's largest
+    ``|dloss|``, whichever is more: rows whose ``dloss`` is 2^16 or more below
+    the largest are more precise in bf16, or in a call of their own), sums are
     fp32 and each output is rounded once.  Ignored rows get a zero
     ``dhidden`` and no part in ``dweight``; an out-of-range target makes the
     gradients NaN.  No reference counterpart."""

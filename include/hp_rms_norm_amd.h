@@ -422,8 +422,9 @@ int hprms_linear_cross_entropy(float* loss, float* lse, const void* hidden, cons
  * dloss[i] of each row's loss:
  *   dz = (exp(z - lse) - [v == target]) * dloss;  dhidden <- dz . weight;  dweight <- dz^T . hidden
  * The logits are computed again, a piece of the vocabulary at a time; dz is
- * rounded to dtype (at a scale that suits the largest dloss), the products are
- * summed in binary32 and rounded once.  Ignored rows get a zero
+ * rounded to dtype at one scale for all rows, which suits the largest |dloss| (an
+ * entry is off by half a step of dtype, in float16 at least 2^-39 of the largest
+ * |dloss|), the products are summed in binary32 and rounded once.  Ignored rows get a zero
  * dhidden and no part in dweight, whatever their hidden values and dloss are; an
  * out-of-range target gives NaN gradients.  Both outputs are written, not added
  * to (rows == 0 zeroes dweight), and overlap none of the inputs.  Workspace:

@@ -179,3 +179,60 @@ def test_opcheck_of_the_training_operators(ops):
             (o.clip_grad_norm_, (norm, [v.clone() for v in grads], 0.5)),
             (o.clip_grad_norm_out, (norm, [torch.empty_like(v) for v in grads], grads, 0.5))):
         torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor", "test_aot_dispatch_static"))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_gradients_of_many_rows_in_many_pieces(ops, dtype):
+    """33000 rows: dz goes in pieces of 3840 vocabulary entries, and dhidden's
+    shares run over 129 row tiles; an odd width and padded rows."""
+    h, w, t, dloss = make(33000, 72, 9001, dtype, 40, 0.1, pad=3, offset=1)
+    loss, lse = ops.linear_cross_entropy(h, w, t)
+    check_forward(loss, lse, h, w, t)
+    dh, dw = ops.linear_cross_entropy_backward(dloss, h, w, t, lse)
+    check_backward(dh, dw, h, w, t, dloss)
+
+
+def test_gradients_of_the_most_rows(ops):
+    """2^22 rows, where the offsets into the turned rows come closest to 2^31
+    bytes, in two pieces of the vocabulary; dhidden is looked at in some rows,
+    dweight whole."""
+    rows, hidden, vocab = 1 << 22, 40, 1100
+    h, w, t, dloss = make(rows, hidden, vocab, torch.bfloat16, 41, 0.05)
+    loss, lse = ops.linear_cross_entropy(h, w, t)
+    dh, dw = ops.linear_cross_entropy_backward(dloss, h, w, t, lse)
+    want_dw, bound_dw = (torch.zeros((vocab, hidden), device=DEV, dtype=torch.float64) for _ in range(2))
+    wd, u = w.double(), 2.0 ** -8
+    for at in torch.arange(rows, device=DEV).split(1 << 17):
+        check_forward(loss[at], lse[at], h[at], w, t[at])
+        kept = t[at] != -100
+        hd, g, to = h[at][kept].double(), dloss[at][kept].double()[:, None], t[at][kept]
+        z = hd @ wd.t()
+        p = torch.softmax(z, 1)
+        d = p.clone()
+        d[torch.arange(len(d), device=DEV), to] -= 1.0
+        d *= g
+        dz = k_of(hidden) * E * (hd.abs() @ wd.abs().t()).amax(1, keepdim=True)
+        db = u * d.abs() + p * g.abs() * (2 * dz + 2.0 ** -16)
+        off = (dh[at][kept].double() - d @ wd).abs()
+        assert bool((off <= ((db + k_of(vocab) * E * d.abs()) @ wd.abs() + u * (d @ wd).abs()) * (1 + u)).all())
+        assert not bool(dh[at][~kept].any())
+        want_dw += d.t() @ hd
+        bound_dw += (db + k_of(rows) * E * d.abs()).t() @ hd.abs()
+    assert bool(((dw.double() - want_dw).abs() <= (bound_dw + u * want_dw.abs()) * (1 + u)).all())
+
+
+def test_float16_rows_of_very_different_dloss(ops):
+    """One scale serves all rows, the one that takes the largest |dloss| to 2^14:
+    an entry of dz is off by half a step of float16 or by 2^-39 of the largest
+    |dloss|, whichever is more.  With dloss down to 2^-24 of the largest that
+    is the bound, and with one row a call each row has half a step."""
+    h, w, t, _ = make(60, 96, 700, torch.float16, 42)
+    g = torch.Generator(device=DEV).manual_seed(43)
+    dloss = 256.0 * torch.exp2(-torch.randint(0, 25, (60,), generator=g, device=DEV).float())
+    dloss[0] = 256.0
+    loss, lse = ops.linear_cross_entropy(h, w, t)
+    dh, dw = ops.linear_cross_entropy_backward(dloss, h, w, t, lse)
+    check_backward(dh, dw, h, w, t, dloss)
+    for i in range(0, 60, 7):
+        dh1, dw1 = ops.linear_cross_entropy_backward(dloss[i:i + 1], h[i:i + 1], w, t[i:i + 1], lse[i:i + 1])
+        check_backward(dh1, dw1, h[i:i + 1], w, t[i:i + 1], dloss[i:i + 1])
