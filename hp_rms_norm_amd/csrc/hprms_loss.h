@@ -22,15 +22,16 @@
 // dz is rounded to 16 bits because the matrix cores take 16-bit operands: a
 // relative error of half a step per entry, as the outputs' own rounding has.
 // dloss is scaled first so that its largest magnitude is 2^14, and the products
-// are scaled back in binary32: float16 then holds dz down to probabilities of
-// 2^-28 (subnormal from there on: off by up to 2^-39 of the largest |dloss|; a row
-// whose dloss is 2^-k of the largest reaches that at probabilities of 2^(k - 28)).
-// Scales of their own would serve such rows' dhidden, but dweight's sum over the
-// rows would then need them in float16's other operand, where they cost more.  And under one dloss for all rows, as a mean
-// of losses has it, an entry's error comes from p - 1 or p alone.  (Scaled by a
-// power of two instead, that dloss's own rounding, up to half a step, was
-// common to all entries of the targets: 0.0031 against 0.0023 relative error of
-// the gradients at 500 rows.)
+// are scaled back in binary32: under one dloss for all rows, as a mean of losses
+// has it, an entry's error then comes from p - 1 or p alone.  (Scaled by a power
+// of two instead, that dloss's own rounding, up to half a step, was common to
+// all entries of the targets: 0.0031 against 0.0023 relative error of the
+// gradients at 500 rows.)  float16 holds dz down to probabilities of 2^-28; from
+// there on it is subnormal, off by up to 2^-39 of the largest |dloss|, and a row
+// whose dloss is 2^-k of the largest gets there at probabilities of 2^(k - 28).
+// A scale for each row would serve such rows' dhidden, but dweight's sum over
+// the rows would then need its inverse in hidden, the other float16 operand,
+// which it would take below float16's normal numbers sooner.
 //
 // Fragments of v_mfma_f32_16x16x32: lane l holds A[l % 16][8 (l / 16) + j] and
 // B[8 (l / 16) + j][l % 16], j = 0 ... 7, and of the product the four rows

@@ -339,7 +339,7 @@ struct SumProduct {
 // the same time.
 //
 // 1.1 TFLOP of each kind, tiles in XCD-contiguous order, TFLOP/s (a library
-// product of the same sizes: 1450, 1100 and 1370):
+// product of the same sizes: 1340, 1070 and 1250):
 //
 //                                  32768 x 4096    4096 x 32768    4096 x 4096
 //                                  x 4096          x 4096          x 32768
@@ -349,10 +349,11 @@ struct SumProduct {
 //   64-byte rows a slice, 4 slices 1240            1240 (both)     1330
 //   the same without the phases    1080            920 (both)      960
 //
-// At 1.4 PFLOP/s a slice of 32 takes 1160-1180 cycles, of which the matrix cores
-// work 1024, and the clock falls from 2.4 to 1.7 GHz: power bounds it (a loop
-// of nothing but these instructions on random values reaches 2080 TFLOP/s at
-// 2.06 GHz; zeros run at 2.4 GHz).
+// A z tile over 4096 entries keeps its CU busy for 168 000 cycles, of which the
+// matrix cores work 131 000 (78%; dweight 68%, dhidden 70%), and under that load
+// the clock stands at 1.8-1.9 GHz.  A loop of nothing but these instructions on
+// random values reaches 2050 TFLOP/s at 2.0 GHz: most of the distance is matrix
+// cores that wait, at a tile's ends and for the slices, the rest the clock.
 template <int DT, bool AKO_, bool BKO_, int WM_ = 4>
 struct RingProduct {
   static constexpr int MT = 256, NT = 256, NW = 8, WM = WM_, WN = NW / WM, MI = MT / WM / 16, NI = NT / WN / 16;

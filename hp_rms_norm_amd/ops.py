@@ -245,7 +245,7 @@ def linear_cross_entropy_out(loss, lse, hidden, weight, target, ignore_index=-10
     without keeping the logits ``z = hidden @ weight.T``: ``lse <-
     logsumexp(z)`` and ``loss <- lse - z[target]`` per row.  ``hidden``: [..., H]
     bf16 or fp16; ``weight``: [V, H] of the same dtype; ``target``: int64
-    [...]; ``loss`` and ``lse``: float32 like ``target``.  Products and sums
+    [...], contiguous; ``loss`` and ``lse``: float32 like ``target``.  Products and sums
     are fp32.  Rows whose target is ``ignore_index`` get 0 and 0 and are never
     read (padding may hold anything); another target outside ``[0, V)`` gives
     a NaN loss.  No reference counterpart."""
