@@ -18,7 +18,7 @@ HPRMS_OK = 0
 HPRMS_E_INVALID = -22
 HPRMS_E_LAUNCH = -5
 HPRMS_E_RANGE = -34
-DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2  # FP32: gradients only
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2  # FP32: gradients and logits only
 STREAM_COPY, STREAM_RELU = 0, 1
 MAX_PARTS = 8
 # the `mode` numbering of hprms_select_config / hprms_kernel_configs
@@ -46,6 +46,15 @@ SYMBOLS = (
     "hprms_grad_norm_workspace",
     "hprms_grad_norm",
     "hprms_clip_grad_norm",
+    "hprms_norm_add_rmsnorm",
+    "hprms_norm_add_rmsnorm_int8",
+    "hprms_norm_add_rmsnorm_backward_workspace",
+    "hprms_norm_add_rmsnorm_backward",
+    "hprms_int8_linear_workspace",
+    "hprms_int8_linear",
+    "hprms_token_log_probs_workspace",
+    "hprms_token_log_probs",
+    "hprms_token_log_probs_backward",
     "hprms_fused_add_rmsnorm_config",
     "hprms_select_config",
     "hprms_select_config_cu",
@@ -99,8 +108,19 @@ def _bind(L, bench):
     L.hprms_grad_norm_workspace.argtypes = [pi64, ci]
     L.hprms_grad_norm.argtypes = [vp, pvp, pci, pi64, ci, vp, i64, vp]
     L.hprms_clip_grad_norm.argtypes = [vp, pvp, pci, pvp, pci, pi64, ci, cd, vp, i64, vp]
+    L.hprms_norm_add_rmsnorm.argtypes = [vp] * 7 + [i64] * 8 + [ci, cd, cd, vp]
+    L.hprms_norm_add_rmsnorm_int8.argtypes = [vp] * 8 + [i64] * 8 + [ci, cd, cd, vp]
+    L.hprms_norm_add_rmsnorm_backward_workspace.argtypes = [i64] * 3
+    L.hprms_norm_add_rmsnorm_backward.argtypes = [vp] * 13 + [i64] * 12 + [ci] * 3 + [cd, cd, vp]
+    L.hprms_int8_linear_workspace.argtypes = [i64] * 3 + [vp, i64, vp, i64]
+    L.hprms_int8_linear.argtypes = [vp] * 7 + [i64] * 7 + [ci, vp]
+    L.hprms_token_log_probs_workspace.argtypes = [i64] * 3 + [ci]
+    L.hprms_token_log_probs.argtypes = [vp] * 8 + [i64] * 6 + [ci, vp]
+    L.hprms_token_log_probs_backward.argtypes = [vp] * 7 + [i64] * 5 + [ci, vp]
     for name in ("hprms_rmsnorm_backward_workspace", "hprms_linear_cross_entropy_workspace",
-                 "hprms_linear_cross_entropy_backward_workspace", "hprms_grad_norm_workspace"):
+                 "hprms_linear_cross_entropy_backward_workspace", "hprms_grad_norm_workspace",
+                 "hprms_norm_add_rmsnorm_backward_workspace", "hprms_int8_linear_workspace",
+                 "hprms_token_log_probs_workspace"):
         getattr(L, name).restype = i64
     L.hprms_streamer.argtypes = [vp, vp, i64, i64, i64, i64, ci, ci, vp]
     L.hprms_select_config.argtypes = [i64, i64, ci, ci, ctypes.POINTER(Config)]
@@ -119,7 +139,8 @@ def _bind(L, bench):
              "hprms_reduce_add_rmsnorm",
              "hprms_fused_add_rmsnorm_mx", "hprms_rmsnorm_backward", "hprms_linear_cross_entropy",
              "hprms_linear_cross_entropy_backward", "hprms_grad_norm", "hprms_clip_grad_norm",
-             "hprms_streamer", "hprms_select_config", "hprms_select_config_cu",
+             "hprms_norm_add_rmsnorm", "hprms_norm_add_rmsnorm_int8", "hprms_norm_add_rmsnorm_backward",
+             "hprms_int8_linear", "hprms_token_log_probs", "hprms_token_log_probs_backward", "hprms_streamer", "hprms_select_config", "hprms_select_config_cu",
              "hprms_device_cu_count", "hprms_kernel_configs", "hprms_set_batch_invariant", "hprms_batch_invariant"]
     if bench:
         L.hprms_bench_fused_timeline.argtypes = [vp, vp, vp, i64, i64, ci, cd, ctypes.POINTER(Config), vp, vp]
@@ -299,6 +320,68 @@ class Library:
         return self._check(self.lib().hprms_clip_grad_norm(norm_ptr, o, od, g, d, c, n, max_norm, workspace_ptr,
                                                            workspace_size, stream))
 
+    def norm_add_rmsnorm(self, out_ptr, residual_out_ptr, input_ptr, post_weight_ptr, weight_ptr, residual_ptr,
+                         gate_ptr, rows, hidden, rows_per_gate, out_stride, residual_out_stride, input_stride,
+                         residual_stride, gate_stride, dtype, residual_scale, eps, stream=0):
+        return self._check(self.lib().hprms_norm_add_rmsnorm(
+            out_ptr, residual_out_ptr, input_ptr, post_weight_ptr, weight_ptr, residual_ptr, gate_ptr, rows, hidden,
+            rows_per_gate, out_stride, residual_out_stride, input_stride, residual_stride, gate_stride, dtype,
+            residual_scale, eps, stream))
+
+    def norm_add_rmsnorm_int8(self, out_ptr, scale_ptr, residual_out_ptr, input_ptr, post_weight_ptr, weight_ptr,
+                              residual_ptr, gate_ptr, rows, hidden, rows_per_gate, out_stride, residual_out_stride,
+                              input_stride, residual_stride, gate_stride, dtype, residual_scale, eps, stream=0):
+        return self._check(self.lib().hprms_norm_add_rmsnorm_int8(
+            out_ptr, scale_ptr, residual_out_ptr, input_ptr, post_weight_ptr, weight_ptr, residual_ptr, gate_ptr, rows,
+            hidden, rows_per_gate, out_stride, residual_out_stride, input_stride, residual_stride, gate_stride, dtype,
+            residual_scale, eps, stream))
+
+    def norm_add_rmsnorm_backward_workspace(self, rows, hidden, gate_rows):
+        return self._bytes(self.lib().hprms_norm_add_rmsnorm_backward_workspace(rows, hidden, gate_rows))
+
+    def norm_add_rmsnorm_backward(self, dinput_ptr, dresidual_in_ptr, dpost_weight_ptr, dweight_ptr, dgate_ptr,
+                                  dout_ptr, dresidual_ptr, input_ptr, residual_ptr, post_weight_ptr, weight_ptr,
+                                  gate_ptr, workspace_ptr, workspace_size, rows, hidden, gate_rows, dinput_stride,
+                                  dresidual_in_stride, dgate_stride, dout_stride, dresidual_stride, input_stride,
+                                  residual_stride, gate_stride, dtype, dpost_weight_dtype, dweight_dtype,
+                                  residual_scale, eps, stream=0):
+        return self._check(self.lib().hprms_norm_add_rmsnorm_backward(
+            dinput_ptr, dresidual_in_ptr, dpost_weight_ptr, dweight_ptr, dgate_ptr, dout_ptr, dresidual_ptr, input_ptr,
+            residual_ptr, post_weight_ptr, weight_ptr, gate_ptr, workspace_ptr, workspace_size, rows, hidden,
+            gate_rows, dinput_stride, dresidual_in_stride, dgate_stride, dout_stride, dresidual_stride, input_stride,
+            residual_stride, gate_stride, dtype, dpost_weight_dtype, dweight_dtype, residual_scale, eps, stream))
+
+    def int8_linear_workspace(self, rows, inner, outer, input_ptr=0, input_stride=None, weight_ptr=0,
+                              weight_stride=None):
+        """For operands at these addresses (default: any aligned ones) with
+        these strides between rows (default: ``inner``)."""
+        return self._bytes(self.lib().hprms_int8_linear_workspace(
+            rows, inner, outer, input_ptr, inner if input_stride is None else input_stride, weight_ptr,
+            inner if weight_stride is None else weight_stride))
+
+    def int8_linear(self, out_ptr, input_ptr, scale_ptr, weight_ptr, weight_scale_ptr, bias_ptr, workspace_ptr,
+                    workspace_size, rows, inner, outer, out_stride, input_stride, weight_stride, dtype, stream=0):
+        return self._check(self.lib().hprms_int8_linear(
+            out_ptr, input_ptr, scale_ptr, weight_ptr, weight_scale_ptr, bias_ptr, workspace_ptr, workspace_size,
+            rows, inner, outer, out_stride, input_stride, weight_stride, dtype, stream))
+
+    def token_log_probs_workspace(self, rows, vocab, top, dtype):
+        return self._bytes(self.lib().hprms_token_log_probs_workspace(rows, vocab, top, dtype))
+
+    def token_log_probs(self, log_prob_ptr, entropy_ptr, lse_ptr, top_log_prob_ptr, top_index_ptr, logits_ptr,
+                        tokens_ptr, workspace_ptr, workspace_size, rows, vocab, top, logits_stride, ignore_index,
+                        dtype, stream=0):
+        return self._check(self.lib().hprms_token_log_probs(
+            log_prob_ptr, entropy_ptr, lse_ptr, top_log_prob_ptr, top_index_ptr, logits_ptr, tokens_ptr, workspace_ptr,
+            workspace_size, rows, vocab, top, logits_stride, ignore_index, dtype, stream))
+
+    def token_log_probs_backward(self, dlogits_ptr, dlog_prob_ptr, dentropy_ptr, logits_ptr, tokens_ptr, lse_ptr,
+                                 entropy_ptr, rows, vocab, dlogits_stride, logits_stride, ignore_index, dtype,
+                                 stream=0):
+        return self._check(self.lib().hprms_token_log_probs_backward(
+            dlogits_ptr, dlog_prob_ptr, dentropy_ptr, logits_ptr, tokens_ptr, lse_ptr, entropy_ptr, rows, vocab,
+            dlogits_stride, logits_stride, ignore_index, dtype, stream))
+
     def streamer(self, out_ptr, in_ptr, rows, hidden, out_stride, in_stride, dtype, op, stream=0):
         return self._check(self.lib().hprms_streamer(out_ptr, in_ptr, rows, hidden, out_stride, in_stride, dtype,
                                                      op, stream))
@@ -390,6 +473,15 @@ linear_cross_entropy_backward = PRODUCT.linear_cross_entropy_backward
 grad_norm_workspace = PRODUCT.grad_norm_workspace
 grad_norm = PRODUCT.grad_norm
 clip_grad_norm = PRODUCT.clip_grad_norm
+norm_add_rmsnorm = PRODUCT.norm_add_rmsnorm
+norm_add_rmsnorm_int8 = PRODUCT.norm_add_rmsnorm_int8
+norm_add_rmsnorm_backward_workspace = PRODUCT.norm_add_rmsnorm_backward_workspace
+norm_add_rmsnorm_backward = PRODUCT.norm_add_rmsnorm_backward
+int8_linear_workspace = PRODUCT.int8_linear_workspace
+int8_linear = PRODUCT.int8_linear
+token_log_probs_workspace = PRODUCT.token_log_probs_workspace
+token_log_probs = PRODUCT.token_log_probs
+token_log_probs_backward = PRODUCT.token_log_probs_backward
 streamer = PRODUCT.streamer
 select_config = PRODUCT.select_config
 device_cu_count = PRODUCT.device_cu_count

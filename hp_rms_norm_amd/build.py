@@ -77,12 +77,13 @@ def _atomic(dst, build_fn):
 def build_kernels(bench=True):
     """Compiles every translation unit of csrc/ at once into a scratch
     directory, then links libhprms.so and (with `bench`) libhprms_bench.so.
-    The two share the variant, general-tier and training objects; hprms.hip is compiled
+    The two share the variant, general-tier, training and serving objects; hprms.hip is compiled
     once per library (HPRMS_BENCH_BUILD adds the bench-only shapes and entry
     point)."""
     hipcc = shutil.which("hipcc") or os.path.join(ROCM, "bin", "hipcc")
     shared_units = ["hprms_unaligned.hip", "hprms_tail.hip", "hprms_general.hip", "hprms_norm_grad.hip",
-                    "hprms_grad_norm.hip", "hprms_loss.hip"]
+                    "hprms_grad_norm.hip", "hprms_loss.hip", "hprms_norm_add.hip", "hprms_norm_add_grad.hip",
+                    "hprms_int8_linear.hip", "hprms_log_probs.hip"]
     units = [("hprms.hip", [])] + [(name, []) for name in shared_units]
     if bench:
         units += [("hprms.hip", ["-DHPRMS_BENCH_BUILD"]), ("hprms_ceiling.hip", [])]

@@ -1,0 +1,352 @@
+// hprms_int8_linear.hip - the product of 8-bit integer rows and weights with a scale
+// for each row and each output feature:
+//
+//   out[t, o] = rne((sum_k input[t, k] * weight[o, k]) * scale[t] * weight_scale[o] + bias[o])
+//
+// The sums are exact in 32-bit integers (up to 131071 terms of at most 2^14), so
+// their order, and with it every choice of tiles below, leaves no trace in the
+// result; a sum is rounded to binary32 once (24 bits of it, a relative error of
+// 2^-24 beside the output's own 2^-9 or 2^-12), then scaled.
+//
+// Few rows: the weight's bytes bound the call.  Up to 8 rows run on dot products of
+// 4 bytes, a wave reading whole KB of a weight's row, so the weight streams in whole
+// lines.  More rows run on the matrix cores (hprms_product.h), tiles by sizes.
+#include <hip/hip_runtime.h>
+
+#include "hprms_host.h"
+#include "hprms_product.h"
+
+namespace hprms {
+namespace {
+
+struct Int8Args {
+  const int8_t* input;
+  const int8_t* weight;
+  const float* scale;
+  const float* weight_scale;
+  const uint16_t* bias;  // null: none
+  uint16_t* out;
+  int64_t out_stride;
+  int64_t input_stride, weight_stride;  // bytes, multiples of 16
+  int32_t rows, inner, outer;           // inner: a multiple of 16
+  int32_t outer_tiles, row_tiles;
+};
+
+__device__ __forceinline__ float scaled(int32_t sum, float scale, float weight_scale, float bias) {
+  return __builtin_fmaf((float)sum * scale, weight_scale, bias);
+}
+
+// ---- few rows ------------------------------------------------------------------------------
+__device__ __forceinline__ int32_t wave_sum(int32_t v) {
+  v += (int32_t)dpp_u32<0xB1>((uint32_t)v);
+  v += (int32_t)dpp_u32<0x4E>((uint32_t)v);
+  v += (int32_t)dpp_u32<0x141>((uint32_t)v);
+  v += (int32_t)dpp_u32<0x140>((uint32_t)v);
+  v += __builtin_amdgcn_ds_swizzle(v, 0x401F);
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 32);
+}
+
+// A workgroup takes W rows of the weight and all N rows of the input; its 4 waves
+// take KB of the summed index in turn.
+template <int DT, int N, int W>
+__global__ __launch_bounds__(256) void int8_few_rows_kernel(Int8Args a) {
+  using F = Fmt<DT>;
+  constexpr int U = 2;  // KB of a row on their way at once, ahead of those in use
+  __shared__ int32_t lds[4][N * W];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t first = blockIdx.x * W;
+  u32x4 w[U][W], x[U][N];
+  auto load = [&](int u, int32_t kb) {
+    const int32_t k = kb * 1024 + lane * 16;
+    const bool in = k < a.inner;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int32_t o = first + i < a.outer ? first + i : a.outer - 1;
+      w[u][i] = u32x4{0, 0, 0, 0};
+      if (in) w[u][i] = __builtin_nontemporal_load((const u32x4*)(a.weight + o * a.weight_stride + k));
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int32_t t = n < a.rows ? n : a.rows - 1;
+      x[u][n] = u32x4{0, 0, 0, 0};
+      if (in) x[u][n] = *(const u32x4*)(a.input + t * a.input_stride + k);
+    }
+  };
+  int32_t acc[N][W];
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < W; ++i) acc[n][i] = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) load(u, wave + 4 * u);
+  const int32_t kbs = (a.inner + 1023) / 1024;
+  for (int32_t kb = wave; kb < kbs; kb += 4 * U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[n][i] = __builtin_amdgcn_sdot4((int)x[u][n][j], (int)w[u][i][j], acc[n][i], false);
+      load(u, kb + 4 * (u + U));
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int32_t s = wave_sum(acc[n][i]);
+      if (lane == 0) lds[wave][n * W + i] = s;
+    }
+  __syncthreads();
+  if (threadIdx.x >= N * W) return;
+  const int32_t t = threadIdx.x / W, o = first + threadIdx.x % W;
+  if (t >= a.rows || o >= a.outer) return;
+  const int32_t s = lds[0][threadIdx.x] + lds[1][threadIdx.x] + lds[2][threadIdx.x] + lds[3][threadIdx.x];
+  const float bias = a.bias ? F::one(a.bias[o]) : 0.0f;
+  a.out[t * a.out_stride + o] = F::pack1(scaled(s, a.scale[t], a.weight_scale[o], bias));
+}
+
+// ---- tiles on the matrix cores ---------------------------------------------------------------
+// A: the weight's rows, so that a lane's four sums are neighbours of an output row.
+template <class P>
+constexpr int kLdsBytes = P::LDS_BYTES > kTileOutBytes<P> ? P::LDS_BYTES : kTileOutBytes<P>;
+
+template <class P, int DT>
+__global__ __launch_bounds__(P::NW * 64) void int8_tile_kernel(Int8Args a, int group) {
+  using F = Fmt<DT>;
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[kLdsBytes<P> / 2];
+  int m, n;
+  if (!tile_of(blockIdx.x, a.outer_tiles, a.row_tiles, group, &m, &n)) return;
+  const int m0 = m * P::MT, n0 = n * P::NT;
+  const Operand weight = {(const uint16_t*)(a.weight + m0 * a.weight_stride),
+                          (a.outer - 1 - m0) * a.weight_stride + a.inner, (int32_t)(a.weight_stride / 2)};
+  const Operand input = {(const uint16_t*)(a.input + n0 * a.input_stride),
+                         (a.rows - 1 - n0) * a.input_stride + a.inner, (int32_t)(a.input_stride / 2)};
+  f32x4 acc[P::MI][P::NI];
+  P::run(weight, input, a.inner / 2, lds, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / P::WN % P::WM, wn = wave % P::WN;
+  const bool one = P::NW > P::WM * P::WN;  // a SumProduct's waves all hold the tile: the first writes it
+  if (one && wave > 0) return;
+  float scale[P::NI];
+#pragma unroll
+  for (int ni = 0; ni < P::NI; ++ni) {
+    const int t = n0 + (wn * P::NI + ni) * 16 + (lane & 15);
+    scale[ni] = t < a.rows ? a.scale[t] : 0.0f;
+  }
+  // a fragment's four values
+  auto value = [&](int mi, int ni) {
+    const int o = m0 + (wm * P::MI + mi) * 16 + (lane >> 4) * 4;
+    const i32x4 s = __builtin_bit_cast(i32x4, acc[mi][ni]);
+    float d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = o + i < a.outer ? o + i : a.outer - 1;
+      d[i] = scaled(s[i], scale[ni], a.weight_scale[at], a.bias ? F::one(a.bias[at]) : 0.0f);
+    }
+    return u32x2{F::pack(d[0], d[1]), F::pack(d[2], d[3])};
+  };
+  if constexpr (P::NW > P::WM * P::WN) {
+#pragma unroll
+    for (int ni = 0; ni < P::NI; ++ni) {
+      const int t = n0 + ni * 16 + (lane & 15);
+      if (t >= a.rows) continue;
+#pragma unroll
+      for (int mi = 0; mi < P::MI; ++mi) {
+        const int o = m0 + mi * 16 + (lane >> 4) * 4;
+        const u32x2 v = value(mi, ni);
+        for (int i = 0; i < 4 && o + i < a.outer; ++i)
+          a.out[t * a.out_stride + o + i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  } else {
+    tile_out<P>(lds, a.outer - m0, value,
+                [&](int row) { return n0 + row < a.rows ? a.out + (n0 + row) * a.out_stride + m0 : nullptr; });
+  }
+}
+
+// Rows that 16-byte loads at 16-byte boundaries cannot take in place, copied to
+// rows of whole 16 bytes with zeros behind.
+__global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* from, int64_t stride, int64_t rows, int32_t width,
+                                                        int32_t packed_width, int8_t* to) {
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int8_t* f = from + row * stride;
+    for (int32_t k = threadIdx.x * 16; k < packed_width; k += 256 * 16) {
+      u32x4 v = {0, 0, 0, 0};
+      if (k + 16 <= width) {
+        typedef u32x4 u32x4_any __attribute__((aligned(1)));
+        v = *(const u32x4_any*)(f + k);
+      } else {
+        for (int j = 0; k + j < width; ++j) v[j / 4] |= (uint32_t)(uint8_t)f[k + j] << (8 * (j & 3));
+      }
+      *(u32x4*)(to + row * packed_width + k) = v;
+    }
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------
+constexpr int64_t kMaxInner = 131071;  // 2^14 each, below 2^31 together
+// a tile's 256 rows at this stride stay within a buffer access's 31-bit offset
+constexpr int64_t kMaxStride = int64_t(1) << 22;
+
+int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+int64_t ceil_div(int64_t v, int64_t m) { return (v + m - 1) / m; }
+bool aligned_to(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+bool in_place(const void* p, int64_t stride, int64_t inner) {
+  return aligned_to(p, 16) && stride % 16 == 0 && inner % 16 == 0 && stride <= kMaxStride;
+}
+
+struct Plan {
+  int64_t packed_inner, weight, total;  // bytes; the packed input at 0
+  bool input_in_place, weight_in_place;
+};
+Plan plan_of(int64_t rows, int64_t inner, int64_t outer, const void* input, int64_t input_stride, const void* weight,
+             int64_t weight_stride) {
+  Plan p;
+  p.packed_inner = round_up(inner, 16);
+  p.input_in_place = in_place(input, input_stride, inner);
+  p.weight_in_place = in_place(weight, weight_stride, inner);
+  p.weight = p.input_in_place ? 0 : round_up(rows * p.packed_inner, 256);
+  p.total = p.weight + (p.weight_in_place ? 0 : outer * p.packed_inner);
+  return p;
+}
+
+int check_sizes(int64_t rows, int64_t inner, int64_t outer) {
+  if (rows < 0) return fail(HPRMS_E_INVALID, "rows must be >= 0 (got %lld)", (long long)rows);
+  if (inner < 1 || outer < 1)
+    return fail(HPRMS_E_INVALID, "inner and outer must be >= 1 (got %lld, %lld)", (long long)inner, (long long)outer);
+  if (inner > kMaxInner)
+    return fail(HPRMS_E_RANGE, "inner %lld exceeds %lld: its sums would not fit 32 bits", (long long)inner,
+                (long long)kMaxInner);
+  if (rows > int64_t(1) << 24 || outer > int64_t(1) << 24)
+    return fail(HPRMS_E_RANGE, "rows and outer must be at most 2^24 (got %lld, %lld)", (long long)rows,
+                (long long)outer);
+  if (ceil_div(rows, 128) * ceil_div(outer, 128) > int64_t(1) << 22)  // a launch holds fewer than 2^32 work-items
+    return fail(HPRMS_E_RANGE, "the output holds more than 2^36 elements (%lld x %lld)", (long long)rows,
+                (long long)outer);
+  return HPRMS_OK;
+}
+
+template <class P, int DT>
+void launch_tiles(Int8Args a, hipStream_t stream) {
+  a.outer_tiles = (int32_t)ceil_div(a.outer, P::MT);
+  a.row_tiles = (int32_t)ceil_div(a.rows, P::NT);
+  int8_tile_kernel<P, DT><<<dim3((unsigned)round_up((int64_t)a.outer_tiles * a.row_tiles, 8)), dim3(P::NW * 64), 0,
+                            stream>>>(a, 4);
+}
+
+template <int DT, int N, int W>
+void launch_few(const Int8Args& a, hipStream_t stream) {
+  int8_few_rows_kernel<DT, N, W><<<dim3((unsigned)ceil_div(a.outer, W)), dim3(256), 0, stream>>>(a);
+}
+
+template <int DT>
+int launch_all(const Int8Args& a, hipStream_t stream) {
+  constexpr int I = kInt8Pairs;
+  const int64_t cus = current_cus();
+  if (a.rows <= 1)
+    launch_few<DT, 1, 4>(a, stream);
+  else if (a.rows <= 2)
+    launch_few<DT, 2, 4>(a, stream);
+  else if (a.rows <= 4)
+    launch_few<DT, 4, 4>(a, stream);
+  else if (a.rows <= 8)
+    launch_few<DT, 8, 4>(a, stream);
+  else if (a.rows <= 16) {
+    if (ceil_div(a.outer, 16) <= cus)
+      launch_tiles<SumProduct<I, 1, 1, 4, 6>, DT>(a, stream);
+    else if (ceil_div(a.outer, 128) < 2 * cus)
+      launch_tiles<Product<I, 64, 16, 4, 1, 64, 6, false, false>, DT>(a, stream);
+    else
+      launch_tiles<Product<I, 128, 16, 4, 1, 64, 4, false, false>, DT>(a, stream);
+  } else if (a.rows <= 64) {
+    if (ceil_div(a.outer, 16) <= cus)
+      launch_tiles<SumProduct<I, 1, 4, 4, 3>, DT>(a, stream);
+    else if (ceil_div(a.outer, 128) < 2 * cus)
+      launch_tiles<Product<I, 64, 64, 4, 1, 64, 5, false, false>, DT>(a, stream);
+    else
+      launch_tiles<Product<I, 128, 64, 4, 1, 64, 3, false, false>, DT>(a, stream);
+  } else if (2 * ceil_div(a.outer, 256) * ceil_div(a.rows, 256) <= cus)
+    launch_tiles<Product<I, 128, 128, 2, 2, 64, 2, false, false>, DT>(a, stream);
+  else if (a.rows <= 128)
+    launch_tiles<Product<I, 256, 128, 4, 2, 32, 3, false, false>, DT>(a, stream);
+  else
+    launch_tiles<RingProduct<I, false, false, 2>, DT>(a, stream);
+  return check_launch("8-bit linear kernel");
+}
+
+void pack(const void* from, int64_t stride, int64_t rows, int64_t inner, int64_t packed_inner, void* to,
+          hipStream_t stream) {
+  int8_pack_kernel<<<dim3((unsigned)(rows < 8192 ? rows : 8192)), dim3(256), 0, stream>>>(
+      (const int8_t*)from, stride, rows, (int32_t)inner, (int32_t)packed_inner, (int8_t*)to);
+}
+
+}  // namespace
+}  // namespace hprms
+
+using namespace hprms;
+
+extern "C" {
+
+int64_t hprms_int8_linear_workspace(int64_t rows, int64_t inner, int64_t outer, const void* input,
+                                    int64_t input_row_stride, const void* weight, int64_t weight_row_stride) {
+  const int rc = check_sizes(rows, inner, outer);
+  return rc != HPRMS_OK ? rc : rows == 0 ? 0
+                                         : plan_of(rows, inner, outer, input, input_row_stride, weight,
+                                                   weight_row_stride)
+                                               .total;
+}
+
+int hprms_int8_linear(void* out, const void* input, const float* scale, const void* weight, const float* weight_scale,
+                      const void* bias, void* workspace, int64_t workspace_size, int64_t rows, int64_t inner,
+                      int64_t outer, int64_t out_row_stride, int64_t input_row_stride, int64_t weight_row_stride,
+                      int dtype, hipStream_t stream) {
+  if (dtype != HPRMS_DTYPE_BF16 && dtype != HPRMS_DTYPE_FP16)
+    return fail(HPRMS_E_INVALID, "dtype must be HPRMS_DTYPE_BF16 or HPRMS_DTYPE_FP16 (got %d)", dtype);
+  const int rc = check_sizes(rows, inner, outer);
+  if (rc != HPRMS_OK) return rc;
+  if (out_row_stride < outer || input_row_stride < inner || weight_row_stride < inner)
+    return fail(HPRMS_E_INVALID, "row strides must be >= the rows' widths");
+  if (!extent_ok(rows, out_row_stride, 2, outer) || !extent_ok(rows, input_row_stride, 1, inner) ||
+      !extent_ok(outer, weight_row_stride, 1, inner))
+    return fail(HPRMS_E_RANGE, "the rows at these row strides span more than 2^56 bytes");
+  if (rows == 0) return HPRMS_OK;
+  if (!out || !input || !scale || !weight || !weight_scale) return fail(HPRMS_E_INVALID, "null tensor pointer");
+  if (!aligned_to(out, 2) || !aligned_to(scale, 4) || !aligned_to(weight_scale, 4) || !aligned_to(bias, 2))
+    return fail(HPRMS_E_INVALID, "tensors must be aligned to their elements");
+  const Plan p = plan_of(rows, inner, outer, input, input_row_stride, weight, weight_row_stride);
+  if (p.total > 0 && (!workspace || workspace_size < p.total || !aligned_to(workspace, 256)))
+    return fail(HPRMS_E_INVALID, "the workspace must hold %lld bytes, 256-byte aligned (got %lld)", (long long)p.total,
+                (long long)workspace_size);
+  char* ws = (char*)workspace;
+  Int8Args a = {};
+  a.input = (const int8_t*)input;
+  a.input_stride = input_row_stride;
+  if (!p.input_in_place) {
+    pack(input, input_row_stride, rows, inner, p.packed_inner, ws, stream);
+    a.input = (const int8_t*)ws;
+    a.input_stride = p.packed_inner;
+  }
+  a.weight = (const int8_t*)weight;
+  a.weight_stride = weight_row_stride;
+  if (!p.weight_in_place) {
+    pack(weight, weight_row_stride, outer, inner, p.packed_inner, ws + p.weight, stream);
+    a.weight = (const int8_t*)(ws + p.weight);
+    a.weight_stride = p.packed_inner;
+  }
+  a.scale = scale;
+  a.weight_scale = weight_scale;
+  a.bias = (const uint16_t*)bias;
+  a.out = (uint16_t*)out;
+  a.out_stride = out_row_stride;
+  a.rows = (int32_t)rows;
+  a.inner = (int32_t)p.packed_inner;
+  a.outer = (int32_t)outer;
+  return dtype == HPRMS_DTYPE_BF16 ? launch_all<HPRMS_DTYPE_BF16>(a, stream) : launch_all<HPRMS_DTYPE_FP16>(a, stream);
+}
+
+}  // extern "C"

@@ -125,43 +125,6 @@ __device__ __forceinline__ void forward_epilogue(const LossArgs& a, const f32x4 
   }
 }
 
-// A tile of 16-bit values on its way out: the fragments hold 4 neighbours of a
-// row (of the output: a column of the product) a lane, which would store 32
-// bytes of 16 rows at a time; through LDS whole rows of the tile go out, 16
-// bytes a lane (dweight of one row, 131072 x 4096: 197 us, 311 with the
-// fragments' own stores).  `from(mi, ni)` gives a fragment's 4 values as 8 bytes; `to(row)`
-// is where a row of the tile begins, null if it does not exist, and `left` the
-// elements from there on that do.
-template <class P>
-constexpr int kTileOutBytes = P::NT * (P::MT + 8) * 2;
-
-template <class P, class From, class To>
-__device__ __forceinline__ void tile_out(uint16_t* lds, int left, From&& from, To&& to) {
-  constexpr int PITCH = P::MT + 8;  // 16 bytes off the banks' period
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / P::WN, wn = wave % P::WN;
-  __syncthreads();  // the tile loop's LDS reads are over
-#pragma unroll
-  for (int ni = 0; ni < P::NI; ++ni)
-#pragma unroll
-    for (int mi = 0; mi < P::MI; ++mi)
-      *(u32x2*)(lds + ((wn * P::NI + ni) * 16 + (lane & 15)) * PITCH + (wm * P::MI + mi) * 16 + (lane >> 4) * 4) =
-          from(mi, ni);
-  __syncthreads();
-  constexpr int LPR = P::MT / 8;  // lanes of a row
-  const int m = threadIdx.x % LPR * 8;
-#pragma unroll 4
-  for (int row = threadIdx.x / LPR; row < P::NT; row += P::NW * 64 / LPR) {
-    uint16_t* p = to(row);
-    if (!p || m >= left) continue;
-    const u32x4 v = *(const u32x4*)(lds + row * PITCH + m);
-    if (left - m >= 8) {
-      *(u32x4_u*)(p + m) = v;
-    } else {
-      for (int j = 0; j < left - m; ++j) p[m + j] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
-    }
-  }
-}
-
 // The piece's dz of the tile, 0 where there is no row or no vocabulary entry.
 // A target outside [0, vocab) gives NaN.
 template <class P>
@@ -267,23 +230,6 @@ __device__ __forceinline__ void dhidden_epilogue(const LossArgs& a, const f32x4 
       }
     }
   }
-}
-
-// ---- tiles of a launch ------------------------------------------------------------------
-// Tile (m, n) of workgroup b, false past the last one.  The hardware hands
-// consecutive workgroups to the 8 XCDs in turn, so XCD k takes one contiguous
-// run of tiles; in a run, `group` column tiles times some row tiles make the
-// block of tiles that an XCD's 32 CUs work on at a time, which share their
-// operands' slices in that XCD's L2.
-__device__ __forceinline__ bool tile_of(int b, int mt, int nt, int group, int* m, int* n) {
-  const int total = mt * nt, per = (total + 7) / 8;
-  const int t = (b & 7) * per + (b >> 3);
-  if ((b >> 3) >= per || t >= total) return false;
-  const int g = t / (group * mt), r = t % (group * mt);
-  const int w = nt - g * group < group ? nt - g * group : group;
-  *m = r / w;
-  *n = g * group + r % w;
-  return true;
 }
 
 }  // namespace hprms

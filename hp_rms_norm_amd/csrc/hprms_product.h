@@ -1,5 +1,6 @@
-// hprms_product.h - the tile product of the loss kernels: C = A . B^T over 16-bit
-// operands with binary32 sums, on the matrix cores.
+// hprms_product.h - the tile product of the loss and of the 8-bit linear kernels: C
+// = A . B^T on the matrix cores, over 16-bit operands with binary32 sums or over
+// 8-bit integers with 32-bit integer sums.
 #pragma once
 
 #include "hprms_device.h"
@@ -11,14 +12,36 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes at any 2-byte boundary
+typedef u32x4 u32x4_out __attribute__((aligned(2)));
+
+// 8-bit integers as a product's element type: everything below counts in pairs of
+// them, 16 bits each, and an accumulator's registers hold integers.  (A lane of
+// v_mfma_i32_16x16x64_i8 holds 16 bytes of a row at byte 16 (l / 16), as one of
+// v_mfma_f32_16x16x32 does.)  Pairs cannot lie k outer.
+constexpr int kInt8Pairs = 16;
+
 template <int DT>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-  if constexpr (DT == HPRMS_DTYPE_BF16)
+  if constexpr (DT == kInt8Pairs)
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
+                                                                           __builtin_bit_cast(i32x4, b),
+                                                                           __builtin_bit_cast(i32x4, c), 0, 0, 0));
+  else if constexpr (DT == HPRMS_DTYPE_BF16)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                   0);
+}
+
+template <int DT>
+__device__ __forceinline__ f32x4 add_sums(f32x4 a, f32x4 b) {
+  if constexpr (DT == kInt8Pairs)
+    return __builtin_bit_cast(f32x4, __builtin_bit_cast(i32x4, a) + __builtin_bit_cast(i32x4, b));
+  else
+    return a + b;
 }
 
 // One operand of a tile: `rows` of its first index (the tile's extent) over the
@@ -317,7 +340,7 @@ struct SumProduct {
       for (int j = 0; j < NI; ++j) {
         acc[i][j] = lds[(i * NI + j) * 64 + lane];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) acc[i][j] += lds[((w * MI + i) * NI + j) * 64 + lane];
+        for (int w = 1; w < NW; ++w) acc[i][j] = add_sums<DT>(acc[i][j], lds[((w * MI + i) * NI + j) * 64 + lane]);
       }
   }
 };
@@ -482,5 +505,60 @@ struct RingProduct {
     __builtin_amdgcn_s_waitcnt(wait_code(0));  // LDS is free again behind the next barrier
   }
 };
+
+// ---- a tile's way out ----------------------------------------------------------------
+// A tile of 16-bit values on its way out: the fragments hold 4 neighbours of a
+// row (of the output: a column of the product) a lane, which would store 32
+// bytes of 16 rows at a time; through LDS whole rows of the tile go out, 16
+// bytes a lane (dweight of one row, 131072 x 4096: 197 us, 311 with the
+// fragments' own stores).  `from(mi, ni)` gives a fragment's 4 values as 8 bytes; `to(row)`
+// is where a row of the tile begins, null if it does not exist, and `left` the
+// elements from there on that do.
+template <class P>
+constexpr int kTileOutBytes = P::NT * (P::MT + 8) * 2;
+
+template <class P, class From, class To>
+__device__ __forceinline__ void tile_out(uint16_t* lds, int left, From&& from, To&& to) {
+  constexpr int PITCH = P::MT + 8;  // 16 bytes off the banks' period
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / P::WN, wn = wave % P::WN;
+  __syncthreads();  // the tile loop's LDS reads are over
+#pragma unroll
+  for (int ni = 0; ni < P::NI; ++ni)
+#pragma unroll
+    for (int mi = 0; mi < P::MI; ++mi)
+      *(u32x2*)(lds + ((wn * P::NI + ni) * 16 + (lane & 15)) * PITCH + (wm * P::MI + mi) * 16 + (lane >> 4) * 4) =
+          from(mi, ni);
+  __syncthreads();
+  constexpr int LPR = P::MT / 8;  // lanes of a row
+  const int m = threadIdx.x % LPR * 8;
+#pragma unroll 4
+  for (int row = threadIdx.x / LPR; row < P::NT; row += P::NW * 64 / LPR) {
+    uint16_t* p = to(row);
+    if (!p || m >= left) continue;
+    const u32x4 v = *(const u32x4*)(lds + row * PITCH + m);
+    if (left - m >= 8) {
+      *(u32x4_out*)(p + m) = v;
+    } else {
+      for (int j = 0; j < left - m; ++j) p[m + j] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+    }
+  }
+}
+
+// ---- tiles of a launch ------------------------------------------------------------------
+// Tile (m, n) of workgroup b, false past the last one.  The hardware hands
+// consecutive workgroups to the 8 XCDs in turn, so XCD k takes one contiguous
+// run of tiles; in a run, `group` column tiles times some row tiles make the
+// block of tiles that an XCD's 32 CUs work on at a time, which share their
+// operands' slices in that XCD's L2.
+__device__ __forceinline__ bool tile_of(int b, int mt, int nt, int group, int* m, int* n) {
+  const int total = mt * nt, per = (total + 7) / 8;
+  const int t = (b & 7) * per + (b >> 3);
+  if ((b >> 3) >= per || t >= total) return false;
+  const int g = t / (group * mt), r = t % (group * mt);
+  const int w = nt - g * group < group ? nt - g * group : group;
+  *m = r / w;
+  *n = g * group + r % w;
+  return true;
+}
 
 }  // namespace hprms

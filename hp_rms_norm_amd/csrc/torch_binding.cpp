@@ -887,6 +887,466 @@ void clip_grad_norm_meta_(at::Tensor& norm, at::TensorList grads, double max_nor
   clip_grad_norm_out_meta(norm, grads, grads, max_norm);
 }
 
+// ---- the edge between two blocks --------------------------------------------------------
+typedef std::optional<at::Tensor> MaybeTensor;
+
+void* data_of(const MaybeTensor& t) { return t ? t->data_ptr() : nullptr; }
+
+// Rows of a gate: one for all rows ([hidden]), or as many as its leading sizes
+// say, which are input's up to some dimension and 1 from there on.
+int64_t gate_rows_of(const at::Tensor& gate, const at::Tensor& input, int64_t* stride) {
+  const int64_t hidden = input.size(-1);
+  TORCH_CHECK(gate.dim() == 1 || gate.dim() == input.dim(), "gate.dim() must be 1 or input.dim()");
+  TORCH_CHECK(gate.size(-1) == hidden, "gate.size(-1) == hidden_dim");
+  TORCH_CHECK(gate.stride(-1) == 1 || hidden <= 1, "gate.stride(-1) == 1");
+  TORCH_CHECK(gate.scalar_type() == input.scalar_type(), "gate.dtype() == input.dtype()");
+  TORCH_CHECK(gate.device() == input.device(), "gate must be on input's device");
+  *stride = hidden;
+  if (gate.dim() == 1) return 1;
+  bool ones = false;
+  for (int64_t i = 0; i + 1 < input.dim(); ++i) {
+    ones = ones || gate.size(i) != input.size(i);
+    TORCH_CHECK(!ones || gate.size(i) == 1,
+                "gate's leading sizes must be input's up to some dimension and 1 from there on");
+  }
+  int64_t rows = 0;
+  rows_of(gate, hidden, &rows, stride);
+  return rows;
+}
+
+struct EdgeShape {
+  int64_t rows, hidden, gate_rows, in_stride, res_stride, gate_stride;
+  int dtype;
+};
+
+// What the forward calls and the gradient read.
+EdgeShape check_edge(const at::Tensor& input, const MaybeTensor& post_weight, const at::Tensor& weight,
+                     const at::Tensor& residual, const MaybeTensor& gate) {
+  TORCH_CHECK(input.dim() >= 2, "input.dim() >= 2");
+  TORCH_CHECK(weight.dim() == 1, "weight.dim() == 1");
+  EdgeShape s;
+  s.hidden = weight.size(0);
+  s.dtype = dtype_code(input);
+  TORCH_CHECK(input.size(-1) == s.hidden, "input.size(-1) == hidden_dim");
+  TORCH_CHECK(s.hidden >= 1, "rows must hold at least one element");
+  TORCH_CHECK(residual.sizes() == input.sizes(), "residual must be shaped like input");
+  TORCH_CHECK((input.stride(-1) == 1 && residual.stride(-1) == 1) || s.hidden == 1,
+              "rows must be contiguous (stride(-1) == 1)");
+  TORCH_CHECK(residual.scalar_type() == input.scalar_type(), "residual.dtype() == input.dtype()");
+  TORCH_CHECK(residual.device() == input.device(), "residual must be on input's device");
+  for (const at::Tensor* w : {&weight, post_weight ? &*post_weight : &weight}) {
+    TORCH_CHECK(w->dim() == 1 && w->size(0) == s.hidden, "post_weight must be shaped like weight");
+    TORCH_CHECK(w->stride(0) == 1 || s.hidden == 1, "weights must be contiguous");
+    TORCH_CHECK(w->scalar_type() == input.scalar_type(), "weight.dtype() == input.dtype()");
+    TORCH_CHECK(w->device() == input.device(), "weights must be on input's device");
+  }
+  int64_t r = 0;
+  rows_of(input, s.hidden, &s.rows, &s.in_stride);
+  rows_of(residual, s.hidden, &r, &s.res_stride);
+  s.gate_rows = 0;
+  s.gate_stride = s.hidden;
+  if (gate) s.gate_rows = gate_rows_of(*gate, input, &s.gate_stride);
+  return s;
+}
+
+// A row tensor to be written: shaped like input, of its dtype unless `dtype` says another.
+int64_t check_row_output(const at::Tensor& out, const at::Tensor& input, at::ScalarType dtype, const char* name) {
+  TORCH_CHECK(out.sizes() == input.sizes(), name, " must be shaped like input");
+  TORCH_CHECK(out.stride(-1) == 1 || input.size(-1) == 1, "rows must be contiguous (stride(-1) == 1)");
+  TORCH_CHECK(out.scalar_type() == dtype, name, ".dtype() must be ", dtype);
+  TORCH_CHECK(out.device() == input.device(), "all tensors must be on input's device");
+  int64_t rows = 0, stride = 0;
+  rows_of(out, input.size(-1), &rows, &stride);
+  return stride;
+}
+
+struct NormAddShape {
+  EdgeShape e;
+  int64_t out_stride, res_out_stride;
+};
+
+NormAddShape check_norm_add(const at::Tensor& out, const at::Tensor* scale, const at::Tensor& residual_out,
+                            const at::Tensor& input, const MaybeTensor& post_weight, const at::Tensor& weight,
+                            const at::Tensor& residual, const MaybeTensor& gate) {
+  NormAddShape s;
+  s.e = check_edge(input, post_weight, weight, residual, gate);
+  s.out_stride = check_row_output(out, input, scale ? at::kChar : input.scalar_type(), "out");
+  s.res_out_stride = check_row_output(residual_out, input, input.scalar_type(), "residual_out");
+  if (scale) {
+    TORCH_CHECK(scale->scalar_type() == at::kFloat, "scale.dtype() == float32");
+    TORCH_CHECK(scale->numel() == s.e.rows, "scale.numel() == number of rows");
+    TORCH_CHECK(scale->is_contiguous(), "scale must be contiguous");
+    TORCH_CHECK(scale->device() == input.device(), "all tensors must be on input's device");
+  }
+  if (s.e.rows > 0) {
+    // a row is read before it is written, by the same workgroup: out may be input
+    // and residual_out may be residual, exactly
+    if (scale)
+      at::assert_no_overlap(out, input);
+    else
+      at::assert_no_partial_overlap(out, input);
+    at::assert_no_partial_overlap(residual_out, residual);
+    at::assert_no_overlap(out, residual);
+    at::assert_no_overlap(residual_out, input);
+    at::assert_no_overlap(out, residual_out);
+    for (const at::Tensor* t : {&out, &residual_out}) {
+      at::assert_no_overlap(*t, weight);
+      if (post_weight) at::assert_no_overlap(*t, *post_weight);
+      if (gate) at::assert_no_overlap(*t, *gate);
+      if (scale) at::assert_no_overlap(*t, *scale);
+    }
+    if (scale) {
+      for (const at::Tensor* t : {&input, &residual, &weight}) at::assert_no_overlap(*scale, *t);
+      if (post_weight) at::assert_no_overlap(*scale, *post_weight);
+      if (gate) at::assert_no_overlap(*scale, *gate);
+    }
+  }
+  return s;
+}
+
+int64_t rows_per_gate(const EdgeShape& e) { return e.gate_rows > 0 && e.rows > 0 ? e.rows / e.gate_rows : 1; }
+
+void norm_add_rms_norm_hip(at::Tensor& out, at::Tensor& residual_out, const at::Tensor& input,
+                           const MaybeTensor& post_weight, const at::Tensor& weight, const at::Tensor& residual,
+                           const MaybeTensor& gate, double residual_scale, double eps) {
+  const NormAddShape s = check_norm_add(out, nullptr, residual_out, input, post_weight, weight, residual, gate);
+  c10::DeviceGuard guard(input.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(input.device().index()).stream();
+  check_status(hprms_norm_add_rmsnorm(out.data_ptr(), residual_out.data_ptr(), input.data_ptr(), data_of(post_weight),
+                                      weight.data_ptr(), residual.data_ptr(), data_of(gate), s.e.rows, s.e.hidden,
+                                      rows_per_gate(s.e), s.out_stride, s.res_out_stride, s.e.in_stride,
+                                      s.e.res_stride, s.e.gate_stride, s.e.dtype, residual_scale, eps, stream));
+}
+
+void norm_add_rms_norm_meta(at::Tensor& out, at::Tensor& residual_out, const at::Tensor& input,
+                            const MaybeTensor& post_weight, const at::Tensor& weight, const at::Tensor& residual,
+                            const MaybeTensor& gate, double residual_scale, double eps) {
+  (void)check_norm_add(out, nullptr, residual_out, input, post_weight, weight, residual, gate);
+  (void)residual_scale, (void)eps;
+}
+
+void norm_add_rms_norm_int8_hip(at::Tensor& out, at::Tensor& scale, at::Tensor& residual_out, const at::Tensor& input,
+                                const MaybeTensor& post_weight, const at::Tensor& weight, const at::Tensor& residual,
+                                const MaybeTensor& gate, double residual_scale, double eps) {
+  const NormAddShape s = check_norm_add(out, &scale, residual_out, input, post_weight, weight, residual, gate);
+  c10::DeviceGuard guard(input.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(input.device().index()).stream();
+  check_status(hprms_norm_add_rmsnorm_int8(
+      out.data_ptr(), scale.data_ptr<float>(), residual_out.data_ptr(), input.data_ptr(), data_of(post_weight),
+      weight.data_ptr(), residual.data_ptr(), data_of(gate), s.e.rows, s.e.hidden, rows_per_gate(s.e), s.out_stride,
+      s.res_out_stride, s.e.in_stride, s.e.res_stride, s.e.gate_stride, s.e.dtype, residual_scale, eps, stream));
+}
+
+void norm_add_rms_norm_int8_meta(at::Tensor& out, at::Tensor& scale, at::Tensor& residual_out, const at::Tensor& input,
+                                 const MaybeTensor& post_weight, const at::Tensor& weight, const at::Tensor& residual,
+                                 const MaybeTensor& gate, double residual_scale, double eps) {
+  (void)check_norm_add(out, &scale, residual_out, input, post_weight, weight, residual, gate);
+  (void)residual_scale, (void)eps;
+}
+
+struct NormAddGradShape {
+  EdgeShape e;
+  int64_t din_stride, dres_in_stride, dgate_stride, dout_stride, dres_stride;
+  int dpost_dtype, dweight_dtype;
+};
+
+NormAddGradShape check_norm_add_backward(const at::Tensor& dinput, const at::Tensor& dresidual_in,
+                                         const MaybeTensor& dpost_weight, const at::Tensor& dweight,
+                                         const MaybeTensor& dgate, const at::Tensor& dout,
+                                         const MaybeTensor& dresidual, const at::Tensor& input,
+                                         const at::Tensor& residual, const MaybeTensor& post_weight,
+                                         const at::Tensor& weight, const MaybeTensor& gate) {
+  NormAddGradShape s;
+  s.e = check_edge(input, post_weight, weight, residual, gate);
+  TORCH_CHECK(dpost_weight.has_value() == post_weight.has_value(), "dpost_weight must come with post_weight");
+  TORCH_CHECK(dgate.has_value() == gate.has_value(), "dgate must come with gate");
+  s.din_stride = check_row_output(dinput, input, input.scalar_type(), "dinput");
+  s.dres_in_stride = check_row_output(dresidual_in, input, input.scalar_type(), "dresidual_in");
+  s.dout_stride = check_row_output(dout, input, input.scalar_type(), "dout");
+  s.dres_stride = dresidual ? check_row_output(*dresidual, input, input.scalar_type(), "dresidual") : s.e.hidden;
+  s.dgate_stride = s.e.hidden;
+  if (dgate) {
+    TORCH_CHECK(dgate->sizes() == gate->sizes(), "dgate must be shaped like gate");
+    (void)gate_rows_of(*dgate, input, &s.dgate_stride);
+  }
+  s.dpost_dtype = s.dweight_dtype = s.e.dtype;
+  for (const at::Tensor* t : {&dweight, dpost_weight ? &*dpost_weight : &dweight}) {
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == s.e.hidden, "dweight and dpost_weight must be shaped like weight");
+    TORCH_CHECK(t->stride(0) == 1 || s.e.hidden == 1, "dweight and dpost_weight must be contiguous");
+    TORCH_CHECK(t->scalar_type() == input.scalar_type() || t->scalar_type() == at::kFloat,
+                "dweight.dtype() must be weight.dtype() or float32");
+    TORCH_CHECK(t->device() == input.device(), "all tensors must be on input's device");
+  }
+  if (dweight.scalar_type() == at::kFloat) s.dweight_dtype = HPRMS_DTYPE_FP32;
+  if (dpost_weight && dpost_weight->scalar_type() == at::kFloat) s.dpost_dtype = HPRMS_DTYPE_FP32;
+  if (s.e.rows > 0) {
+    std::vector<const at::Tensor*> rows = {&dout, &input, &residual};
+    if (dresidual) rows.push_back(&*dresidual);
+    std::vector<const at::Tensor*> read = {&weight};
+    if (post_weight) read.push_back(&*post_weight);
+    std::vector<const at::Tensor*> sums = {&dweight};
+    if (dpost_weight) sums.push_back(&*dpost_weight);
+    // a row is read before it is written, by the same workgroup
+    at::assert_no_overlap(dinput, dresidual_in);
+    for (const at::Tensor* out : {&dinput, &dresidual_in}) {
+      for (const at::Tensor* t : rows) at::assert_no_partial_overlap(*out, *t);
+      for (const at::Tensor* t : read) at::assert_no_overlap(*out, *t);
+      for (const at::Tensor* t : sums) at::assert_no_overlap(*out, *t);
+      if (gate) at::assert_no_overlap(*out, *gate);
+      if (dgate) at::assert_no_overlap(*out, *dgate);
+    }
+    for (const at::Tensor* out : sums) {
+      for (const at::Tensor* t : rows) at::assert_no_overlap(*out, *t);
+      for (const at::Tensor* t : read) at::assert_no_overlap(*out, *t);
+      if (gate) at::assert_no_overlap(*out, *gate);
+      if (dgate) at::assert_no_overlap(*out, *dgate);
+    }
+    if (dpost_weight) at::assert_no_overlap(dweight, *dpost_weight);
+    if (dgate) {
+      for (const at::Tensor* t : rows) at::assert_no_overlap(*dgate, *t);
+      for (const at::Tensor* t : read) at::assert_no_overlap(*dgate, *t);
+      if (s.e.gate_rows == s.e.rows)
+        at::assert_no_partial_overlap(*dgate, *gate);
+      else
+        at::assert_no_overlap(*dgate, *gate);
+    }
+  }
+  return s;
+}
+
+void norm_add_rms_norm_backward_hip(at::Tensor& dinput, at::Tensor& dresidual_in, const MaybeTensor& dpost_weight,
+                                    at::Tensor& dweight, const MaybeTensor& dgate, const at::Tensor& dout,
+                                    const MaybeTensor& dresidual, const at::Tensor& input, const at::Tensor& residual,
+                                    const MaybeTensor& post_weight, const at::Tensor& weight, const MaybeTensor& gate,
+                                    double residual_scale, double eps) {
+  const NormAddGradShape s = check_norm_add_backward(dinput, dresidual_in, dpost_weight, dweight, dgate, dout,
+                                                     dresidual, input, residual, post_weight, weight, gate);
+  c10::DeviceGuard guard(input.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(input.device().index()).stream();
+  const at::Tensor ws =
+      workspace_of(hprms_norm_add_rmsnorm_backward_workspace(s.e.rows, s.e.hidden, s.e.gate_rows), input);
+  check_status(hprms_norm_add_rmsnorm_backward(
+      dinput.data_ptr(), dresidual_in.data_ptr(), data_of(dpost_weight), dweight.data_ptr(), data_of(dgate),
+      dout.data_ptr(), data_of(dresidual), input.data_ptr(), residual.data_ptr(), data_of(post_weight),
+      weight.data_ptr(), data_of(gate), ws.data_ptr(), ws.numel(), s.e.rows, s.e.hidden, s.e.gate_rows, s.din_stride,
+      s.dres_in_stride, s.dgate_stride, s.dout_stride, s.dres_stride, s.e.in_stride, s.e.res_stride, s.e.gate_stride,
+      s.e.dtype, s.dpost_dtype, s.dweight_dtype, residual_scale, eps, stream));
+}
+
+void norm_add_rms_norm_backward_meta(at::Tensor& dinput, at::Tensor& dresidual_in, const MaybeTensor& dpost_weight,
+                                     at::Tensor& dweight, const MaybeTensor& dgate, const at::Tensor& dout,
+                                     const MaybeTensor& dresidual, const at::Tensor& input, const at::Tensor& residual,
+                                     const MaybeTensor& post_weight, const at::Tensor& weight, const MaybeTensor& gate,
+                                     double residual_scale, double eps) {
+  (void)check_norm_add_backward(dinput, dresidual_in, dpost_weight, dweight, dgate, dout, dresidual, input, residual,
+                                post_weight, weight, gate);
+  (void)residual_scale, (void)eps;
+}
+
+// ---- the product of 8-bit integers ---------------------------------------------------------
+struct Int8Shape {
+  int64_t rows, inner, outer, out_stride, in_stride, weight_stride;
+  int dtype;
+};
+
+Int8Shape check_int8_linear(const at::Tensor& out, const at::Tensor& input, const at::Tensor& scale,
+                            const at::Tensor& weight, const at::Tensor& weight_scale, const MaybeTensor& bias) {
+  TORCH_CHECK(input.dim() >= 2, "input.dim() >= 2");
+  TORCH_CHECK(weight.dim() == 2, "weight.dim() == 2");
+  TORCH_CHECK(input.scalar_type() == at::kChar && weight.scalar_type() == at::kChar,
+              "input and weight must be int8");
+  Int8Shape s;
+  s.outer = weight.size(0);
+  s.inner = weight.size(1);
+  s.dtype = dtype_code(out);
+  TORCH_CHECK(s.inner >= 1 && s.outer >= 1, "weight must hold at least one element");
+  TORCH_CHECK(input.size(-1) == s.inner, "input.size(-1) == weight.size(1)");
+  TORCH_CHECK(out.dim() == input.dim() && out.size(-1) == s.outer &&
+                  out.sizes().slice(0, out.dim() - 1) == input.sizes().slice(0, input.dim() - 1),
+              "out must have one row of weight.size(0) elements per row of input");
+  TORCH_CHECK((input.stride(-1) == 1 && weight.stride(1) == 1) || s.inner == 1,
+              "rows must be contiguous (stride(-1) == 1)");
+  TORCH_CHECK(out.stride(-1) == 1 || s.outer == 1, "out.stride(-1) == 1");
+  rows_of(input, s.inner, &s.rows, &s.in_stride);
+  int64_t r = 0;
+  rows_of(out, s.outer, &r, &s.out_stride);
+  s.weight_stride = matrix_stride(weight, s.inner);
+  TORCH_CHECK(scale.scalar_type() == at::kFloat && weight_scale.scalar_type() == at::kFloat,
+              "scale and weight_scale must be float32");
+  TORCH_CHECK(scale.numel() == s.rows && scale.is_contiguous(), "scale must hold one contiguous element per row");
+  TORCH_CHECK(weight_scale.numel() == s.outer && weight_scale.is_contiguous(),
+              "weight_scale must hold one contiguous element per row of weight");
+  if (bias) {
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == s.outer && bias->is_contiguous(),
+                "bias must hold one contiguous element per row of weight");
+    TORCH_CHECK(bias->scalar_type() == out.scalar_type(), "bias.dtype() == out.dtype()");
+    TORCH_CHECK(bias->device() == input.device(), "all tensors must be on input's device");
+  }
+  for (const at::Tensor* t : {&out, &scale, &weight, &weight_scale})
+    TORCH_CHECK(t->device() == input.device(), "all tensors must be on input's device");
+  if (s.rows > 0) {
+    for (const at::Tensor* t : {&input, &scale, &weight, &weight_scale}) at::assert_no_overlap(out, *t);
+    if (bias) at::assert_no_overlap(out, *bias);
+  }
+  return s;
+}
+
+void int8_linear_hip(at::Tensor& out, const at::Tensor& input, const at::Tensor& scale, const at::Tensor& weight,
+                     const at::Tensor& weight_scale, const MaybeTensor& bias) {
+  const Int8Shape s = check_int8_linear(out, input, scale, weight, weight_scale, bias);
+  if (s.rows == 0) return;
+  c10::DeviceGuard guard(input.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(input.device().index()).stream();
+  const int64_t need = hprms_int8_linear_workspace(s.rows, s.inner, s.outer, input.data_ptr(), s.in_stride,
+                                                   weight.data_ptr(), s.weight_stride);
+  at::Tensor ws;
+  if (need != 0) ws = workspace_of(need, input);
+  check_status(hprms_int8_linear(out.data_ptr(), input.data_ptr(), scale.data_ptr<float>(), weight.data_ptr(),
+                                 weight_scale.data_ptr<float>(), data_of(bias), need ? ws.data_ptr() : nullptr, need,
+                                 s.rows, s.inner, s.outer, s.out_stride, s.in_stride, s.weight_stride, s.dtype,
+                                 stream));
+}
+
+void int8_linear_meta(at::Tensor& out, const at::Tensor& input, const at::Tensor& scale, const at::Tensor& weight,
+                      const at::Tensor& weight_scale, const MaybeTensor& bias) {
+  (void)check_int8_linear(out, input, scale, weight, weight_scale, bias);
+}
+
+// ---- log probabilities -----------------------------------------------------------------------
+struct LogitsShape {
+  int64_t rows, vocab, stride;
+  int dtype;
+};
+
+int logits_dtype_code(const at::Tensor& t) {
+  if (t.scalar_type() == at::kFloat) return HPRMS_DTYPE_FP32;
+  if (t.scalar_type() == at::kBFloat16) return HPRMS_DTYPE_BF16;
+  if (t.scalar_type() == at::kHalf) return HPRMS_DTYPE_FP16;
+  TORCH_CHECK(false, "logits must be bfloat16, float16 or float32");
+  return -1;
+}
+
+LogitsShape check_logits(const at::Tensor& logits, const at::Tensor& tokens,
+                         std::initializer_list<const at::Tensor*> per_row) {
+  TORCH_CHECK(logits.dim() >= 2, "logits.dim() >= 2");
+  LogitsShape s;
+  s.vocab = logits.size(-1);
+  s.dtype = logits_dtype_code(logits);
+  TORCH_CHECK(s.vocab >= 1, "logits must hold at least one element per row");
+  TORCH_CHECK(logits.stride(-1) == 1 || s.vocab == 1, "logits.stride(-1) == 1");
+  TORCH_CHECK(tokens.scalar_type() == at::kLong, "tokens.dtype() == int64");
+  TORCH_CHECK(tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1), "tokens must have one element per row");
+  TORCH_CHECK(tokens.is_contiguous(), "tokens must be contiguous");
+  TORCH_CHECK(tokens.device() == logits.device(), "all tensors must be on logits' device");
+  for (const at::Tensor* t : per_row) {
+    TORCH_CHECK(t->scalar_type() == at::kFloat, "log_prob, entropy, lse and their gradients must be float32");
+    TORCH_CHECK(t->sizes() == tokens.sizes(), "log_prob, entropy, lse and their gradients must be shaped like tokens");
+    TORCH_CHECK(t->is_contiguous(), "log_prob, entropy, lse and their gradients must be contiguous");
+    TORCH_CHECK(t->device() == logits.device(), "all tensors must be on logits' device");
+  }
+  rows_of(logits, s.vocab, &s.rows, &s.stride);
+  return s;
+}
+
+LogitsShape check_log_probs(const at::Tensor& log_prob, const at::Tensor& entropy, const at::Tensor& lse,
+                            const at::Tensor& top_log_prob, const at::Tensor& top_index, const at::Tensor& logits,
+                            const at::Tensor& tokens) {
+  const LogitsShape s = check_logits(logits, tokens, {&log_prob, &entropy, &lse});
+  TORCH_CHECK(top_log_prob.scalar_type() == at::kFloat, "top_log_prob.dtype() == float32");
+  TORCH_CHECK(top_index.scalar_type() == at::kLong, "top_index.dtype() == int64");
+  TORCH_CHECK(top_index.dim() == logits.dim() &&
+                  top_index.sizes().slice(0, logits.dim() - 1) == tokens.sizes() &&
+                  top_log_prob.sizes() == top_index.sizes(),
+              "top_log_prob and top_index must be shaped like tokens, with the alternatives behind");
+  TORCH_CHECK(top_index.size(-1) <= 64 && top_index.size(-1) <= s.vocab,
+              "at most 64 alternatives, and no more than the vocabulary has");
+  for (const at::Tensor* t : {&top_log_prob, &top_index}) {
+    TORCH_CHECK(t->is_contiguous(), "top_log_prob and top_index must be contiguous");
+    TORCH_CHECK(t->device() == logits.device(), "all tensors must be on logits' device");
+  }
+  if (s.rows > 0) {
+    const at::Tensor* outs[5] = {&log_prob, &entropy, &lse, &top_log_prob, &top_index};
+    for (int i = 0; i < 5; ++i) {
+      at::assert_no_overlap(*outs[i], logits);
+      at::assert_no_overlap(*outs[i], tokens);
+      for (int j = 0; j < i; ++j) at::assert_no_overlap(*outs[i], *outs[j]);
+    }
+  }
+  return s;
+}
+
+void token_log_probs_hip(at::Tensor& log_prob, at::Tensor& entropy, at::Tensor& lse, at::Tensor& top_log_prob,
+                         at::Tensor& top_index, const at::Tensor& logits, const at::Tensor& tokens,
+                         int64_t ignore_index) {
+  const LogitsShape s = check_log_probs(log_prob, entropy, lse, top_log_prob, top_index, logits, tokens);
+  if (s.rows == 0) return;
+  c10::DeviceGuard guard(logits.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(logits.device().index()).stream();
+  const int64_t top = top_index.size(-1);
+  const at::Tensor ws = workspace_of(hprms_token_log_probs_workspace(s.rows, s.vocab, top, s.dtype), logits);
+  check_status(hprms_token_log_probs(log_prob.data_ptr<float>(), entropy.data_ptr<float>(), lse.data_ptr<float>(),
+                                     top_log_prob.data_ptr<float>(), top_index.data_ptr<int64_t>(), logits.data_ptr(),
+                                     tokens.data_ptr<int64_t>(), ws.data_ptr(), ws.numel(), s.rows, s.vocab, top,
+                                     s.stride, ignore_index, s.dtype, stream));
+}
+
+void token_log_probs_meta(at::Tensor& log_prob, at::Tensor& entropy, at::Tensor& lse, at::Tensor& top_log_prob,
+                          at::Tensor& top_index, const at::Tensor& logits, const at::Tensor& tokens,
+                          int64_t ignore_index) {
+  (void)check_log_probs(log_prob, entropy, lse, top_log_prob, top_index, logits, tokens);
+  (void)ignore_index;
+}
+
+struct LogitsGradShape {
+  LogitsShape f;
+  int64_t dlogits_stride;
+};
+
+LogitsGradShape check_log_probs_backward(const at::Tensor& dlogits, const at::Tensor& dlog_prob,
+                                         const MaybeTensor& dentropy, const at::Tensor& logits,
+                                         const at::Tensor& tokens, const at::Tensor& lse, const MaybeTensor& entropy) {
+  LogitsGradShape s;
+  TORCH_CHECK(!dentropy || entropy, "dentropy needs the forward call's entropy");
+  s.f = check_logits(logits, tokens,
+                     {&dlog_prob, &lse, dentropy ? &*dentropy : &lse, dentropy ? &*entropy : &lse});
+  TORCH_CHECK(dlogits.sizes() == logits.sizes(), "dlogits must be shaped like logits");
+  TORCH_CHECK(dlogits.scalar_type() == logits.scalar_type(), "dlogits.dtype() == logits.dtype()");
+  TORCH_CHECK(dlogits.stride(-1) == 1 || s.f.vocab == 1, "dlogits.stride(-1) == 1");
+  TORCH_CHECK(dlogits.device() == logits.device(), "all tensors must be on logits' device");
+  int64_t r = 0;
+  rows_of(dlogits, s.f.vocab, &r, &s.dlogits_stride);
+  if (s.f.rows > 0) {
+    at::assert_no_partial_overlap(dlogits, logits);
+    for (const at::Tensor* t : {&dlog_prob, &tokens, &lse}) at::assert_no_overlap(dlogits, *t);
+    if (dentropy) {
+      at::assert_no_overlap(dlogits, *dentropy);
+      at::assert_no_overlap(dlogits, *entropy);
+    }
+  }
+  return s;
+}
+
+void token_log_probs_backward_hip(at::Tensor& dlogits, const at::Tensor& dlog_prob, const MaybeTensor& dentropy,
+                                  const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& lse,
+                                  const MaybeTensor& entropy, int64_t ignore_index) {
+  const LogitsGradShape s = check_log_probs_backward(dlogits, dlog_prob, dentropy, logits, tokens, lse, entropy);
+  if (s.f.rows == 0) return;
+  c10::DeviceGuard guard(logits.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStream(logits.device().index()).stream();
+  check_status(hprms_token_log_probs_backward(
+      dlogits.data_ptr(), dlog_prob.data_ptr<float>(), dentropy ? dentropy->data_ptr<float>() : nullptr,
+      logits.data_ptr(), tokens.data_ptr<int64_t>(), lse.data_ptr<float>(),
+      dentropy ? entropy->data_ptr<float>() : nullptr, s.f.rows, s.f.vocab, s.dlogits_stride, s.f.stride, ignore_index,
+      s.f.dtype, stream));
+}
+
+void token_log_probs_backward_meta(at::Tensor& dlogits, const at::Tensor& dlog_prob, const MaybeTensor& dentropy,
+                                   const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& lse,
+                                   const MaybeTensor& entropy, int64_t ignore_index) {
+  (void)check_log_probs_backward(dlogits, dlog_prob, dentropy, logits, tokens, lse, entropy);
+  (void)ignore_index;
+}
+
 // _C.set_batch_invariant(enable) -> previous setting; _C.batch_invariant()
 // -> current setting (hprms_set_batch_invariant / hprms_batch_invariant).
 PyObject* py_set_batch_invariant(PyObject*, PyObject* arg) {
@@ -952,6 +1412,19 @@ TORCH_LIBRARY(hp_rms_norm, m) {
   m.def("grad_norm(Tensor(a!) norm, Tensor[] grads) -> ()");
   m.def("clip_grad_norm_(Tensor(a!) norm, Tensor(b!)[] grads, float max_norm) -> ()");
   m.def("clip_grad_norm_out(Tensor(a!) norm, Tensor(b!)[] outs, Tensor[] grads, float max_norm) -> ()");
+  m.def("norm_add_rms_norm(Tensor(a!) out, Tensor(b!) residual_out, Tensor input, Tensor? post_weight, Tensor weight, "
+        "Tensor residual, Tensor? gate, float residual_scale, float eps) -> ()");
+  m.def("norm_add_rms_norm_int8(Tensor(a!) out, Tensor(b!) scale, Tensor(c!) residual_out, Tensor input, "
+        "Tensor? post_weight, Tensor weight, Tensor residual, Tensor? gate, float residual_scale, float eps) -> ()");
+  m.def("norm_add_rms_norm_backward(Tensor(a!) dinput, Tensor(b!) dresidual_in, Tensor(c!)? dpost_weight, "
+        "Tensor(d!) dweight, Tensor(e!)? dgate, Tensor dout, Tensor? dresidual, Tensor input, Tensor residual, "
+        "Tensor? post_weight, Tensor weight, Tensor? gate, float residual_scale, float eps) -> ()");
+  m.def("int8_linear(Tensor(a!) out, Tensor input, Tensor scale, Tensor weight, Tensor weight_scale, Tensor? bias) "
+        "-> ()");
+  m.def("token_log_probs(Tensor(a!) log_prob, Tensor(b!) entropy, Tensor(c!) lse, Tensor(d!) top_log_prob, "
+        "Tensor(e!) top_index, Tensor logits, Tensor tokens, int ignore_index) -> ()");
+  m.def("token_log_probs_backward(Tensor(a!) dlogits, Tensor dlog_prob, Tensor? dentropy, Tensor logits, "
+        "Tensor tokens, Tensor lse, Tensor? entropy, int ignore_index) -> ()");
 }
 
 // ROCm builds of PyTorch expose HIP devices under the CUDA dispatch key.
@@ -973,6 +1446,12 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, CUDA, m) {
   m.impl("grad_norm", &grad_norm_hip);
   m.impl("clip_grad_norm_", &clip_grad_norm_hip_);
   m.impl("clip_grad_norm_out", &clip_grad_norm_out_hip);
+  m.impl("norm_add_rms_norm", &norm_add_rms_norm_hip);
+  m.impl("norm_add_rms_norm_int8", &norm_add_rms_norm_int8_hip);
+  m.impl("norm_add_rms_norm_backward", &norm_add_rms_norm_backward_hip);
+  m.impl("int8_linear", &int8_linear_hip);
+  m.impl("token_log_probs", &token_log_probs_hip);
+  m.impl("token_log_probs_backward", &token_log_probs_backward_hip);
 }
 
 // Shape checks only, for fake tensors / torch.compile tracing.  Meta tensors
@@ -995,4 +1474,10 @@ TORCH_LIBRARY_IMPL(hp_rms_norm, Meta, m) {
   m.impl("grad_norm", &grad_norm_meta);
   m.impl("clip_grad_norm_", &clip_grad_norm_meta_);
   m.impl("clip_grad_norm_out", &clip_grad_norm_out_meta);
+  m.impl("norm_add_rms_norm", &norm_add_rms_norm_meta);
+  m.impl("norm_add_rms_norm_int8", &norm_add_rms_norm_int8_meta);
+  m.impl("norm_add_rms_norm_backward", &norm_add_rms_norm_backward_meta);
+  m.impl("int8_linear", &int8_linear_meta);
+  m.impl("token_log_probs", &token_log_probs_meta);
+  m.impl("token_log_probs_backward", &token_log_probs_backward_meta);
 }

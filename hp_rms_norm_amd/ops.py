@@ -12,6 +12,11 @@ __all__ = ["hp_rms_norm", "relu", "relu_max0", "rms_norm", "fused_add_rms_norm",
            "rms_norm_backward", "rms_norm_backward_out", "linear_cross_entropy", "linear_cross_entropy_out",
            "linear_cross_entropy_backward", "linear_cross_entropy_backward_out",
            "grad_norm", "clip_grad_norm_", "clip_grad_norm_out",
+           "norm_add_rms_norm", "norm_add_rms_norm_out", "norm_add_rms_norm_int8", "norm_add_rms_norm_int8_out",
+           "hp_rms_norm_int8", "fused_add_rms_norm_int8",
+           "norm_add_rms_norm_backward", "norm_add_rms_norm_backward_out",
+           "int8_linear", "int8_linear_out",
+           "token_log_probs", "token_log_probs_out", "token_log_probs_backward", "token_log_probs_backward_out",
            "set_batch_invariant", "batch_invariant"]
 
 MXFP8, MXFP4 = 0, 1  # element formats of the OCP MX output
@@ -321,6 +326,201 @@ def clip_grad_norm_out(outs, grads, max_norm):
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device if grads else None)
     torch.ops.hp_rms_norm.clip_grad_norm_out.default(norm, outs, grads, max_norm)
     return norm
+
+
+def norm_add_rms_norm_out(out, residual_out, input, residual, post_weight, weight, eps, gate=None,
+                          residual_scale=1.0):
+    """The edge between two blocks in one pass: the norm behind a block, its
+    gate, the scaled residual and the norm before the next block.  ``n =
+    rms_norm(input) * post_weight`` (``post_weight`` None: ``n = input``);
+    ``residual_out <- residual_scale * residual + gate * n`` (rounded to the
+    tensor dtype); ``out <- rms_norm(residual_out) * weight``.  Sums are fp32;
+    both norms take ``eps``.  ``input``, ``residual``: [..., H] bf16 or fp16;
+    the weights: [H]; ``gate``: None, [H] (one for each channel), or of as many
+    dimensions as ``input`` with its leading sizes up to some dimension and 1
+    from there on, e.g. [B, 1, H] (one for each sequence) or [B, S, H].  Apply
+    the gate's own activation (a sigmoid, a tanh) before.  ``out`` may be
+    ``input`` and ``residual_out`` may be ``residual``.  No reference
+    counterpart."""
+    torch.ops.hp_rms_norm.norm_add_rms_norm.default(out, residual_out, input, post_weight, weight, residual, gate,
+                                                    residual_scale, eps)
+
+
+def _like(t):
+    """A new contiguous tensor of ``t``'s shape."""
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def norm_add_rms_norm(input, residual, post_weight, weight, eps, gate=None, residual_scale=1.0):
+    """Allocating form of ``norm_add_rms_norm_out``: returns ``(out,
+    residual_out)`` and leaves the arguments untouched."""
+    out, residual_out = _like(input), _like(residual)
+    norm_add_rms_norm_out(out, residual_out, input, residual, post_weight, weight, eps, gate, residual_scale)
+    return out, residual_out
+
+
+def norm_add_rms_norm_int8_out(output, scale, residual_out, input, residual, post_weight, weight, eps, gate=None,
+                               residual_scale=1.0):
+    """``norm_add_rms_norm_out`` with an 8-bit integer output, dynamic per row:
+    with ``y`` the 16-bit output, ``scale[r] = max(amax|y[r]| / 127, FLT_MIN)``
+    and ``output[r] = round(clamp(y[r] * (1 / scale[r]), -127, 127))`` (ties to
+    even), what ``int8_linear`` takes.  ``output``: int8, shaped like
+    ``input``; ``scale``: float32 with one element per row.  A row that holds
+    NaN or infinity has that as its scale and zeros as elements.
+    ``residual_out`` may be ``residual``.  No reference counterpart."""
+    torch.ops.hp_rms_norm.norm_add_rms_norm_int8.default(output, scale, residual_out, input, post_weight, weight,
+                                                         residual, gate, residual_scale, eps)
+
+
+def _int8_rows(input):
+    q = torch.empty(input.shape, dtype=torch.int8, device=input.device)
+    return q, torch.empty(input.shape[:-1] + (1,), dtype=torch.float32, device=input.device)
+
+
+def norm_add_rms_norm_int8(input, residual, post_weight, weight, eps, gate=None, residual_scale=1.0):
+    """Allocating form of ``norm_add_rms_norm_int8_out``: returns ``(q, scale,
+    residual_out)`` with ``scale`` of shape ``input.shape[:-1] + (1,)``, and
+    leaves the arguments untouched."""
+    q, scale = _int8_rows(input)
+    residual_out = _like(residual)
+    norm_add_rms_norm_int8_out(q, scale, residual_out, input, residual, post_weight, weight, eps, gate,
+                               residual_scale)
+    return q, scale, residual_out
+
+
+def hp_rms_norm_int8(output, scale, input, weight, residual, eps):
+    """``hp_rms_norm_fp8`` with 8-bit integers: ``residual <- input +
+    residual`` in place and ``output``, ``scale`` as for
+    ``norm_add_rms_norm_int8_out``.  ``input`` is only read.  No reference
+    counterpart."""
+    torch.ops.hp_rms_norm.norm_add_rms_norm_int8.default(output, scale, residual, input, None, weight, residual, None,
+                                                         1.0, eps)
+
+
+def fused_add_rms_norm_int8(input, residual, weight, eps):
+    """Allocating form of ``hp_rms_norm_int8``: returns ``(q, scale)`` with
+    ``q`` int8 shaped like ``input`` and ``scale`` float32 of shape
+    ``input.shape[:-1] + (1,)``; ``residual`` is updated in place."""
+    q, scale = _int8_rows(input)
+    hp_rms_norm_int8(q, scale, input, weight, residual, eps)
+    return q, scale
+
+
+def norm_add_rms_norm_backward_out(dinput, dresidual_in, dpost_weight, dweight, dgate, dout, input, residual,
+                                   post_weight, weight, eps, gate=None, residual_scale=1.0, dresidual=None):
+    """Gradient of ``norm_add_rms_norm`` into given tensors.  ``residual`` is
+    the forward call's ``residual_out``, ``dout`` the gradient of its ``out``
+    and ``dresidual`` (or None) that of ``residual_out`` by its other uses.
+    With ``r`` and ``q`` the reciprocal roots of the mean squares of
+    ``residual`` and ``input``: ``dh = r * (dout * weight) - residual * (r^3 *
+    mean(dout * weight * residual)) + dresidual``; ``dresidual_in <-
+    residual_scale * dh``; ``dweight <- sum over rows of dout * residual * r``;
+    ``dgate <- dh * n``, summed over the rows that share a gate;
+    ``dpost_weight <- sum over rows of gate * dh * input * q``; ``dinput`` the
+    gradient of ``input`` by the first norm.  ``dpost_weight`` and ``dgate``
+    are None without ``post_weight`` and ``gate``; ``dweight`` and
+    ``dpost_weight`` may be float32.  Sums are fp32, each output is rounded
+    once.  ``dinput`` and ``dresidual_in`` may each be one of ``dout``,
+    ``dresidual``, ``input`` and ``residual`` (not the same).  No reference
+    counterpart."""
+    torch.ops.hp_rms_norm.norm_add_rms_norm_backward.default(
+        dinput, dresidual_in, dpost_weight, dweight, dgate, dout, dresidual, input, residual, post_weight, weight,
+        gate, residual_scale, eps)
+
+
+def norm_add_rms_norm_backward(dout, input, residual, post_weight, weight, eps, gate=None, residual_scale=1.0,
+                               dresidual=None):
+    """Allocating form of ``norm_add_rms_norm_backward_out``: returns
+    ``(dinput, dresidual_in, dpost_weight, dweight, dgate)``, None for what
+    there is not.  ``dout`` and ``dresidual`` may have any strides, as for
+    ``rms_norm_backward``."""
+    dout = _rows(dout)
+    if dresidual is not None:
+        dresidual = _rows(dresidual)
+    dinput, dresidual_in, dweight = _like(input), _like(residual), _like(weight)
+    dpost_weight = None if post_weight is None else _like(post_weight)
+    dgate = None if gate is None else _like(gate)
+    norm_add_rms_norm_backward_out(dinput, dresidual_in, dpost_weight, dweight, dgate, dout, input, residual,
+                                   post_weight, weight, eps, gate, residual_scale, dresidual)
+    return dinput, dresidual_in, dpost_weight, dweight, dgate
+
+
+def int8_linear_out(out, input, scale, weight, weight_scale, bias=None):
+    """The product of 8-bit integer rows and weights, each row of both with a
+    scale: ``out <- (input @ weight.T) * scale * weight_scale + bias``.
+    ``input``: [..., K] int8 (as ``fused_add_rms_norm_int8`` gives it) with
+    ``scale`` float32, one element per row; ``weight``: [N, K] int8 with
+    ``weight_scale`` float32, one element per row; ``bias``: [N] of ``out``'s
+    dtype or None; ``out``: [..., N] bf16 or fp16.  Sums are exact integers (K
+    up to 131071), rounded to fp32 and scaled, and ``out`` is rounded once, so
+    a row's bits do not depend on the other rows.  Operands whose rows are not
+    whole 16 bytes at 16-byte boundaries are copied by each call: lay a weight
+    out with K % 16 == 0.  No reference counterpart."""
+    torch.ops.hp_rms_norm.int8_linear.default(out, input, scale, weight, weight_scale, bias)
+
+
+def int8_linear(input, scale, weight, weight_scale, bias=None, dtype=torch.bfloat16):
+    """Allocating form of ``int8_linear_out``: returns ``out`` of ``dtype``
+    (bf16 or fp16)."""
+    out = torch.empty(input.shape[:-1] + (weight.shape[0],), dtype=dtype, device=input.device)
+    torch.ops.hp_rms_norm.int8_linear.default(out, input, scale, weight, weight_scale, bias)
+    return out
+
+
+def token_log_probs_out(log_prob, entropy, lse, top_log_prob, top_index, logits, tokens, ignore_index=-100):
+    """Log probabilities of given tokens under rows of logits, with the entropy
+    and the most likely alternatives: ``lse <- logsumexp(logits)``, ``log_prob
+    <- logits[token] - lse``, ``entropy <- -sum(p * log(p))``, ``top_index <-``
+    the largest logits, equal ones by the lower index, and ``top_log_prob <-``
+    theirs minus ``lse``.  ``logits``: [..., V] bf16, fp16 or fp32 (V up to
+    2^20); ``tokens``: int64 [...], contiguous; ``log_prob``, ``entropy`` and
+    ``lse``: float32 like ``tokens``; ``top_log_prob`` and ``top_index``:
+    float32 and int64 [..., k], k from 0 to 64.  Rows whose token is
+    ``ignore_index`` get zeros (and index -1) and are never read; another token
+    outside ``[0, V)`` gives a NaN ``log_prob``.  Logits of -inf (forbidden
+    tokens) have probability 0; a row of nothing else has entropy 0 and log
+    probabilities of -inf.  NaN or +inf makes a row's ``lse`` NaN; NaN ranks
+    first.  No reference counterpart."""
+    torch.ops.hp_rms_norm.token_log_probs.default(log_prob, entropy, lse, top_log_prob, top_index, logits, tokens,
+                                                  ignore_index)
+
+
+def token_log_probs(logits, tokens, top=0, ignore_index=-100):
+    """Allocating form of ``token_log_probs_out`` with ``top`` alternatives:
+    returns ``(log_prob, entropy, lse, top_log_prob, top_index)``; the backward
+    call takes ``lse`` and ``entropy``."""
+    log_prob = torch.empty(tokens.shape, dtype=torch.float32, device=tokens.device)
+    entropy, lse = torch.empty_like(log_prob), torch.empty_like(log_prob)
+    shape = tuple(tokens.shape) + (top,)
+    top_log_prob = torch.empty(shape, dtype=torch.float32, device=tokens.device)
+    top_index = torch.empty(shape, dtype=torch.int64, device=tokens.device)
+    token_log_probs_out(log_prob, entropy, lse, top_log_prob, top_index, logits, tokens, ignore_index)
+    return log_prob, entropy, lse, top_log_prob, top_index
+
+
+def token_log_probs_backward_out(dlogits, dlog_prob, logits, tokens, lse, entropy=None, dentropy=None,
+                                 ignore_index=-100):
+    """Gradient of ``token_log_probs``' ``log_prob`` and ``entropy``: with ``p =
+    exp(logits - lse)``, ``dlogits <- dlog_prob * (onehot(token) - p) - dentropy
+    * p * (log(p) + entropy)``.  ``lse`` and ``entropy`` are the forward
+    call's, ``dlog_prob`` and ``dentropy`` (or None) float32 like ``tokens``.
+    Ignored rows and rows of nothing but -inf get zeros; a token out of range
+    makes its row NaN.  ``dlogits`` may be ``logits``.  No reference
+    counterpart."""
+    torch.ops.hp_rms_norm.token_log_probs_backward.default(dlogits, dlog_prob, dentropy, logits, tokens, lse,
+                                                           entropy, ignore_index)
+
+
+def token_log_probs_backward(dlog_prob, logits, tokens, lse, entropy=None, dentropy=None, ignore_index=-100):
+    """Allocating form of ``token_log_probs_backward_out``: returns
+    ``dlogits``.  ``dlog_prob`` and ``dentropy`` may be any float32 tensors
+    that expand to ``tokens``' shape."""
+    dlogits = _like(logits)
+    if dentropy is not None:
+        dentropy = dentropy.expand(tokens.shape).contiguous()
+    token_log_probs_backward_out(dlogits, dlog_prob.expand(tokens.shape).contiguous(), logits, tokens, lse, entropy,
+                                 dentropy, ignore_index)
+    return dlogits
 
 
 def set_batch_invariant(enable):

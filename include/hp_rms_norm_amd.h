@@ -23,14 +23,14 @@
 extern "C" {
 #endif
 
-#define HPRMS_ABI_VERSION 9
+#define HPRMS_ABI_VERSION 10
 
 /* element types (the reference accepts exactly these two:
  * hp_rms_norm/csrc/cuda/hp_rms_norm.cu:29-49) */
 typedef enum {
   HPRMS_DTYPE_BF16 = 0,
   HPRMS_DTYPE_FP16 = 1,
-  HPRMS_DTYPE_FP32 = 2  /* gradients only: dweight_dtype, and the dtypes of a list of gradients */
+  HPRMS_DTYPE_FP32 = 2  /* dweight_dtype, the dtypes of a list of gradients, logits */
 } hprms_dtype;
 
 /* status codes */
@@ -458,6 +458,118 @@ int hprms_grad_norm(float* norm, const void* const* grads, const int* dtypes, co
 int hprms_clip_grad_norm(float* norm, void* const* outs, const int* out_dtypes, const void* const* grads,
                          const int* dtypes, const int64_t* counts, int n, double max_norm, void* workspace,
                          int64_t workspace_size, hipStream_t stream);
+
+/*
+ * The edge between two blocks: the norm behind a block, its gate, the scaled
+ * residual and the norm before the next block.
+ *   n <- input * rsqrt(mean(input^2) + eps) * post_weight   (post_weight NULL: n = input)
+ *   residual_out[r, :] <- rne(residual_scale * residual + gate * n)   (gate NULL: n itself)
+ *   out[r, :] <- rne(residual_out * rsqrt(mean(residual_out^2) + eps) * weight)
+ * in binary32.  Row r takes row r / rows_per_gate of the gate (rows_per_gate >=
+ * rows: one for all, 1: one for each).  The _int8 form quantises the 16-bit
+ * output y per row instead: scale[r] <- max(max|y| / 127, FLT_MIN), out[r, :] <-
+ * rne(clamp(y * (1 / scale[r]), -127, 127)); a row that holds NaN or infinity has
+ * that as its scale and zeros as elements.  `out` (16-bit form) may be `input`
+ * and `residual_out` may be `residual`, exactly; nothing else is shared.  The
+ * kernel shape follows from hidden alone in either batch-invariant mode.  No
+ * workspace.  rows == 0 is a no-op.  No counterpart in the reference.
+ */
+int hprms_norm_add_rmsnorm(void* out, void* residual_out, const void* input, const void* post_weight,
+                           const void* weight, const void* residual, const void* gate, int64_t rows, int64_t hidden,
+                           int64_t rows_per_gate, int64_t out_row_stride, int64_t residual_out_row_stride,
+                           int64_t input_row_stride, int64_t residual_row_stride, int64_t gate_row_stride, int dtype,
+                           double residual_scale, double eps, hipStream_t stream);
+int hprms_norm_add_rmsnorm_int8(void* out, float* scale, void* residual_out, const void* input,
+                                const void* post_weight, const void* weight, const void* residual, const void* gate,
+                                int64_t rows, int64_t hidden, int64_t rows_per_gate, int64_t out_row_stride,
+                                int64_t residual_out_row_stride, int64_t input_row_stride,
+                                int64_t residual_row_stride, int64_t gate_row_stride, int dtype,
+                                double residual_scale, double eps, hipStream_t stream);
+
+/*
+ * Gradient of hprms_norm_add_rmsnorm().  `residual` is the forward call's
+ * residual_out, `dout` the gradient of its out and `dresidual` (may be NULL) that
+ * of residual_out by its other uses.  With h = residual, r = rsqrt(mean(h^2) +
+ * eps), q = rsqrt(mean(input^2) + eps), n as above:
+ *   dh           =  r * (dout * weight) - h * (r^3 * mean(dout * weight * h)) + dresidual
+ *   dresidual_in <- rne(residual_scale * dh)
+ *   dweight      <- sum over rows of dout * h * r
+ *   dgate        <- dh * n, summed over the rows that share a gate
+ *   dpost_weight <- sum over rows of gate * dh * input * q
+ *   dinput       <- rne(q * (gate * dh * post_weight) - input * (q^3 * mean(gate * dh * post_weight * input)))
+ * (without post_weight dinput = gate * dh).  The gate has gate_rows rows, which
+ * divide rows: row r takes row r / (rows / gate_rows); 0 and NULL without one.
+ * Sums are binary32, in an order fixed for given sizes and CU count, rounded
+ * once; dgate is of dtype, dweight and dpost_weight of their dtypes (dtype or
+ * HPRMS_DTYPE_FP32).  All outputs are written, not added to (rows == 0 writes
+ * zeros to the weights' and the gate's).  `dinput` and `dresidual_in` may each
+ * be one of dout, dresidual, input and residual exactly, not the same one, and
+ * with a gate for each row `dgate` may be `gate`.  The workspace is as for
+ * hprms_rmsnorm_backward(), of hprms_norm_add_rmsnorm_backward_workspace()
+ * bytes.  No counterpart in the reference.
+ */
+int64_t hprms_norm_add_rmsnorm_backward_workspace(int64_t rows, int64_t hidden, int64_t gate_rows);
+int hprms_norm_add_rmsnorm_backward(void* dinput, void* dresidual_in, void* dpost_weight, void* dweight, void* dgate,
+                                    const void* dout, const void* dresidual, const void* input, const void* residual,
+                                    const void* post_weight, const void* weight, const void* gate, void* workspace,
+                                    int64_t workspace_size, int64_t rows, int64_t hidden, int64_t gate_rows,
+                                    int64_t dinput_row_stride, int64_t dresidual_in_row_stride,
+                                    int64_t dgate_row_stride, int64_t dout_row_stride, int64_t dresidual_row_stride,
+                                    int64_t input_row_stride, int64_t residual_row_stride, int64_t gate_row_stride,
+                                    int dtype, int dpost_weight_dtype, int dweight_dtype, double residual_scale,
+                                    double eps, hipStream_t stream);
+
+/*
+ * The product of 8-bit integer rows and weights:
+ *   out[t, o] <- rne((sum_k input[t, k] * weight[o, k]) * scale[t] * weight_scale[o] + bias[o])
+ * input [rows, inner] and weight [outer, inner] int8 at row strides, scale [rows],
+ * weight_scale [outer] binary32, bias [outer] of dtype or NULL, out [rows, outer]
+ * of dtype.  The sums are exact (inner is at most 131071), so a row's bits do not
+ * depend on the other rows.  Workspace: hprms_int8_linear_workspace() bytes,
+ * 256-byte aligned, none (and NULL) where both operands have 16-byte aligned
+ * rows of whole 16 bytes no more than 4 MiB apart; others are copied there by
+ * each call.  rows and outer go up to 2^24, out up to 2^36 elements.  rows == 0
+ * is a no-op.  No counterpart in the reference.
+ */
+int64_t hprms_int8_linear_workspace(int64_t rows, int64_t inner, int64_t outer, const void* input,
+                                    int64_t input_row_stride, const void* weight, int64_t weight_row_stride);
+int hprms_int8_linear(void* out, const void* input, const float* scale, const void* weight, const float* weight_scale,
+                      const void* bias, void* workspace, int64_t workspace_size, int64_t rows, int64_t inner,
+                      int64_t outer, int64_t out_row_stride, int64_t input_row_stride, int64_t weight_row_stride,
+                      int dtype, hipStream_t stream);
+
+/*
+ * Log probabilities of given tokens under rows of logits z [rows, vocab] (any
+ * hprms_dtype):
+ *   lse <- log(sum_v exp(z[v]));  log_prob <- z[tokens] - lse;  entropy <- -sum_v p[v] log p[v], p = exp(z - lse)
+ *   top_index <- the `top` (0 ... 64) largest z, equal ones by the lower index; top_log_prob <- theirs minus lse
+ * in binary32.  Rows whose token is ignore_index are not read and get 0 (and
+ * index -1); another token outside [0, vocab) gives a NaN log_prob.  A logit of
+ * -infinity has probability 0; a row of nothing else gives lse = log_prob =
+ * top_log_prob = -infinity and entropy 0.  NaN or +infinity makes a row's lse
+ * NaN; NaN ranks above every number.  Workspace: as for
+ * hprms_rmsnorm_backward(), of hprms_token_log_probs_workspace() bytes.  rows
+ * == 0 is a no-op; vocab goes up to 2^20.  A row's bits do not depend on the
+ * other rows.  No counterpart in the reference.
+ */
+int64_t hprms_token_log_probs_workspace(int64_t rows, int64_t vocab, int64_t top, int dtype);
+int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* top_log_prob, int64_t* top_index,
+                          const void* logits, const int64_t* tokens, void* workspace, int64_t workspace_size,
+                          int64_t rows, int64_t vocab, int64_t top, int64_t logits_row_stride, int64_t ignore_index,
+                          int dtype, hipStream_t stream);
+
+/*
+ * Gradient of hprms_token_log_probs()'s log_prob and entropy, from its lse and
+ * entropy:
+ *   dlogits <- dlog_prob * ([v == token] - p) - dentropy * p * (log p + entropy)
+ * `dentropy` may be NULL (and then `entropy`).  Ignored rows and rows of nothing
+ * but -infinity get zeros, a token out of range NaN.  `dlogits` may be `logits`
+ * exactly.  No workspace.  No counterpart in the reference.
+ */
+int hprms_token_log_probs_backward(void* dlogits, const float* dlog_prob, const float* dentropy, const void* logits,
+                                   const int64_t* tokens, const float* lse, const float* entropy, int64_t rows,
+                                   int64_t vocab, int64_t dlogits_row_stride, int64_t logits_row_stride,
+                                   int64_t ignore_index, int dtype, hipStream_t stream);
 
 /* Lists the vector-tier configurations built into the library for (dtype,
  * mode, numbered as for hprms_select_config).  Writes up to `capacity`
