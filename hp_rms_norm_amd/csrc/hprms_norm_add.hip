@@ -74,7 +74,6 @@ __device__ __forceinline__ uint32_t to_int8(float v, const RowScale& s) {
 
 template <int DT, int LPR, int VPL, int BLOCK, bool POST, bool INT8, bool NT>
 __global__ __launch_bounds__(BLOCK) void norm_add_kernel(NormAddArgs a) {
-  using F = Fmt<DT>;
   constexpr int RPB = BLOCK / LPR;
   __shared__ float sums[2][BLOCK / 64];
   __shared__ uint32_t tops[BLOCK / 64];
@@ -98,6 +97,10 @@ __global__ __launch_bounds__(BLOCK) void norm_add_kernel(NormAddArgs a) {
       x[k] = load_row8_once<NT>(a.input + row * a.input_stride + off[k]);
       s[k] = load_row8_once<NT>(a.residual + row * a.residual_stride + off[k]);
     }
+    if (tail) {
+      drop_first(x[k], skip[k]);
+      drop_first(s[k], skip[k]);
+    }
   }
   float ix = 1.0f;
   if constexpr (POST) {
@@ -107,7 +110,7 @@ __global__ __launch_bounds__(BLOCK) void norm_add_kernel(NormAddArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float v = element<DT>(x[k], j);
-        if (j >= skip[k]) ss[0] += v * v;
+        ss[0] += v * v;
       }
     sum_rows<1, LPR, BLOCK>(ss, sums[0]);
     ix = inverse_rms(ss[0], a.hidden, a.eps);
@@ -116,6 +119,8 @@ __global__ __launch_bounds__(BLOCK) void norm_add_kernel(NormAddArgs a) {
 #pragma unroll
   for (int k = 0; k < VPL; ++k) {
     u32x4 p = {0, 0, 0, 0}, g = {0, 0, 0, 0};
+    packed_again(x[k]);
+    packed_again(s[k]);
     if (POST && on[k]) p = load_row8(a.post_weight + off[k]);
     if (gate && on[k]) g = load_row8(gate + off[k]);
     float h[8];
@@ -130,7 +135,7 @@ __global__ __launch_bounds__(BLOCK) void norm_add_kernel(NormAddArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float v = element<DT>(s[k], j);
-      if (j >= skip[k]) ss[0] += v * v;
+      ss[0] += v * v;
     }
     if (on[k]) store_row8(a.residual_out + row * a.residual_out_stride + off[k], s[k], skip[k]);
   }
@@ -146,7 +151,7 @@ __global__ __launch_bounds__(BLOCK) void norm_add_kernel(NormAddArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       y[j] = element<DT>(s[k], j) * ih * element<DT>(w[k], j);
-      if (INT8 && on[k] && j >= skip[k]) top = __builtin_elementwise_max(top, __float_as_uint(y[j]) & 0x7fffffffu);
+      if constexpr (INT8) top = __builtin_elementwise_max(top, __float_as_uint(y[j]) & 0x7fffffffu);
     }
     s[k] = pack8<DT>(y);
     if (!INT8 && on[k]) store_row8((uint16_t*)a.out + row * a.out_stride + off[k], s[k], skip[k]);

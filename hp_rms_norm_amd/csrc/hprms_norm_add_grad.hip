@@ -49,7 +49,6 @@ struct NormAddGradArgs {
   float* post_sums;    // [gridDim.x, hidden]
   float* gate_sums;    // [units, hidden] if parts > 1
   int64_t rows, gates, rows_per_gate, units;
-  int64_t part_rows;  // rows of a unit
   int32_t parts;      // units of a gate
   int64_t dout_stride, dresidual_stride, input_stride, residual_stride, gate_stride, dinput_stride,
       dresidual_in_stride, dgate_stride;
@@ -59,9 +58,60 @@ struct NormAddGradArgs {
 
 enum GateKind { kNoGate, kSharedGate, kElementGate };
 
-template <int DT, int LPR, int VPL, int BLOCK, int PER_SIMD, bool POST, int GATE, bool AHEAD>
-__global__ __launch_bounds__(BLOCK, PER_SIMD) void norm_add_grad_kernel(NormAddGradArgs a) {
+// A lane's sums of its columns, N times 8: in registers, or (LDS) in its own slots
+// of LDS.
+template <bool LDS, int N, int BLOCK>
+struct ColumnSums {
+  float v[N][8];
+  __device__ __forceinline__ void clear(int i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+  }
+  __device__ __forceinline__ void add(int i, const float (&t)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] += t[j];
+  }
+  __device__ __forceinline__ void get(int i, float (&t)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = v[i][j];
+  }
+};
+template <int N, int BLOCK>
+struct ColumnSums<true, N, BLOCK> {
+  f32x4* at;
+  __device__ __forceinline__ ColumnSums() {
+    __shared__ f32x4 slots[2 * N * BLOCK];
+    at = slots + threadIdx.x;
+  }
+  __device__ __forceinline__ void clear(int i) { at[2 * i * BLOCK] = at[(2 * i + 1) * BLOCK] = f32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void add(int i, const float (&t)[8]) {
+    at[2 * i * BLOCK] += f32x4{t[0], t[1], t[2], t[3]};
+    at[(2 * i + 1) * BLOCK] += f32x4{t[4], t[5], t[6], t[7]};
+  }
+  __device__ __forceinline__ void get(int i, float (&t)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = at[(2 * i + j / 4) * BLOCK][j % 4];
+  }
+};
+
+// LPR lanes a row, VPL vectors of 8 elements a lane (slots as in hprms_rows.h).
+// Per element and row, with m the product of what scales it behind dh (gate *
+// post_weight, or the one there is):
+//
+//   first pass   squares of h and x, weight * (d * h)
+//   second       dh; v = dh * x; z += q * v; sum of m * v; dweight += r * (d * h)
+//   third        dx = q * (m * dh) - x * c
+//
+// z alone gives both columns' sums of a shared gate: its gradient is post_weight *
+// z, and gate * z is its unit's share of dpost.  HOLD keeps weight and m as
+// binary32 in registers (8 instructions an element fewer than unpacking them for
+// each row); LACC keeps the columns' sums in LDS.
+template <int DT, int LPR, int VPL, int BLOCK, bool POST, int GATE, bool AHEAD, bool HOLD, bool LACC>
+__global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a) {
   constexpr int RPB = BLOCK / LPR;
+  constexpr bool SHARED = GATE == kSharedGate, ELEMENT = GATE == kElementGate;
+  constexpr bool SCALED = POST || SHARED;  // m is more than 1 (or a row's own gate)
+  constexpr bool Z = POST || SHARED;
   __shared__ float sums[2][BLOCK / 64 * 3];
   __shared__ float sums2[2][BLOCK / 64];
   __shared__ float cols[RPB > 1 ? RPB * LPR * 8 : 1];
@@ -70,175 +120,227 @@ __global__ __launch_bounds__(BLOCK, PER_SIMD) void norm_add_grad_kernel(NormAddG
   const int dup = tail ? 8 - tail : 0;  // the tail vector's elements that a whole vector holds
   int off[VPL], skip[VPL];
   bool on[VPL];
-  float aw[VPL][8], ap[POST ? VPL : 1][8], ag[GATE == kSharedGate ? VPL : 1][8];
+  ColumnSums<LACC, (Z ? 2 : 1) * VPL, BLOCK> acc;  // dweight's, then z
+  float* post_sums = a.post_sums + (int64_t)blockIdx.x * a.hidden;
 #pragma unroll
   for (int k = 0; k < VPL; ++k) {
     const int v = k * LPR + lane;
     on[k] = v < nvec + (tail ? 1 : 0);
     off[k] = v < nvec ? v * 8 : a.hidden - 8;
     skip[k] = v < nvec ? 0 : dup;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      aw[k][j] = 0.0f;
-      if constexpr (POST) ap[k][j] = 0.0f;
-      if constexpr (GATE == kSharedGate) ag[k][j] = 0.0f;
-    }
+    acc.clear(k);
+    if constexpr (Z) acc.clear(VPL + k);
   }
   // a column's sums over the row groups of the workgroup, in row group 0
-  auto join = [&](float (&acc)[8]) {
+  auto join = [&](float (&t)[8]) {
     if constexpr (RPB > 1) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) cols[(sub * LPR + lane) * 8 + j] = acc[j];
+      for (int j = 0; j < 8; ++j) cols[(sub * LPR + lane) * 8 + j] = t[j];
       __syncthreads();
       if (sub == 0) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          for (int i = 1; i < RPB; ++i) acc[j] += cols[(i * LPR + lane) * 8 + j];
+          for (int i = 1; i < RPB; ++i) t[j] += cols[(i * LPR + lane) * 8 + j];
       }
     }
   };
-  auto put = [&](float* to, int k, const float (&acc)[8]) {
+  auto put = [&](float* to, int k, const float (&t)[8]) {
     if (sub != 0 || !on[k]) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j >= skip[k]) to[off[k] + j] = acc[j];
+      if (j >= skip[k]) to[off[k] + j] = t[j];
   };
+  const u32x4 zeros = {0, 0, 0, 0};
   u32x4 nd[VPL], ne[VPL], nx[VPL], nh[VPL], ng[VPL];
   auto load = [&](int64_t row, bool in) {
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
-      nd[k] = ne[k] = nx[k] = nh[k] = u32x4{0, 0, 0, 0};
-      if constexpr (GATE == kElementGate) ng[k] = u32x4{0, 0, 0, 0};
+      nd[k] = ne[k] = nx[k] = nh[k] = ng[k] = zeros;
       if (in && on[k]) {
         nd[k] = load_row8_once<true>(a.dout + row * a.dout_stride + off[k]);
         nh[k] = load_row8_once<true>(a.residual + row * a.residual_stride + off[k]);
         nx[k] = load_row8_once<true>(a.input + row * a.input_stride + off[k]);
         if (a.dresidual) ne[k] = load_row8_once<true>(a.dresidual + row * a.dresidual_stride + off[k]);
-        if constexpr (GATE == kElementGate) ng[k] = load_row8_once<true>(a.gate + row * a.gate_stride + off[k]);
+        if constexpr (ELEMENT) ng[k] = load_row8_once<true>(a.gate + row * a.gate_stride + off[k]);
       }
     }
   };
+  const uint16_t* gate = a.gate;  // the unit's row of a shared one
+  float wf[HOLD ? VPL : 1][8], mf[HOLD && SCALED ? VPL : 1][8];
+  auto scales = [&](int k, float (&m)[8]) {
+    const u32x4 p = POST && on[k] ? load_row8(a.post_weight + off[k]) : zeros;
+    const u32x4 g = SHARED && on[k] ? load_row8(gate + off[k]) : zeros;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      m[j] = POST && SHARED ? element<DT>(p, j) * element<DT>(g, j) : POST ? element<DT>(p, j) : element<DT>(g, j);
+  };
+  auto weights = [&](int k, float (&w)[8]) {
+    const u32x4 v = on[k] ? load_row8(a.weight + off[k]) : zeros;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = element<DT>(v, j);
+  };
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) weights(k, wf[k]);
+  }
   int phase = 0;
   for (int64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
     // unit u is part u / gates of gate u % gates; a unit's rows are whole
     // workgroup steps, `parts` steps apart
-    const int64_t gate = GATE == kSharedGate ? unit % a.gates : 0;
-    const int64_t part = GATE == kSharedGate ? unit / a.gates : unit;
-    const int64_t end = GATE == kSharedGate ? (gate + 1) * a.rows_per_gate : a.rows;
+    const int64_t at = SHARED ? unit % a.gates : 0;
+    const int64_t part = SHARED ? unit / a.gates : unit;
+    const int64_t end = SHARED ? (at + 1) * a.rows_per_gate : a.rows;
     const int64_t step = (int64_t)a.parts * RPB;
-    const int64_t first = (GATE == kSharedGate ? gate * a.rows_per_gate : 0) + part * RPB;
+    const int64_t first = (SHARED ? at * a.rows_per_gate : 0) + part * RPB;
     if (first < end) load(first + sub, first + sub < end);
+    if constexpr (SHARED) gate = a.gate + at * a.gate_stride;
+    if constexpr (HOLD && SCALED) {
+#pragma unroll
+      for (int k = 0; k < VPL; ++k) scales(k, mf[k]);
+    }
     for (int64_t row0 = first; row0 < end; row0 += step) {
       const int64_t row = row0 + sub;
       const bool live = RPB == 1 || row < end;
-      u32x4 d[VPL], e[VPL], x[VPL], h[VPL], g[VPL], w[VPL], p[VPL];
+      u32x4 d[VPL], e[VPL], x[VPL], h[VPL], g[VPL];
 #pragma unroll
       for (int k = 0; k < VPL; ++k) {
         d[k] = nd[k];
+        e[k] = ne[k];
         x[k] = nx[k];
         h[k] = nh[k];
-        e[k] = ne[k];
-        if constexpr (GATE == kElementGate) g[k] = ng[k];
-        w[k] = p[k] = u32x4{0, 0, 0, 0};
-        if constexpr (GATE == kSharedGate) g[k] = u32x4{0, 0, 0, 0};
-        if (on[k]) {
-          w[k] = load_row8(a.weight + off[k]);
-          if constexpr (POST) p[k] = load_row8(a.post_weight + off[k]);
-          if constexpr (GATE == kSharedGate) g[k] = load_row8(a.gate + gate * a.gate_stride + off[k]);
+        g[k] = ng[k];
+        if (tail) {
+          drop_first(d[k], skip[k]);
+          drop_first(e[k], skip[k]);
+          drop_first(x[k], skip[k]);
+          drop_first(h[k], skip[k]);
         }
       }
       if constexpr (AHEAD) load(row + step, row + step < end);
-      float s[3] = {0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < VPL; ++k)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j < skip[k]) continue;
-          const float hf = element<DT>(h[k], j);
-          s[0] += hf * hf;
-          s[1] += element<DT>(d[k], j) * element<DT>(w[k], j) * hf;
-          if constexpr (POST) s[2] += element<DT>(x[k], j) * element<DT>(x[k], j);
-        }
-      if constexpr (POST) {
-        sum_rows<3, LPR, BLOCK>(s, sums[phase]);
-      } else {
-        float t[2] = {s[0], s[1]};
-        sum_rows<2, LPR, BLOCK>(t, sums[phase]);
-        s[0] = t[0];
-        s[1] = t[1];
-      }
-      const float n = (float)a.hidden;
-      const float r = 1.0f / sqrtf(s[0] / n + a.eps);
-      const float rc = r * r * (r * (s[1] / n));
-      const float q = POST ? 1.0f / sqrtf(s[2] / n + a.eps) : 1.0f;
-      float du[1] = {0.0f};
-      float u[VPL][8];  // the gradient of what is normed behind the block, or of the block's output
+      float s[POST ? 3 : 2] = {};
 #pragma unroll
       for (int k = 0; k < VPL; ++k) {
-        float o[8], dg[8];
+        float w[8];
+        if constexpr (!HOLD) weights(k, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float hf = element<DT>(h[k], j);
+          s[0] += hf * hf;
+          s[1] += (element<DT>(d[k], j) * hf) * (HOLD ? wf[HOLD ? k : 0][j] : w[j]);
+          if constexpr (POST) s[2] += element<DT>(x[k], j) * element<DT>(x[k], j);
+        }
+        packed_again(d[k]);
+        packed_again(x[k]);
+        packed_again(h[k]);
+      }
+      sum_rows<POST ? 3 : 2, LPR, BLOCK>(s, sums[phase]);
+      const float n = (float)a.hidden;
+      // (a row group without a row holds zeros, and adds zeros to the columns' sums)
+      const float r = live ? 1.0f / sqrtf(s[0] / n + a.eps) : 0.0f;
+      const float rc = r * r * (r * (s[1] / n));
+      const float q = !POST ? 1.0f : live ? 1.0f / sqrtf(s[POST ? 2 : 0] / n + a.eps) : 0.0f;
+      float mv[1] = {0.0f};
+      float u[POST ? VPL : 1][8];
+#pragma unroll
+      for (int k = 0; k < VPL; ++k) {
+        float w[8], m[8], o[8], dx[8], dg[8], tw[8], tz[8];
+        if constexpr (!HOLD) weights(k, w);
+        if constexpr (!HOLD && SCALED) scales(k, m);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float hf = element<DT>(h[k], j), df = element<DT>(d[k], j), xf = element<DT>(x[k], j);
-          float dh = r * (df * element<DT>(w[k], j)) - hf * rc;
-          dh += element<DT>(e[k], j);
+          const float wj = HOLD ? wf[HOLD ? k : 0][j] : w[j];
+          float dh = r * (df * wj) - hf * rc + element<DT>(e[k], j);
           o[j] = dh * a.residual_scale;
-          float t = dh;
-          if constexpr (GATE != kNoGate) t *= element<DT>(g[k], j);
-          const float nx = xf * q;
-          if constexpr (POST) {
-            const float pf = element<DT>(p[k], j);
-            if constexpr (GATE != kNoGate) dg[j] = dh * (nx * pf);
-            if (live) ap[k][j] += t * nx;
-            t *= pf;
-            if (j >= skip[k]) du[0] += t * xf;
-          } else {
-            if constexpr (GATE != kNoGate) dg[j] = dh * xf;
+          tw[j] = (df * hf) * r;
+          float v = dh * xf;  // q times this: what the first norm passes on, without its weight
+          if constexpr (SCALED) {
+            const float mj = HOLD ? mf[HOLD && SCALED ? k : 0][j] : m[j];
+            if constexpr (ELEMENT) {
+              const float gf = element<DT>(g[k], j);
+              dg[j] = (v * q) * mj;
+              dh *= gf;
+              v *= gf;
+            }
+            tz[j] = v * q;
+            mv[0] += v * mj;
+            dh *= mj;
+          } else if constexpr (ELEMENT) {
+            dg[j] = v;
+            dh *= element<DT>(g[k], j);
           }
-          u[k][j] = t;
-          if (live) aw[k][j] += df * (hf * r);
-          if constexpr (GATE == kSharedGate) {
-            if (live) ag[k][j] += dg[j];
-          }
+          if constexpr (POST)
+            u[k][j] = dh;
+          else
+            dx[j] = dh;
         }
+        acc.add(k, tw);
+        if constexpr (Z) acc.add(VPL + k, tz);
         if (live && on[k]) {
           store_row8(a.dresidual_in + row * a.dresidual_in_stride + off[k], pack8<DT>(o), skip[k]);
-          if constexpr (GATE == kElementGate)
-            store_row8(a.dgate + row * a.dgate_stride + off[k], pack8<DT>(dg), skip[k]);
+          if constexpr (ELEMENT) store_row8(a.dgate + row * a.dgate_stride + off[k], pack8<DT>(dg), skip[k]);
+          if constexpr (!POST) store_row8(a.dinput + row * a.dinput_stride + off[k], pack8<DT>(dx), skip[k]);
+        }
+        packed_again(x[k]);
+      }
+      if constexpr (POST) {
+        sum_rows<1, LPR, BLOCK>(mv, sums2[phase]);
+        const float c = q * q * (q * (mv[0] / n));
+#pragma unroll
+        for (int k = 0; k < VPL; ++k) {
+          float dx[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dx[j] = q * u[k][j] - element<DT>(x[k], j) * c;
+          if (live && on[k])
+            store_row8(a.dinput + row * a.dinput_stride + off[k], pack8<DT>(dx), skip[k]);
         }
       }
-      if constexpr (POST) sum_rows<1, LPR, BLOCK>(du, sums2[phase]);
       phase ^= 1;
-      const float c = q * q * (q * (du[0] / n));
-#pragma unroll
-      for (int k = 0; k < VPL; ++k) {
-        float o[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = POST ? q * u[k][j] - element<DT>(x[k], j) * c : u[k][j];
-        if (live && on[k]) store_row8(a.dinput + row * a.dinput_stride + off[k], pack8<DT>(o), skip[k]);
-      }
       if constexpr (!AHEAD) load(row + step, row + step < end);
     }
-    if constexpr (GATE == kSharedGate) {
+    if constexpr (SHARED) {
 #pragma unroll
       for (int k = 0; k < VPL; ++k) {
-        join(ag[k]);
-        if (a.parts > 1)
-          put(a.gate_sums + unit * a.hidden, k, ag[k]);
-        else if (sub == 0 && on[k])
-          store_row8(a.dgate + gate * a.dgate_stride + off[k], pack8<DT>(ag[k]), skip[k]);
+        float t[8];
+        acc.get(VPL + k, t);
+        acc.clear(VPL + k);
+        const u32x4 p = POST && on[k] ? load_row8(a.post_weight + off[k]) : zeros;
+        if constexpr (POST) {
+          const u32x4 g = on[k] ? load_row8(gate + off[k]) : zeros;
+          float share[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ag[k][j] = 0.0f;
+          for (int j = 0; j < 8; ++j) {
+            share[j] = t[j] * element<DT>(g, j);
+            t[j] *= element<DT>(p, j);
+          }
+          join(share);
+          // the workgroup's row of sums of dpost grows by each of its units
+          if (unit >= gridDim.x && sub == 0 && on[k]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (j >= skip[k]) share[j] += post_sums[off[k] + j];
+          }
+          put(post_sums, k, share);
+        }
+        join(t);
+        if (a.parts > 1)
+          put(a.gate_sums + unit * a.hidden, k, t);
+        else if (sub == 0 && on[k])
+          store_row8(a.dgate + at * a.dgate_stride + off[k], pack8<DT>(t), skip[k]);
       }
     }
   }
 #pragma unroll
   for (int k = 0; k < VPL; ++k) {
-    join(aw[k]);
-    put(a.weight_sums + (int64_t)blockIdx.x * a.hidden, k, aw[k]);
-    if constexpr (POST) {
-      join(ap[k]);
-      put(a.post_sums + (int64_t)blockIdx.x * a.hidden, k, ap[k]);
+    float t[8];
+    acc.get(k, t);
+    join(t);
+    put(a.weight_sums + (int64_t)blockIdx.x * a.hidden, k, t);
+    if constexpr (POST && !SHARED) {
+      acc.get(VPL + k, t);
+      join(t);
+      put(post_sums, k, t);
     }
   }
 }
@@ -396,19 +498,30 @@ __global__ __launch_bounds__(1024) void norm_add_grad_join_kernel(JoinArgs a, in
 constexpr int64_t kMaxHidden = int64_t(1) << 24;
 constexpr int64_t kVectorHidden = 16384;  // the register-resident kernels' widest rows
 
+// Shapes by width.  Up to 8192 elements a workgroup of 8 waves a CU, 2 vectors a
+// lane where the width has them, with the next rows' loads ahead and weights and
+// sums in registers.  Times on bf16 rows with dresidual and one gate for all (none
+// up to 512), both kernels, lanes x vectors x workgroup x workgroups per CU (33.5 M
+// elements, 403 MB): 128 16 x 1 x 512 x 2 83.1 us, 16 x 1 x 256 x 4 87.7; 256 32 x
+// 1 x 512 x 2 77.3, 64 x 1 96.3; 512 32 x 2 x 512 x 1 78.0, 64 x 1 82.2; 1024 64 x
+// 2 x 512 x 1 77.0, x 256 x 2 78.6, 128 x 2 87.6; 2048 128 x 2 x 512 x 1 78.0, x
+// 256 x 2 84.4, 256 x 2 90.0; 4096 256 x 2 x 512 x 1 81.6, 512 x 1 x 512 x 2 96.9,
+// 512 x 1 x 1024 x 1 94.6; 8192 512 x 2 x 512 x 1 90.2, 1024 x 1 105.  Without the
+// loads ahead 4096 takes 99.3, with weights unpacked for each row 108.  Past 8192
+// the registers hold neither the sums (they lie in LDS) nor a second row: 16384
+// 512 x 4 135.6 us, 1024 x 2 138.4, sums in registers 224 (120 to 180 spilled).
 struct Shape {
   int lpr, vpl, block, per_cu;
 };
 
 Shape shape_of(int64_t hidden) {
   const int64_t slots = (hidden + 7) / 8;
-  if (slots <= 16) return {16, 1, 256, 4};
-  if (slots <= 32) return {32, 1, 256, 4};
-  if (slots <= 64) return {64, 1, 256, 4};
-  if (slots <= 128) return {64, 2, 256, 2};
-  if (slots <= 256) return {128, 2, 256, 2};
-  if (slots <= 512) return {512, 1, 512, 2};
-  if (slots <= 768) return {256, 3, 512, 1};
+  if (slots <= 16) return {16, 1, 512, 2};
+  if (slots <= 32) return {32, 1, 512, 2};
+  if (slots <= 64) return {32, 2, 512, 1};
+  if (slots <= 128) return {64, 2, 512, 1};
+  if (slots <= 256) return {128, 2, 512, 1};
+  if (slots <= 512) return {256, 2, 512, 1};
   if (slots <= 1024) return {512, 2, 512, 1};
   return {512, 4, 512, 1};
 }
@@ -450,28 +563,23 @@ Plan plan_of(int64_t rows, int64_t hidden, int64_t gate_rows, bool post) {
   return p;
 }
 
-template <int DT, int LPR, int VPL, int BLOCK, int PER_SIMD, bool AHEAD, bool POST, int GATE>
-void launch(const NormAddGradArgs& a, int64_t grid, hipStream_t stream) {
-  norm_add_grad_kernel<DT, LPR, VPL, BLOCK, PER_SIMD, POST, GATE, AHEAD><<<dim3((unsigned)grid), dim3(BLOCK), 0,
-                                                                           stream>>>(a);
-}
-
-template <int DT, int LPR, int VPL, int BLOCK, int PER_SIMD, bool AHEAD, bool POST>
+template <int DT, int LPR, int VPL, int BLOCK, bool AHEAD, bool HOLD, bool LACC, bool POST>
 void launch_gate(const NormAddGradArgs& a, const Plan& p, hipStream_t stream) {
+  const dim3 grid((unsigned)p.grid), block(BLOCK);
   if (p.element)
-    launch<DT, LPR, VPL, BLOCK, PER_SIMD, AHEAD, POST, kElementGate>(a, p.grid, stream);
+    norm_add_grad_kernel<DT, LPR, VPL, BLOCK, POST, kElementGate, AHEAD, HOLD, LACC><<<grid, block, 0, stream>>>(a);
   else if (p.shared)
-    launch<DT, LPR, VPL, BLOCK, PER_SIMD, AHEAD, POST, kSharedGate>(a, p.grid, stream);
+    norm_add_grad_kernel<DT, LPR, VPL, BLOCK, POST, kSharedGate, AHEAD, HOLD, LACC><<<grid, block, 0, stream>>>(a);
   else
-    launch<DT, LPR, VPL, BLOCK, PER_SIMD, AHEAD, POST, kNoGate>(a, p.grid, stream);
+    norm_add_grad_kernel<DT, LPR, VPL, BLOCK, POST, kNoGate, AHEAD, HOLD, LACC><<<grid, block, 0, stream>>>(a);
 }
 
-template <int DT, int LPR, int VPL, int BLOCK, int PER_SIMD, bool AHEAD>
+template <int DT, int LPR, int VPL, int BLOCK, bool AHEAD, bool HOLD, bool LACC>
 void launch_rows(const NormAddGradArgs& a, const Plan& p, hipStream_t stream) {
   if (a.post_weight)
-    launch_gate<DT, LPR, VPL, BLOCK, PER_SIMD, AHEAD, true>(a, p, stream);
+    launch_gate<DT, LPR, VPL, BLOCK, AHEAD, HOLD, LACC, true>(a, p, stream);
   else
-    launch_gate<DT, LPR, VPL, BLOCK, PER_SIMD, AHEAD, false>(a, p, stream);
+    launch_gate<DT, LPR, VPL, BLOCK, AHEAD, HOLD, LACC, false>(a, p, stream);
 }
 
 template <int DT>
@@ -487,15 +595,14 @@ void launch_all(const NormAddGradArgs& a, const Plan& p, char* ws, hipStream_t s
   }
   const Shape s = shape_of(a.hidden);
   switch (s.lpr * 8 + s.vpl) {
-    case 16 * 8 + 1: launch_rows<DT, 16, 1, 256, 1, true>(a, p, stream); break;
-    case 32 * 8 + 1: launch_rows<DT, 32, 1, 256, 1, true>(a, p, stream); break;
-    case 64 * 8 + 1: launch_rows<DT, 64, 1, 256, 1, true>(a, p, stream); break;
-    case 64 * 8 + 2: launch_rows<DT, 64, 2, 256, 1, true>(a, p, stream); break;
-    case 128 * 8 + 2: launch_rows<DT, 128, 2, 256, 1, true>(a, p, stream); break;
-    case 512 * 8 + 1: launch_rows<DT, 512, 1, 512, 4, true>(a, p, stream); break;
-    case 256 * 8 + 3: launch_rows<DT, 256, 3, 512, 2, true>(a, p, stream); break;
-    case 512 * 8 + 2: launch_rows<DT, 512, 2, 512, 2, true>(a, p, stream); break;
-    default: launch_rows<DT, 512, 4, 512, 2, false>(a, p, stream); break;
+    case 16 * 8 + 1: launch_rows<DT, 16, 1, 512, true, true, false>(a, p, stream); break;
+    case 32 * 8 + 1: launch_rows<DT, 32, 1, 512, true, true, false>(a, p, stream); break;
+    case 32 * 8 + 2: launch_rows<DT, 32, 2, 512, true, true, false>(a, p, stream); break;
+    case 64 * 8 + 2: launch_rows<DT, 64, 2, 512, true, true, false>(a, p, stream); break;
+    case 128 * 8 + 2: launch_rows<DT, 128, 2, 512, true, true, false>(a, p, stream); break;
+    case 256 * 8 + 2: launch_rows<DT, 256, 2, 512, true, true, false>(a, p, stream); break;
+    case 512 * 8 + 2: launch_rows<DT, 512, 2, 512, true, true, false>(a, p, stream); break;
+    default: launch_rows<DT, 512, 4, 512, false, false, true>(a, p, stream); break;
   }
 }
 

@@ -4,7 +4,8 @@
 // A row of H elements is H / 8 whole vectors of 8; for H % 8 != 0 the slot after
 // the last whole vector holds the row's last 8 elements (H >= 8), of which only
 // those that no whole vector holds count and are stored.  The others are loaded
-// and dropped, so it does not matter if their owner has overwritten them.
+// and set to 0 (drop_first), so it does not matter if their owner has overwritten
+// them, and zeros change no sum and no maximum.
 #pragma once
 
 #include "hprms_device.h"
@@ -31,11 +32,26 @@ __device__ __forceinline__ void store_row8(uint16_t* p, u32x4 v, int skip) {
   if (skip == 0) {
     __builtin_nontemporal_store(v, (u32x4_any*)p);
   } else {
+    asm volatile("" : "+v"(skip));  // or a loop's lane masks of all 7 comparisons would be kept
 #pragma unroll
     for (int j = 1; j < 8; ++j)
       if (j >= skip) p[j] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
   }
 }
+
+// v with its first `skip` (0 ... 7) elements 0
+__device__ __forceinline__ void drop_first(u32x4& v, int skip) {
+  asm volatile("" : "+v"(skip));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (skip > 2 * i) v[i] &= 0xffff0000u;
+    if (skip > 2 * i + 1) v[i] = 0;
+  }
+}
+
+// v through an empty asm statement: what is unpacked from it again afterwards
+// need not stay in registers until then.
+__device__ __forceinline__ void packed_again(u32x4& v) { asm volatile("" : "+v"(v)); }
 
 template <int DT>
 __device__ __forceinline__ float element(const u32x4& v, int j) {
