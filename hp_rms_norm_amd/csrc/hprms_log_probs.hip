@@ -6,12 +6,12 @@
 //   top alternatives: the largest z, equal ones by the lower index, minus lse
 //   dz = dlog_prob * ([v == token] - p) - dentropy * p * (log p + entropy)
 //
-// Forward, first kernel: a wave takes a part of a row, kPartBytes of it, into
-// registers at once, 16 bytes a lane and step, and leaves the part's m, S and sum
-// of e^(z - m) (z - m) and its `top` largest as sorted keys.  Its loads are all on
-// their way before the first is used, waves need no barrier, and the logits are
-// read once.  Second kernel: a wave joins a row's parts.  The gradient is one pass
-// over the logits, from the forward call's lse and entropy.
+// Forward, first kernel: a workgroup takes a part of a row, up to kPartBytes of it,
+// into registers at once, 16 bytes a lane and step, and leaves the part's m, S and
+// sum of e^(z - m) (z - m) and its `top` largest as sorted keys: its loads are all
+// on their way before the first is used, and the logits are read once.  Second
+// kernel: a wave joins a row's parts; a row of one part needs none.  The gradient
+// is one pass over the logits, from the forward call's lse and entropy.
 #include <hip/hip_runtime.h>
 
 #include "hprms_host.h"
@@ -22,8 +22,10 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kSteps = 16;                 // 16-byte loads of a lane
-constexpr int kPartBytes = kSteps * 1024;  // a part: 8192 16-bit or 4096 32-bit logits
+constexpr int kSteps = 16;                 // 16-byte loads of a lane, at most
+constexpr int kStepBytes = 256 * 16;       // of a workgroup
+constexpr int kPartBytes = kSteps * kStepBytes;  // 32768 16-bit or 16384 32-bit logits
+constexpr int kMaxParts = 64;
 constexpr int kMaxTop = 64;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 // exponents of 2 below this give 0; bounds what 0 is multiplied with at -infinity
@@ -33,7 +35,6 @@ template <int DT>
 struct Logits {
   static constexpr int N = DT == HPRMS_DTYPE_FP32 ? 4 : 8;  // of a vector
   static constexpr int SIZE = DT == HPRMS_DTYPE_FP32 ? 4 : 2;
-  static constexpr int PART = kPartBytes / SIZE;
   static constexpr uint32_t MINUS_INF =
       DT == HPRMS_DTYPE_FP32 ? 0xff800000u : DT == HPRMS_DTYPE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
   __device__ static __forceinline__ float get(const u32x4& v, int j) {
@@ -92,39 +93,138 @@ struct LogProbArgs {
   int64_t row_bytes, ignore_index;
   int64_t row_from;                 // first row of the launch
   int32_t rows, parts, top, vocab;  // rows of the launch
+  int32_t steps;                    // of a part
 };
 
-template <int DT, bool TOP>
-__global__ __launch_bounds__(256, 4) void log_probs_part_kernel(LogProbArgs a) {
+// ---- the largest values --------------------------------------------------------------------
+// Both kernels find the `top` largest keys in two steps.  A bound first: each lane
+// has the largest of its own values, and a bound that `top` of a wave's lanes reach
+// is found bit by bit (ballots), so at least `top` values reach it and, of values
+// in no particular place, not many more (64 ln(64 / (64 - top)): 24 for 20; from
+// kLaneBound on it is sought among the largest of each vector).  Those that reach the largest of the four waves' bounds are listed in LDS, and each
+// one's place is the number of larger keys.  Where a wave's list would be longer
+// (equal values without end) or no bound above -infinity is reached, that wave's
+// keys are taken one by one instead, a maximum over its lanes each.
+constexpr int kListed = 512;
+constexpr int kLaneBound = 32;
+constexpr uint32_t kOrderMinusInf = 0x007fffffu;
+
+// The largest (or, once they are counted exactly, some) bound that at least `count`
+// of some values reach, reached(b) of them b; 0 if there are fewer.
+template <class Reached>
+__device__ __forceinline__ uint32_t bound_of(Reached&& reached, int count) {
+  uint32_t bound = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t b = bound | 1u << bit;
+    const int n = reached(b);
+    if (n >= count) bound = b;
+    if (n == count) break;
+  }
+  return bound;
+}
+
+// Appends the keys of `lanes` to a wave's list; *count goes on past its end.
+template <class Key>
+__device__ __forceinline__ void append(u64* list, int* count, u64 lanes, Key&& key) {
+  const int at = *count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32),
+                                                         __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u));
+  if ((lanes >> (threadIdx.x & 63) & 1) && at < kListed) list[at] = key();
+  *count += __popcll(lanes);
+}
+
+// The number of keys above `key` in a list.
+__device__ __forceinline__ int above(const u64* list, int count, u64 key) {
+  int n = 0;
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) n += list[i] > key;
+  return n;
+}
+
+// What a row's sums give.
+__device__ __forceinline__ void store_row(const LogProbArgs& a, int64_t row, int64_t token, int dtype, float m, float s,
+                                          float t) {
+  const bool none = m == -__builtin_inff();
+  const float log_s = logf(s), lse = none ? m : m + log_s;
+  float z = __builtin_nanf("");
+  if (token >= 0 && token < a.vocab) {
+    const char* p = a.logits + row * a.row_bytes;
+    z = dtype == HPRMS_DTYPE_FP32   ? ((const float*)p)[token]
+        : dtype == HPRMS_DTYPE_BF16 ? Fmt<HPRMS_DTYPE_BF16>::one(((const uint16_t*)p)[token])
+                                    : Fmt<HPRMS_DTYPE_FP16>::one(((const uint16_t*)p)[token]);
+  }
+  a.log_prob[row] = none ? z : z - lse;
+  a.entropy[row] = none ? 0.0f : log_s - t / s;
+  a.lse[row] = lse;
+}
+
+__device__ __forceinline__ void store_top(const LogProbArgs& a, int64_t row, int place, u64 key, float lse) {
+  const float v = value_of((uint32_t)(key >> 32));
+  a.top_log_prob[row * a.top + place] = lse == -__builtin_inff() ? v : v - lse;
+  a.top_index[row * a.top + place] = 0xffffffffu - (uint32_t)key;
+}
+
+// Parts' maxima and sums, as one.
+struct Sums {
+  float m, s, t;
+  __device__ __forceinline__ void add(float om, float os, float ot) {
+    if (om == -__builtin_inff()) return;  // nothing there
+    const float top = __builtin_elementwise_maximum(m, om);
+    const float d = m == -__builtin_inff() ? kLowest : __builtin_elementwise_maximum(m - top, kLowest);
+    const float od = __builtin_elementwise_maximum(om - top, kLowest), f = expf(d), of = expf(od);
+    t = f * (t + s * d) + of * (ot + os * od);
+    s = f * s + of * os;
+    m = top;
+  }
+};
+
+template <int DT, bool TOP, int STEPS>
+__global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(LogProbArgs a) {
   using L = Logits<DT>;
-  const int lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int32_t here = (int32_t)(at / a.parts), part = (int32_t)(at % a.parts);
-  if (here >= a.rows) return;
+  __shared__ u64 lists[TOP ? 4 : 1][TOP ? kListed : 1];
+  __shared__ f32x4 stats[4];
+  __shared__ uint32_t bounds[4];
+  __shared__ int counts[4];
+  __shared__ float row_lse;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t here = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int64_t row = a.row_from + here;
-  if (a.tokens[row] == a.ignore_index) return;
+  const int64_t token = a.tokens[row];
+  if (token == a.ignore_index) {
+    if (a.parts == 1) {
+      if (threadIdx.x == 0) a.log_prob[row] = a.entropy[row] = a.lse[row] = 0.0f;
+      if (TOP && threadIdx.x < a.top) {
+        a.top_log_prob[row * a.top + threadIdx.x] = 0.0f;
+        a.top_index[row * a.top + threadIdx.x] = -1;
+      }
+    }
+    return;
+  }
   const char* z = a.logits + row * a.row_bytes;
-  const int32_t first = part * L::PART + lane * L::N;
-  u32x4 v[kSteps];
+  const int32_t first = part * (a.steps * 256 * L::N) + threadIdx.x * L::N;
+  u32x4 v[STEPS];
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) v[i] = L::load(z, first + i * 64 * L::N, a.vocab);
-  float top[kSteps], m = -__builtin_inff();
+  for (int i = 0; i < STEPS; ++i)
+    if (i < a.steps) v[i] = L::load(z, first + i * 256 * L::N, a.vocab);
+  float top[STEPS], m = -__builtin_inff();
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
+  for (int i = 0; i < STEPS; ++i) {
+    if (i >= a.steps) continue;
     top[i] = L::get(v[i], 0);
 #pragma unroll
     for (int j = 1; j < L::N; ++j) top[i] = __builtin_elementwise_maximum(top[i], L::get(v[i], j));
     m = __builtin_elementwise_maximum(m, top[i]);
   }
+  const float lane_top = m;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, d));
   // unpacked again below: the compiler would keep the 128 values otherwise
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(v[i]));
+  for (int i = 0; i < STEPS; ++i) packed_again(v[i]);
   const float shift = m == -__builtin_inff() ? 0.0f : m;  // nothing but -infinity: every exponential is 0
   float s = 0.0f, t = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i)
+  for (int i = 0; i < STEPS; ++i) {
+    if (i >= a.steps) continue;
 #pragma unroll
     for (int j = 0; j < L::N; ++j) {
       const float x = __builtin_elementwise_maximum((L::get(v[i], j) - shift) * kLog2e, kLowest);
@@ -132,144 +232,208 @@ __global__ __launch_bounds__(256, 4) void log_probs_part_kernel(LogProbArgs a) {
       s += e;
       t += e * x;
     }
+  }
   s = group_sum<64>(s);
   t = group_sum<64>(t);
-  if (lane == 0) a.stats[(int64_t)here * a.parts + part] = f32x4{m, s, t * kLn2, 0.0f};
+  if (lane == 0) stats[wave] = f32x4{m, s, t * kLn2, 0.0f};
+  uint32_t bound = 0;
   if constexpr (TOP) {
+    const uint32_t lane_order = first < a.vocab ? order_of(lane_top) : 0u;
+    if (a.top <= kLaneBound) {
+      bound = bound_of([&](uint32_t b) { return __popcll(__ballot(lane_order >= b)); }, a.top);
+    } else {
+      uint32_t order[STEPS];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(v[i]));
-    uint32_t order[kSteps];     // of each vector's largest value that is left
-    uint32_t gone[kSteps / 4];  // what is taken, 8 bits a vector
+      for (int i = 0; i < STEPS; ++i)
+        order[i] = i < a.steps && first + i * 256 * L::N < a.vocab ? order_of(top[i]) : 0u;
+      bound = bound_of(
+          [&](uint32_t b) {
+            int n = 0;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) order[i] = first + i * 64 * L::N < a.vocab ? order_of(top[i]) : 0u;
+            for (int i = 0; i < STEPS; ++i) n += __popcll(__ballot(order[i] >= b));
+            return n;
+          },
+          a.top);
+    }
+    if (lane == 0) bounds[wave] = bound;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    Sums sums = {stats[0][0], stats[0][1], stats[0][2]};
+    for (int w = 1; w < 4; ++w) sums.add(stats[w][0], stats[w][1], stats[w][2]);
+    if (a.parts == 1) {
+      if (lane == 0) store_row(a, row, token, DT, sums.m, sums.s, sums.t);
+      if (TOP && lane == 0) row_lse = sums.m == -__builtin_inff() ? sums.m : sums.m + logf(sums.s);
+    } else if (lane == 0) {
+      a.stats[(int64_t)here * a.parts + part] = f32x4{sums.m, sums.s, sums.t, 0.0f};
+    }
+  }
+  if constexpr (TOP) {
+    u64* list = lists[wave];
+    int count = 0;
 #pragma unroll
-    for (int i = 0; i < kSteps / 4; ++i) gone[i] = 0;
-    u64* to = a.keys + ((int64_t)here * a.parts + part) * a.top;
-    for (int n = 0; n < a.top; ++n) {
-      uint32_t best = 0;
+    for (int w = 0; w < 4; ++w) bound = __builtin_elementwise_max(bound, bounds[w]);
+    const float least = value_of(bound);
+    // (below, what a bound at -infinity would let pass: elements past the row's end)
+    bool listed = bound > kOrderMinusInf && bound <= 0xff800000u;
+    if (listed) {
+      uint32_t hits = 0;  // the lane's steps with a value that reaches it
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) best = __builtin_elementwise_max(best, order[i]);
-      const uint32_t most = group_max_u32<64>(best);
-      if (most == 0) {  // fewer values than alternatives
-        if (lane == 0)
-          for (int i = n; i < a.top; ++i) to[i] = 0;
-        break;
-      }
-      // the first vector that holds it: step, then lane
-      int step = kSteps;
-#pragma unroll
-      for (int i = kSteps - 1; i >= 0; --i)
-        if (order[i] == most) step = i;
-      const uint32_t place = 0xffffffffu - group_max_u32<64>(0xffffffffu - (uint32_t)(step * 64 + lane));
-      const int s0 = (int)(place >> 6);
-      const bool mine = (int)(place & 63) == lane;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        if (i != s0) continue;  // the same for all lanes
-        const int32_t index = first + i * 64 * L::N;
-        // opaque: the orders of all 128 values would be kept over the loop otherwise
-        u32x4 w = v[i];
-        uint32_t taken = gone[i / 4] >> (8 * (i & 3));
-        int valid = a.vocab - index;
-        asm volatile("" : "+v"(w), "+v"(taken), "+v"(valid));
-        uint32_t left = 0;
-        int found = -1;
+      for (int i = 0; i < STEPS; ++i)
+        if (i < a.steps && !(top[i] < least)) hits |= 1u << i;
+      // their vectors again, from the caches: few, and the loop is short
+      while (__ballot(hits != 0) != 0) {
+        const int32_t index = first + (hits ? __builtin_ctz(hits) : 0) * 256 * L::N;
+        u32x4 w = {L::MINUS_INF, L::MINUS_INF, L::MINUS_INF, L::MINUS_INF};
+        if (hits) w = L::load(z, index, a.vocab);
+        hits &= hits - 1;
 #pragma unroll
         for (int j = 0; j < L::N; ++j) {
-          uint32_t o = order_of(L::get(w, j));
-          if (taken & (1u << j) || j >= valid) o = 0;
-          if (o == most && found < 0)
-            found = j;
-          else
-            left = __builtin_elementwise_max(left, o);
+          const float f = L::get(w, j);
+          const u64 lanes = __ballot(!(f < least));
+          if (lanes != 0) append(list, &count, lanes, [&] { return key_of(order_of(f), index + j); });
         }
-        if (mine) {
-          to[n] = key_of(most, index + found);
-          gone[i / 4] |= 1u << (8 * (i & 3) + found);
-          order[i] = left;
+        if (count > kListed) break;
+      }
+      listed = count <= kListed;
+    }
+    if (!listed) {
+      uint32_t order[STEPS];  // of each vector's largest value that is left
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i)
+        order[i] = i < a.steps && first + i * 256 * L::N < a.vocab ? order_of(top[i]) : 0u;
+      u64 last_key = 0;
+      int last_step = -1;
+      for (count = 0; count < a.top; ++count) {
+        uint32_t best = 0;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) best = __builtin_elementwise_max(best, order[i]);
+        const uint32_t most = group_max_u32<64>(best);
+        if (most == 0) break;  // nothing is left
+        // the first vector that holds it: step, then lane
+        int step = STEPS;
+#pragma unroll
+        for (int i = STEPS - 1; i >= 0; --i)
+          if (order[i] == most) step = i;
+        const uint32_t place = 0xffffffffu - group_max_u32<64>(0xffffffffu - (uint32_t)(step * 64 + lane));
+        step = (int)(place >> 6);
+        if ((int)(place & 63) == lane) {
+          const int32_t index = first + step * 256 * L::N;
+          const u32x4 w = L::load(z, index, a.vocab);
+          // Left of the vector is what is below the last key taken from it: nothing
+          // above `most`, and of values equal to it (taken one after the other, as a
+          // vector's elements are neighbours) none up to the last one.
+          const u64 end = step == last_step ? last_key - 1 : (u64)most << 32 | 0xffffffffu;
+          u64 found = 0, next = 0;
+#pragma unroll
+          for (int j = 0; j < L::N; ++j) {
+            const u64 key = index + j < a.vocab ? key_of(order_of(L::get(w, j)), index + j) : 0;
+            if (key > end) continue;
+            next = key > found ? found : key > next ? key : next;
+            found = key > found ? key : found;
+          }
+          list[count] = found;
+          last_key = found;
+          last_step = step;
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i)
+            if (i == step) order[i] = (uint32_t)(next >> 32);
         }
       }
     }
+    if (lane == 0) counts[wave] = count;
+    __syncthreads();
+    const float lse = row_lse;
+    u64* to = a.keys + ((int64_t)here * a.parts + part) * a.top;
+    for (int i = lane; i < count; i += 64) {
+      const u64 key = list[i];
+      int place = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) place += above(lists[w], counts[w], key);
+      if (place >= a.top) continue;
+      if (a.parts == 1)
+        store_top(a, row, place, key, lse);
+      else
+        to[place] = key;
+    }
+    // a part of fewer values than alternatives
+    const int all = counts[0] + counts[1] + counts[2] + counts[3];
+    if (a.parts > 1 && (int)threadIdx.x >= all && (int)threadIdx.x < a.top) to[threadIdx.x] = 0;
   }
 }
 
 // Joins the parts of a row, one wave each.
 __global__ __launch_bounds__(256) void log_probs_join_kernel(LogProbArgs a, int dtype) {
-  const int lane = threadIdx.x & 63;
-  const int32_t here = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ u64 lists[4][kListed];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t here = blockIdx.x * 4 + wave;
   if (here >= a.rows) return;
   const int64_t row = a.row_from + here;
   const int64_t token = a.tokens[row];
-  float* top_log_prob = a.top_log_prob + row * a.top;
-  int64_t* top_index = a.top_index + row * a.top;
   if (token == a.ignore_index) {
     if (lane == 0) a.log_prob[row] = a.entropy[row] = a.lse[row] = 0.0f;
     if (lane < a.top) {
-      top_log_prob[lane] = 0.0f;
-      top_index[lane] = -1;
+      a.top_log_prob[row * a.top + lane] = 0.0f;
+      a.top_index[row * a.top + lane] = -1;
     }
     return;
   }
-  const f32x4* stats = a.stats + (int64_t)here * a.parts;
-  float m = -__builtin_inff();
-  for (int i = lane; i < a.parts; i += 64) m = __builtin_elementwise_maximum(m, stats[i][0]);
+  // lane l has part l, and its list, in descending order
+  const bool mine = lane < a.parts;
+  const u64* keys = a.keys + ((int64_t)here * a.parts + (mine ? lane : 0)) * a.top;
+  constexpr int U = 4;  // loads on their way at once
+  u64 key[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) key[u] = mine && u < a.top ? keys[u] : 0;
+  const f32x4 p = mine ? a.stats[(int64_t)here * a.parts + lane] : f32x4{-__builtin_inff(), 0.0f, 0.0f, 0.0f};
+  float m = p[0];
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, d));
   float s = 0.0f, t = 0.0f;
-  for (int i = lane; i < a.parts; i += 64) {
-    const f32x4 p = stats[i];
-    if (p[0] == -__builtin_inff()) continue;  // nothing there
+  if (p[0] != -__builtin_inff()) {
     const float d = __builtin_elementwise_maximum(p[0] - m, kLowest), f = expf(d);
-    s += f * p[1];
-    t += f * (p[2] + p[1] * d);
+    s = f * p[1];
+    t = f * (p[2] + p[1] * d);
   }
   s = group_sum<64>(s);
   t = group_sum<64>(t);
-  const bool none = m == -__builtin_inff();
-  const float lse = none ? m : m + logf(s);
-  if (lane == 0) {
-    float z = __builtin_nanf("");
-    if (token >= 0 && token < a.vocab) {
-      const char* p = a.logits + row * a.row_bytes;
-      z = dtype == HPRMS_DTYPE_FP32   ? ((const float*)p)[token]
-          : dtype == HPRMS_DTYPE_BF16 ? Fmt<HPRMS_DTYPE_BF16>::one(((const uint16_t*)p)[token])
-                                      : Fmt<HPRMS_DTYPE_FP16>::one(((const uint16_t*)p)[token]);
-    }
-    a.log_prob[row] = none ? z : z - lse;
-    a.entropy[row] = none ? 0.0f : logf(s) - t / s;
-    a.lse[row] = lse;
-  }
+  if (lane == 0) store_row(a, row, token, dtype, m, s, t);
   if (a.top == 0) return;
-  // lane l has the lists of parts l, l + 64, ...: their first keys that are left
-  constexpr int LISTS = 4;
-  const u64* keys = a.keys + (int64_t)here * a.parts * a.top;
-  u64 head[LISTS];
-  int used[LISTS];
+  const float lse = m == -__builtin_inff() ? m : m + logf(s);
+  // a bound from the lists' r-th keys: r of them each in enough lists
+  const int r = (a.top + a.parts - 1) / a.parts, enough = (a.top + r - 1) / r;
+  uint32_t reach = mine ? (uint32_t)(keys[r - 1] >> 32) : 0u;
+  const uint32_t bound = bound_of([&](uint32_t b) { return __popcll(__ballot(reach >= b)); }, enough);
+  u64* list = lists[wave];
+  int count = 0;
+  bool more = mine;
+  for (int n = 0; n < a.top; n += U) {
 #pragma unroll
-  for (int i = 0; i < LISTS; ++i) {
-    used[i] = 0;
-    head[i] = lane + i * 64 < a.parts ? keys[(int64_t)(lane + i * 64) * a.top] : 0;
+    for (int u = 0; u < U; ++u) {
+      more = more && key[u] != 0 && (uint32_t)(key[u] >> 32) >= bound;
+      const u64 lanes = __ballot(more);
+      if (lanes != 0) append(list, &count, lanes, [&] { return key[u]; });
+    }
+    if (count > kListed || __ballot(more) == 0) break;
+#pragma unroll
+    for (int u = 0; u < U; ++u) key[u] = more && n + U + u < a.top ? keys[n + U + u] : 0;
   }
-  u64 mine = 0;  // lane n ends with alternative n
+  if (count <= kListed) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the lanes' writes, in order within the wave
+    for (int i = lane; i < count; i += 64) {
+      const int place = above(list, count, list[i]);
+      if (place < a.top) store_top(a, row, place, list[i], lse);
+    }
+    return;
+  }
+  u64 head = mine ? keys[0] : 0;
+  int used = 0;
   for (int n = 0; n < a.top; ++n) {
-    u64 best = 0;
-#pragma unroll
-    for (int i = 0; i < LISTS; ++i) best = head[i] > best ? head[i] : best;
-    const uint32_t hi = group_max_u32<64>((uint32_t)(best >> 32));
-    const uint32_t lo = group_max_u32<64>((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+    const uint32_t hi = group_max_u32<64>((uint32_t)(head >> 32));
+    const uint32_t lo = group_max_u32<64>((uint32_t)(head >> 32) == hi ? (uint32_t)head : 0u);
     const u64 most = (u64)hi << 32 | lo;
-    if (lane == n) mine = most;
-#pragma unroll
-    for (int i = 0; i < LISTS; ++i)
-      if (head[i] == most) {
-        ++used[i];
-        head[i] = used[i] < a.top ? keys[(int64_t)(lane + i * 64) * a.top + used[i]] : 0;
-      }
-  }
-  if (lane < a.top) {
-    const float v = value_of((uint32_t)(mine >> 32));
-    top_log_prob[lane] = none ? v : v - lse;
-    top_index[lane] = 0xffffffffu - (uint32_t)mine;
+    if (lane == 0) store_top(a, row, n, most, lse);
+    if (head == most) head = ++used < a.top ? keys[used] : 0;
   }
 }
 
@@ -348,20 +512,31 @@ constexpr int64_t kMaxPartials = int64_t(1) << 26;  // bytes of partial results:
 
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t size_of(int dtype) { return dtype == HPRMS_DTYPE_FP32 ? 4 : 2; }
-int64_t parts_of(int64_t vocab, int dtype) { return (vocab * size_of(dtype) + kPartBytes - 1) / kPartBytes; }
+
+// Parts of a row: as few as hold it, or, for few rows, so many that two workgroups
+// a CU have some, of 2 steps at least.  In batch-invariant mode always the fewest:
+// other parts sum a row's exponentials in another order, which shows in last bits.
+int64_t parts_of(int64_t rows, int64_t vocab, int dtype, bool invariant) {
+  const int64_t bytes = vocab * size_of(dtype);
+  const int64_t least = (bytes + kPartBytes - 1) / kPartBytes, most = (bytes + 2 * kStepBytes - 1) / (2 * kStepBytes);
+  int64_t parts = least;
+  if (!invariant && rows > 0) parts = (2 * (int64_t)current_cus() + rows - 1) / rows;
+  if (parts > most) parts = most;
+  if (parts > kMaxParts) parts = kMaxParts;
+  return parts < least ? least : parts;
+}
 
 struct Plan {
   int64_t parts, rows_at, keys, total;  // rows of a launch; bytes
 };
-Plan plan_of(int64_t rows, int64_t vocab, int64_t top, int dtype) {
+Plan plan_of(int64_t rows, int64_t vocab, int64_t top, int dtype, bool invariant) {
   Plan p;
-  p.parts = parts_of(vocab, dtype);
+  p.parts = parts_of(rows, vocab, dtype, invariant);
   const int64_t row = p.parts * (16 + 8 * top);
   p.rows_at = kMaxPartials / row;
-  if (p.rows_at < 1) p.rows_at = 1;
   if (p.rows_at > rows) p.rows_at = rows;
   p.keys = round_up(p.rows_at * p.parts * 16, 256);
-  p.total = p.keys + p.rows_at * p.parts * top * 8;
+  p.total = p.parts == 1 ? 0 : p.keys + p.rows_at * p.parts * top * 8;
   return p;
 }
 
@@ -380,17 +555,25 @@ int check_sizes(int64_t rows, int64_t vocab, int64_t top, int dtype) {
 
 bool aligned_to(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
+template <int DT, bool TOP>
+void launch_parts(const LogProbArgs& a, dim3 grid, dim3 block, hipStream_t stream) {
+  if (a.steps <= 4)
+    log_probs_part_kernel<DT, TOP, 4><<<grid, block, 0, stream>>>(a);
+  else
+    log_probs_part_kernel<DT, TOP, kSteps><<<grid, block, 0, stream>>>(a);
+}
+
 template <int DT>
 int run_forward(LogProbArgs a, const Plan& p, int64_t rows, hipStream_t stream) {
   for (int64_t from = 0; from < rows; from += p.rows_at) {
     a.row_from = from;
     a.rows = (int32_t)(rows - from < p.rows_at ? rows - from : p.rows_at);
-    const dim3 grid((unsigned)((a.rows * p.parts + 3) / 4)), block(256);
+    const dim3 grid((unsigned)(a.rows * p.parts)), block(256);
     if (a.top > 0)
-      log_probs_part_kernel<DT, true><<<grid, block, 0, stream>>>(a);
+      launch_parts<DT, true>(a, grid, block, stream);
     else
-      log_probs_part_kernel<DT, false><<<grid, block, 0, stream>>>(a);
-    log_probs_join_kernel<<<dim3((unsigned)((a.rows + 3) / 4)), block, 0, stream>>>(a, DT);
+      launch_parts<DT, false>(a, grid, block, stream);
+    if (p.parts > 1) log_probs_join_kernel<<<dim3((unsigned)((a.rows + 3) / 4)), block, 0, stream>>>(a, DT);
   }
   return check_launch("log probability kernel");
 }
@@ -417,7 +600,10 @@ extern "C" {
 
 int64_t hprms_token_log_probs_workspace(int64_t rows, int64_t vocab, int64_t top, int dtype) {
   const int rc = check_sizes(rows, vocab, top, dtype);
-  return rc != HPRMS_OK ? rc : rows == 0 ? 0 : plan_of(rows, vocab, top, dtype).total;
+  if (rc != HPRMS_OK || rows == 0) return rc;
+  // enough for either mode, which may change between the query and the call
+  const int64_t n = plan_of(rows, vocab, top, dtype, false).total, i = plan_of(rows, vocab, top, dtype, true).total;
+  return n > i ? n : i;
 }
 
 int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* top_log_prob, int64_t* top_index,
@@ -436,8 +622,8 @@ int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* to
   if (!aligned_to(log_prob, 4) || !aligned_to(entropy, 4) || !aligned_to(lse, 4) || !aligned_to(logits, size) ||
       !aligned_to(tokens, 8) || (top > 0 && (!aligned_to(top_log_prob, 4) || !aligned_to(top_index, 8))))
     return fail(HPRMS_E_INVALID, "tensors must be aligned to their elements");
-  const Plan p = plan_of(rows, vocab, top, dtype);
-  if (!workspace || workspace_size < p.total || !aligned_to(workspace, 16))
+  const Plan p = plan_of(rows, vocab, top, dtype, hprms_batch_invariant() != 0);
+  if (p.total > 0 && (!workspace || workspace_size < p.total || !aligned_to(workspace, 16)))
     return fail(HPRMS_E_INVALID, "the workspace must hold %lld bytes, 16-byte aligned (got %lld)", (long long)p.total,
                 (long long)workspace_size);
   LogProbArgs a = {};
@@ -454,6 +640,7 @@ int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* to
   a.vocab = (int32_t)vocab;
   a.ignore_index = ignore_index;
   a.parts = (int32_t)p.parts;
+  a.steps = (int32_t)((vocab * size + p.parts * kStepBytes - 1) / (p.parts * kStepBytes));
   a.top = (int32_t)top;
   return dtype == HPRMS_DTYPE_FP32   ? run_forward<HPRMS_DTYPE_FP32>(a, p, rows, stream)
          : dtype == HPRMS_DTYPE_BF16 ? run_forward<HPRMS_DTYPE_BF16>(a, p, rows, stream)

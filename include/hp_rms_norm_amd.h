@@ -548,9 +548,10 @@ int hprms_int8_linear(void* out, const void* input, const float* scale, const vo
  * -infinity has probability 0; a row of nothing else gives lse = log_prob =
  * top_log_prob = -infinity and entropy 0.  NaN or +infinity makes a row's lse
  * NaN; NaN ranks above every number.  Workspace: as for
- * hprms_rmsnorm_backward(), of hprms_token_log_probs_workspace() bytes.  rows
- * == 0 is a no-op; vocab goes up to 2^20.  A row's bits do not depend on the
- * other rows.  No counterpart in the reference.
+ * hprms_rmsnorm_backward(), of hprms_token_log_probs_workspace() bytes, enough in
+ * either batch-invariant mode.  rows == 0 is a no-op; vocab goes up to 2^20.  Few
+ * rows are cut into more parts (other last bits) unless that mode is on.  No
+ * counterpart in the reference.
  */
 int64_t hprms_token_log_probs_workspace(int64_t rows, int64_t vocab, int64_t top, int dtype);
 int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* top_log_prob, int64_t* top_index,

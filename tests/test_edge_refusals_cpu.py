@@ -228,7 +228,7 @@ def test_workspace_sizes():
     assert i(0, 64, 64) == 0 and i(5, 64, 64) == 0 and i(5, 63, 64, input_stride=64, weight_stride=64) >= 69 * 64
     assert i(5, 64, 64, weight_ptr=8) >= 64 * 64 and i(5, 64, 64, input_stride=72) >= 5 * 64
     p = abi.token_log_probs_workspace
-    assert p(0, 100, 5, 0) == 0 and p(1, 100, 0, 0) >= 16 and p(1 << 30, 131072, 64, 2) <= (1 << 26) + 4096
+    assert p(0, 100, 5, 0) == 0 and p(1, 200000, 0, 0) >= 16 and p(1 << 30, 131072, 64, 2) <= (1 << 26) + 4096
     for call in (lambda: n(-1, 64, 0), lambda: n(1, 0, 0), lambda: n(1, (1 << 24) + 1, 0), lambda: n(6, 64, 4),
                  lambda: n(6, 64, -1), lambda: n(1 << 31, 64, 0), lambda: i(-1, 64, 64), lambda: i(1, 0, 64),
                  lambda: i(1, 64, 0), lambda: i(1, 131072, 64), lambda: i((1 << 24) + 1, 64, 64),
@@ -336,8 +336,9 @@ def log_probs_abi(**kw):
     (dict(vocab=4, stride=4), "top"), (dict(stride=99), "strides"), (dict(lp=0), "null"), (dict(h=0), "null"),
     (dict(lse=0), "null"), (dict(tl=0), "null"), (dict(ti=0), "null"), (dict(logits=0), "null"),
     (dict(tokens=0), "null"), (dict(dtype=2, logits=0x6002), "aligned"), (dict(tokens=0x7004), "aligned"),
-    (dict(ti=0x5004), "aligned"), (dict(ws=0), "workspace"), (dict(ws=0x10008), "workspace"),
-    (dict(ws_size=100), "workspace"),
+    (dict(ti=0x5004), "aligned"), (dict(ws=0, vocab=200000, stride=200000), "workspace"),
+    (dict(ws=0x10008, vocab=200000, stride=200000), "workspace"),
+    (dict(ws_size=100, vocab=200000, stride=200000), "workspace"),
 ])
 def test_log_probs_abi_refuses(kw, msg):
     assert log_probs_abi(**kw) == abi.HPRMS_E_INVALID

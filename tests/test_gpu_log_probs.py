@@ -260,6 +260,48 @@ def test_more_rows_than_one_launch_takes(ops):
         assert torch.equal(a, b[at])
 
 
+@pytest.mark.parametrize("vocab,dtype", [(300, torch.bfloat16), (20000, torch.float32), (131072, torch.float16),
+                                         (300001, torch.bfloat16)])
+def test_batch_invariant_mode(ops, vocab, dtype):
+    """In the mode a row's bits depend on no other row; out of it the results are
+    right with any number of rows, few of which are cut into more parts."""
+    z, t = make(600, vocab, dtype, 8, 0.0, 0.1)
+    previous = ops.set_batch_invariant(True)
+    try:
+        whole = ops.token_log_probs(z, t, top=7)
+        for at in (slice(0, 1), slice(5, 12), slice(100, 300), slice(599, 600)):
+            for a, b in zip(ops.token_log_probs(z[at], t[at], top=7), whole):
+                assert torch.equal(a, b[at])
+    finally:
+        ops.set_batch_invariant(previous)
+    for rows in (1, 2, 9, 40, 150):
+        check(ops.token_log_probs(z[:rows], t[:rows], top=7), z[:rows], t[:rows], 7)
+
+
+def test_values_in_particular_places(ops):
+    """Rows whose largest values stand close together, in one lane's vectors, or
+    reach the bound in numbers: in each the list or the way without it serves."""
+    for dtype in DTYPES:
+        n = 4 if dtype == torch.float32 else 8  # of a vector
+        z, t = make(12, 33000, dtype, 15, spread=0.5)
+        z[0, -200:] += 9.0                     # at the end
+        z[1, :200] += 9.0                      # at the beginning
+        z[2, 1000:1000 + 256 * n * 8:256 * n] += 9.0  # one lane's vectors
+        z[3, 512 * n:513 * n] += 9.0           # one vector
+        z[4] = z[4].round()                    # thousands of equal values
+        z[5, ::3] = 4.0                        # a third of the row
+        z[6] = -INF
+        z[6, 30000:30040] = 1.5                # fewer allowed than alternatives
+        z[7] = -INF
+        z[7, ::700] = torch.arange(48, device=DEV).to(dtype)
+        z[8, :600] = 9.0                       # more equal values than a list holds
+        z[9] = z[9].abs()
+        t[6], t[7] = 30001, 700
+        for top in (1, 20, 47, 64):
+            check(ops.token_log_probs(z, t, top=top), z, t, top)
+            check(ops.token_log_probs(z[4:9], t[4:9], top=top), z[4:9], t[4:9], top)
+
+
 def test_leading_dimensions_and_no_rows(ops):
     z, t = make(12, 300, torch.float16, 6)
     want = ops.token_log_probs(z, t, top=2)
