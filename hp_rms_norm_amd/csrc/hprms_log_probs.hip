@@ -49,21 +49,60 @@ struct Logits {
     else
       return Fmt<DT>::one(*(const uint16_t*)p);
   }
-  // the vector at element i of a row, -infinity past the row's end
-  __device__ static __forceinline__ u32x4 load(const char* row, int32_t i, int32_t vocab) {
-    if (i + N <= vocab) return __builtin_nontemporal_load((const u32x4_any*)(row + i * SIZE));
-    u32x4 v = {MINUS_INF, MINUS_INF, MINUS_INF, MINUS_INF};
+  // Rows are cut into vectors at 16-byte boundaries: the first begins this many
+  // elements before the row (4096 rows of 50001 16-bit logits: 79 us, 90 with vectors
+  // from the row's own beginning; at 128-byte boundaries 77, but 2000 of a row 15.5
+  // against 12.8).
+  __device__ static __forceinline__ int32_t before(const char* row) {
+    return (int32_t)((uintptr_t)row & 15) / SIZE;
+  }
+  // STEPS vectors `step` elements apart from element `first` (> -N) of a row on,
+  // -infinity before its beginning and past its end.  First all loads of whole
+  // vectors; what a row's ends cut is few lanes' business, and in the same loop its
+  // shifts would keep every lane waiting (4096 x 50048: 104 us against 70).
+  template <int STEPS>
+  __device__ static __forceinline__ void load(const char* row, int32_t first, int32_t step, int32_t steps,
+                                              int32_t vocab, u32x4 (&v)[STEPS]) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      if (i >= steps) continue;
+      const int32_t at = first + i * step;
+      v[i] = u32x4{MINUS_INF, MINUS_INF, MINUS_INF, MINUS_INF};
+      if (at >= 0 && at + N <= vocab) v[i] = __builtin_nontemporal_load((const u32x4_any*)(row + (int64_t)at * SIZE));
+    }
+    if (first < 0) v[0] = cut(row, first, vocab);
+    const int32_t left = vocab - first;
+    int32_t last = left / step;  // the vector that the row's end may cut
+    if (left > 0 && left - last * step > 0 && left - last * step < N && last < steps) {
+      const u32x4 t = cut(row, first + last * step, vocab);
+      asm volatile("" : "+v"(last));  // or the lane masks of all comparisons would be kept
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = i == last ? t[j] : v[i][j];
+    }
+  }
+  // One vector of which only some elements exist.  All its loads travel together (in
+  // branches they came one after the other, and every workgroup has such a vector).
+  __device__ static __forceinline__ u32x4 cut(const char* row, int32_t at, int32_t vocab) {
+    uint32_t e[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int32_t in = at + j < 0 ? 0 : at + j < vocab ? at + j : vocab - 1;
+      const char* p = row + (int64_t)in * SIZE;
+      e[j] = SIZE == 4 ? *(const uint32_t*)p : (uint32_t) * (const uint16_t*)p;
+    }
+    u32x4 v;
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      if (i + j < vocab) {
-        if constexpr (DT == HPRMS_DTYPE_FP32)
-          v[j] = *(const uint32_t*)(row + (i + j) * 4);
-        else if (j & 1)
-          v[j / 2] = (v[j / 2] & 0xffffu) | (uint32_t) * (const uint16_t*)(row + (i + j) * 2) << 16;
-        else
-          v[j / 2] = (v[j / 2] & 0xffff0000u) | *(const uint16_t*)(row + (i + j) * 2);
-      }
+      if (at + j < 0 || at + j >= vocab) e[j] = SIZE == 4 ? MINUS_INF : MINUS_INF & 0xffffu;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = SIZE == 4 ? e[j] : e[2 * j % N] | e[(2 * j + 1) % N] << 16;
     return v;
+  }
+  __device__ static __forceinline__ u32x4 load_one(const char* row, int32_t at, int32_t vocab) {
+    if (at >= 0 && at + N <= vocab) return *(const u32x4_any*)(row + (int64_t)at * SIZE);
+    return cut(row, at, vocab);
   }
 };
 
@@ -94,6 +133,7 @@ struct LogProbArgs {
   int64_t row_from;                 // first row of the launch
   int32_t rows, parts, top, vocab;  // rows of the launch
   int32_t steps;                    // of a part
+  bool cut;                         // into vectors at 16-byte boundaries
 };
 
 // ---- the largest values --------------------------------------------------------------------
@@ -137,6 +177,23 @@ __device__ __forceinline__ int above(const u64* list, int count, u64 key) {
   int n = 0;
 #pragma unroll 8
   for (int i = 0; i < count; ++i) n += list[i] > key;
+  return n;
+}
+
+// ... among the first `count` lanes' keys, the others' being 0: through the scalar
+// registers, 8 at a time (one by one, 50 keys take 2 us: each waits for the last).
+__device__ __forceinline__ int above_in_lanes(int count, u64 key) {
+  const int lo = (int)(uint32_t)key, hi = (int)(uint32_t)(key >> 32);
+  int n = 0;
+  for (int i = 0; i < count; i += 8) {
+    u64 other[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      other[j] = (u64)(uint32_t)__builtin_amdgcn_readlane(hi, i + j) << 32 |
+                 (uint32_t)__builtin_amdgcn_readlane(lo, i + j);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) n += other[j] > key;
+  }
   return n;
 }
 
@@ -200,11 +257,9 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
     return;
   }
   const char* z = a.logits + row * a.row_bytes;
-  const int32_t first = part * (a.steps * 256 * L::N) + threadIdx.x * L::N;
+  const int32_t first = part * (a.steps * 256 * L::N) + threadIdx.x * L::N - (a.cut ? L::before(z) : 0);
   u32x4 v[STEPS];
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i)
-    if (i < a.steps) v[i] = L::load(z, first + i * 256 * L::N, a.vocab);
+  L::template load<STEPS>(z, first, 256 * L::N, a.steps, a.vocab, v);
   float top[STEPS], m = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
@@ -237,6 +292,8 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
   t = group_sum<64>(t);
   if (lane == 0) stats[wave] = f32x4{m, s, t * kLn2, 0.0f};
   uint32_t bound = 0;
+  // whether a vector holds an element of the row
+  auto has = [&](int32_t at) { return at < a.vocab; };
   if constexpr (TOP) {
     const uint32_t lane_order = first < a.vocab ? order_of(lane_top) : 0u;
     if (a.top <= kLaneBound) {
@@ -245,7 +302,7 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
       uint32_t order[STEPS];
 #pragma unroll
       for (int i = 0; i < STEPS; ++i)
-        order[i] = i < a.steps && first + i * 256 * L::N < a.vocab ? order_of(top[i]) : 0u;
+        order[i] = i < a.steps && has(first + i * 256 * L::N) ? order_of(top[i]) : 0u;
       bound = bound_of(
           [&](uint32_t b) {
             int n = 0;
@@ -281,11 +338,17 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
 #pragma unroll
       for (int i = 0; i < STEPS; ++i)
         if (i < a.steps && !(top[i] < least)) hits |= 1u << i;
-      // their vectors again, from the caches: few, and the loop is short
+      // Each lane's first such vector, picked from its registers by selects: 80
+      // instructions, where a load of it again waits (32 rows x 131072, top 20: 17.8 us
+      // for both kernels, 17.0 so).
       while (__ballot(hits != 0) != 0) {
-        const int32_t index = first + (hits ? __builtin_ctz(hits) : 0) * 256 * L::N;
+        const int step = hits ? __builtin_ctz(hits) : STEPS;
+        const int32_t index = first + step * 256 * L::N;
         u32x4 w = {L::MINUS_INF, L::MINUS_INF, L::MINUS_INF, L::MINUS_INF};
-        if (hits) w = L::load(z, index, a.vocab);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = i == step ? v[i][j] : w[j];
         hits &= hits - 1;
 #pragma unroll
         for (int j = 0; j < L::N; ++j) {
@@ -301,7 +364,7 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
       uint32_t order[STEPS];  // of each vector's largest value that is left
 #pragma unroll
       for (int i = 0; i < STEPS; ++i)
-        order[i] = i < a.steps && first + i * 256 * L::N < a.vocab ? order_of(top[i]) : 0u;
+        order[i] = i < a.steps && has(first + i * 256 * L::N) ? order_of(top[i]) : 0u;
       u64 last_key = 0;
       int last_step = -1;
       for (count = 0; count < a.top; ++count) {
@@ -319,7 +382,7 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
         step = (int)(place >> 6);
         if ((int)(place & 63) == lane) {
           const int32_t index = first + step * 256 * L::N;
-          const u32x4 w = L::load(z, index, a.vocab);
+          const u32x4 w = L::load_one(z, index, a.vocab);
           // Left of the vector is what is below the last key taken from it: nothing
           // above `most`, and of values equal to it (taken one after the other, as a
           // vector's elements are neighbours) none up to the last one.
@@ -327,7 +390,8 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
           u64 found = 0, next = 0;
 #pragma unroll
           for (int j = 0; j < L::N; ++j) {
-            const u64 key = index + j < a.vocab ? key_of(order_of(L::get(w, j)), index + j) : 0;
+            const bool in = index + j >= 0 && index + j < a.vocab;
+            const u64 key = in ? key_of(order_of(L::get(w, j)), index + j) : 0;
             if (key > end) continue;
             next = key > found ? found : key > next ? key : next;
             found = key > found ? key : found;
@@ -345,19 +409,32 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
     __syncthreads();
     const float lse = row_lse;
     u64* to = a.keys + ((int64_t)here * a.parts + part) * a.top;
-    for (int i = lane; i < count; i += 64) {
-      const u64 key = list[i];
-      int place = 0;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) place += above(lists[w], counts[w], key);
-      if (place >= a.top) continue;
+    auto store = [&](int place, u64 key) {
+      if (place >= a.top) return;
       if (a.parts == 1)
         store_top(a, row, place, key, lse);
       else
         to[place] = key;
+    };
+    const int c0 = counts[0], c1 = c0 + counts[1], c2 = c1 + counts[2], all = c2 + counts[3];
+    if (all <= 64) {
+      if (wave == 0) {
+        const int w = lane < c0 ? 0 : lane < c1 ? 1 : lane < c2 ? 2 : 3;
+        const int at = lane - (w == 0 ? 0 : w == 1 ? c0 : w == 2 ? c1 : c2);
+        const u64 key = lane < all ? lists[w][at] : 0;
+        const int place = above_in_lanes(all, key);
+        if (lane < all) store(place, key);
+      }
+    } else {
+      for (int i = lane; i < count; i += 64) {
+        const u64 key = list[i];
+        int place = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) place += above(lists[w], counts[w], key);
+        store(place, key);
+      }
     }
     // a part of fewer values than alternatives
-    const int all = counts[0] + counts[1] + counts[2] + counts[3];
     if (a.parts > 1 && (int)threadIdx.x >= all && (int)threadIdx.x < a.top) to[threadIdx.x] = 0;
   }
 }
@@ -420,6 +497,12 @@ __global__ __launch_bounds__(256) void log_probs_join_kernel(LogProbArgs a, int 
   }
   if (count <= kListed) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the lanes' writes, in order within the wave
+    if (count <= 64) {
+      const u64 one = lane < count ? list[lane] : 0;
+      const int place = above_in_lanes(count, one);
+      if (lane < count && place < a.top) store_top(a, row, place, one, lse);
+      return;
+    }
     for (int i = lane; i < count; i += 64) {
       const int place = above(list, count, list[i]);
       if (place < a.top) store_top(a, row, place, list[i], lse);
@@ -454,9 +537,10 @@ template <int DT>
 __global__ __launch_bounds__(256) void log_probs_grad_kernel(LogProbGradArgs a) {
   using L = Logits<DT>;
   const int64_t row = a.row_from + blockIdx.x / a.parts;
-  const int32_t first = (int32_t)(blockIdx.x % a.parts) * (256 * kGradSteps * L::N) + threadIdx.x * L::N;
   const char* z = a.logits + row * a.logits_bytes;
   char* to = a.dlogits + row * a.dlogits_bytes;
+  const int32_t first =
+      (int32_t)(blockIdx.x % a.parts) * (256 * kGradSteps * L::N) + threadIdx.x * L::N - L::before(to);
   const int64_t token = a.tokens[row];
   const bool ignored = token == a.ignore_index;
   const float lse = a.lse[row];
@@ -465,10 +549,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(LogProbGradArgs a) 
   const float gh = a.dentropy ? a.dentropy[row] : 0.0f, entropy = a.dentropy ? a.entropy[row] : 0.0f;
   const float by = -g - gh * entropy, per = -gh * kLn2;  // dz = p * (by + per * log2 p) + [v == token] g
   u32x4 v[kGradSteps];
-  if (!ignored) {
-#pragma unroll
-    for (int i = 0; i < kGradSteps; ++i) v[i] = L::load(z, first + i * 256 * L::N, a.vocab);
-  }
+  if (!ignored) L::template load<kGradSteps>(z, first, 256 * L::N, kGradSteps, a.vocab, v);
 #pragma unroll
   for (int i = 0; i < kGradSteps; ++i) {
     const int32_t index = first + i * 256 * L::N;
@@ -490,12 +571,12 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(LogProbGradArgs a) 
     } else {
       o = pack8<DT>(d);
     }
-    if (index + L::N <= a.vocab) {
+    if (index >= 0 && index + L::N <= a.vocab) {
       __builtin_nontemporal_store(o, (u32x4_any*)(to + index * L::SIZE));
     } else {
 #pragma unroll
       for (int j = 0; j < L::N; ++j)
-        if (index + j < a.vocab) {
+        if (index + j >= 0 && index + j < a.vocab) {
           if constexpr (DT == HPRMS_DTYPE_FP32)
             *(uint32_t*)(to + (index + j) * 4) = o[j];
           else
@@ -513,11 +594,15 @@ constexpr int64_t kMaxPartials = int64_t(1) << 26;  // bytes of partial results:
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t size_of(int dtype) { return dtype == HPRMS_DTYPE_FP32 ? 4 : 2; }
 
+// A row's bytes, with what its first vector may hold before it.
+int64_t row_bytes_of(int64_t vocab, int dtype, bool cut) {
+  return vocab * size_of(dtype) + (cut ? 16 - size_of(dtype) : 0);
+}
+
 // Parts of a row: as few as hold it, or, for few rows, so many that two workgroups
 // a CU have some, of 2 steps at least.  In batch-invariant mode always the fewest:
 // other parts sum a row's exponentials in another order, which shows in last bits.
-int64_t parts_of(int64_t rows, int64_t vocab, int dtype, bool invariant) {
-  const int64_t bytes = vocab * size_of(dtype);
+int64_t parts_of(int64_t rows, int64_t bytes, bool invariant) {
   const int64_t least = (bytes + kPartBytes - 1) / kPartBytes, most = (bytes + 2 * kStepBytes - 1) / (2 * kStepBytes);
   int64_t parts = least;
   if (!invariant && rows > 0) parts = (2 * (int64_t)current_cus() + rows - 1) / rows;
@@ -527,11 +612,17 @@ int64_t parts_of(int64_t rows, int64_t vocab, int dtype, bool invariant) {
 }
 
 struct Plan {
-  int64_t parts, rows_at, keys, total;  // rows of a launch; bytes
+  int64_t parts, steps, rows_at, keys, total;  // rows of a launch; bytes
+  bool cut;
 };
-Plan plan_of(int64_t rows, int64_t vocab, int64_t top, int dtype, bool invariant) {
+// `aligned`: every row begins at a 16-byte boundary
+Plan plan_of(int64_t rows, int64_t vocab, int64_t top, int dtype, bool invariant, bool aligned) {
   Plan p;
-  p.parts = parts_of(rows, vocab, dtype, invariant);
+  // (the largest vocabularies fill the most parts there can be)
+  p.cut = !aligned && row_bytes_of(vocab, dtype, true) <= kMaxParts * kPartBytes;
+  const int64_t bytes = row_bytes_of(vocab, dtype, p.cut);
+  p.parts = parts_of(rows, bytes, invariant);
+  p.steps = (bytes + p.parts * kStepBytes - 1) / (p.parts * kStepBytes);
   const int64_t row = p.parts * (16 + 8 * top);
   p.rows_at = kMaxPartials / row;
   if (p.rows_at > rows) p.rows_at = rows;
@@ -581,7 +672,7 @@ int run_forward(LogProbArgs a, const Plan& p, int64_t rows, hipStream_t stream) 
 template <int DT>
 int run_backward(LogProbGradArgs a, int64_t rows, hipStream_t stream) {
   const int64_t span = 256 * kGradSteps * Logits<DT>::N;
-  a.parts = (int32_t)((a.vocab + span - 1) / span);
+  a.parts = (int32_t)((a.vocab + Logits<DT>::N - 1 + span - 1) / span);
   const int64_t rows_at = (int64_t(1) << 23) / a.parts;  // a launch holds fewer than 2^32 work-items
   for (int64_t from = 0; from < rows; from += rows_at) {
     a.row_from = from;
@@ -601,9 +692,13 @@ extern "C" {
 int64_t hprms_token_log_probs_workspace(int64_t rows, int64_t vocab, int64_t top, int dtype) {
   const int rc = check_sizes(rows, vocab, top, dtype);
   if (rc != HPRMS_OK || rows == 0) return rc;
-  // enough for either mode, which may change between the query and the call
-  const int64_t n = plan_of(rows, vocab, top, dtype, false).total, i = plan_of(rows, vocab, top, dtype, true).total;
-  return n > i ? n : i;
+  // enough for either mode, which may change between the query and the call, and wherever the rows begin
+  int64_t most = 0;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = plan_of(rows, vocab, top, dtype, i & 1, i & 2).total;
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* top_log_prob, int64_t* top_index,
@@ -622,7 +717,8 @@ int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* to
   if (!aligned_to(log_prob, 4) || !aligned_to(entropy, 4) || !aligned_to(lse, 4) || !aligned_to(logits, size) ||
       !aligned_to(tokens, 8) || (top > 0 && (!aligned_to(top_log_prob, 4) || !aligned_to(top_index, 8))))
     return fail(HPRMS_E_INVALID, "tensors must be aligned to their elements");
-  const Plan p = plan_of(rows, vocab, top, dtype, hprms_batch_invariant() != 0);
+  const Plan p = plan_of(rows, vocab, top, dtype, hprms_batch_invariant() != 0,
+                         aligned_to(logits, 16) && (rows == 1 || logits_row_stride * size % 16 == 0));
   if (p.total > 0 && (!workspace || workspace_size < p.total || !aligned_to(workspace, 16)))
     return fail(HPRMS_E_INVALID, "the workspace must hold %lld bytes, 16-byte aligned (got %lld)", (long long)p.total,
                 (long long)workspace_size);
@@ -640,7 +736,8 @@ int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* to
   a.vocab = (int32_t)vocab;
   a.ignore_index = ignore_index;
   a.parts = (int32_t)p.parts;
-  a.steps = (int32_t)((vocab * size + p.parts * kStepBytes - 1) / (p.parts * kStepBytes));
+  a.steps = (int32_t)p.steps;
+  a.cut = p.cut;
   a.top = (int32_t)top;
   return dtype == HPRMS_DTYPE_FP32   ? run_forward<HPRMS_DTYPE_FP32>(a, p, rows, stream)
          : dtype == HPRMS_DTYPE_BF16 ? run_forward<HPRMS_DTYPE_BF16>(a, p, rows, stream)
