@@ -8,9 +8,11 @@
 // result; a sum is rounded to binary32 once (24 bits of it, a relative error of
 // 2^-24 beside the output's own 2^-9 or 2^-12), then scaled.
 //
-// Few rows: the weight's bytes bound the call.  Up to 8 rows run on dot products of
-// 4 bytes, a wave reading whole KB of a weight's row, so the weight streams in whole
-// lines.  More rows run on the matrix cores (hprms_product.h), tiles by sizes.
+// Few rows: the weight's bytes bound the call.  One and two rows run on dot products
+// of 4 bytes, a wave reading whole KB of a weight's row, so the weight streams in
+// whole lines (1 x 4096 x 14336: 10.6 us, 5.5 TB/s; on the matrix cores 14.4).  More
+// rows run on the matrix cores (hprms_product.h), in tiles by a model of their
+// times, and long sums of few tiles in shares.
 #include <hip/hip_runtime.h>
 
 #include "hprms_host.h"
@@ -30,6 +32,9 @@ struct Int8Args {
   int64_t input_stride, weight_stride;  // bytes, multiples of 16
   int32_t rows, inner, outer;           // inner: a multiple of 16
   int32_t outer_tiles, row_tiles;
+  // a sum in several workgroups' shares, or null: [splits, rows, sum_stride]
+  int32_t* sums;
+  int32_t splits, span, sum_stride;  // span: of the summed index, a multiple of 128
 };
 
 __device__ __forceinline__ float scaled(int32_t sum, float scale, float weight_scale, float bias) {
@@ -46,7 +51,7 @@ __device__ __forceinline__ int32_t wave_sum(int32_t v) {
   return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 32);
 }
 
-// A workgroup takes W rows of the weight and all N rows of the input; its 4 waves
+// A workgroup takes W rows of the weight and the N rows of the input; its 4 waves
 // take KB of the summed index in turn.
 template <int DT, int N, int W>
 __global__ __launch_bounds__(256) void int8_few_rows_kernel(Int8Args a) {
@@ -67,9 +72,8 @@ __global__ __launch_bounds__(256) void int8_few_rows_kernel(Int8Args a) {
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int32_t t = n < a.rows ? n : a.rows - 1;
       x[u][n] = u32x4{0, 0, 0, 0};
-      if (in) x[u][n] = *(const u32x4*)(a.input + t * a.input_stride + k);
+      if (in) x[u][n] = *(const u32x4*)(a.input + n * a.input_stride + k);
     }
   };
   int32_t acc[N][W];
@@ -103,7 +107,7 @@ __global__ __launch_bounds__(256) void int8_few_rows_kernel(Int8Args a) {
   __syncthreads();
   if (threadIdx.x >= N * W) return;
   const int32_t t = threadIdx.x / W, o = first + threadIdx.x % W;
-  if (t >= a.rows || o >= a.outer) return;
+  if (o >= a.outer) return;
   const int32_t s = lds[0][threadIdx.x] + lds[1][threadIdx.x] + lds[2][threadIdx.x] + lds[3][threadIdx.x];
   const float bias = a.bias ? F::one(a.bias[o]) : 0.0f;
   a.out[t * a.out_stride + o] = F::pack1(scaled(s, a.scale[t], a.weight_scale[o], bias));
@@ -118,19 +122,35 @@ template <class P, int DT>
 __global__ __launch_bounds__(P::NW * 64) void int8_tile_kernel(Int8Args a, int group) {
   using F = Fmt<DT>;
   __shared__ __attribute__((aligned(1024))) uint16_t lds[kLdsBytes<P> / 2];
-  int m, n;
-  if (!tile_of(blockIdx.x, a.outer_tiles, a.row_tiles, group, &m, &n)) return;
+  int m, ns;
+  if (!tile_of(blockIdx.x, a.outer_tiles, a.row_tiles * a.splits, group, &m, &ns)) return;
+  const int n = ns % a.row_tiles, split = ns / a.row_tiles, from = split * a.span;
   const int m0 = m * P::MT, n0 = n * P::NT;
-  const Operand weight = {(const uint16_t*)(a.weight + m0 * a.weight_stride),
-                          (a.outer - 1 - m0) * a.weight_stride + a.inner, (int32_t)(a.weight_stride / 2)};
-  const Operand input = {(const uint16_t*)(a.input + n0 * a.input_stride),
-                         (a.rows - 1 - n0) * a.input_stride + a.inner, (int32_t)(a.input_stride / 2)};
+  const int depth = a.inner - from < a.span ? a.inner - from : a.span;
+  const Operand weight = {(const uint16_t*)(a.weight + m0 * a.weight_stride + from),
+                          (a.outer - 1 - m0) * a.weight_stride + a.inner - from, (int32_t)(a.weight_stride / 2)};
+  const Operand input = {(const uint16_t*)(a.input + n0 * a.input_stride + from),
+                         (a.rows - 1 - n0) * a.input_stride + a.inner - from, (int32_t)(a.input_stride / 2)};
   f32x4 acc[P::MI][P::NI];
-  P::run(weight, input, a.inner / 2, lds, acc);
+  P::run(weight, input, depth / 2, lds, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN % P::WM, wn = wave % P::WN;
   const bool one = P::NW > P::WM * P::WN;  // a SumProduct's waves all hold the tile: the first writes it
   if (one && wave > 0) return;
+  if (a.sums) {
+    int32_t* to = a.sums + (int64_t)split * a.rows * a.sum_stride;
+#pragma unroll
+    for (int ni = 0; ni < P::NI; ++ni) {
+      const int t = n0 + (wn * P::NI + ni) * 16 + (lane & 15);
+      if (t >= a.rows) continue;
+#pragma unroll
+      for (int mi = 0; mi < P::MI; ++mi) {
+        const int o = m0 + (wm * P::MI + mi) * 16 + (lane >> 4) * 4;
+        if (o < a.outer) *(f32x4*)(to + (int64_t)t * a.sum_stride + o) = acc[mi][ni];
+      }
+    }
+    return;
+  }
   float scale[P::NI];
 #pragma unroll
   for (int ni = 0; ni < P::NI; ++ni) {
@@ -168,6 +188,33 @@ __global__ __launch_bounds__(P::NW * 64) void int8_tile_kernel(Int8Args a, int g
   }
 }
 
+// The output from its sums' shares, four neighbours a lane.
+template <int DT>
+__global__ __launch_bounds__(256) void int8_sum_kernel(Int8Args a) {
+  using F = Fmt<DT>;
+  const int o = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (o >= a.outer) return;
+  for (int t = blockIdx.y; t < a.rows; t += gridDim.y) {
+    const int32_t* from = a.sums + (int64_t)t * a.sum_stride + o;
+    i32x4 s = {0, 0, 0, 0};
+    constexpr int U = 8;  // loads on their way at once
+    for (int i = 0; i < a.splits; i += U) {
+      i32x4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        v[u] = i + u < a.splits ? *(const i32x4*)(from + (int64_t)(i + u) * a.rows * a.sum_stride) : i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int u = 0; u < U; ++u) s += v[u];
+    }
+    const float scale = a.scale[t];
+    uint16_t* to = a.out + t * a.out_stride + o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (o + i < a.outer)
+        to[i] = F::pack1(scaled(s[i], scale, a.weight_scale[o + i], a.bias ? F::one(a.bias[o + i]) : 0.0f));
+  }
+}
+
 // Rows that 16-byte loads at 16-byte boundaries cannot take in place, copied to
 // rows of whole 16 bytes with zeros behind.
 __global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* from, int64_t stride, int64_t rows, int32_t width,
@@ -200,9 +247,64 @@ bool in_place(const void* p, int64_t stride, int64_t inner) {
   return aligned_to(p, 16) && stride % 16 == 0 && inner % 16 == 0 && stride <= kMaxStride;
 }
 
+// Tiles of output features x rows, and what a workgroup of them takes for 128
+// summed entries, ns, with `round` workgroups on 256 CUs at once (a slice's time is
+// its latency while there is one workgroup a CU or none: 0.85 of that).  Measured
+// at 4 to 1024 rows of 4096 to 4096, 4096 to 14336, 14336 to 4096 and 4096 to 1024,
+// where a call takes 2.5 us besides.  The model's choice is the fastest of these, or
+// within 10% of it, at all of them, e.g. (us; model's first) 48 x 4096 x 4096 64 x
+// 16 10.7, 64 x 64 14.0; 512 x 4096 x 14336 128 x 128 43.6, 256 x 256 48.5, 64 x 128
+// 56; 1024 x 4096 x 14336 256 x 256 55.7, 128 x 128 81; 256 x 4096 x 14336 64 x 128
+// 32.1, 128 x 128 40.8.
+enum Tile { kFewRows, kSum16, k64x16, k64x32, k64x64, k64x128, k128x128, k256x256 };
+struct TileCost {
+  Tile tile;
+  int32_t outer, rows, round, ns;
+};
+constexpr TileCost kTiles[] = {{kSum16, 16, 16, 256, 140},    {k64x16, 64, 16, 512, 300},
+                               {k64x32, 64, 32, 512, 500},    {k64x64, 64, 64, 512, 550},
+                               {k64x128, 64, 128, 512, 900},  {k128x128, 128, 128, 512, 1300},
+                               {k256x256, 256, 256, 256, 1660}};
+constexpr int64_t kSplitInner = 8192, kLeastShare = 1792;
+
+struct Choice {
+  Tile tile;
+  int32_t splits, span;
+};
+
+// A sum of 8192 entries or more is cut into shares, of 1792 at least, where that
+// fills the CUs: a second launch, 3 us, adds them (4 bytes of each written and read
+// again).  16 x 14336 x 4096 18.9 us whole and 16.2 in 4 shares, 48 rows 30.3 and
+// 17.5, 256 rows 40.0 and 35.0; at 4096 entries it gains nothing (48 x 4096 x 4096
+// 10.7 and 11.2).
+Choice choose(int64_t rows, int64_t inner, int64_t outer) {
+  if (rows <= 2) return {kFewRows, 1, (int32_t)inner};
+  Choice best = {};
+  double least = 0.0;
+  for (const TileCost& t : kTiles) {
+    const int64_t tiles = ceil_div(outer, t.outer) * ceil_div(rows, t.rows);
+    const double round = (double)t.round * current_cus() / kRefCUs;
+    int64_t most = inner >= kSplitInner && t.tile != kSum16 ? inner / kLeastShare : 1;
+    for (int64_t splits = 1; splits <= most; splits *= 2) {
+      if (splits > 1 && (double)(tiles * splits) > round) break;
+      const int64_t span = round_up(ceil_div(inner, splits), 128);
+      const double rounds = (double)(tiles * splits) / round;
+      double us = (rounds <= 0.5 && t.round > kRefCUs ? 0.85 : rounds <= 1.0 ? 1.0 : (double)ceil_div(tiles, (int64_t)round)) *
+                  (double)ceil_div(span, 128) * t.ns * 1e-3;
+      if (splits > 1) us += 3.0 + (double)rows * outer * splits * 8 / 5e6;
+      if (best.tile == kFewRows || us < least) {
+        best = {t.tile, (int32_t)ceil_div(inner, span), (int32_t)span};
+        least = us;
+      }
+    }
+  }
+  return best;
+}
+
 struct Plan {
-  int64_t packed_inner, weight, total;  // bytes; the packed input at 0
+  int64_t packed_inner, weight, sums, total;  // bytes; the packed input at 0
   bool input_in_place, weight_in_place;
+  Choice choice;
 };
 Plan plan_of(int64_t rows, int64_t inner, int64_t outer, const void* input, int64_t input_stride, const void* weight,
              int64_t weight_stride) {
@@ -210,8 +312,10 @@ Plan plan_of(int64_t rows, int64_t inner, int64_t outer, const void* input, int6
   p.packed_inner = round_up(inner, 16);
   p.input_in_place = in_place(input, input_stride, inner);
   p.weight_in_place = in_place(weight, weight_stride, inner);
+  p.choice = choose(rows, p.packed_inner, outer);
   p.weight = p.input_in_place ? 0 : round_up(rows * p.packed_inner, 256);
-  p.total = p.weight + (p.weight_in_place ? 0 : outer * p.packed_inner);
+  p.sums = p.weight + (p.weight_in_place ? 0 : round_up(outer * p.packed_inner, 256));
+  p.total = p.sums + (p.choice.splits > 1 ? p.choice.splits * rows * round_up(outer, 4) * 4 : 0);
   return p;
 }
 
@@ -235,8 +339,11 @@ template <class P, int DT>
 void launch_tiles(Int8Args a, hipStream_t stream) {
   a.outer_tiles = (int32_t)ceil_div(a.outer, P::MT);
   a.row_tiles = (int32_t)ceil_div(a.rows, P::NT);
-  int8_tile_kernel<P, DT><<<dim3((unsigned)round_up((int64_t)a.outer_tiles * a.row_tiles, 8)), dim3(P::NW * 64), 0,
-                            stream>>>(a, 4);
+  const int64_t tiles = (int64_t)a.outer_tiles * a.row_tiles * a.splits;
+  int8_tile_kernel<P, DT><<<dim3((unsigned)round_up(tiles, 8)), dim3(P::NW * 64), 0, stream>>>(a, 4);
+  if (a.sums)
+    int8_sum_kernel<DT><<<dim3((unsigned)ceil_div(a.outer, 1024), (unsigned)(a.rows < 8192 ? a.rows : 8192)),
+                          dim3(256), 0, stream>>>(a);
 }
 
 template <int DT, int N, int W>
@@ -245,37 +352,23 @@ void launch_few(const Int8Args& a, hipStream_t stream) {
 }
 
 template <int DT>
-int launch_all(const Int8Args& a, hipStream_t stream) {
+int launch_all(const Int8Args& a, Tile tile, hipStream_t stream) {
   constexpr int I = kInt8Pairs;
-  const int64_t cus = current_cus();
-  if (a.rows <= 1)
-    launch_few<DT, 1, 4>(a, stream);
-  else if (a.rows <= 2)
-    launch_few<DT, 2, 4>(a, stream);
-  else if (a.rows <= 4)
-    launch_few<DT, 4, 4>(a, stream);
-  else if (a.rows <= 8)
-    launch_few<DT, 8, 4>(a, stream);
-  else if (a.rows <= 16) {
-    if (ceil_div(a.outer, 16) <= cus)
-      launch_tiles<SumProduct<I, 1, 1, 4, 6>, DT>(a, stream);
-    else if (ceil_div(a.outer, 128) < 2 * cus)
-      launch_tiles<Product<I, 64, 16, 4, 1, 64, 6, false, false>, DT>(a, stream);
-    else
-      launch_tiles<Product<I, 128, 16, 4, 1, 64, 4, false, false>, DT>(a, stream);
-  } else if (a.rows <= 64) {
-    if (ceil_div(a.outer, 16) <= cus)
-      launch_tiles<SumProduct<I, 1, 4, 4, 3>, DT>(a, stream);
-    else if (ceil_div(a.outer, 128) < 2 * cus)
-      launch_tiles<Product<I, 64, 64, 4, 1, 64, 5, false, false>, DT>(a, stream);
-    else
-      launch_tiles<Product<I, 128, 64, 4, 1, 64, 3, false, false>, DT>(a, stream);
-  } else if (2 * ceil_div(a.outer, 256) * ceil_div(a.rows, 256) <= cus)
-    launch_tiles<Product<I, 128, 128, 2, 2, 64, 2, false, false>, DT>(a, stream);
-  else if (a.rows <= 128)
-    launch_tiles<Product<I, 256, 128, 4, 2, 32, 3, false, false>, DT>(a, stream);
-  else
-    launch_tiles<RingProduct<I, false, false, 2>, DT>(a, stream);
+  switch (tile) {
+    case kFewRows:
+      if (a.rows == 1)
+        launch_few<DT, 1, 4>(a, stream);
+      else
+        launch_few<DT, 2, 4>(a, stream);
+      break;
+    case kSum16: launch_tiles<SumProduct<I, 1, 1, 8, 4>, DT>(a, stream); break;
+    case k64x16: launch_tiles<Product<I, 64, 16, 4, 1, 64, 6, false, false>, DT>(a, stream); break;
+    case k64x32: launch_tiles<Product<I, 64, 32, 4, 1, 64, 6, false, false>, DT>(a, stream); break;
+    case k64x64: launch_tiles<Product<I, 64, 64, 2, 2, 64, 4, false, false>, DT>(a, stream); break;
+    case k64x128: launch_tiles<Product<I, 64, 128, 2, 2, 64, 3, false, false>, DT>(a, stream); break;
+    case k128x128: launch_tiles<Product<I, 128, 128, 2, 2, 64, 2, false, false>, DT>(a, stream); break;
+    case k256x256: launch_tiles<RingProduct<I, false, false, 2>, DT>(a, stream); break;
+  }
   return check_launch("8-bit linear kernel");
 }
 
@@ -345,8 +438,13 @@ int hprms_int8_linear(void* out, const void* input, const float* scale, const vo
   a.out_stride = out_row_stride;
   a.rows = (int32_t)rows;
   a.inner = (int32_t)p.packed_inner;
+  a.splits = p.choice.splits;
+  a.span = p.choice.span;
+  a.sum_stride = (int32_t)round_up(outer, 4);
+  if (a.splits > 1) a.sums = (int32_t*)(ws + p.sums);
   a.outer = (int32_t)outer;
-  return dtype == HPRMS_DTYPE_BF16 ? launch_all<HPRMS_DTYPE_BF16>(a, stream) : launch_all<HPRMS_DTYPE_FP16>(a, stream);
+  return dtype == HPRMS_DTYPE_BF16 ? launch_all<HPRMS_DTYPE_BF16>(a, p.choice.tile, stream)
+                                   : launch_all<HPRMS_DTYPE_FP16>(a, p.choice.tile, stream);
 }
 
 }  // extern "C"

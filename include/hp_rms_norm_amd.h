@@ -526,9 +526,9 @@ int hprms_norm_add_rmsnorm_backward(void* dinput, void* dresidual_in, void* dpos
  * weight_scale [outer] binary32, bias [outer] of dtype or NULL, out [rows, outer]
  * of dtype.  The sums are exact (inner is at most 131071), so a row's bits do not
  * depend on the other rows.  Workspace: hprms_int8_linear_workspace() bytes,
- * 256-byte aligned, none (and NULL) where both operands have 16-byte aligned
- * rows of whole 16 bytes no more than 4 MiB apart; others are copied there by
- * each call.  rows and outer go up to 2^24, out up to 2^36 elements.  rows == 0
+ * 256-byte aligned (0, and NULL, for most calls): shares of the sums where inner is
+ * 8192 or more, and operands whose rows are not 16-byte aligned, of whole 16
+ * bytes and at most 4 MiB apart, which each call copies there.  rows and outer go up to 2^24, out up to 2^36 elements.  rows == 0
  * is a no-op.  No counterpart in the reference.
  */
 int64_t hprms_int8_linear_workspace(int64_t rows, int64_t inner, int64_t outer, const void* input,

@@ -52,7 +52,7 @@ ROWS = [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 31, 48, 64, 65, 127, 128, 129, 256, 257,
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 def test_matches_the_formula(ops, rows, dtype):
     for i, (inner, outer) in enumerate(((64, 16), (16, 1), (128, 100), (1024, 4096), (1040, 4100), (2048, 257),
-                                        (4096, 512), (4112, 130), (48, 66000), (9216, 33))):
+                                        (4096, 512), (4112, 130), (48, 66000), (9216, 33), (16400, 515))):
         x, scale, w, weight_scale, bias = make(rows, inner, outer, rows + i)
         bias = bias.to(dtype) if i % 2 else None
         out = ops.int8_linear(x, scale, w, weight_scale, bias=bias, dtype=dtype)
