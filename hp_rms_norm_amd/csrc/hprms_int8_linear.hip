@@ -157,16 +157,33 @@ __global__ __launch_bounds__(P::NW * 64) void int8_tile_kernel(Int8Args a, int g
     const int t = n0 + (wn * P::NI + ni) * 16 + (lane & 15);
     scale[ni] = t < a.rows ? a.scale[t] : 0.0f;
   }
+  // the features' scales and biases, read once for all rows of the tile
+  typedef f32x4 f32x4_any __attribute__((aligned(4)));
+  f32x4 weight_scale[P::MI];
+  u32x2 bias[P::MI];
+#pragma unroll
+  for (int mi = 0; mi < P::MI; ++mi) {
+    const int o = m0 + (wm * P::MI + mi) * 16 + (lane >> 4) * 4;
+    bias[mi] = u32x2{0, 0};
+    if (o + 4 <= a.outer) {
+      weight_scale[mi] = *(const f32x4_any*)(a.weight_scale + o);
+      if (a.bias) bias[mi] = *(const u32x2_out*)(a.bias + o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = o + i < a.outer ? o + i : a.outer - 1;
+        weight_scale[mi][i] = a.weight_scale[at];
+        if (a.bias) bias[mi][i / 2] |= (uint32_t)a.bias[at] << (16 * (i & 1));
+      }
+    }
+  }
   // a fragment's four values
   auto value = [&](int mi, int ni) {
-    const int o = m0 + (wm * P::MI + mi) * 16 + (lane >> 4) * 4;
     const i32x4 s = __builtin_bit_cast(i32x4, acc[mi][ni]);
     float d[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = o + i < a.outer ? o + i : a.outer - 1;
-      d[i] = scaled(s[i], scale[ni], a.weight_scale[at], a.bias ? F::one(a.bias[at]) : 0.0f);
-    }
+    for (int i = 0; i < 4; ++i)
+      d[i] = scaled(s[i], scale[ni], weight_scale[mi][i], i & 1 ? F::hi(bias[mi][i / 2]) : F::lo(bias[mi][i / 2]));
     return u32x2{F::pack(d[0], d[1]), F::pack(d[2], d[3])};
   };
   if constexpr (P::NW > P::WM * P::WN) {
@@ -340,7 +357,7 @@ void launch_tiles(Int8Args a, hipStream_t stream) {
   a.outer_tiles = (int32_t)ceil_div(a.outer, P::MT);
   a.row_tiles = (int32_t)ceil_div(a.rows, P::NT);
   const int64_t tiles = (int64_t)a.outer_tiles * a.row_tiles * a.splits;
-  int8_tile_kernel<P, DT><<<dim3((unsigned)round_up(tiles, 8)), dim3(P::NW * 64), 0, stream>>>(a, 4);
+  int8_tile_kernel<P, DT><<<dim3((unsigned)round_up(tiles, 8)), dim3(P::NW * 64), 0, stream>>>(a, 8);
   if (a.sums)
     int8_sum_kernel<DT><<<dim3((unsigned)ceil_div(a.outer, 1024), (unsigned)(a.rows < 8192 ? a.rows : 8192)),
                           dim3(256), 0, stream>>>(a);

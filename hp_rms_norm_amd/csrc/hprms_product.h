@@ -13,8 +13,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-// 16 bytes at any 2-byte boundary
+// 16 and 8 bytes at any 2-byte boundary
 typedef u32x4 u32x4_out __attribute__((aligned(2)));
+typedef u32x2 u32x2_out __attribute__((aligned(2)));
 
 // 8-bit integers as a product's element type: everything below counts in pairs of
 // them, 16 bits each, and an accumulator's registers hold integers.  (A lane of

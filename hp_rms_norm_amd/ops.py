@@ -346,15 +346,10 @@ def norm_add_rms_norm_out(out, residual_out, input, residual, post_weight, weigh
                                                     residual_scale, eps)
 
 
-def _like(t):
-    """A new contiguous tensor of ``t``'s shape."""
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-
 def norm_add_rms_norm(input, residual, post_weight, weight, eps, gate=None, residual_scale=1.0):
     """Allocating form of ``norm_add_rms_norm_out``: returns ``(out,
     residual_out)`` and leaves the arguments untouched."""
-    out, residual_out = _like(input), _like(residual)
+    out, residual_out = torch.empty_like(input), torch.empty_like(residual)
     norm_add_rms_norm_out(out, residual_out, input, residual, post_weight, weight, eps, gate, residual_scale)
     return out, residual_out
 
@@ -373,8 +368,7 @@ def norm_add_rms_norm_int8_out(output, scale, residual_out, input, residual, pos
 
 
 def _int8_rows(input):
-    q = torch.empty(input.shape, dtype=torch.int8, device=input.device)
-    return q, torch.empty(input.shape[:-1] + (1,), dtype=torch.float32, device=input.device)
+    return torch.empty_like(input, dtype=torch.int8), input.new_empty(input.shape[:-1] + (1,), dtype=torch.float32)
 
 
 def norm_add_rms_norm_int8(input, residual, post_weight, weight, eps, gate=None, residual_scale=1.0):
@@ -382,7 +376,7 @@ def norm_add_rms_norm_int8(input, residual, post_weight, weight, eps, gate=None,
     residual_out)`` with ``scale`` of shape ``input.shape[:-1] + (1,)``, and
     leaves the arguments untouched."""
     q, scale = _int8_rows(input)
-    residual_out = _like(residual)
+    residual_out = torch.empty_like(residual)
     norm_add_rms_norm_int8_out(q, scale, residual_out, input, residual, post_weight, weight, eps, gate,
                                residual_scale)
     return q, scale, residual_out
@@ -437,9 +431,9 @@ def norm_add_rms_norm_backward(dout, input, residual, post_weight, weight, eps, 
     dout = _rows(dout)
     if dresidual is not None:
         dresidual = _rows(dresidual)
-    dinput, dresidual_in, dweight = _like(input), _like(residual), _like(weight)
-    dpost_weight = None if post_weight is None else _like(post_weight)
-    dgate = None if gate is None else _like(gate)
+    dinput, dresidual_in, dweight = torch.empty_like(input), torch.empty_like(residual), torch.empty_like(weight)
+    dpost_weight = None if post_weight is None else torch.empty_like(post_weight)
+    dgate = None if gate is None else torch.empty_like(gate)
     norm_add_rms_norm_backward_out(dinput, dresidual_in, dpost_weight, dweight, dgate, dout, input, residual,
                                    post_weight, weight, eps, gate, residual_scale, dresidual)
     return dinput, dresidual_in, dpost_weight, dweight, dgate
@@ -462,7 +456,7 @@ def int8_linear_out(out, input, scale, weight, weight_scale, bias=None):
 def int8_linear(input, scale, weight, weight_scale, bias=None, dtype=torch.bfloat16):
     """Allocating form of ``int8_linear_out``: returns ``out`` of ``dtype``
     (bf16 or fp16)."""
-    out = torch.empty(input.shape[:-1] + (weight.shape[0],), dtype=dtype, device=input.device)
+    out = input.new_empty(input.shape[:-1] + (weight.shape[0],), dtype=dtype)
     torch.ops.hp_rms_norm.int8_linear.default(out, input, scale, weight, weight_scale, bias)
     return out
 
@@ -489,11 +483,10 @@ def token_log_probs(logits, tokens, top=0, ignore_index=-100):
     """Allocating form of ``token_log_probs_out`` with ``top`` alternatives:
     returns ``(log_prob, entropy, lse, top_log_prob, top_index)``; the backward
     call takes ``lse`` and ``entropy``."""
-    log_prob = torch.empty(tokens.shape, dtype=torch.float32, device=tokens.device)
+    log_prob = torch.empty_like(tokens, dtype=torch.float32)
     entropy, lse = torch.empty_like(log_prob), torch.empty_like(log_prob)
-    shape = tuple(tokens.shape) + (top,)
-    top_log_prob = torch.empty(shape, dtype=torch.float32, device=tokens.device)
-    top_index = torch.empty(shape, dtype=torch.int64, device=tokens.device)
+    shape = (*tokens.shape, top)
+    top_log_prob, top_index = log_prob.new_empty(shape), tokens.new_empty(shape)
     token_log_probs_out(log_prob, entropy, lse, top_log_prob, top_index, logits, tokens, ignore_index)
     return log_prob, entropy, lse, top_log_prob, top_index
 
@@ -515,7 +508,7 @@ def token_log_probs_backward(dlog_prob, logits, tokens, lse, entropy=None, dentr
     """Allocating form of ``token_log_probs_backward_out``: returns
     ``dlogits``.  ``dlog_prob`` and ``dentropy`` may be any float32 tensors
     that expand to ``tokens``' shape."""
-    dlogits = _like(logits)
+    dlogits = torch.empty_like(logits)
     if dentropy is not None:
         dentropy = dentropy.expand(tokens.shape).contiguous()
     token_log_probs_backward_out(dlogits, dlog_prob.expand(tokens.shape).contiguous(), logits, tokens, lse, entropy,
