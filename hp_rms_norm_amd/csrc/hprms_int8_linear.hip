@@ -233,21 +233,34 @@ __global__ __launch_bounds__(256) void int8_sum_kernel(Int8Args a) {
 }
 
 // Rows that 16-byte loads at 16-byte boundaries cannot take in place, copied to
-// rows of whole 16 bytes with zeros behind.
-__global__ __launch_bounds__(256) void int8_pack_kernel(const int8_t* from, int64_t stride, int64_t rows, int32_t width,
-                                                        int32_t packed_width, int8_t* to) {
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int8_t* f = from + row * stride;
-    for (int32_t k = threadIdx.x * 16; k < packed_width; k += 256 * 16) {
-      u32x4 v = {0, 0, 0, 0};
-      if (k + 16 <= width) {
-        typedef u32x4 u32x4_any __attribute__((aligned(1)));
-        v = *(const u32x4_any*)(f + k);
-      } else {
-        for (int j = 0; k + j < width; ++j) v[j / 4] |= (uint32_t)(uint8_t)f[k + j] << (8 * (j & 3));
-      }
-      *(u32x4*)(to + row * packed_width + k) = v;
+// rows of whole 16 bytes with zeros behind: 16 bytes a lane, of the input's rows,
+// then of the weight's.
+struct PackJob {
+  const int8_t* from;
+  int8_t* to;
+  int64_t stride, chunks;  // chunks: rows x 16-byte pieces, 0 for none
+};
+
+__global__ __launch_bounds__(256) void int8_pack_kernel(PackJob input, PackJob weight, int32_t width,
+                                                        int32_t row_chunks) {
+  const int64_t step = (int64_t)gridDim.x * 256;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < input.chunks + weight.chunks; at += step) {
+    const bool second = at >= input.chunks;
+    const PackJob& job = second ? weight : input;
+    const int64_t c = second ? at - input.chunks : at;
+    const int64_t row = (c | row_chunks) >> 31 ? c / row_chunks : (int64_t)((uint32_t)c / (uint32_t)row_chunks);
+    const int32_t k = (int32_t)(c - row * row_chunks) * 16;
+    const int8_t* f = job.from + row * job.stride + k;
+    u32x4 v = {0, 0, 0, 0};
+    if (k + 16 <= width) {
+      typedef u32x4 u32x4_any __attribute__((aligned(1)));
+      v = *(const u32x4_any*)f;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (k + j < width) v[j / 4] |= (uint32_t)(uint8_t)f[j] << (8 * (j & 3));
     }
+    *(u32x4*)(job.to + c * 16) = v;
   }
 }
 
@@ -389,12 +402,6 @@ int launch_all(const Int8Args& a, Tile tile, hipStream_t stream) {
   return check_launch("8-bit linear kernel");
 }
 
-void pack(const void* from, int64_t stride, int64_t rows, int64_t inner, int64_t packed_inner, void* to,
-          hipStream_t stream) {
-  int8_pack_kernel<<<dim3((unsigned)(rows < 8192 ? rows : 8192)), dim3(256), 0, stream>>>(
-      (const int8_t*)from, stride, rows, (int32_t)inner, (int32_t)packed_inner, (int8_t*)to);
-}
-
 }  // namespace
 }  // namespace hprms
 
@@ -436,17 +443,23 @@ int hprms_int8_linear(void* out, const void* input, const float* scale, const vo
   Int8Args a = {};
   a.input = (const int8_t*)input;
   a.input_stride = input_row_stride;
+  a.weight = (const int8_t*)weight;
+  a.weight_stride = weight_row_stride;
+  PackJob jobs[2] = {};
   if (!p.input_in_place) {
-    pack(input, input_row_stride, rows, inner, p.packed_inner, ws, stream);
+    jobs[0] = {a.input, (int8_t*)ws, a.input_stride, rows * (p.packed_inner / 16)};
     a.input = (const int8_t*)ws;
     a.input_stride = p.packed_inner;
   }
-  a.weight = (const int8_t*)weight;
-  a.weight_stride = weight_row_stride;
   if (!p.weight_in_place) {
-    pack(weight, weight_row_stride, outer, inner, p.packed_inner, ws + p.weight, stream);
+    jobs[1] = {a.weight, (int8_t*)(ws + p.weight), a.weight_stride, outer * (p.packed_inner / 16)};
     a.weight = (const int8_t*)(ws + p.weight);
     a.weight_stride = p.packed_inner;
+  }
+  if (const int64_t chunks = jobs[0].chunks + jobs[1].chunks) {
+    const int64_t groups = ceil_div(chunks, 256);
+    int8_pack_kernel<<<dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, stream>>>(
+        jobs[0], jobs[1], (int32_t)inner, (int32_t)(p.packed_inner / 16));
   }
   a.scale = scale;
   a.weight_scale = weight_scale;
