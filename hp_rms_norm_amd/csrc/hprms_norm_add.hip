@@ -231,8 +231,6 @@ __global__ __launch_bounds__(256) void norm_add_any_kernel(NormAddArgs a) {
 // ---- host ------------------------------------------------------------------------------
 constexpr int64_t kMaxHidden = int64_t(1) << 24;
 constexpr int64_t kVectorHidden = 32768;
-// past 2^24 elements the rows exceed what the caches keep between operators
-constexpr int64_t kCachedElements = int64_t(1) << 24;
 
 // a launch holds fewer than 2^32 work-items
 constexpr int64_t kMaxGroups = int64_t(1) << 21;
@@ -241,17 +239,26 @@ template <int DT, bool POST, bool INT8, int LPR, int VPL, int BLOCK>
 void launch(NormAddArgs a, hipStream_t stream) {
   constexpr int RPB = BLOCK / LPR;
   const int64_t groups = (a.rows + RPB - 1) / RPB;
+  const bool nt = past_caches(a.rows, a.hidden, {{a.input, a.input_stride}, {a.residual, a.residual_stride}});
   for (int64_t from = 0; from < groups; from += kMaxGroups) {
     const dim3 grid((unsigned)(groups - from < kMaxGroups ? groups - from : kMaxGroups)), block(BLOCK);
     a.row_from = from * RPB;
-    if (a.rows > kCachedElements / a.hidden)
+    if (nt)
       norm_add_kernel<DT, LPR, VPL, BLOCK, POST, INT8, true><<<grid, block, 0, stream>>>(a);
     else
       norm_add_kernel<DT, LPR, VPL, BLOCK, POST, INT8, false><<<grid, block, 0, stream>>>(a);
   }
 }
 
-// Shapes go by the width alone, so a row's bits do not depend on the call's rows.
+// Shapes go by the width alone, so a row's bits do not depend on the call's rows;
+// each is the fastest of those tried, or within 3% of it.  Lanes a row x vectors a
+// lane, bf16 with both norms, 33.5M elements (268 MB) or as many rows as noted, us:
+//   128 16 x 1 44.6; 256 32 x 1 44.4; 512 64 x 1 44.7; 1024 64 x 2 44.8
+//   2048 128 x 2 44.9; 4096 256 x 2 45.9, 512 x 1 45.2, 128 x 4 48.3, but with 8-bit
+//   output 256 x 2 42.0, 512 x 1 46.4
+//   5120 (5000 rows) 256 x 3 36.4, 384 x 2 37.6, 512 x 2 38.8; 6144 256 x 3 43.0
+//   8192 512 x 2 46.5, 256 x 4 46.7, 1024 x 1 48.6
+//   12288 512 x 4 49.0, 512 x 3 47.5; 16384 512 x 4 48.3, 1024 x 2 47.9; 32768 1024 x 4 49.8
 template <int DT, bool POST, bool INT8>
 int launch_all(const NormAddArgs& a, hipStream_t stream) {
   const int32_t slots = (a.hidden + 7) / 8;

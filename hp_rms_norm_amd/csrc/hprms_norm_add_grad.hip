@@ -106,7 +106,7 @@ struct ColumnSums<true, N, BLOCK> {
 // z, and gate * z is its unit's share of dpost.  HOLD keeps weight and m as
 // binary32 in registers (8 instructions an element fewer than unpacking them for
 // each row); LACC keeps the columns' sums in LDS.
-template <int DT, int LPR, int VPL, int BLOCK, bool POST, int GATE, bool AHEAD, bool HOLD, bool LACC>
+template <int DT, int LPR, int VPL, int BLOCK, bool POST, int GATE, bool AHEAD, bool HOLD, bool LACC, bool NT>
 __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a) {
   constexpr int RPB = BLOCK / LPR;
   constexpr bool SHARED = GATE == kSharedGate, ELEMENT = GATE == kElementGate;
@@ -158,11 +158,11 @@ __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a)
     for (int k = 0; k < VPL; ++k) {
       nd[k] = ne[k] = nx[k] = nh[k] = ng[k] = zeros;
       if (in && on[k]) {
-        nd[k] = load_row8_once<true>(a.dout + row * a.dout_stride + off[k]);
-        nh[k] = load_row8_once<true>(a.residual + row * a.residual_stride + off[k]);
-        nx[k] = load_row8_once<true>(a.input + row * a.input_stride + off[k]);
-        if (a.dresidual) ne[k] = load_row8_once<true>(a.dresidual + row * a.dresidual_stride + off[k]);
-        if constexpr (ELEMENT) ng[k] = load_row8_once<true>(a.gate + row * a.gate_stride + off[k]);
+        nd[k] = load_row8_once<NT>(a.dout + row * a.dout_stride + off[k]);
+        nh[k] = load_row8_once<NT>(a.residual + row * a.residual_stride + off[k]);
+        nx[k] = load_row8_once<NT>(a.input + row * a.input_stride + off[k]);
+        if (a.dresidual) ne[k] = load_row8_once<NT>(a.dresidual + row * a.dresidual_stride + off[k]);
+        if constexpr (ELEMENT) ng[k] = load_row8(a.gate + row * a.gate_stride + off[k]);
       }
     }
   };
@@ -563,23 +563,32 @@ Plan plan_of(int64_t rows, int64_t hidden, int64_t gate_rows, bool post) {
   return p;
 }
 
-template <int DT, int LPR, int VPL, int BLOCK, bool AHEAD, bool HOLD, bool LACC, bool POST>
+template <int DT, int LPR, int VPL, int BLOCK, bool AHEAD, bool HOLD, bool LACC, bool POST, bool NT>
 void launch_gate(const NormAddGradArgs& a, const Plan& p, hipStream_t stream) {
   const dim3 grid((unsigned)p.grid), block(BLOCK);
   if (p.element)
-    norm_add_grad_kernel<DT, LPR, VPL, BLOCK, POST, kElementGate, AHEAD, HOLD, LACC><<<grid, block, 0, stream>>>(a);
+    norm_add_grad_kernel<DT, LPR, VPL, BLOCK, POST, kElementGate, AHEAD, HOLD, LACC, NT><<<grid, block, 0, stream>>>(a);
   else if (p.shared)
-    norm_add_grad_kernel<DT, LPR, VPL, BLOCK, POST, kSharedGate, AHEAD, HOLD, LACC><<<grid, block, 0, stream>>>(a);
+    norm_add_grad_kernel<DT, LPR, VPL, BLOCK, POST, kSharedGate, AHEAD, HOLD, LACC, NT><<<grid, block, 0, stream>>>(a);
   else
-    norm_add_grad_kernel<DT, LPR, VPL, BLOCK, POST, kNoGate, AHEAD, HOLD, LACC><<<grid, block, 0, stream>>>(a);
+    norm_add_grad_kernel<DT, LPR, VPL, BLOCK, POST, kNoGate, AHEAD, HOLD, LACC, NT><<<grid, block, 0, stream>>>(a);
 }
 
 template <int DT, int LPR, int VPL, int BLOCK, bool AHEAD, bool HOLD, bool LACC>
 void launch_rows(const NormAddGradArgs& a, const Plan& p, hipStream_t stream) {
-  if (a.post_weight)
-    launch_gate<DT, LPR, VPL, BLOCK, AHEAD, HOLD, LACC, true>(a, p, stream);
+  const bool nt = past_caches(a.rows, a.hidden,
+                              {{a.dout, a.dout_stride},
+                               {a.residual, a.residual_stride},
+                               {a.input, a.input_stride},
+                               {a.dresidual, a.dresidual ? a.dresidual_stride : 0}});
+  if (a.post_weight && nt)
+    launch_gate<DT, LPR, VPL, BLOCK, AHEAD, HOLD, LACC, true, true>(a, p, stream);
+  else if (a.post_weight)
+    launch_gate<DT, LPR, VPL, BLOCK, AHEAD, HOLD, LACC, true, false>(a, p, stream);
+  else if (nt)
+    launch_gate<DT, LPR, VPL, BLOCK, AHEAD, HOLD, LACC, false, true>(a, p, stream);
   else
-    launch_gate<DT, LPR, VPL, BLOCK, AHEAD, HOLD, LACC, false>(a, p, stream);
+    launch_gate<DT, LPR, VPL, BLOCK, AHEAD, HOLD, LACC, false, false>(a, p, stream);
 }
 
 template <int DT>

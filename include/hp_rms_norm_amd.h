@@ -528,8 +528,9 @@ int hprms_norm_add_rmsnorm_backward(void* dinput, void* dresidual_in, void* dpos
  * depend on the other rows.  Workspace: hprms_int8_linear_workspace() bytes,
  * 256-byte aligned (0, and NULL, for most calls): shares of the sums where inner is
  * 8192 or more, and operands whose rows are not 16-byte aligned, of whole 16
- * bytes and at most 4 MiB apart, which each call copies there.  rows and outer go up to 2^24, out up to 2^36 elements.  rows == 0
- * is a no-op.  No counterpart in the reference.
+ * bytes and at most 4 MiB apart, which each call copies there.  Asked for with the
+ * device current that the call has.  rows and outer go up to 2^24, out up to 2^36
+ * elements.  rows == 0 is a no-op.  No counterpart in the reference.
  */
 int64_t hprms_int8_linear_workspace(int64_t rows, int64_t inner, int64_t outer, const void* input,
                                     int64_t input_row_stride, const void* weight, int64_t weight_row_stride);
@@ -564,7 +565,8 @@ int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* to
  * entropy:
  *   dlogits <- dlog_prob * ([v == token] - p) - dentropy * p * (log p + entropy)
  * `dentropy` may be NULL (and then `entropy`).  Ignored rows and rows of nothing
- * but -infinity get zeros, a token out of range NaN.  `dlogits` may be `logits`
+ * but -infinity get zeros, a token out of range NaN.  A p is off by up to
+ * 2^-22 (|lse| + |log p|) of itself, as lse is binary32.  `dlogits` may be `logits`
  * exactly.  No workspace.  No counterpart in the reference.
  */
 int hprms_token_log_probs_backward(void* dlogits, const float* dlog_prob, const float* dentropy, const void* logits,
