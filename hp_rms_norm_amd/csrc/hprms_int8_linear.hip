@@ -8,9 +8,10 @@
 // result; a sum is rounded to binary32 once (24 bits of it, a relative error of
 // 2^-24 beside the output's own 2^-9 or 2^-12), then scaled.
 //
-// Few rows: the weight's bytes bound the call.  One and two rows run on dot products
-// of 4 bytes, a wave reading whole KB of a weight's row, so the weight streams in
-// whole lines (1 x 4096 x 14336: 10.6 us, 5.5 TB/s; on the matrix cores 14.4).  More
+// Few rows: the weight's bytes bound the call.  Up to 4 rows run on dot products of 4
+// bytes, a wave reading whole KB of a weight's row, so the weight streams in whole
+// lines (1 x 4096 x 14336: 10.6 us, 5.5 TB/s; on the matrix cores 14.4; 4 x 8192 x 8192
+// 15.3 and 19.6, 4 x 4096 x 4096 6.7 and 6.9, but 8 rows of it 10.1 and 6.9).  More
 // rows run on the matrix cores (hprms_product.h), in tiles by a model of their
 // times, and long sums of few tiles in shares.
 #include <hip/hip_runtime.h>
@@ -56,7 +57,9 @@ __device__ __forceinline__ int32_t wave_sum(int32_t v) {
 template <int DT, int N, int W>
 __global__ __launch_bounds__(256) void int8_few_rows_kernel(Int8Args a) {
   using F = Fmt<DT>;
-  constexpr int U = 2;  // KB of a row on their way at once, ahead of those in use
+  // KB of a row on their way at once, ahead of those in use (4 rows of 8192 x 8192:
+  // 15.3 us with 1, 16.7 with 2, as fewer waves fit a CU)
+  constexpr int U = N <= 2 ? 2 : 1;
   __shared__ int32_t lds[4][N * W];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t first = blockIdx.x * W;
@@ -308,7 +311,7 @@ struct Choice {
 // 17.5, 256 rows 40.0 and 35.0; at 4096 entries it gains nothing (48 x 4096 x 4096
 // 10.7 and 11.2).
 Choice choose(int64_t rows, int64_t inner, int64_t outer) {
-  if (rows <= 2) return {kFewRows, 1, (int32_t)inner};
+  if (rows <= 4) return {kFewRows, 1, (int32_t)inner};
   Choice best = {};
   double least = 0.0;
   for (const TileCost& t : kTiles) {
@@ -388,8 +391,12 @@ int launch_all(const Int8Args& a, Tile tile, hipStream_t stream) {
     case kFewRows:
       if (a.rows == 1)
         launch_few<DT, 1, 4>(a, stream);
-      else
+      else if (a.rows == 2)
         launch_few<DT, 2, 4>(a, stream);
+      else if (a.rows == 3)
+        launch_few<DT, 3, 4>(a, stream);
+      else
+        launch_few<DT, 4, 4>(a, stream);
       break;
     case kSum16: launch_tiles<SumProduct<I, 1, 1, 8, 4>, DT>(a, stream); break;
     case k64x16: launch_tiles<Product<I, 64, 16, 4, 1, 64, 6, false, false>, DT>(a, stream); break;
