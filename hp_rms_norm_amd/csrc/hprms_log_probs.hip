@@ -35,6 +35,7 @@ template <int DT>
 struct Logits {
   static constexpr int N = DT == HPRMS_DTYPE_FP32 ? 4 : 8;  // of a vector
   static constexpr int SIZE = DT == HPRMS_DTYPE_FP32 ? 4 : 2;
+  static constexpr int LAST_BIT = DT == HPRMS_DTYPE_FP32 ? 0 : DT == HPRMS_DTYPE_BF16 ? 16 : 13;  // as binary32
   static constexpr uint32_t MINUS_INF =
       DT == HPRMS_DTYPE_FP32 ? 0xff800000u : DT == HPRMS_DTYPE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
   __device__ static __forceinline__ float get(const u32x4& v, int j) {
@@ -138,23 +139,24 @@ struct LogProbArgs {
 
 // ---- the largest values --------------------------------------------------------------------
 // Both kernels find the `top` largest keys in two steps.  A bound first: each lane
-// has the largest of its own values, and a bound that `top` of a wave's lanes reach
-// is found bit by bit (ballots), so at least `top` values reach it and, of values
-// in no particular place, not many more (64 ln(64 / (64 - top)): 24 for 20; from
-// kLaneBound on it is sought among the largest of each vector).  Those that reach the largest of the four waves' bounds are listed in LDS, and each
-// one's place is the number of larger keys.  Where a wave's list would be longer
-// (equal values without end) or no bound above -infinity is reached, that wave's
-// keys are taken one by one instead, a maximum over its lanes each.
+// has the largest of its own values, and a bound that `top` of the workgroup's lanes
+// reach is found bit by bit (ballots), so at least `top` values reach it and, of
+// values in no particular place, not many more (256 ln(256 / (256 - top)): 21 for
+// 20; with a bound for each wave's 64 lanes four times as many, and 4096 x 50048
+// with 20 takes 113 us, 97 so, with 50 211 and 117).  Those that reach it are listed
+// in LDS, and each one's place is the number of larger keys.  Where a wave's list
+// would be longer (equal values without end) or no bound above -infinity is reached,
+// that wave's keys are taken one by one instead, a maximum over its lanes each.
 constexpr int kListed = 512;
-constexpr int kLaneBound = 32;
 constexpr uint32_t kOrderMinusInf = 0x007fffffu;
 
 // The largest (or, once they are counted exactly, some) bound that at least `count`
-// of some values reach, reached(b) of them b; 0 if there are fewer.
-template <class Reached>
+// of some values reach, reached(b) of them b; 0 if there are fewer.  Values of 16
+// bits have no bits below LAST.
+template <int LAST, class Reached>
 __device__ __forceinline__ uint32_t bound_of(Reached&& reached, int count) {
   uint32_t bound = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit >= LAST; --bit) {
     const uint32_t b = bound | 1u << bit;
     const int n = reached(b);
     if (n >= count) bound = b;
@@ -234,12 +236,15 @@ struct Sums {
   }
 };
 
+// 5 workgroups a CU, where 16 vectors a lane take 64 of the 96 registers (with 4
+// 4096 x 50048 and 5 alternatives takes 87 us, 82 so; with 8 vectors a lane and 8
+// workgroups 87).
 template <int DT, bool TOP, int STEPS>
-__global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(LogProbArgs a) {
+__global__ __launch_bounds__(256, STEPS > 4 ? 5 : 8) void log_probs_part_kernel(LogProbArgs a) {
   using L = Logits<DT>;
   __shared__ u64 lists[TOP ? 4 : 1][TOP ? kListed : 1];
   __shared__ f32x4 stats[4];
-  __shared__ uint32_t bounds[4];
+  __shared__ uint32_t tops[TOP ? 256 : 1];
   __shared__ int counts[4];
   __shared__ float row_lse;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -291,29 +296,7 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
   s = group_sum<64>(s);
   t = group_sum<64>(t);
   if (lane == 0) stats[wave] = f32x4{m, s, t * kLn2, 0.0f};
-  uint32_t bound = 0;
-  // whether a vector holds an element of the row
-  auto has = [&](int32_t at) { return at < a.vocab; };
-  if constexpr (TOP) {
-    const uint32_t lane_order = first < a.vocab ? order_of(lane_top) : 0u;
-    if (a.top <= kLaneBound) {
-      bound = bound_of([&](uint32_t b) { return __popcll(__ballot(lane_order >= b)); }, a.top);
-    } else {
-      uint32_t order[STEPS];
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i)
-        order[i] = i < a.steps && has(first + i * 256 * L::N) ? order_of(top[i]) : 0u;
-      bound = bound_of(
-          [&](uint32_t b) {
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) n += __popcll(__ballot(order[i] >= b));
-            return n;
-          },
-          a.top);
-    }
-    if (lane == 0) bounds[wave] = bound;
-  }
+  if constexpr (TOP) tops[threadIdx.x] = first < a.vocab ? order_of(lane_top) : 0u;
   __syncthreads();
   if (wave == 0) {
     Sums sums = {stats[0][0], stats[0][1], stats[0][2]};
@@ -328,8 +311,17 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
   if constexpr (TOP) {
     u64* list = lists[wave];
     int count = 0;
+    uint32_t reach[4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) bound = __builtin_elementwise_max(bound, bounds[w]);
+    for (int w = 0; w < 4; ++w) reach[w] = tops[w * 64 + lane];
+    const uint32_t bound = bound_of<L::LAST_BIT>(
+        [&](uint32_t b) {
+          int n = 0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) n += __popcll(__ballot(reach[w] >= b));
+          return n;
+        },
+        a.top);
     const float least = value_of(bound);
     // (below, what a bound at -infinity would let pass: elements past the row's end)
     bool listed = bound > kOrderMinusInf && bound <= 0xff800000u;
@@ -364,7 +356,7 @@ __global__ __launch_bounds__(256, STEPS > 4 ? 4 : 8) void log_probs_part_kernel(
       uint32_t order[STEPS];  // of each vector's largest value that is left
 #pragma unroll
       for (int i = 0; i < STEPS; ++i)
-        order[i] = i < a.steps && has(first + i * 256 * L::N) ? order_of(top[i]) : 0u;
+        order[i] = i < a.steps && first + i * 256 * L::N < a.vocab ? order_of(top[i]) : 0u;
       u64 last_key = 0;
       int last_step = -1;
       for (count = 0; count < a.top; ++count) {
@@ -480,7 +472,7 @@ __global__ __launch_bounds__(256) void log_probs_join_kernel(LogProbArgs a, int 
   // a bound from the lists' r-th keys: r of them each in enough lists
   const int r = (a.top + a.parts - 1) / a.parts, enough = (a.top + r - 1) / r;
   uint32_t reach = mine ? (uint32_t)(keys[r - 1] >> 32) : 0u;
-  const uint32_t bound = bound_of([&](uint32_t b) { return __popcll(__ballot(reach >= b)); }, enough);
+  const uint32_t bound = bound_of<0>([&](uint32_t b) { return __popcll(__ballot(reach >= b)); }, enough);
   u64* list = lists[wave];
   int count = 0;
   bool more = mine;
