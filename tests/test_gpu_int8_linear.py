@@ -120,3 +120,17 @@ def test_a_large_product(ops):
     x, scale, w, weight_scale, bias = make(5000, 1024, 9000, 10)
     out = ops.int8_linear(x, scale, w, weight_scale, bias=bias.bfloat16())
     check(out, x, scale, w, weight_scale, bias.bfloat16())
+
+
+@pytest.mark.parametrize("rows", [2, 3, 4])
+def test_a_few_rows_of_odd_sizes_strides_and_the_largest_sums(ops, rows):
+    for inner, outer, pads in ((1, 1, (0, 0, 0, 0)), (17, 3, (0, 0, 0, 0)), (1001, 6, (3, 1, 16, 0)),
+                               (4096, 5, (16, 16, 32, 16)), (5000, 1027, (0, 8, 0, 4)),
+                               (1024, 4, (0, 0, 0, 0)), (8208, 9, (0, 0, 0, 0))):
+        x, scale, w, weight_scale, bias = make(rows, inner, outer, rows, *pads)
+        out = ops.int8_linear(x, scale, w, weight_scale, bias=bias.half(), dtype=torch.float16)
+        check(out, x, scale, w, weight_scale, bias.half())
+    x = torch.full((rows, 131071), -128, device=DEV, dtype=torch.int8)
+    w = torch.full((7, 131071), -128, device=DEV, dtype=torch.int8)
+    scale, weight_scale = torch.full((rows,), 2.0 ** -14, device=DEV), torch.full((7,), 0.5, device=DEV)
+    check(ops.int8_linear(x, scale, w, weight_scale), x, scale, w, weight_scale, None)

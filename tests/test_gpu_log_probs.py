@@ -135,6 +135,21 @@ def test_equal_values_go_by_the_lower_index(ops, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("top", [2, 19, 20, 21, 32, 33, 50, 63, 64])
+def test_where_the_largest_values_lie(ops, top, dtype):
+    """Spread out, neighbours in few lanes, in one wave, at a row's end, all
+    negative, and one lane's apart from the others; few rows and many."""
+    for rows, vocab in ((6, 2000), (6, 50001), (600, 9001)):
+        z, t = make(rows, vocab, dtype, top)
+        z[1::6, 100:100 + top] += 30.0
+        z[2::6, :512] += 20.0
+        z[3::6, vocab - top + 1:] += 25.0
+        z[4::6] -= 40.0
+        z[5::6, ::2048] += 30.0
+        check(ops.token_log_probs(z, t, top=top), z, t, top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("vocab", [3, 700, 20000])
 def test_rows_without_a_value_and_values_that_are_not_numbers(ops, vocab, dtype):
     z, t = make(6, vocab, dtype, 3)
