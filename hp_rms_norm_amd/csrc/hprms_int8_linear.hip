@@ -281,23 +281,25 @@ bool in_place(const void* p, int64_t stride, int64_t inner) {
 }
 
 // Tiles of output features x rows, and what a workgroup of them takes for 128
-// summed entries, ns, with `round` workgroups on 256 CUs at once (a slice's time is
-// its latency while there is one workgroup a CU or none: 0.85 of that).  Measured
-// at 4 to 1024 rows of 4096 to 4096, 4096 to 14336, 14336 to 4096 and 4096 to 1024,
-// where a call takes 2.5 us besides.  The model's choice is the fastest of these, or
-// within 10% of it, at all of them, e.g. (us; model's first) 48 x 4096 x 4096 64 x
-// 16 10.7, 64 x 64 14.0; 512 x 4096 x 14336 128 x 128 43.6, 256 x 256 48.5, 64 x 128
-// 56; 1024 x 4096 x 14336 256 x 256 55.7, 128 x 128 81; 256 x 4096 x 14336 64 x 128
-// 32.1, 128 x 128 40.8.
+// summed entries, ns, with `round` workgroups on 256 CUs at once, or `alone` with
+// one a CU at most (a slice's latency).  Measured at 4 to 1024 rows of 4096 to 4096,
+// 4096 to 14336, 14336 to 4096 and 4096 to 1024, where a call takes 2.5 us besides.
+// The model's choice is the fastest of these, or within 13% of it, at all of them,
+// e.g. (us; model's first) 48 x 4096 x 4096 64 x 16 8.4, 64 x 32 10.9, 64 x 64 14.0; 24 x
+// 4096 x 14336 64 x 32 14.4, 64 x 16 16.7; 512 x 4096 x 14336 128 x 128 41.6, 256 x
+// 256 48.5, 64 x 128 56; 1024 x 4096 x 14336 256 x 256 53.6, 128 x 128 81; 256 x 4096 x
+// 14336 64 x 128 32.2, 128 x 128 40.8.  The two smallest take slices of 256 bytes in
+// 3 stages: 48 x 4096 x 4096 8.4 us, with 128 bytes in 6 stages, twice the barriers,
+// 10.6 (64 x 64 so: 128 x 4096 x 14336 26.5, one workgroup a CU, as it is 20 to 23).
 enum Tile { kFewRows, kSum16, k64x16, k64x32, k64x64, k64x128, k128x128, k256x256 };
 struct TileCost {
   Tile tile;
-  int32_t outer, rows, round, ns;
+  int32_t outer, rows, round, ns, alone;
 };
-constexpr TileCost kTiles[] = {{kSum16, 16, 16, 256, 140},    {k64x16, 64, 16, 512, 300},
-                               {k64x32, 64, 32, 512, 500},    {k64x64, 64, 64, 512, 550},
-                               {k64x128, 64, 128, 512, 900},  {k128x128, 128, 128, 512, 1300},
-                               {k256x256, 256, 256, 256, 1660}};
+constexpr TileCost kTiles[] = {{kSum16, 16, 16, 256, 140, 140},       {k64x16, 64, 16, 512, 300, 190},
+                               {k64x32, 64, 32, 512, 480, 275},       {k64x64, 64, 64, 512, 550, 470},
+                               {k64x128, 64, 128, 512, 900, 765},     {k128x128, 128, 128, 512, 1300, 1105},
+                               {k256x256, 256, 256, 256, 1660, 1660}};
 constexpr int64_t kSplitInner = 8192, kLeastShare = 1792;
 
 struct Choice {
@@ -309,7 +311,7 @@ struct Choice {
 // fills the CUs: a second launch, 3 us, adds them (4 bytes of each written and read
 // again).  16 x 14336 x 4096 18.9 us whole and 16.2 in 4 shares, 48 rows 30.3 and
 // 17.5, 256 rows 40.0 and 35.0; at 4096 entries it gains nothing (48 x 4096 x 4096
-// 10.7 and 11.2).
+// 10.7 and 11.2 when both were measured).
 Choice choose(int64_t rows, int64_t inner, int64_t outer) {
   if (rows <= 4) return {kFewRows, 1, (int32_t)inner};
   Choice best = {};
@@ -321,9 +323,8 @@ Choice choose(int64_t rows, int64_t inner, int64_t outer) {
     for (int64_t splits = 1; splits <= most; splits *= 2) {
       if (splits > 1 && (double)(tiles * splits) > round) break;
       const int64_t span = round_up(ceil_div(inner, splits), 128);
-      const double rounds = (double)(tiles * splits) / round;
-      double us = (rounds <= 0.5 && t.round > kRefCUs ? 0.85 : rounds <= 1.0 ? 1.0 : (double)ceil_div(tiles, (int64_t)round)) *
-                  (double)ceil_div(span, 128) * t.ns * 1e-3;
+      double us = (double)ceil_div(span, 128) * 1e-3 *
+                  (tiles * splits <= current_cus() ? t.alone : t.ns * (double)ceil_div(tiles * splits, (int64_t)round));
       if (splits > 1) us += 3.0 + (double)rows * outer * splits * 8 / 5e6;
       if (best.tile == kFewRows || us < least) {
         best = {t.tile, (int32_t)ceil_div(inner, span), (int32_t)span};
@@ -399,8 +400,8 @@ int launch_all(const Int8Args& a, Tile tile, hipStream_t stream) {
         launch_few<DT, 4, 4>(a, stream);
       break;
     case kSum16: launch_tiles<SumProduct<I, 1, 1, 8, 4>, DT>(a, stream); break;
-    case k64x16: launch_tiles<Product<I, 64, 16, 4, 1, 64, 6, false, false>, DT>(a, stream); break;
-    case k64x32: launch_tiles<Product<I, 64, 32, 4, 1, 64, 6, false, false>, DT>(a, stream); break;
+    case k64x16: launch_tiles<Product<I, 64, 16, 4, 1, 128, 3, false, false>, DT>(a, stream); break;
+    case k64x32: launch_tiles<Product<I, 64, 32, 4, 1, 128, 3, false, false>, DT>(a, stream); break;
     case k64x64: launch_tiles<Product<I, 64, 64, 2, 2, 64, 4, false, false>, DT>(a, stream); break;
     case k64x128: launch_tiles<Product<I, 64, 128, 2, 2, 64, 3, false, false>, DT>(a, stream); break;
     case k128x128: launch_tiles<Product<I, 128, 128, 2, 2, 64, 2, false, false>, DT>(a, stream); break;

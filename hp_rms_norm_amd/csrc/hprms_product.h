@@ -76,7 +76,7 @@ __device__ __forceinline__ void phase_end() {
 // swizzled through the addresses that the lanes load from, so that fragment
 // reads touch every bank once:
 //   k contiguous: LDS row r holds 2 * BK bytes, its 16-byte chunk p the row's
-//     chunk p ^ (r mod 8) (BK = 64) or p ^ (r / 2 mod 4) (BK = 32); a
+//     chunk p ^ (r mod 8) (BK = 64, 128) or p ^ (r / 2 mod 4) (BK = 32); a
 //     fragment is one 16-byte read a lane.
 //   k outer: LDS row k holds 2 * extent bytes, its 32-byte unit u the unit
 //     u ^ (k mod 4 + 4 (k / 8 mod 2)), as far as the extent has units; a
@@ -96,7 +96,7 @@ struct Product {
   static constexpr int STAGE = ABYTES + BBYTES;
   static constexpr int LA = (ABYTES / 1024 + NW - 1) / NW, LB = (BBYTES / 1024 + NW - 1) / NW;
   static constexpr int LDS_BYTES = STAGE * ST;
-  static_assert(BK == 64 || BK == 32, "slice depth");
+  static_assert(BK == 128 || BK == 64 || BK == 32, "slice depth");
   static_assert(MT % (WM * 16) == 0 && NT % (WN * 16) == 0, "wave tiles");
   static_assert(ABYTES % 1024 == 0 && BBYTES % 1024 == 0, "whole loads");
 
@@ -109,7 +109,7 @@ struct Product {
     if constexpr (!KO) {
       constexpr int RB = BK * 2;
       const int r = at / RB, p = at % RB / 16;
-      const int c = BK == 64 ? p ^ (r & 7) : p ^ ((r >> 1) & 3);
+      const int c = BK >= 64 ? p ^ (r & 7) : p ^ ((r >> 1) & 3);
       *k = c * 8;
       return ((uint32_t)r * (uint32_t)stride + c * 8) * 2;
     } else {
@@ -131,7 +131,7 @@ struct Product {
   __device__ static __forceinline__ u32x4 fragment(lds_u16* slice, int r0, int kk, int lane) {
     if constexpr (!KO) {
       const int r = r0 + (lane & 15), c = kk * 4 + (lane >> 4);
-      const int p = BK == 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
+      const int p = BK >= 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
       return *(__attribute__((address_space(3))) u32x4*)(slice + r * BK + p * 8);
     } else {
       // 16 lanes read 4 rows of k (lane & 15) / 4, 4 columns each
