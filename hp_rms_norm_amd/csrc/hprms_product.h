@@ -76,7 +76,7 @@ __device__ __forceinline__ void phase_end() {
 // swizzled through the addresses that the lanes load from, so that fragment
 // reads touch every bank once:
 //   k contiguous: LDS row r holds 2 * BK bytes, its 16-byte chunk p the row's
-//     chunk p ^ (r mod 8) (BK = 64, 128) or p ^ (r / 2 mod 4) (BK = 32); a
+//     chunk p ^ (r mod 16) (BK = 128), p ^ (r mod 8) (64) or p ^ (r / 2 mod 4) (32); a
 //     fragment is one 16-byte read a lane.
 //   k outer: LDS row k holds 2 * extent bytes, its 32-byte unit u the unit
 //     u ^ (k mod 4 + 4 (k / 8 mod 2)), as far as the extent has units; a
@@ -100,6 +100,9 @@ struct Product {
   static_assert(MT % (WM * 16) == 0 && NT % (WN * 16) == 0, "wave tiles");
   static_assert(ABYTES % 1024 == 0 && BBYTES % 1024 == 0, "whole loads");
 
+  // What a row's 16-byte chunks are permuted by (k contiguous).
+  __device__ static __forceinline__ int swizzle(int r) { return BK == 128 ? r & 15 : BK == 64 ? r & 7 : (r >> 1) & 3; }
+
   // Byte offset, from the operand's base, of what lane `lane` loads in load j
   // of a slice (1024 bytes of LDS), for an operand of EXT rows; *k: the slice's
   // summed entry where the lane's 8 elements begin (k contiguous).
@@ -109,7 +112,7 @@ struct Product {
     if constexpr (!KO) {
       constexpr int RB = BK * 2;
       const int r = at / RB, p = at % RB / 16;
-      const int c = BK >= 64 ? p ^ (r & 7) : p ^ ((r >> 1) & 3);
+      const int c = p ^ swizzle(r);
       *k = c * 8;
       return ((uint32_t)r * (uint32_t)stride + c * 8) * 2;
     } else {
@@ -131,7 +134,7 @@ struct Product {
   __device__ static __forceinline__ u32x4 fragment(lds_u16* slice, int r0, int kk, int lane) {
     if constexpr (!KO) {
       const int r = r0 + (lane & 15), c = kk * 4 + (lane >> 4);
-      const int p = BK >= 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
+      const int p = c ^ swizzle(r);
       return *(__attribute__((address_space(3))) u32x4*)(slice + r * BK + p * 8);
     } else {
       // 16 lanes read 4 rows of k (lane & 15) / 4, 4 columns each
