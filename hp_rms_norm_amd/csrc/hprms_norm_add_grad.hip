@@ -542,7 +542,9 @@ Plan plan_of(int64_t rows, int64_t hidden, int64_t gate_rows, bool post) {
   const Shape s = general ? Shape{1, 1, 1, 0} : shape_of(hidden);
   const int64_t rpb = s.block / s.lpr;
   const int64_t most = general ? 64 : (int64_t)current_cus() * s.per_cu;
-  p.element = gate_rows > 0 && gate_rows == rows && rows > 1;
+  // (the general path's columns kernel writes a shared gate's gradient before its rows kernel reads the
+  // gate, on which dgate may lie where every row has its own: there one row is such a case too)
+  p.element = gate_rows > 0 && gate_rows == rows && (rows > 1 || general);
   p.shared = gate_rows > 0 && !p.element;
   p.gates = p.shared ? gate_rows : 1;
   if (rows > 0) {

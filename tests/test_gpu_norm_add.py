@@ -362,3 +362,19 @@ def test_gradient_against_differences(ops):
         slope = (model(*up) - model(*down)) / (2 * step)
         size = (d.double() * way).abs().sum()
         assert abs(float((d.double() * way).sum() - slope)) <= float((U[c.dtype] + 1e-4) * size)
+
+
+@pytest.mark.parametrize("hidden", [1, 7, 9, 1001, 4096, 16384, 16385, 33000])
+@pytest.mark.parametrize("gate", ["channel", "sequence", "element"])
+@pytest.mark.parametrize("post", [True, False])
+def test_gradient_of_one_row_in_place_of_its_gate(ops, hidden, gate, post):
+    """One row has a gate of its own, whichever shape the gate has."""
+    c = Case(1, 1, hidden, torch.bfloat16, 14, gate, post, 0.9)
+    want, res, dout, dres = run_backward(ops, c)
+    check_backward(c, want, res, dout, dres)
+    held = c.gate.clone()
+    di, dr, dw = torch.empty_like(c.x), torch.empty_like(c.x), torch.empty_like(c.w)
+    dp = torch.empty_like(c.p) if post else None
+    ops.norm_add_rms_norm_backward_out(di, dr, dp, dw, held, dout, c.x, res, c.p, c.w, EPS, held, 0.9, dres)
+    for a, b in zip((di, dr, dp, dw, held), want):
+        assert (a is None and b is None) or torch.equal(a, b)
