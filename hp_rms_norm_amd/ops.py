@@ -474,7 +474,8 @@ def token_log_probs_out(log_prob, entropy, lse, top_log_prob, top_index, logits,
     outside ``[0, V)`` gives a NaN ``log_prob``.  Logits of -inf (forbidden
     tokens) have probability 0; a row of nothing else has entropy 0 and log
     probabilities of -inf.  NaN or +inf makes a row's ``lse`` NaN; NaN ranks
-    first.  No reference counterpart."""
+    first.  A row's last bits follow the row count and the row's address, in
+    batch-invariant mode neither.  No reference counterpart."""
     torch.ops.hp_rms_norm.token_log_probs.default(log_prob, entropy, lse, top_log_prob, top_index, logits, tokens,
                                                   ignore_index)
 

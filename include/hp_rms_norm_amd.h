@@ -550,9 +550,10 @@ int hprms_int8_linear(void* out, const void* input, const float* scale, const vo
  * top_log_prob = -infinity and entropy 0.  NaN or +infinity makes a row's lse
  * NaN; NaN ranks above every number.  Workspace: as for
  * hprms_rmsnorm_backward(), of hprms_token_log_probs_workspace() bytes, enough in
- * either batch-invariant mode.  rows == 0 is a no-op; vocab goes up to 2^20.  Few
- * rows are cut into more parts (other last bits) unless that mode is on.  No
- * counterpart in the reference.
+ * either batch-invariant mode.  rows == 0 is a no-op; vocab goes up to 2^20.  By
+ * default few rows are cut into more parts, and rows off 16-byte boundaries
+ * where their addresses say (other last bits); with that mode on a row's bits
+ * follow from the row alone, wherever it lies.  No counterpart in the reference.
  */
 int64_t hprms_token_log_probs_workspace(int64_t rows, int64_t vocab, int64_t top, int dtype);
 int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* top_log_prob, int64_t* top_index,

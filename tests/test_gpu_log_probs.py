@@ -331,3 +331,28 @@ def test_leading_dimensions_and_no_rows(ops):
     got = ops.token_log_probs(z[:0], t[:0], top=2)
     assert got[0].shape == (0,) and got[4].shape == (0, 2)
     assert ops.token_log_probs_backward(torch.empty(0, device=DEV), z[:0], t[:0], got[2]).shape == (0, 300)
+
+
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("vocab,dtype", [
+    (32767, torch.bfloat16), (32768, torch.bfloat16), (50001, torch.bfloat16), (65535, torch.float16),
+    (65536, torch.bfloat16), (131071, torch.float16), (131072, torch.bfloat16), (32767, torch.float32),
+    (131072, torch.float32), (1001, torch.bfloat16), (77, torch.float32)])
+def test_batch_invariant_mode_at_any_address(ops, vocab, dtype, pad):
+    """In the mode a row's bits depend on neither the other rows nor on where the
+    row lies: rows of odd strides alone, among others and copied to other
+    addresses.  The vocabularies are those whose rows fill their parts to the
+    last step, where a few bytes more would change the parts."""
+    z, t = make(24, vocab, dtype, 8, 0.0, 0.1, pad)
+    moved = make(24, vocab, dtype, 9, 0.0, 0.0, 4, 3)[0]
+    moved.copy_(z)
+    previous = ops.set_batch_invariant(True)
+    try:
+        whole = ops.token_log_probs(z, t, top=7)
+        check(whole, z, t, 7)
+        for rows in (z, moved):
+            for at in (slice(0, 24), slice(0, 1), slice(8, 9), slice(3, 9), slice(23, 24)):
+                for a, b in zip(ops.token_log_probs(rows[at], t[at], top=7), whole):
+                    assert torch.equal(a, b[at])
+    finally:
+        ops.set_batch_invariant(previous)
