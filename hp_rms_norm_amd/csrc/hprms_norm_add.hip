@@ -40,6 +40,8 @@ struct NormAddArgs {
   float eps, residual_scale;
 };
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
 __device__ __forceinline__ int64_t gate_row(const NormAddArgs& a, int64_t row) {
   // one gate for all rows, or one for each, or one for every so many
   if (a.rows_per_gate >= a.rows) return 0;
@@ -51,7 +53,7 @@ __device__ __forceinline__ float inverse_rms(float squares, int32_t hidden, floa
   return 1.0f / sqrtf(squares / (float)hidden + eps);
 }
 
-// A row's scale and its reciprocal from the bits of max |y|; a row that holds NaN
+// A row's scale and its reciprocal from the 16 bits of max |y|; a row that holds NaN
 // or infinity has that as its scale, and zeros as elements.
 struct RowScale {
   float scale, inverse;
@@ -59,7 +61,7 @@ struct RowScale {
 };
 template <int DT>
 __device__ __forceinline__ RowScale row_scale(uint32_t top) {
-  const float amax = Fmt<DT>::lo(Fmt<DT>::pack(__uint_as_float(top), 0.0f));  // rounded as y is
+  const float amax = Fmt<DT>::lo(top);
   const bool finite = __float_as_uint(amax) < 0x7f800000u;
   const float scale = finite ? fmaxf(amax / 127.0f, 1.17549435e-38f) : amax;
   return {scale, finite ? 1.0f / scale : 0.0f, finite};
@@ -132,6 +134,7 @@ __global__ __launch_bounds__(BLOCK) void norm_add_kernel(NormAddArgs a) {
       h[j] = element<DT>(s[k], j) * a.residual_scale + n;
     }
     s[k] = pack8<DT>(h);
+    if (skip[k] > 0) drop_first(s[k], skip[k]);  // (0 times an infinite gate or weight: NaN)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float v = element<DT>(s[k], j);
@@ -144,21 +147,27 @@ __global__ __launch_bounds__(BLOCK) void norm_add_kernel(NormAddArgs a) {
   for (int k = 0; k < VPL; ++k) w[k] = on[k] ? load_row8(a.weight + off[k]) : u32x4{0, 0, 0, 0};
   sum_rows<1, LPR, BLOCK>(ss, sums[1]);
   const float ih = inverse_rms(ss[0], a.hidden, a.eps);
-  uint32_t top = 0;
+  u16x2 top = {0, 0};
 #pragma unroll
   for (int k = 0; k < VPL; ++k) {
     float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      y[j] = element<DT>(s[k], j) * ih * element<DT>(w[k], j);
-      if constexpr (INT8) top = __builtin_elementwise_max(top, __float_as_uint(y[j]) & 0x7fffffffu);
-    }
+    for (int j = 0; j < 8; ++j) y[j] = element<DT>(s[k], j) * ih * element<DT>(w[k], j);
     s[k] = pack8<DT>(y);
-    if (!INT8 && on[k]) store_row8((uint16_t*)a.out + row * a.out_stride + off[k], s[k], skip[k]);
+    if constexpr (INT8) {
+      if (skip[k] > 0) drop_first(s[k], skip[k]);  // (0 times an infinite weight or ih)
+      u16x2 t = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, s[k][j] & 0x7fff7fffu));
+      top = on[k] ? __builtin_elementwise_max(top, t) : top;
+    } else if (on[k]) {
+      store_row8((uint16_t*)a.out + row * a.out_stride + off[k], s[k], skip[k]);
+    }
   }
   if constexpr (INT8) {
-    top = max_rows<LPR, BLOCK>(top, tops);
-    const RowScale q = row_scale<DT>(top);
+    const RowScale q =
+        row_scale<DT>(max_rows<LPR, BLOCK>(__builtin_elementwise_max((uint32_t)top[0], (uint32_t)top[1]), tops));
     if (live && lane == 0) a.scale[row] = q.scale;
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
@@ -218,8 +227,7 @@ __global__ __launch_bounds__(256) void norm_add_any_kernel(NormAddArgs a) {
       int8_t* out = (int8_t*)a.out + row * a.out_stride;
       uint32_t top = 0;
       for (int32_t i = threadIdx.x; i < a.hidden; i += 256)
-        top = __builtin_elementwise_max(top,
-                                        __float_as_uint(F::one(h[i]) * ih * F::one(a.weight[i])) & 0x7fffffffu);
+        top = __builtin_elementwise_max(top, (uint32_t)F::pack1(F::one(h[i]) * ih * F::one(a.weight[i])) & 0x7fffu);
       const RowScale q = row_scale<DT>(max_rows<256, 256>(top, tops));
       if (threadIdx.x == 0) a.scale[row] = q.scale;
       for (int32_t i = threadIdx.x; i < a.hidden; i += 256)

@@ -5,7 +5,9 @@
 // the last whole vector holds the row's last 8 elements (H >= 8), of which only
 // those that no whole vector holds count and are stored.  The others are loaded
 // and set to 0 (drop_first), so it does not matter if their owner has overwritten
-// them, and zeros change no sum and no maximum.
+// them, and zeros change no sum and no maximum.  What multiplies them is either
+// set to 0 as well or their product is: a weight, a gate or a reciprocal root may be
+// infinite there.
 #pragma once
 
 #include <initializer_list>

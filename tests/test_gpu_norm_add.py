@@ -378,3 +378,64 @@ def test_gradient_of_one_row_in_place_of_its_gate(ops, hidden, gate, post):
     ops.norm_add_rms_norm_backward_out(di, dr, dp, dw, held, dout, c.x, res, c.p, c.w, EPS, held, 0.9, dres)
     for a, b in zip((di, dr, dp, dw, held), want):
         assert (a is None and b is None) or torch.equal(a, b)
+
+
+# the last vector of a row overlaps the one before, in elements hidden - 8 ... hidden / 8 * 8 - 1
+OVERLAPPED = [9, 121, 250, 257, 505, 1001, 2047, 4097, 5003, 8187, 12001, 16383, 17001, 32761]
+
+
+def alike(got, want):
+    """The same infinities and NaN, and elsewhere the same numbers up to roundings."""
+    u = U[got.dtype]
+    off = (got.double() - want).abs()
+    same = (got.double() == want) | (torch.isnan(got) & torch.isnan(want))
+    return bool((same | (torch.isfinite(want) & (off <= (u + 2 * k_of(want.shape[-1]) * E) * want.abs()
+                                                 + TINY[got.dtype]))).all())
+
+
+@pytest.mark.parametrize("hidden", OVERLAPPED)
+@pytest.mark.parametrize("where", ["gate", "gate of a row", "post_weight", "weight"])
+def test_infinities_where_a_rows_vectors_overlap(ops, hidden, where):
+    """An infinity in the gate or a weight makes its own element infinite, the
+    others 0 (its mean square is infinite) and no more than that NaN."""
+    for at in (hidden - 8, hidden // 8 * 8 - 1):
+        c = Case(1, 6, hidden, torch.bfloat16, 15, "element" if where == "gate of a row" else "channel", True, 0.5)
+        if where == "post_weight":
+            c.p[at] = float("inf")
+        elif where == "weight":
+            c.w[at] = float("inf")
+        else:
+            c.gate.view(-1, hidden)[-1, at] = -float("inf")
+        out, res = c.forward(ops)
+        x, gate = c.x.double(), c.gate.double()
+        n = gate * (x * (x.pow(2).mean(-1, keepdim=True) + EPS).rsqrt() * c.p.double())
+        want = c.scale * c.s.double() + n
+        assert torch.equal(torch.isinf(res), torch.isinf(want)) and not bool(torch.isnan(res).any())
+        assert torch.equal(res[torch.isinf(want)].double(), want[torch.isinf(want)])
+        h = res.double()
+        y = h * (h.pow(2).mean(-1, keepdim=True) + EPS).rsqrt() * c.w.double()
+        assert alike(out, y)
+        q, scale, qres = ops.norm_add_rms_norm_int8(c.x, c.s, c.p, c.w, EPS, gate=c.gate, residual_scale=c.scale)
+        assert torch.equal(qres, res)
+        top = out.abs().amax(-1, keepdim=True).double()  # NaN where a row has one
+        bad = ~torch.isfinite(top)
+        assert alike(scale[bad], top[bad]) and not bool(q.masked_select(bad).any())
+        fine = ~bad.view(-1)
+        want_q, want_scale = quantised(out[:, fine])
+        assert torch.equal(q[:, fine], want_q) and torch.equal(scale[:, fine], want_scale)
+
+
+@pytest.mark.parametrize("hidden", [9, 40, 257, 1001, 2048, 4097, 5003, 5120, 12001, 33000])
+def test_8_bit_rows_whose_mean_square_is_lost(ops, hidden):
+    """Without eps, a row too small to be squared in binary32 has an infinite
+    output where it is not 0, and that is its scale."""
+    c = Case(1, 4, hidden, torch.bfloat16, 17, post=False)
+    x, s = torch.zeros_like(c.x), c.s.clone()
+    s[0, 1] = torch.where(s[0, 1] >= 0, 1e-30, -1e-30).to(torch.bfloat16)
+    q, scale, res = ops.norm_add_rms_norm_int8(x, s, None, c.w, 0.0)
+    out, _ = ops.norm_add_rms_norm(x, s, None, c.w, 0.0)
+    assert torch.equal(res, s) and bool(torch.isinf(out[0, 1]).all())
+    assert float(scale[0, 1]) == float("inf") and not bool(q[0, 1].any())
+    fine = [0, 2, 3]
+    want, want_scale = quantised(out[:, fine])
+    assert torch.equal(q[:, fine], want) and torch.equal(scale[:, fine], want_scale)
