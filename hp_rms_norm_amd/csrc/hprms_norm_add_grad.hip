@@ -120,6 +120,7 @@ __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a)
   const int dup = tail ? 8 - tail : 0;  // the tail vector's elements that a whole vector holds
   int off[VPL], skip[VPL];
   bool on[VPL];
+  u32x4 own[VPL];
   ColumnSums<LACC, (Z ? 2 : 1) * VPL, BLOCK> acc;  // dweight's, then z
   float* post_sums = a.post_sums + (int64_t)blockIdx.x * a.hidden;
 #pragma unroll
@@ -128,6 +129,7 @@ __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a)
     on[k] = v < nvec + (tail ? 1 : 0);
     off[k] = v < nvec ? v * 8 : a.hidden - 8;
     skip[k] = v < nvec ? 0 : dup;
+    own[k] = k >= VPL / 2 ? without_first(skip[k]) : without_first(0);
     acc.clear(k);
     if constexpr (Z) acc.clear(VPL + k);
   }
@@ -169,14 +171,19 @@ __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a)
   const uint16_t* gate = a.gate;  // the unit's row of a shared one
   float wf[HOLD ? VPL : 1][8], mf[HOLD && SCALED ? VPL : 1][8];
   auto scales = [&](int k, float (&m)[8]) {
-    const u32x4 p = POST && on[k] ? load_row8(a.post_weight + off[k]) : zeros;
-    const u32x4 g = SHARED && on[k] ? load_row8(gate + off[k]) : zeros;
+    u32x4 p = POST && on[k] ? load_row8(a.post_weight + off[k]) : zeros;
+    u32x4 g = SHARED && on[k] ? load_row8(gate + off[k]) : zeros;
+    if (tail && k >= VPL / 2) {
+      p &= own[k];
+      g &= own[k];
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       m[j] = POST && SHARED ? element<DT>(p, j) * element<DT>(g, j) : POST ? element<DT>(p, j) : element<DT>(g, j);
   };
   auto weights = [&](int k, float (&w)[8]) {
-    const u32x4 v = on[k] ? load_row8(a.weight + off[k]) : zeros;
+    u32x4 v = on[k] ? load_row8(a.weight + off[k]) : zeros;
+    if (tail && k >= VPL / 2) v &= own[k];
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = element<DT>(v, j);
   };
@@ -210,11 +217,12 @@ __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a)
         x[k] = nx[k];
         h[k] = nh[k];
         g[k] = ng[k];
-        if (tail) {
-          drop_first(d[k], skip[k]);
-          drop_first(e[k], skip[k]);
-          drop_first(x[k], skip[k]);
-          drop_first(h[k], skip[k]);
+        if (tail && k >= VPL / 2) {
+          d[k] &= own[k];
+          e[k] &= own[k];
+          x[k] &= own[k];
+          h[k] &= own[k];
+          g[k] &= own[k];
         }
       }
       if constexpr (AHEAD) load(row + step, row + step < end);

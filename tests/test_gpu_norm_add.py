@@ -439,3 +439,49 @@ def test_8_bit_rows_whose_mean_square_is_lost(ops, hidden):
     fine = [0, 2, 3]
     want, want_scale = quantised(out[:, fine])
     assert torch.equal(q[:, fine], want) and torch.equal(scale[:, fine], want_scale)
+
+
+@pytest.mark.parametrize("hidden", [h for h in OVERLAPPED if h != 32761])
+@pytest.mark.parametrize("where", ["gate of a row", "gate", "post_weight", "weight"])
+@pytest.mark.parametrize("post", [True, False])
+def test_gradient_of_infinities_where_a_rows_vectors_overlap(ops, hidden, where, post):
+    """Infinities and NaN as the formula has them; what it leaves finite is what
+    it is without the infinity, bit by bit."""
+    if where == "post_weight" and not post:
+        return
+    for at in (hidden - 8, hidden // 8 * 8 - 1):
+        c = Case(1, 6, hidden, torch.bfloat16, 16, "element" if where == "gate of a row" else "channel", post, 0.5)
+        c.p = None if c.p is None else c.p.clone()
+        base, res, dout, dres = run_backward(ops, c)
+        if where == "post_weight":
+            c.p[at] = float("inf")
+        elif where == "weight":
+            c.w[at] = float("inf")
+        else:
+            c.gate.view(-1, hidden)[-1, at] = -float("inf")
+        got = ops.norm_add_rms_norm_backward(dout, c.x, res, c.p, c.w, EPS, gate=c.gate, residual_scale=c.scale,
+                                             dresidual=dres)
+        h, d, x, gate = res.double(), dout.double(), c.x.double(), c.gate.double()
+        r = (h.pow(2).mean(-1, keepdim=True) + EPS).rsqrt()
+        g = d * c.w.double()
+        dh = r * g - h * (r ** 3 * (g * h).mean(-1, keepdim=True)) + dres.double()
+        a, n, dpost = gate * dh, x, None
+        dx = a
+        if post:
+            q = (x.pow(2).mean(-1, keepdim=True) + EPS).rsqrt()
+            n = x * q * c.p.double()
+            dpost = (a * x * q).sum((0, 1))
+            a = a * c.p.double()
+            dx = q * a - x * (q ** 3 * (a * x).mean(-1, keepdim=True))
+        wants = (dx, c.scale * dh, dpost, (d * h * r).sum((0, 1)), (dh * n).sum_to_size(gate.shape))
+        for name, v, want, b in zip(("dinput", "dresidual_in", "dpost", "dweight", "dgate"), got, wants, base):
+            if want is None:
+                assert v is None
+                continue
+            fine = torch.isfinite(want)
+            assert torch.equal(v[fine], b[fine]), name
+            if v.shape == c.shape:
+                inf = torch.isinf(want)
+                assert torch.equal(torch.isnan(v), torch.isnan(want)) and torch.equal(v[inf].double(), want[inf]), name
+            else:  # a factor that rows share multiplies their sum: infinite where the sum of products is NaN
+                assert not bool(torch.isfinite(v[~fine]).any()), name
