@@ -757,6 +757,8 @@ int hprms_token_log_probs_backward(void* dlogits, const float* dlog_prob, const 
   if (!aligned_to(dlogits, size) || !aligned_to(logits, size) || !aligned_to(dlog_prob, 4) || !aligned_to(lse, 4) ||
       !aligned_to(dentropy, 4) || (dentropy && !aligned_to(entropy, 4)) || !aligned_to(tokens, 8))
     return fail(HPRMS_E_INVALID, "tensors must be aligned to their elements");
+  if (dlogits == logits && rows > 1 && dlogits_row_stride != logits_row_stride)
+    return fail(HPRMS_E_INVALID, "an in-place alias needs equal row strides");
   LogProbGradArgs a = {};
   a.dlogits = (char*)dlogits;
   a.logits = (const char*)logits;

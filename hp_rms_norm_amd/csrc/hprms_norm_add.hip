@@ -331,6 +331,9 @@ int check(const NormAddArgs& a, int64_t hidden, int dtype, bool int8, double eps
     return fail(HPRMS_E_INVALID, "tensors must be aligned to their elements");
   if (a.out == a.residual_out || a.out == a.residual || a.residual_out == a.input || (int8 && a.out == a.input))
     return fail(HPRMS_E_INVALID, "outputs alias each other or another row tensor than their own");
+  if (a.rows > 1 && ((a.out == a.input && a.out_stride != a.input_stride) ||
+                     (a.residual_out == a.residual && a.residual_out_stride != a.residual_stride)))
+    return fail(HPRMS_E_INVALID, "an in-place alias needs equal row strides");
   return HPRMS_OK;
 }
 

@@ -692,6 +692,22 @@ int hprms_norm_add_rmsnorm_backward(void* dinput, void* dresidual_in, void* dpos
     return fail(HPRMS_E_INVALID, "tensors must be aligned to their elements");
   if (rows > 0 && dinput == dresidual_in)
     return fail(HPRMS_E_INVALID, "dinput and dresidual_in alias each other");
+  // a row is read before it is written, by the workgroup that has it
+  auto moves = [&](const void* out, int64_t out_stride, const void* in, int64_t in_stride) {
+    return in && out == in && rows > 1 && out_stride != in_stride;
+  };
+  if (moves(dinput, dinput_row_stride, dout, dout_row_stride) ||
+      moves(dinput, dinput_row_stride, dresidual, dresidual_row_stride) ||
+      moves(dinput, dinput_row_stride, input, input_row_stride) ||
+      moves(dinput, dinput_row_stride, residual, residual_row_stride) ||
+      moves(dresidual_in, dresidual_in_row_stride, dout, dout_row_stride) ||
+      moves(dresidual_in, dresidual_in_row_stride, dresidual, dresidual_row_stride) ||
+      moves(dresidual_in, dresidual_in_row_stride, input, input_row_stride) ||
+      moves(dresidual_in, dresidual_in_row_stride, residual, residual_row_stride) ||
+      moves(dgate, dgate_row_stride, gate, gate_row_stride))
+    return fail(HPRMS_E_INVALID, "an in-place alias needs equal row strides");
+  if (rows > 0 && gate && dgate == gate && gate_rows != rows)
+    return fail(HPRMS_E_INVALID, "dgate aliases a gate that rows share");
   const Plan p = plan_of(rows, hidden, gate_rows, post_weight != nullptr);
   if (p.total > 0 && (!workspace || workspace_size < p.total || ((uintptr_t)workspace & 15) != 0))
     return fail(HPRMS_E_INVALID, "the workspace must hold %lld bytes, 16-byte aligned (got %lld)", (long long)p.total,

@@ -368,3 +368,26 @@ def test_log_probs_abi_ranges_and_no_rows():
     assert log_probs_backward_abi(rows=1 << 20, s0=1 << 40) == abi.HPRMS_E_RANGE
     assert log_probs_abi(rows=0, lp=0, h=0, lse=0, tl=0, ti=0, logits=0, tokens=0, ws=0) == abi.HPRMS_OK
     assert log_probs_backward_abi(rows=0, d=0, g=0, logits=0, tokens=0, lse=0) == abi.HPRMS_OK
+
+
+def test_in_place_with_other_strides():
+    """A tensor in another's place has its row stride too: the rows of one would lie
+    on others' of the other."""
+    for kw in (dict(out=0x3000, s0=72), dict(res_out=0x6000, s1=72)):
+        assert edge_abi(**kw) == abi.HPRMS_E_INVALID and "strides" in abi.last_error()
+    assert edge_abi("hprms_norm_add_rmsnorm_int8", res_out=0x6000, s3=72) == abi.HPRMS_E_INVALID
+    assert "strides" in abi.last_error()
+    for out, stride in (("di", "s0"), ("dr", "s1")):
+        for at in (0x5000, 0x6000, 0x7000, 0xa000):  # dout, input, residual, dresidual
+            assert edge_backward_abi(dres=0xa000, **{out: at, stride: 72}) == abi.HPRMS_E_INVALID
+            assert "equal row strides" in abi.last_error()
+    assert edge_backward_abi(gate=0xb000, dg=0xb000, gates=4, s2=72) == abi.HPRMS_E_INVALID
+    assert "equal row strides" in abi.last_error()
+    assert log_probs_backward_abi(d=0x4000, s0=108) == abi.HPRMS_E_INVALID
+    assert "equal row strides" in abi.last_error()
+
+
+@pytest.mark.parametrize("gates", [1, 2])
+def test_dgate_in_place_of_a_shared_gate(gates):
+    assert edge_backward_abi(gate=0xb000, dg=0xb000, gates=gates) == abi.HPRMS_E_INVALID
+    assert "rows share" in abi.last_error()
