@@ -105,3 +105,53 @@ def test_logits_of_more_than_2_31_elements(ops, rows, vocab, dtype, pad):
     lp.check([v[at] for v in got], z[at], t[at], 4)
     lp.check_backward(d[at], z[at], t[at], adv[at], adv[at])
     assert bool(torch.isfinite(got[0]).all())
+
+
+@pytest.mark.parametrize("groups,length,hidden,gate,lanes", [
+    (1, 530000, 4096, "element", 512), (1, 540000, 4097, "none", 256), (1, 33600000, 64, "channel", 16384),
+    (2, 525000, 2048, "sequence", 1024), (1, 130000, 16600, "none", 64)])
+def test_column_sums_of_more_than_2_31_elements(ops, groups, length, hidden, gate, lanes):
+    """The weights' gradients and a shared gate's over all rows.  The gradients
+    that reach the edge follow its own tensors, so a column's terms have one
+    sign nearly throughout (for each gate) and none may be missing.  `lanes` lanes share the
+    rows of a column on 256 CUs: each adds rows / lanes terms, and 16 + 32
+    partial sums of up to 32 row groups are joined."""
+    c = edge.Case(groups, 8, hidden, BF, 1, gate, True, 0.75)
+    rows = groups * length
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    c.shape = (groups, length, hidden)
+    c.x, c.s = (torch.randn(c.shape, generator=g, device=DEV, dtype=BF) for _ in range(2))
+    if gate == "element":
+        c.gate = torch.rand(c.shape, generator=g, device=DEV, dtype=BF)
+    out, res = c.forward(ops)
+    di, dr = torch.empty_like(c.x), torch.empty_like(c.x)
+    dw, dp = torch.empty(hidden, device=DEV), torch.empty(hidden, device=DEV)
+    dg = None if c.gate is None else torch.empty_like(c.gate)
+    ops.norm_add_rms_norm_backward_out(di, dr, dp, dw, dg, out, c.x, res, c.p, c.w, EPS, c.gate, 0.75, c.x)
+    del di, dr
+    sums = torch.zeros((6, groups, hidden), device=DEV, dtype=torch.float64)
+    block = 1 << 27 >> hidden.bit_length()
+    for at in range(0, length, max(1, block // groups)):
+        part = slice(at, at + max(1, block // groups))
+        x, h, d = c.x[:, part].double(), res[:, part].double(), out[:, part].double()
+        r = (h.pow(2).mean(-1, keepdim=True) + EPS).rsqrt()
+        w = d * c.w.double()
+        dh = r * w - h * r ** 3 * (w * h).mean(-1, keepdim=True) + x
+        size = (r * w).abs() + h.abs() * r ** 3 * (w * h).abs().mean(-1, keepdim=True) + x.abs()
+        t = d * h * r
+        nx = x * (x.pow(2).mean(-1, keepdim=True) + EPS).rsqrt()
+        by = 1.0 if c.gate is None else (c.gate[:, part] if gate == "element" else c.gate).double()
+        n = nx * c.p.double()
+        for i, v in enumerate((t, t.abs(), by * dh * nx, (by * size * nx).abs(), dh * n, (size * n).abs())):
+            sums[i] += v.sum(1)
+    steps = rows / lanes + 16 + 32 + 32 + 4 * edge.k_of(hidden)
+    checks = [(dw, sums[0].sum(0), sums[1].sum(0)), (dp, sums[2].sum(0), sums[3].sum(0))]
+    if gate == "channel":
+        checks.append((dg, sums[4].sum(0), sums[5].sum(0)))
+    elif gate == "sequence":
+        checks.append((dg[:, 0], sums[4], sums[5]))
+    for got, want, size in checks:
+        u = edge.U[got.dtype]
+        assert float((want.abs() / size).median()) > 0.1  # (or the bound would say little)
+        off = (got.double() - want).abs()
+        assert bool((off <= u * want.abs() + steps * edge.E * (1 + u) * size).all()), (off / size).max()
