@@ -5,12 +5,13 @@
 //
 // The sums are exact in 32-bit integers (up to 131071 terms of at most 2^14), so
 // their order, and with it every choice of tiles below, leaves no trace in the
-// result; a sum is rounded to binary32 once (24 bits of it, a relative error of
-// 2^-24 beside the output's own 2^-9 or 2^-12), then scaled.
+// result; a sum is rounded to binary32 once (24 bits of it, a relative error of at
+// most 2^-24 beside the output's own 2^-8 or 2^-11), then scaled.
 //
 // Few rows: the weight's bytes bound the call.  Up to 4 rows run on dot products of 4
 // bytes, a wave reading whole KB of a weight's row, so the weight streams in whole
-// lines (1 x 4096 x 14336: 10.6 us, 5.5 TB/s; on the matrix cores 14.4; 4 x 8192 x 8192
+// lines (1 x 4096 x 14336: 9.9 us over three weights in turn, 10.9 over more than the
+// caches hold, 5.4 TB/s; on the matrix cores 14.4; 4 x 8192 x 8192
 // 15.3 and 19.6, 4 x 4096 x 4096 6.7 and 6.9, but 8 rows of it 10.1 and 6.9).  More
 // rows run on the matrix cores (hprms_product.h), in tiles by a model of their
 // times, and long sums of few tiles in shares.
@@ -309,9 +310,12 @@ struct Choice {
 
 // A sum of 8192 entries or more is cut into shares, of 1792 at least, where that
 // fills the CUs: a second launch, 3 us, adds them (4 bytes of each written and read
-// again).  16 x 14336 x 4096 18.9 us whole and 16.2 in 4 shares, 48 rows 30.3 and
-// 17.5, 256 rows 40.0 and 35.0; at 4096 entries it gains nothing (48 x 4096 x 4096
-// 10.7 and 11.2 when both were measured).
+// again).  Whole and in shares, us: 16 x 14336 x 4096 18.5 and 15.7, 48 rows 27.0 and
+// 18.8, 256 rows 39.3 and 35.3; 24 x 16384 x 4096 29.7 and 18.8; 24 x 8192 x 1024
+// 10.6 and 8.4.  With many outputs the model takes shares where the whole sum is
+// faster: 16 x 8192 x 8192 18.5 and 17.9, but 48 rows 19.6 and 21.0, 128 rows 25.0 and
+// 30.7.  At 4096 entries they gain nothing (48 x 4096 x 4096 8.2 either way, x 14336
+// 16.1 and 18.3).
 Choice choose(int64_t rows, int64_t inner, int64_t outer) {
   if (rows <= 4) return {kFewRows, 1, (int32_t)inner};
   Choice best = {};

@@ -499,10 +499,10 @@ def token_log_probs_backward_out(dlogits, dlog_prob, logits, tokens, lse, entrop
     * p * (log(p) + entropy)``.  ``lse`` and ``entropy`` are the forward
     call's, ``dlog_prob`` and ``dentropy`` (or None) float32 like ``tokens``.
     Ignored rows and rows of nothing but -inf get zeros; a token out of range
-    makes its row NaN.  A probability p is off by up to ``2^-22 (|lse| +
-    |log p|)`` of itself, as ``lse`` is float32: a row masked with the dtype's
-    lowest value throughout needs an ignored token.  ``dlogits`` may be
-    ``logits``.  No reference counterpart."""
+    makes its row NaN.  A probability p is off by up to ``2^-16 + 2^-22 (|lse|
+    + |log p|)`` of itself, as ``lse`` is float32: a row masked with the
+    dtype's lowest value throughout needs an ignored token.  ``dlogits`` may
+    be ``logits``.  No reference counterpart."""
     torch.ops.hp_rms_norm.token_log_probs_backward.default(dlogits, dlog_prob, dentropy, logits, tokens, lse,
                                                            entropy, ignore_index)
 

@@ -471,9 +471,9 @@ int hprms_clip_grad_norm(float* norm, void* const* outs, const int* out_dtypes, 
  * rne(clamp(y * (1 / scale[r]), -127, 127)); a row that holds NaN or infinity has
  * that as its scale and zeros as elements.  `out` (16-bit form) may be `input`
  * and `residual_out` may be `residual`, exactly, with the same row stride; nothing
- * else is shared.  The
- * kernel shape follows from hidden alone in either batch-invariant mode.  No
- * workspace.  rows == 0 is a no-op.  No counterpart in the reference.
+ * else is shared.  The kernel shape follows from hidden alone in either
+ * batch-invariant mode.  No workspace.  rows == 0 is a no-op.  No counterpart in
+ * the reference.
  */
 int hprms_norm_add_rmsnorm(void* out, void* residual_out, const void* input, const void* post_weight,
                            const void* weight, const void* residual, const void* gate, int64_t rows, int64_t hidden,
@@ -506,9 +506,9 @@ int hprms_norm_add_rmsnorm_int8(void* out, float* scale, void* residual_out, con
  * zeros to the weights' and the gate's).  `dinput` and `dresidual_in` may each
  * be one of dout, dresidual, input and residual exactly, not the same one, and
  * with a gate for each row `dgate` may be `gate` (each with the same row stride).
- * The workspace is as for
- * hprms_rmsnorm_backward(), of hprms_norm_add_rmsnorm_backward_workspace()
- * bytes.  No counterpart in the reference.
+ * The workspace is as for hprms_rmsnorm_backward(), of
+ * hprms_norm_add_rmsnorm_backward_workspace() bytes.  No counterpart in the
+ * reference.
  */
 int64_t hprms_norm_add_rmsnorm_backward_workspace(int64_t rows, int64_t hidden, int64_t gate_rows);
 int hprms_norm_add_rmsnorm_backward(void* dinput, void* dresidual_in, void* dpost_weight, void* dweight, void* dgate,
@@ -569,7 +569,8 @@ int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* to
  *   dlogits <- dlog_prob * ([v == token] - p) - dentropy * p * (log p + entropy)
  * `dentropy` may be NULL (and then `entropy`).  Ignored rows and rows of nothing
  * but -infinity get zeros, a token out of range NaN.  A p is off by up to
- * 2^-22 (|lse| + |log p|) of itself, as lse is binary32.  `dlogits` may be `logits`
+ * 2^-16 + 2^-22 (|lse| + |log p|) of itself: the sum's own error, and lse is
+ * binary32.  `dlogits` may be `logits`
  * exactly, with the same row stride.  No workspace.  No counterpart in the reference.
  */
 int hprms_token_log_probs_backward(void* dlogits, const float* dlog_prob, const float* dentropy, const void* logits,
