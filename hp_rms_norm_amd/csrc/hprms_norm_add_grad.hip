@@ -108,13 +108,17 @@ struct ColumnSums<true, N, BLOCK> {
 // z alone gives both columns' sums of a shared gate: its gradient is post_weight *
 // z, and gate * z is its unit's share of dpost.  HOLD keeps weight and m as
 // binary32 in registers (8 instructions an element fewer than unpacking them for
-// each row); LACC keeps the columns' sums in LDS.
+// each row), or weight and post_weight as they are (PACKED); LACC keeps the columns'
+// sums in LDS.
 template <int DT, int LPR, int VPL, int BLOCK, bool POST, int GATE, bool AHEAD, bool HOLD, bool LACC, bool NT>
 __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a) {
   constexpr int RPB = BLOCK / LPR;
   constexpr bool SHARED = GATE == kSharedGate, ELEMENT = GATE == kElementGate;
   constexpr bool SCALED = POST || SHARED;  // m is more than 1 (or a row's own gate)
   constexpr bool Z = POST || SHARED;
+  // a row's own gate beside post_weight leaves no registers for both as binary32 (1021
+  // x 5003: 36.1 us so, 32.3 with the two packed)
+  constexpr bool PACKED = HOLD && ELEMENT && POST, FLOATS = HOLD && !PACKED;
   __shared__ float sums[2][BLOCK / 64 * 3];
   __shared__ float sums2[2][BLOCK / 64];
   __shared__ float cols[RPB > 1 ? RPB * LPR * 8 : 1];
@@ -172,27 +176,33 @@ __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a)
     }
   };
   const uint16_t* gate = a.gate;  // the unit's row of a shared one
-  float wf[HOLD ? VPL : 1][8], mf[HOLD && SCALED ? VPL : 1][8];
+  float wf[FLOATS ? VPL : 1][8], mf[FLOATS && SCALED ? VPL : 1][8];
+  u32x4 wp[PACKED ? VPL : 1], pp[PACKED ? VPL : 1];
+  auto vector = [&](const uint16_t* from, int k) {
+    u32x4 v = on[k] ? load_row8(from + off[k]) : zeros;
+    if (tail && k >= VPL / 2) v &= own[k];
+    return v;
+  };
   auto scales = [&](int k, float (&m)[8]) {
-    u32x4 p = POST && on[k] ? load_row8(a.post_weight + off[k]) : zeros;
-    u32x4 g = SHARED && on[k] ? load_row8(gate + off[k]) : zeros;
-    if (tail && k >= VPL / 2) {
-      p &= own[k];
-      g &= own[k];
-    }
+    const u32x4 p = PACKED ? pp[PACKED ? k : 0] : POST ? vector(a.post_weight, k) : zeros;
+    const u32x4 g = SHARED ? vector(gate, k) : zeros;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       m[j] = POST && SHARED ? element<DT>(p, j) * element<DT>(g, j) : POST ? element<DT>(p, j) : element<DT>(g, j);
   };
   auto weights = [&](int k, float (&w)[8]) {
-    u32x4 v = on[k] ? load_row8(a.weight + off[k]) : zeros;
-    if (tail && k >= VPL / 2) v &= own[k];
+    const u32x4 v = PACKED ? wp[PACKED ? k : 0] : vector(a.weight, k);
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = element<DT>(v, j);
   };
   if constexpr (HOLD) {
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) weights(k, wf[k]);
+    for (int k = 0; k < VPL; ++k) {
+      if constexpr (PACKED)
+        wp[k] = vector(a.weight, k);
+      else
+        weights(k, wf[k]);
+    }
   }
   int phase = 0;
   for (int64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
@@ -207,7 +217,12 @@ __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a)
     if constexpr (SHARED) gate = a.gate + at * a.gate_stride;
     if constexpr (HOLD && SCALED) {
 #pragma unroll
-      for (int k = 0; k < VPL; ++k) scales(k, mf[k]);
+      for (int k = 0; k < VPL; ++k) {
+        if constexpr (PACKED)
+          pp[k] = vector(a.post_weight, k);  // (before the units: 8192 x 4096 112 us, 97 here)
+        else
+          scales(k, mf[k]);
+      }
     }
     for (int64_t row0 = first; row0 < end; row0 += step) {
       const int64_t row = row0 + sub;
@@ -233,12 +248,12 @@ __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a)
 #pragma unroll
       for (int k = 0; k < VPL; ++k) {
         float w[8];
-        if constexpr (!HOLD) weights(k, w);
+        if constexpr (!FLOATS) weights(k, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float hf = element<DT>(h[k], j);
           s[0] += hf * hf;
-          s[1] += (element<DT>(d[k], j) * hf) * (HOLD ? wf[HOLD ? k : 0][j] : w[j]);
+          s[1] += (element<DT>(d[k], j) * hf) * (FLOATS ? wf[FLOATS ? k : 0][j] : w[j]);
           if constexpr (POST) s[2] += element<DT>(x[k], j) * element<DT>(x[k], j);
         }
         packed_again(d[k]);
@@ -256,27 +271,35 @@ __global__ __launch_bounds__(BLOCK) void norm_add_grad_kernel(NormAddGradArgs a)
 #pragma unroll
       for (int k = 0; k < VPL; ++k) {
         float w[8], m[8], o[8], dx[8], dg[8], tw[8], tz[8];
-        if constexpr (!HOLD) weights(k, w);
-        if constexpr (!HOLD && SCALED) scales(k, m);
+        if constexpr (PACKED) {
+          packed_again(wp[k]);
+          packed_again(pp[k]);
+        }
+        if constexpr (!FLOATS) weights(k, w);
+        if constexpr (!FLOATS && SCALED) scales(k, m);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float hf = element<DT>(h[k], j), df = element<DT>(d[k], j), xf = element<DT>(x[k], j);
-          const float wj = HOLD ? wf[HOLD ? k : 0][j] : w[j];
+          const float wj = FLOATS ? wf[FLOATS ? k : 0][j] : w[j];
           float dh = r * (df * wj) - hf * rc + element<DT>(e[k], j);
           o[j] = dh * a.residual_scale;
           tw[j] = (df * hf) * r;
           float v = dh * xf;  // q times this: what the first norm passes on, without its weight
           if constexpr (SCALED) {
-            const float mj = HOLD ? mf[HOLD && SCALED ? k : 0][j] : m[j];
+            const float mj = FLOATS ? mf[FLOATS && SCALED ? k : 0][j] : m[j];
             if constexpr (ELEMENT) {
-              const float gf = element<DT>(g[k], j);
+              // gate * post_weight first, as a shared gate has it (in binary32 exact): a
+              // row's bits are the same whichever kind its gate is
+              const float gf = element<DT>(g[k], j), mg = mj * gf;
               dg[j] = (v * q) * mj;
-              dh *= gf;
-              v *= gf;
+              tz[j] = (v * gf) * q;
+              mv[0] += v * mg;
+              dh *= mg;
+            } else {
+              tz[j] = v * q;
+              mv[0] += v * mj;
+              dh *= mj;
             }
-            tz[j] = v * q;
-            mv[0] += v * mj;
-            dh *= mj;
           } else if constexpr (ELEMENT) {
             dg[j] = v;
             dh *= element<DT>(g[k], j);

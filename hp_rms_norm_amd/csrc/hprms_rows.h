@@ -72,9 +72,9 @@ __device__ __forceinline__ void drop_first(u32x4& v, int skip) {
 
 // The same as a mask, made once for all rows of a lane.  A lane's first VPL / 2
 // vectors are whole (a shape's lanes hold more than half of what they could) and need
-// none.  The gradient takes masks (1021 x 5003, a gate for each element: 31.7 us, 35.5
-// with drop_first), the forward call, a row a workgroup, does not (8192 x 4096: 47.4 us
-// with them, 46.3 without).
+// none.  The gradient takes masks (1021 x 5003, a gate for each element, when both were
+// measured: 31.8 us, 35.5 with drop_first), the forward call, a row a workgroup, does
+// not (8192 x 4096: 47.4 us with them, 46.3 without).
 __device__ __forceinline__ u32x4 without_first(int skip) {
   u32x4 m;
 #pragma unroll

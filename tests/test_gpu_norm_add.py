@@ -485,3 +485,21 @@ def test_gradient_of_infinities_where_a_rows_vectors_overlap(ops, hidden, where,
                 assert torch.equal(torch.isnan(v), torch.isnan(want)) and torch.equal(v[inf].double(), want[inf]), name
             else:  # a factor that rows share multiplies their sum: infinite where the sum of products is NaN
                 assert not bool(torch.isfinite(v[~fine]).any()), name
+
+
+@pytest.mark.parametrize("hidden", [7, 64, 129, 512, 1000, 2048, 4096, 5003, 8192, 12001, 16384, 17000])
+@pytest.mark.parametrize("gate", GATES)
+def test_rows_of_the_gradient_do_not_depend_on_the_others(ops, hidden, gate):
+    """A row alone, whose gate is then one for all rows and one for each alike,
+    among few and among many."""
+    for dtype in DTYPES:
+        for post in (True, False):
+            c = Case(1, 240, hidden, dtype, 18, gate, post, 0.7)
+            want, res, dout, dres = run_backward(ops, c)
+            for at in [slice(i, i + 1) for i in range(0, 240, 6)] + [slice(3, 5), slice(100, 160)]:
+                g = c.gate[:, at] if gate == "element" else c.gate
+                got = ops.norm_add_rms_norm_backward(dout[:, at], c.x[:, at], res[:, at], c.p, c.w, EPS, gate=g,
+                                                     residual_scale=0.7, dresidual=dres[:, at])
+                assert torch.equal(got[0], want[0][:, at]) and torch.equal(got[1], want[1][:, at])
+                if gate == "element":
+                    assert torch.equal(got[4], want[4][:, at])
