@@ -570,8 +570,8 @@ int hprms_token_log_probs(float* log_prob, float* entropy, float* lse, float* to
  * `dentropy` may be NULL (and then `entropy`).  Ignored rows and rows of nothing
  * but -infinity get zeros, a token out of range NaN.  A p is off by up to
  * 2^-16 + 2^-22 (|lse| + |log p|) of itself: the sum's own error, and lse is
- * binary32.  `dlogits` may be `logits`
- * exactly, with the same row stride.  No workspace.  No counterpart in the reference.
+ * binary32.  `dlogits` may be `logits` exactly, with the same row stride.  No
+ * workspace.  No counterpart in the reference.
  */
 int hprms_token_log_probs_backward(void* dlogits, const float* dlog_prob, const float* dentropy, const void* logits,
                                    const int64_t* tokens, const float* lse, const float* entropy, int64_t rows,
